@@ -1,0 +1,293 @@
+// GroupNorm (+ ReLU) whose backward pass works on an 8-bit copy of its input (kept8.cuh), so that the bf16 input need
+// not live until then: 1.0625 bytes per element instead of 2.
+//
+// Forward (gn8_apply_kernel, behind the statistics pass of group_norm.cu or a convolution's own partials):
+//   y = relu(x a + c), a = rstd w, c = b - mean a, and the copy, in one pass over x.
+//   A value that the rounding would move across the ReLU's border is kept one step further towards x instead (its error
+//   is then up to a step): the backward pass takes the mask from the copy and finds the forward's own mask, and the
+//   only thing that differs from the ordinary backward pass is xhat by at most a step.
+// Backward: the two passes of group_norm.cu with the copy in the place of x:
+//   gn8_bwd_partial  per (split, n) and channel: sum(dy') and sum(dy' xhat), dy' = dy gated by the mask
+//   gn8_bwd_dx       dx = rstd (dy' w - c1 - xhat c2), c1 / c2 the group's means of dy' w and dy' w xhat
+//
+// Every thread owns 8 channels (half a block) of a voxel; the two halves find their largest magnitude by one shuffle.
+// Channels are a multiple of 16, so a block never leaves its voxel. Bound: memory (forward 5.06 bytes an element behind
+// the statistics, backward 3.06 + 5.06 against 4 + 6 of the bf16 kernels).
+#include "common.cuh"
+#include "host_api.h"
+#include "kept8.cuh"
+
+namespace sb {
+
+constexpr int GN8_THREADS = 256;
+
+struct Gn8Params {
+  const __nv_bfloat16* x;
+  const __nv_bfloat16* dy;
+  __nv_bfloat16* y;  // forward output / backward dx
+  uint8_t* q;        // [N S C] int8
+  uint8_t* exps;     // [N S C / 16]
+  const float* w;
+  const float* b;
+  float* mean;
+  float* rstd;
+  const float* fin;  // forward: [N][G][3] statistics; dx: [N][C][2] sums
+  float* part;       // [N][nsplit][C][2]
+  float* dw;
+  float* db;
+  int N, C, G, nsplit, relu, accumulate;
+  long long S;
+  float eps, group_elems;
+};
+
+__device__ __forceinline__ void gn8_unpack(const uint4& v, float (&f)[8]) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __bfloat1622float2(h[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+__device__ __forceinline__ uint4 gn8_pack(const float (&f)[8]) {
+  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+}
+__device__ __forceinline__ void gn8_values(uint2 q, float step, float (&f)[8]) {
+  float lo[4], hi[4];
+  kept_unpack4(q.x, lo);
+  kept_unpack4(q.y, hi);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { f[i] = lo[i] * step; f[4 + i] = hi[i] * step; }
+}
+
+__global__ void __launch_bounds__(GN8_THREADS, 3) gn8_apply_kernel(const Gn8Params p) {
+  __shared__ float s_mean[256], s_rstd[256];
+  const int n = blockIdx.y;
+  for (int g = threadIdx.x; g < p.G; g += GN8_THREADS) {
+    const float* e = p.fin + ((long long)n * p.G + g) * 3;
+    const float m = e[1], r = rsqrtf(e[2] / e[0] + p.eps);
+    s_mean[g] = m;
+    s_rstd[g] = r;
+    if (blockIdx.x == 0) { p.mean[n * p.G + g] = m; p.rstd[n * p.G + g] = r; }
+  }
+  __syncthreads();
+  const int tpv = p.C / 8, vpb = GN8_THREADS / tpv;
+  const int oct = threadIdx.x % tpv, vl = threadIdx.x / tpv;
+  const int cg = p.C / p.G;
+  float a[8], c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int ch = oct * 8 + i, g = ch / cg;
+    a[i] = s_rstd[g] * p.w[ch];
+    c[i] = p.b[ch] - s_mean[g] * a[i];
+  }
+  const long long base = (long long)n * p.S * p.C + oct * 8;
+  // the loop is uniform over the block, for the shuffle: a thread without a voxel takes part with zeros
+  for (long long v0 = (long long)blockIdx.x * vpb; v0 < p.S; v0 += (long long)gridDim.x * vpb) {
+    const long long v = v0 + vl;
+    const bool live = vl < vpb && v < p.S;
+    const long long at = base + v * p.C;
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (live) raw = __ldg(reinterpret_cast<const uint4*>(p.x + at));
+    float f[8], t[8];
+    gn8_unpack(raw, f);
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    const uint32_t b = kept_exponent(amax);
+    const float step = kept_step(b), inv = b == 255u ? 0.f : kept_inv(b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      t[i] = fmaf(f[i], inv, KEPT_MAGIC);
+      float yv = fmaf(f[i], a[i], c[i]);
+      if (p.relu) {
+        const bool on = yv > 0.f, kept_on = fmaf((t[i] - KEPT_MAGIC) * step, a[i], c[i]) > 0.f;
+        if (on != kept_on) t[i] += on == (a[i] > 0.f) ? 1.f : -1.f;
+        yv = yv <= 0.f ? 0.f : yv;  // NaN propagates
+      }
+      if (b >= KEPT_TOP_BF16) t[i] = b == 255u ? KEPT_MAGIC : kept_cap(t[i]);
+      f[i] = yv;
+    }
+    if (live) {
+      *reinterpret_cast<uint4*>(p.y + at) = gn8_pack(f);
+      *reinterpret_cast<uint2*>(p.q + at) =
+          make_uint2(kept_pack4(t[0], t[1], t[2], t[3]), kept_pack4(t[4], t[5], t[6], t[7]));
+      if ((oct & 1) == 0) p.exps[at / KEPT_BLOCK] = (uint8_t)b;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(GN8_THREADS, 3) gn8_bwd_partial_kernel(const Gn8Params p) {
+  __shared__ float s_a[GN8_THREADS * 8], s_b[GN8_THREADS * 8];
+  const int split = blockIdx.x, n = blockIdx.y;
+  const int tpv = p.C / 8, vpb = GN8_THREADS / tpv;
+  const int oct = threadIdx.x % tpv, vl = threadIdx.x / tpv;
+  const int cg = p.C / p.G;
+  const long long chunk = (p.S + p.nsplit - 1) / p.nsplit;
+  const long long v0 = (long long)split * chunk;
+  const long long v1 = v0 + chunk < p.S ? v0 + chunk : p.S;
+  float a[8], c[8], A[8], B[8], mu[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int ch = oct * 8 + i, g = ch / cg;
+    mu[i] = p.mean[n * p.G + g];
+    a[i] = p.rstd[n * p.G + g] * p.w[ch];
+    c[i] = p.b[ch] - mu[i] * a[i];
+    A[i] = 0.f;
+    B[i] = 0.f;
+  }
+  const long long base = (long long)n * p.S * p.C + oct * 8;
+  if (vl < vpb) {
+    for (long long v = v0 + vl; v < v1; v += vpb) {
+      const long long at = base + v * p.C;
+      float fx[8], fd[8];
+      gn8_values(__ldg(reinterpret_cast<const uint2*>(p.q + at)), kept_step(__ldg(p.exps + at / KEPT_BLOCK)), fx);
+      gn8_unpack(__ldg(reinterpret_cast<const uint4*>(p.dy + at)), fd);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float d = fd[i];
+        if (p.relu && fmaf(fx[i], a[i], c[i]) <= 0.f) d = 0.f;
+        A[i] += d;
+        B[i] = fmaf(d, fx[i] - mu[i], B[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    s_a[threadIdx.x * 8 + i] = A[i];
+    s_b[threadIdx.x * 8 + i] = B[i] * p.rstd[n * p.G + (oct * 8 + i) / cg];
+  }
+  __syncthreads();
+  for (int ch = threadIdx.x; ch < p.C; ch += GN8_THREADS) {
+    float sa = 0.f, sb = 0.f;
+    for (int v = 0; v < vpb; ++v) {
+      const int t = (v * tpv + ch / 8) * 8 + ch % 8;
+      sa += s_a[t];
+      sb += s_b[t];
+    }
+    float* dst = p.part + (((long long)n * p.nsplit + split) * p.C + ch) * 2;
+    dst[0] = sa;
+    dst[1] = sb;
+  }
+}
+
+__global__ void __launch_bounds__(GN8_THREADS, 3) gn8_bwd_dx_kernel(const Gn8Params p) {
+  __shared__ float s_c1[256], s_c2[256];
+  const int n = blockIdx.y;
+  const int tpv = p.C / 8, vpb = GN8_THREADS / tpv;
+  const int oct = threadIdx.x % tpv, vl = threadIdx.x / tpv;
+  const int cg = p.C / p.G;
+  const float* fin = p.fin + (long long)n * p.C * 2;
+  for (int g = threadIdx.x; g < p.G; g += GN8_THREADS) {
+    float c1 = 0.f, c2 = 0.f;
+    for (int ch = g * cg; ch < (g + 1) * cg; ++ch) {
+      c1 = fmaf(p.w[ch], fin[2 * ch], c1);
+      c2 = fmaf(p.w[ch], fin[2 * ch + 1], c2);
+    }
+    s_c1[g] = c1 / p.group_elems;
+    s_c2[g] = c2 / p.group_elems;
+  }
+  // dweight / dbias: summed over samples in index order
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    for (int ch = threadIdx.x; ch < p.C; ch += GN8_THREADS) {
+      float sa = 0.f, sb = 0.f;
+      for (int nn = 0; nn < p.N; ++nn) {
+        sa += p.fin[((long long)nn * p.C + ch) * 2];
+        sb += p.fin[((long long)nn * p.C + ch) * 2 + 1];
+      }
+      p.db[ch] = p.accumulate ? p.db[ch] + sa : sa;
+      p.dw[ch] = p.accumulate ? p.dw[ch] + sb : sb;
+    }
+  }
+  __syncthreads();
+  if (vl >= vpb) return;
+  // dx = rstd (d w - c1 - xhat c2) = d a + (x - mean) q + r
+  float a[8], c[8], mu[8], q[8], r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int ch = oct * 8 + i, g = ch / cg;
+    const float rs = p.rstd[n * p.G + g];
+    mu[i] = p.mean[n * p.G + g];
+    a[i] = rs * p.w[ch];
+    c[i] = p.b[ch] - mu[i] * a[i];
+    q[i] = -rs * rs * s_c2[g];
+    r[i] = -rs * s_c1[g];
+  }
+  const long long base = (long long)n * p.S * p.C + oct * 8;
+  for (long long v = (long long)blockIdx.x * vpb + vl; v < p.S; v += (long long)gridDim.x * vpb) {
+    const long long at = base + v * p.C;
+    float fx[8], fd[8];
+    gn8_values(__ldg(reinterpret_cast<const uint2*>(p.q + at)), kept_step(__ldg(p.exps + at / KEPT_BLOCK)), fx);
+    gn8_unpack(__ldg(reinterpret_cast<const uint4*>(p.dy + at)), fd);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float d = fd[i];
+      if (p.relu && fmaf(fx[i], a[i], c[i]) <= 0.f) d = 0.f;
+      fx[i] = fmaf(d, a[i], fmaf(fx[i] - mu[i], q[i], r[i]));
+    }
+    *reinterpret_cast<uint4*>(p.y + at) = gn8_pack(fx);
+  }
+}
+
+static int gn8_fill(const SbGn8Args* a, Gn8Params& p) {
+  if (!sb_gn_supported(a->C, a->G) || a->C % KEPT_BLOCK || a->N < 1 || a->N > 65535 || a->S < 1) return SB_ERR_SHAPE;
+  if (a->w == nullptr || a->b == nullptr || a->kept == nullptr || a->mean == nullptr || a->rstd == nullptr)
+    return SB_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->dy) | reinterpret_cast<uintptr_t>(a->y) |
+       reinterpret_cast<uintptr_t>(a->kept)) & 15)
+    return SB_ERR_ALIGN;
+  memset(&p, 0, sizeof(p));
+  p.x = (const __nv_bfloat16*)a->x;
+  p.dy = (const __nv_bfloat16*)a->dy;
+  p.y = (__nv_bfloat16*)a->y;
+  p.q = (uint8_t*)a->kept;
+  p.exps = p.q + (long long)a->N * a->S * a->C;
+  p.w = a->w; p.b = a->b; p.mean = a->mean; p.rstd = a->rstd;
+  p.fin = a->fin; p.part = a->part; p.dw = a->dw; p.db = a->db;
+  p.N = a->N; p.C = a->C; p.G = a->G; p.S = a->S;
+  p.nsplit = a->nsplit; p.relu = a->relu; p.accumulate = a->accumulate;
+  p.eps = a->eps;
+  p.group_elems = (float)((double)a->S * (a->C / a->G));
+  return 0;
+}
+static int gn8_blocks(const Gn8Params& p) {
+  const int vpb = GN8_THREADS / (p.C / 8);
+  const long long need = (p.S + vpb - 1) / vpb, cap = 148LL * 3 / p.N;  // one wave
+  const long long b = need < cap ? need : cap;
+  return (int)(b < 1 ? 1 : b);
+}
+
+}  // namespace sb
+
+using namespace sb;
+
+extern "C" int sb_gn8_apply(const SbGn8Args* a, cudaStream_t stream) {
+  Gn8Params p;
+  const int rc = gn8_fill(a, p);
+  if (rc) return rc;
+  if (p.x == nullptr || p.y == nullptr || p.fin == nullptr) return SB_ERR_SHAPE;
+  gn8_apply_kernel<<<dim3(gn8_blocks(p), p.N), GN8_THREADS, 0, stream>>>(p);
+  sb_count_launch(1);
+  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+}
+
+extern "C" int sb_gn8_bwd_partial(const SbGn8Args* a, cudaStream_t stream) {
+  Gn8Params p;
+  const int rc = gn8_fill(a, p);
+  if (rc) return rc;
+  if (p.dy == nullptr || p.part == nullptr || p.nsplit < 1) return SB_ERR_SHAPE;
+  gn8_bwd_partial_kernel<<<dim3(p.nsplit, p.N), GN8_THREADS, 0, stream>>>(p);
+  sb_count_launch(1);
+  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+}
+
+extern "C" int sb_gn8_bwd_dx(const SbGn8Args* a, cudaStream_t stream) {
+  Gn8Params p;
+  const int rc = gn8_fill(a, p);
+  if (rc) return rc;
+  if (p.dy == nullptr || p.y == nullptr || p.fin == nullptr || p.dw == nullptr || p.db == nullptr) return SB_ERR_SHAPE;
+  gn8_bwd_dx_kernel<<<dim3(gn8_blocks(p), p.N), GN8_THREADS, 0, stream>>>(p);
+  sb_count_launch(1);
+  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+}

@@ -174,10 +174,45 @@ typedef struct {
 int sb_gn_share(const float* fin, long long count, void* const* dst, void* const* flags, int world,
                 unsigned epoch, cudaStream_t stream);
 
+// The 8-bit copy of an activation (kept8.cuh): sb_kept8_bytes(n) bytes for n elements, 16-byte aligned.
+// kind: 0 bf16, 1 fp16, 2 fp32.
+long long sb_kept8_bytes(long long n);
+int sb_keep8(const void* x, int kind, long long n, void* kept, cudaStream_t stream);
+int sb_restore8(const void* kept, int kind, long long n, void* y, cudaStream_t stream);
+
+// GroupNorm (+ReLU) with an 8-bit copy of its input for the backward pass (group_norm_kept8.cu); C a multiple of 16.
+// `kept` is the copy of x as one row of N S C elements. Forward: x, fin (the [N][G][3] block of sb_gn_stats) -> y, kept,
+// mean, rstd. Backward: dy, kept, mean, rstd -> part [N][nsplit][C][2]; sb_gn_bwd_finalize makes fin [N][C][2] of it,
+// which sb_gn8_bwd_dx turns into y (= dx), dw and db.
+typedef struct {
+  const void* x;
+  const void* dy;
+  void* y;
+  void* kept;
+  const float* w;
+  const float* b;
+  float* mean;
+  float* rstd;
+  const float* fin;
+  float* part;
+  float* dw;
+  float* db;
+  int N, C, G;
+  long long S;
+  int nsplit;
+  float eps;
+  int relu;
+  int accumulate;  // add to dw / db instead of overwriting them
+} SbGn8Args;
+int sb_gn8_apply(const SbGn8Args* a, cudaStream_t stream);
+int sb_gn8_bwd_partial(const SbGn8Args* a, cudaStream_t stream);
+int sb_gn8_bwd_dx(const SbGn8Args* a, cudaStream_t stream);
+
 // number of kernels this library launched so far in the process
 long long sb_launch_count(void);
 void sb_count_launch(int n);
 
+int sb_gn_supported(int C, int G);
 int sb_gn_nsplit(int N, long long S, int C);
 int sb_gn_stats(const SbGnArgs* a, cudaStream_t stream);
 int sb_gn_apply(const SbGnArgs* a, cudaStream_t stream);

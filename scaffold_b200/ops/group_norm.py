@@ -61,8 +61,70 @@ class _GnFn(torch.autograd.Function):
         return dx, dw, db, None, None, None, None, None
 
 
+class _Gn8Fn(torch.autograd.Function):
+    """:class:`_GnFn` that keeps an 8-bit copy of ``x`` for its backward pass instead of ``x``."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, relu, partials):
+        w32, b32 = weight.detach().float().contiguous(), bias.detach().float().contiguous()
+        fin = None
+        if partials is not None:
+            part, splits, pg = partials
+            if pg == groups and part.numel() == x.shape[0] * splits * groups * 3:
+                fin = gk.gn_finalize(part, x.shape[0], groups, splits)
+        y, kept, mean, rstd = gk.gn8_forward(x, w32, b32, groups, eps, relu, fin=fin)
+        ctx.save_for_backward(kept, w32, b32, mean, rstd)
+        ctx.cfg = (groups, relu)
+        ctx.params = (weight, bias)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        kept, w32, b32, mean, rstd = ctx.saved_tensors
+        groups, relu = ctx.cfg
+        into = None
+        if ctx.needs_input_grad[1] and ctx.needs_input_grad[2]:
+            into = tuple(direct_grad_target(p, ctx) for p in ctx.params)
+            if any(t is None for t in into):
+                into = None
+        dx, dw, db = gk.gn8_backward(gy.contiguous(), kept, w32, b32, mean, rstd, groups, relu, into=into)
+        if into is not None:
+            dw = db = None
+            for p in ctx.params:
+                notify_grad_written(p)
+        return dx, dw, db, None, None, None, None
+
+
+def group_norm_kept8(x: torch.Tensor, num_groups: int, weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-5,
+                     activation: Optional[str] = None) -> torch.Tensor:
+    """GroupNorm (+ ReLU) of bf16 ``x [N, C, D, H, W]`` whose backward pass works on an 8-bit copy of ``x``
+    (:mod:`scaffold_b200.ops.kept8`), so ``x`` itself need not live until then.
+
+    The result and its statistics are those of the ordinary :class:`GroupNorm`. The gradients are the formula's at the
+    kept values: a step of the copy for xhat, and the ReLU's mask exactly (a value that rounding would move across the
+    border is kept one step further towards ``x``). CUDA and bf16 only, channels a multiple of 16.
+    """
+    if activation not in (None, "relu"):
+        raise ValueError(f"activation must be None or 'relu'; got {activation!r}")
+    if x.dim() != 5 or x.dtype != torch.bfloat16 or not x.is_cuda:
+        raise ValueError(f"group_norm_kept8 takes bf16 CUDA tensors [N, C, D, H, W]; got {x.dtype} {tuple(x.shape)} on "
+                         f"{x.device}")
+    c = x.shape[1]
+    if not gk.supported_kept8(c, num_groups):
+        raise ValueError(f"{c} channels in {num_groups} groups are outside the kernels' range: a multiple of 16 up to "
+                         "2048, and groups of whole octets (or of 2 or 4 channels)")
+    if weight.shape != (c,) or bias.shape != (c,) or weight.device != x.device or bias.device != x.device:
+        raise ValueError(f"weight and bias must be [{c}] on {x.device}")
+    if x.numel() == 0:
+        raise ValueError(f"group_norm_kept8 has no statistics of an empty tensor {tuple(x.shape)}")
+    with torch.cuda.device(x.device):
+        return from_vm(_Gn8Fn.apply(to_vm(x), weight, bias, num_groups, eps, activation == "relu", None))
+
+
 class GroupNorm(nn.GroupNorm):
     """``nn.GroupNorm`` + optional fused ``activation="relu"``."""
+
+    keep_bits = 16  # 8: the backward pass of the kernel path works on an 8-bit copy of the input (group_norm_kept8)
 
     def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True,
                  activation: Optional[str] = None, device=None, dtype=None):
@@ -84,11 +146,20 @@ class GroupNorm(nn.GroupNorm):
         group that is a whole number of channel octets (or 2 / 4 channels). Other pairs run the ATen formula."""
         return self.affine and gk.supported(self.num_channels, self.num_groups)
 
+    def keeps8(self) -> bool:
+        """Whether the kernel path keeps 8 bits for its backward pass: asked to, with a backward pass to come, on a whole
+        volume (the statistics that shards exchange are those of the bf16 input) and channels a multiple of 16."""
+        return (self.keep_bits == 8 and torch.is_grad_enabled() and self._spatial is None
+                and gk.supported_kept8(self.num_channels, self.num_groups))
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         relu = self.activation == "relu"
         if use_cuda_kernels(x) and x.dim() == 5 and self.kernel_supported():
             partials = getattr(x, "_sb_gn_partials", None)  # left by the convolution that produced x, if it could
-            y = _GnFn.apply(to_vm(x), self.weight, self.bias, self.num_groups, self.eps, relu, self._spatial, partials)
+            if self.keeps8():
+                y = _Gn8Fn.apply(to_vm(x), self.weight, self.bias, self.num_groups, self.eps, relu, partials)
+            else:
+                y = _GnFn.apply(to_vm(x), self.weight, self.bias, self.num_groups, self.eps, relu, self._spatial, partials)
             return from_vm(y)
         if x.is_cuda and use_cuda_kernels(x) and not self._warned:
             self._warned = True
