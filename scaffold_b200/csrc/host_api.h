@@ -208,6 +208,44 @@ int sb_gn8_apply(const SbGn8Args* a, cudaStream_t stream);
 int sb_gn8_bwd_partial(const SbGn8Args* a, cudaStream_t stream);
 int sb_gn8_bwd_dx(const SbGn8Args* a, cudaStream_t stream);
 
+// Cross entropy of a head of K classes over V voxels of C channels without its logits (head_loss.cu).
+// Arrays marked v / k are padded to a multiple of 128 voxels / classes.
+typedef struct {
+  const void* x;       // bf16 [V][C]
+  const void* w;       // bf16 [K][C]
+  const void* bias;    // optional [K]
+  int bias_kind;       // of bias and db: 0 bf16, 2 fp32
+  const void* labels;  // [V]
+  int label_kind;      // 2 int16, 4 int32, 8 int64
+  int has_ignore;
+  long long ignore;    // label of voxels that take no part
+  const float* cw;     // optional class weights [K], not negative
+  long long V;
+  int K, C;
+  int* y;              // v: forward out: label, -1 takes no part
+  float* bias2;        // k: forward out
+  float* lse2;         // v: forward out: log2 of the sum of exponentials
+  double* total;       // [2] forward out: sums of u nll and u
+  float* loss;         // [1]
+  float* den;          // [1]
+  float* g;            // v: sb_head_weights out
+  float* lse2g;        // v: sb_head_weights out
+  void* dx;            // bf16 [V][C]
+  void* dw;            // [K][C]
+  int dw_kind;         // 0 bf16, 2 fp32
+  void* db;            // optional [K]
+  float* scratch;      // sb_head_scratch() floats, 16-byte aligned
+  long long scratch_floats;
+  uint32_t* status;
+} SbHeadArgs;
+int sb_head_max_width(void);
+long long sb_head_scratch(const SbHeadArgs* a, int mode);  // 0 forward, 1 dx, 2 dw
+int sb_head_forward(const SbHeadArgs* a, cudaStream_t stream);
+int sb_head_total(const double* sums, int blocks, double* total, float* loss, float* den, cudaStream_t stream);
+int sb_head_weights(const SbHeadArgs* a, const float* gout, cudaStream_t stream);
+int sb_head_dx(const SbHeadArgs* a, cudaStream_t stream);
+int sb_head_dw(const SbHeadArgs* a, cudaStream_t stream);
+
 // number of kernels this library launched so far in the process
 long long sb_launch_count(void);
 void sb_count_launch(int n);

@@ -224,6 +224,15 @@ SITES = {
     41: "gradient all-reduce: waiting for the peers' gradients",
     42: "gradient all-reduce: waiting for the peers' completion",
     61: "fused loss: a label outside [0, n_classes) (detail = label value, sample); the voxel was skipped",
+    63: "head loss: a label outside [0, n_classes) (detail = label value, voxel); the voxel takes no part",
+    71: "head loss: producer waiting for a free tile",
+    72: "head loss: MMA waiting for a free accumulator",
+    73: "head loss: MMA waiting for the probabilities",
+    74: "head loss: MMA waiting for the resident tile",
+    75: "head loss: MMA waiting for a streamed tile",
+    76: "head loss: MMA waiting for a free tile of logits",
+    77: "head loss: epilogue waiting for the accumulator",
+    78: "head loss: epilogue waiting for a tile of logits",
     62: "fused loss gradient: a label outside [0, n_classes) (detail = label value, sample); the voxel was skipped",
 }
 

@@ -1,0 +1,215 @@
+"""Cross entropy of a head with many classes, taken from the features in front of it.
+
+``head_cross_entropy(features, weight, bias, labels)`` is the class-weighted mean cross entropy
+(:func:`scaffold_b200.ops.loss.sharded_cross_entropy`) of ``features @ weight.T + bias``, with its gradients, without the
+logits: a head of some hundred classes over a 128-cubed volume would keep gigabytes of them, several times over. The fused
+segmentation loss keeps a voxel's classes in registers and ends at 32 classes; this one has no limit on the classes.
+
+On CUDA with bf16 features (or under bf16 autocast) the kernels of ``csrc/head_loss.cu`` multiply features and weight
+tile by tile, once for the loss and once for each gradient; other tensors take the PyTorch formula.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .layout import use_cuda_kernels
+
+_P = C.c_void_p
+
+
+class SbHeadArgs(C.Structure):
+    _fields_ = [
+        ("x", _P), ("w", _P), ("bias", _P), ("bias_kind", C.c_int),
+        ("labels", _P), ("label_kind", C.c_int), ("has_ignore", C.c_int), ("ignore", C.c_longlong),
+        ("cw", _P),
+        ("V", C.c_longlong), ("K", C.c_int), ("C", C.c_int),
+        ("y", _P), ("bias2", _P), ("lse2", _P), ("total", _P), ("loss", _P), ("den", _P),
+        ("g", _P), ("lse2g", _P),
+        ("dx", _P), ("dw", _P), ("dw_kind", C.c_int), ("db", _P),
+        ("scratch", _P), ("scratch_floats", C.c_longlong),
+        ("status", _P),
+    ]
+
+
+_lib.register("sb_head_max_width", [], C.c_int)
+_lib.register("sb_head_scratch", [C.POINTER(SbHeadArgs), C.c_int], C.c_longlong)
+_lib.register("sb_head_forward", [C.POINTER(SbHeadArgs), _P])
+_lib.register("sb_head_total", [_P, C.c_int, _P, _P, _P, _P])
+_lib.register("sb_head_weights", [C.POINTER(SbHeadArgs), _P, _P])
+_lib.register("sb_head_dx", [C.POINTER(SbHeadArgs), _P])
+_lib.register("sb_head_dw", [C.POINTER(SbHeadArgs), _P])
+
+_LABEL_KIND = {torch.int16: 2, torch.int32: 4, torch.int64: 8}
+_KIND = {torch.bfloat16: 0, torch.float32: 2}
+MAX_WIDTH = 256  # HD_MAX_C of csrc/head_loss.cu
+
+
+def head_supported(width: int) -> bool:
+    """Feature widths of the kernels."""
+    return 8 <= width <= MAX_WIDTH and width % 8 == 0
+
+
+def _pad128(n: int) -> int:
+    return (n + 127) // 128 * 128
+
+
+def _scratch(a: SbHeadArgs, mode: int, dev):
+    n = _lib.lib().sb_head_scratch(C.byref(a), mode)
+    if n < 0:
+        raise _lib.NativeError(f"sb_head_scratch refused {a.V} voxels, {a.K} classes, width {a.C}")
+    t = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    a.scratch, a.scratch_floats = _lib.ptr(t), n
+    return t
+
+
+def _args(x, w16, bias, cw) -> SbHeadArgs:
+    a = SbHeadArgs()
+    a.V, a.C = x.shape
+    a.K = w16.shape[0]
+    a.x, a.w, a.cw = x.data_ptr(), w16.data_ptr(), _lib.ptr(cw)
+    if bias is not None:
+        a.bias, a.bias_kind = bias.data_ptr(), _KIND[bias.dtype]
+    a.status = _lib.status_tensor(x.device).data_ptr()
+    return a
+
+
+class _HeadLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, labels, cw, ignore, spatial):
+        """x [V, C] bf16, weight [K, C], both contiguous."""
+        dev = x.device
+        w16 = weight.to(torch.bfloat16)
+        a = _args(x, w16, bias, cw)
+        a.labels, a.label_kind = labels.data_ptr(), _LABEL_KIND[labels.dtype]
+        if ignore is not None:
+            a.has_ignore, a.ignore = 1, ignore
+        vp, kp = _pad128(a.V), _pad128(a.K)
+        y = torch.empty(vp, dtype=torch.int32, device=dev)
+        lse2 = torch.empty(vp, dtype=torch.float32, device=dev)
+        bias2 = torch.empty(kp, dtype=torch.float32, device=dev)
+        total = torch.empty(2, dtype=torch.float64, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        den = torch.empty(1, dtype=torch.float32, device=dev)
+        a.y, a.lse2, a.bias2, a.total, a.loss, a.den = (t.data_ptr() for t in (y, lse2, bias2, total, loss, den))
+        keep = _scratch(a, 0, dev)  # noqa: F841  (freed in stream order)
+        _lib.check(_lib.lib().sb_head_forward(C.byref(a), _lib.stream_ptr()), "sb_head_forward")
+        if spatial is not None and spatial.size > 1:
+            spatial.all_reduce_sum(total)
+            _lib.check(_lib.lib().sb_head_total(total.data_ptr(), 1, total.data_ptr(), loss.data_ptr(), den.data_ptr(),
+                                                _lib.stream_ptr()), "sb_head_total")
+        ctx.save_for_backward(x, w16, y, lse2, bias2, den, cw)
+        ctx.like = weight.dtype, None if bias is None else bias.dtype
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        x, w16, y, lse2, bias2, den, cw = ctx.saved_tensors
+        dev = x.device
+        w_type, b_type = ctx.like
+        L, st = _lib.lib(), _lib.stream_ptr()
+        a = _args(x, w16, None, cw)
+        g, lse2g = torch.empty_like(lse2), torch.empty_like(lse2)
+        a.y, a.lse2, a.bias2, a.den, a.g, a.lse2g = (t.data_ptr() for t in (y, lse2, bias2, den, g, lse2g))
+        gout = gout.float().contiguous()
+        _lib.check(L.sb_head_weights(C.byref(a), gout.data_ptr(), st), "sb_head_weights")
+        dx = dw = db = None
+        if ctx.needs_input_grad[0]:
+            dx = torch.empty_like(x)
+            a.dx = dx.data_ptr()
+            keep = _scratch(a, 1, dev)
+            _lib.check(L.sb_head_dx(C.byref(a), st), "sb_head_dx")
+            del keep
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dw = torch.empty(w16.shape, dtype=w_type, device=dev)
+            a.dw, a.dw_kind = dw.data_ptr(), _KIND[w_type]
+            if ctx.needs_input_grad[2]:
+                db = torch.empty(w16.shape[0], dtype=b_type, device=dev)
+                a.db, a.bias_kind = db.data_ptr(), _KIND[b_type]
+            keep = _scratch(a, 2, dev)
+            _lib.check(L.sb_head_dw(C.byref(a), st), "sb_head_dw")
+            del keep
+        return dx, dw if ctx.needs_input_grad[1] else None, db, None, None, None, None
+
+
+def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], labels: torch.Tensor,
+                       class_weights: Optional[torch.Tensor] = None, ignore_label: Optional[int] = None,
+                       spatial=None) -> torch.Tensor:
+    """The cross entropy of ``features @ weight.T + bias`` against ``labels``, as an fp32 scalar.
+
+    ``features [..., C]`` (voxel-major, the classes' axis of the logits is the last), ``weight [K, C]`` (or the
+    ``[K, C, 1, 1, 1]`` of a 1x1x1 convolution), ``bias [K]`` or None, ``labels [...]`` int16, int32 or int64.
+    ``class_weights [K]`` (not negative) weigh the voxels by their label; the result is the sum of the weighted terms over
+    the sum of the weights, over all shards with ``spatial``. Voxels of ``ignore_label`` take no part; without any other
+    voxel the loss and its gradients are zero. A label outside the classes takes no part either and is reported by
+    :func:`scaffold_b200.ops._lib.check_status`. Features of voxels that take no part have to be finite, as for the
+    formula: they reach the weight's gradient as ``0 * x``.
+
+    The kernels read bf16: an fp32 ``weight`` is rounded, its gradient comes back in fp32. Gradients: features in bf16,
+    weight and bias in their own types.
+    """
+    if features.dim() < 1 or labels.shape != features.shape[:-1]:
+        raise ValueError(f"features {tuple(features.shape)} need labels {tuple(features.shape[:-1])}; "
+                         f"got {tuple(labels.shape)}")
+    c = features.shape[-1]
+    if weight.dim() < 2 or weight.shape[1] != c or weight.numel() != weight.shape[0] * c or weight.shape[0] < 1:
+        raise ValueError(f"weight must be [classes, {c}] (or [classes, {c}, 1, 1, 1]); got {tuple(weight.shape)}")
+    k = weight.shape[0]
+    if bias is not None and bias.shape != (k,):
+        raise ValueError(f"bias must be [{k}]; got {tuple(bias.shape)}")
+    if class_weights is not None and class_weights.shape != (k,):
+        raise ValueError(f"class_weights must be [{k}]; got {tuple(class_weights.shape)}")
+    if labels.dtype not in _LABEL_KIND:
+        raise TypeError(f"labels must be int16, int32 or int64; got {labels.dtype}")
+    for name, t in (("weight", weight), ("bias", bias), ("labels", labels), ("class_weights", class_weights)):
+        if t is not None and t.device != features.device:
+            raise ValueError(f"{name} is on {t.device}, the features are on {features.device}")
+    if ignore_label is not None and not -2 ** 63 <= ignore_label < 2 ** 63:
+        raise ValueError(f"ignore_label {ignore_label} is no 64-bit number")
+    weight = weight.reshape(k, c)
+    if not use_cuda_kernels(features):
+        return _formula(features, weight, bias, labels, class_weights, ignore_label, spatial)
+    if not head_supported(c):
+        raise ValueError(f"the kernels read features of 8 to {MAX_WIDTH} channels in multiples of 8; got {c}")
+    if weight.dtype not in _KIND or (bias is not None and bias.dtype not in _KIND):
+        raise TypeError("weight and bias must be bf16 or fp32")
+    if features.numel() // c > 2 ** 31 - 256:
+        raise ValueError(f"{features.numel() // c} voxels are more than the kernels count")
+    x = features.to(torch.bfloat16).reshape(-1, c)
+    if not x.is_contiguous() or x.data_ptr() % 16:  # a tensor map starts on 16 bytes
+        x = x.clone(memory_format=torch.contiguous_format)
+    weight = weight.contiguous()
+    if weight.dtype == torch.bfloat16 and weight.data_ptr() % 16:
+        weight = weight.clone()
+    if class_weights is not None:
+        class_weights = class_weights.detach().float().contiguous()
+    if x.shape[0] == 0:  # a shard without voxels: its terms are zero, the other shards' sums are not
+        return _formula(x.float(), weight.float(), None if bias is None else bias.float(), labels.reshape(-1),
+                        class_weights, ignore_label, spatial)
+    with torch.cuda.device(features.device):
+        return _HeadLossFn.apply(x, weight, None if bias is None else bias.contiguous(), labels.reshape(-1).contiguous(),
+                                 class_weights, ignore_label, spatial)
+
+
+def _formula(features, weight, bias, labels, class_weights, ignore_label, spatial):
+    """The definition: the CPU path, and the oracle of the GPU tests in 64 bits."""
+    from .loss import spatial_all_reduce
+    k = weight.shape[0]
+    y = labels.reshape(-1).long()
+    live = (y >= 0) & (y < k)
+    if ignore_label is not None:
+        live &= y != ignore_label
+    x, y = features.reshape(-1, features.shape[-1])[live], y[live]
+    kind = torch.promote_types(torch.promote_types(x.dtype, weight.dtype), torch.float32)
+    logits = x.to(kind) @ weight.to(kind).T
+    if bias is not None:
+        logits = logits + bias.to(kind)
+    u = torch.ones(len(y), dtype=kind, device=y.device) if class_weights is None else class_weights.to(kind)[y]
+    nll = torch.logsumexp(logits, 1) - logits.gather(1, y[:, None])[:, 0]
+    total = spatial_all_reduce(torch.stack([(u * nll).sum(), u.sum()]), spatial)
+    return total[0] / total[1].detach().clamp_min(torch.finfo(torch.float32).eps)
