@@ -19,12 +19,9 @@
 // take one half of its columns each. Column parameters (bias; log-sum-exp, weight and label of a voxel) travel with
 // their tile as bulk copies. All waits are bounded.
 #include "common.cuh"
-#include "host_api.h"
+#include "head_loss.cuh"
 
 namespace sb {
-
-int make_map_bf16(CUtensorMap* m, const void* base, int rank, const long long* dims, const long long* strides,
-                  const int* box, int rowb);
 
 constexpr int HD_THREADS = 320;
 constexpr int HD_EPI_WARPS = 8;
@@ -32,9 +29,6 @@ constexpr int HD_TILE = 128;
 constexpr int HD_BOX = HD_TILE * 128;  // bytes of a 128-row box of 64 channels
 constexpr int HD_MAX_STAGES = 4;
 constexpr int HD_MAX_C = 256;          // TMEM: two or three tiles of s and the accumulator in 512 columns
-constexpr float HD_LOG2E = 1.4426950408889634f;
-constexpr float HD_LN2 = 0.6931471805599453f;
-
 enum HeadMode { HEAD_FWD = 0, HEAD_DX = 1, HEAD_DW = 2 };
 
 struct HeadParams {
@@ -57,11 +51,6 @@ struct HeadParams {
   int stages, rbufs, bufs;
 };
 
-__device__ __forceinline__ float hd_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // D[tmem] (+)= A[tmem] * B[smem]: A holds two bf16 of K per 32-bit column, one row per lane
 __device__ __forceinline__ void hd_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
                                           uint32_t accumulate) {
@@ -82,31 +71,11 @@ __device__ __forceinline__ void hd_tmem_st_x16(uint32_t taddr, const uint32_t* v
       : "memory");
 }
 __device__ __forceinline__ void hd_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void hd_tma_2d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
-      : "memory");
-}
 __device__ __forceinline__ void hd_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-// barrier of the 256 threads of the epilogue warps; the same answer in all of them: whether every one said `ok`
-__device__ __forceinline__ bool hd_epi_vote(bool ok) {
-  uint32_t all;
-  asm volatile(
-      "{\n\t.reg .pred a, q;\n\t"
-      "setp.ne.u32 a, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 256, a;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(all)
-      : "r"(ok ? 1u : 0u)
-      : "memory");
-  return all != 0;
-}
-
 template <int MODE>
 __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_constant__ HeadParams p) {
   constexpr int MAXB = 4;
@@ -162,13 +131,13 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         const int rt = job % p.row_tiles, sp = job / p.row_tiles;
         const int t0 = sp * p.tiles_per_split;
         const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
-        if (!mbar_wait(&r_empty[rb], rph ^ 1u, abort_flag, p.status, 71)) break;
+        if (!mbar_wait(&r_empty[rb], rph ^ 1u, abort_flag, p.status, 91)) break;
         mbar_expect_tx(&r_full[rb], tile_bytes);
         for (int k = 0; k < p.kboxes; ++k)
           hd_tma_2d(smem_r + rb * tile_bytes + k * HD_BOX, &p.mapR, &r_full[rb], k * 64, rt * HD_TILE);
         if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
         for (int t = t0; t < t1; ++t) {
-          if (!mbar_wait(&q_empty[st], ph ^ 1u, abort_flag, p.status, 71)) { ok = false; break; }
+          if (!mbar_wait(&q_empty[st], ph ^ 1u, abort_flag, p.status, 91)) { ok = false; break; }
           mbar_expect_tx(&q_full[st], tile_bytes + NPAR * HD_TILE * 4);
           for (int k = 0; k < p.kboxes; ++k)
             hd_tma_2d(smem_q + st * tile_bytes + k * HD_BOX, &p.mapQ, &q_full[st], k * 64, t * HD_TILE);
@@ -196,10 +165,10 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
     bool ok = true;
     auto second = [&]() -> bool {
       if (prev_first) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty, aph ^ 1u, abort_flag, p.status, 72))) return false;
+        if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty, aph ^ 1u, abort_flag, p.status, 92))) return false;
         aph ^= 1u;
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_done[prev_b], prev_bph, abort_flag, p.status, 73))) return false;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_done[prev_b], prev_bph, abort_flag, p.status, 93))) return false;
       tc_fence_after();
       if (leader) {
         const uint32_t lo = desc_lo(q0 + prev_st * tile_bytes, lbo);
@@ -218,12 +187,12 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       const int sp = job / p.row_tiles;
       const int t0 = sp * p.tiles_per_split;
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
-      if (!__all_sync(0xffffffffu, mbar_wait(&r_full[rb], rph, abort_flag, p.status, 74))) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, mbar_wait(&r_full[rb], rph, abort_flag, p.status, 94))) { ok = false; break; }
       for (int t = t0; t < t1; ++t) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 75))) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95))) { ok = false; break; }
         // the buffer is free: read by the epilogue (FWD), or its P read by the second MMA that used it
         uint64_t* bar = MODE == HEAD_FWD ? &s_done[b] : &s_free[b];
-        if (!__all_sync(0xffffffffu, mbar_wait(bar, bph ^ 1u, abort_flag, p.status, 76))) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait(bar, bph ^ 1u, abort_flag, p.status, 96))) { ok = false; break; }
         tc_fence_after();
         const int nc = cols_of(t);
         if (leader) {
@@ -261,7 +230,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
     float pend_g = 0.f, pend_db = 0.f;
     // the accumulator of a finished job
     auto drain = [&]() -> bool {
-      if (!mbar_wait(&acc_full, aph, abort_flag, p.status, 77)) return false;
+      if (!mbar_wait(&acc_full, aph, abort_flag, p.status, 97)) return false;
       aph ^= 1u;
       tc_fence_after();
       const long long r = (long long)pend_rt * HD_TILE + row;
@@ -310,8 +279,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       if (MODE == HEAD_DX) g = p.rowg[r];
       float m = -INFINITY, s = 0.f, tl = 0.f;
       for (int t = t0; t < t1; ++t) {
-        if (!mbar_wait(&q_full[st], ph, abort_flag, p.status, 78) ||
-            !mbar_wait(&s_full[b], bph, abort_flag, p.status, 78)) { ok = false; break; }
+        if (!mbar_wait(&q_full[st], ph, abort_flag, p.status, 98) ||
+            !mbar_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
         tc_fence_after();
         const float* par = smem_p + st * NPAR * HD_TILE + half * 64;
         const int nc = cols_of(t) - half * 64;  // this group's columns: none, 32 or (64 and more) 64
@@ -552,10 +521,6 @@ __global__ void __launch_bounds__(256) head_weights_kernel(const float* __restri
   }
 }
 
-template <typename T> __device__ __forceinline__ T hd_cast(float v);
-template <> __device__ __forceinline__ float hd_cast<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 hd_cast<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
-
 // out[r][c] = sum over the slices of ws[slice][rows_pad][ld], in slice order; r < rows, c < C
 template <typename T>
 __global__ void __launch_bounds__(256) head_reduce_kernel(const float* __restrict__ ws, int slices, long long rows,
@@ -588,9 +553,7 @@ static void head_split(int row_tiles, int col_tiles, int* splits, int* tps) {
   }
 }
 
-static int head_geometry(const SbHeadArgs* a, int mode, HeadParams& p) {
-  if (a->V < 1 || a->V > (1LL << 31) - 256 || a->K < 1 || a->K > (1 << 30) || a->C < 8 || a->C % 8 || a->C > HD_MAX_C)
-    return SB_ERR_SHAPE;
+static void head_geometry(const SbHeadArgs* a, int mode, HeadParams& p) {
   memset(&p, 0, sizeof(p));
   p.C = a->C;
   p.cpad = (a->C + 15) / 16 * 16;
@@ -600,7 +563,7 @@ static int head_geometry(const SbHeadArgs* a, int mode, HeadParams& p) {
   p.cols = mode == HEAD_DW ? a->V : a->K;
   p.row_tiles = (int)((p.rows + HD_TILE - 1) / HD_TILE);
   p.col_tiles = (int)((p.cols + HD_TILE - 1) / HD_TILE);
-  p.rows_pad = (long long)p.row_tiles * HD_TILE;
+  p.rows_pad = (p.rows + HD_PAD - 1) / HD_PAD * HD_PAD;
   head_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
   p.bufs = mode == HEAD_FWD ? 4 : p.cpad <= 128 ? 3 : 2;
   // shared memory: 12 boxes of 16 KB (kboxes per tile); one or two resident tiles and two to four in the ring
@@ -608,7 +571,6 @@ static int head_geometry(const SbHeadArgs* a, int mode, HeadParams& p) {
   p.stages = 12 / p.kboxes - p.rbufs;
   if (p.stages > HD_MAX_STAGES) p.stages = HD_MAX_STAGES;
   p.status = a->status;
-  return 0;
 }
 
 template <int MODE>
@@ -635,43 +597,56 @@ static int head_launch(const SbHeadArgs* a, HeadParams& p, cudaStream_t stream) 
 
 using namespace sb;
 
-static long long pad128(long long n) { return (n + 127) / 128 * 128; }
+static long long pad(long long n) { return (n + HD_PAD - 1) / HD_PAD * HD_PAD; }
+static bool shape_ok(const SbHeadArgs* a) {
+  return a->V >= 1 && a->V <= (1LL << 31) - 512 && a->K >= 1 && a->K <= (1 << 30) && a->C >= 8 && a->C % 8 == 0 &&
+         a->C <= 32768;
+}
+static bool wide(const SbHeadArgs* a) { return a->C > HD_MAX_C; }
+constexpr int HD_SUM_BLOCKS = 148 * 4;
 
-extern "C" int sb_head_max_width(void) { return HD_MAX_C; }
-
-// fp32 scratch of the forward pass (mode 0), the gradient of x (1) or of w and b (2); -1: outside the kernels' range
+// fp32 scratch of the forward (mode 0) and the backward pass (1); -1: outside the kernels' range
 extern "C" long long sb_head_scratch(const SbHeadArgs* a, int mode) {
+  if (mode < 0 || mode > 1 || !shape_ok(a)) return -1;
   HeadParams p;
-  if (mode < 0 || mode > 2 || head_geometry(a, mode, p)) return -1;
-  if (mode == HEAD_FWD) return 2 * (long long)p.splits * p.rows_pad + p.rows_pad + 4 * 148 * 4;
-  if (mode == HEAD_DX && p.splits == 1) return 0;
-  return (long long)p.splits * p.rows_pad * p.cpad + (mode == HEAD_DW ? 2LL * p.splits * p.rows_pad : 0);
+  if (mode == 0) {
+    head_geometry(a, HEAD_FWD, p);
+    const int splits = wide(a) ? head_wide_splits(a->V, a->K) : p.splits;
+    return 4LL * HD_SUM_BLOCKS + (2LL * splits + 1) * p.rows_pad;
+  }
+  if (wide(a)) return head_wide_scratch(a);
+  head_geometry(a, HEAD_DX, p);
+  const long long dx = p.splits == 1 ? 0 : p.splits * p.rows_pad * p.cpad;
+  head_geometry(a, HEAD_DW, p);
+  const long long dw = p.splits * p.rows_pad * (p.cpad + 2);
+  return dx > dw ? dx : dw;
 }
 
 // labels, bias -> y, bias2, lse2, total, loss, den
 extern "C" int sb_head_forward(const SbHeadArgs* a, cudaStream_t stream) {
-  HeadParams p;
-  int rc = head_geometry(a, HEAD_FWD, p);
-  if (rc) return rc;
-  if (!a->x || !a->w || !a->labels || !a->y || !a->bias2 || !a->lse2 || !a->total || !a->loss || !a->den || !a->scratch)
+  if (!shape_ok(a) || !a->x || !a->w || !a->labels || !a->y || !a->bias2 || !a->lse2 || !a->total || !a->loss ||
+      !a->den || !a->scratch)
     return SB_ERR_SHAPE;
-  if (a->scratch_floats < sb_head_scratch(a, HEAD_FWD)) return SB_ERR_TOO_LARGE;
-  const long long v_pad = pad128(a->V);
-  const int k_pad = (int)pad128(a->K);
+  if (a->scratch_floats < sb_head_scratch(a, 0)) return SB_ERR_TOO_LARGE;
+  HeadParams p;
+  head_geometry(a, HEAD_FWD, p);
+  const long long v_pad = pad(a->V);
+  const int k_pad = (int)pad(a->K);
   head_prep_kernel<<<hd_blocks(v_pad > k_pad ? v_pad : k_pad, 8), 256, 0, stream>>>(
       a->labels, a->label_kind, a->V, v_pad, a->K, k_pad, a->has_ignore, a->ignore, a->y, a->bias, a->bias_kind, a->bias2,
       a->status);
   sb_count_launch(1);
   // scratch: block sums (double), running maxima and sums, t at the labels
   double* sums = (double*)a->scratch;
-  p.part = (float2*)(a->scratch + 4 * 148 * 4);
-  p.tl = (float*)(p.part + (long long)p.splits * p.rows_pad);
+  const int splits = wide(a) ? head_wide_splits(a->V, a->K) : p.splits;
+  p.part = (float2*)(a->scratch + 4LL * HD_SUM_BLOCKS);
+  p.tl = (float*)(p.part + splits * p.rows_pad);
   p.colp = a->bias2;
   p.rowy = a->y;
-  rc = head_launch<HEAD_FWD>(a, p, stream);
+  const int rc = wide(a) ? head_wide_forward(a, p.part, p.tl, splits, stream) : head_launch<HEAD_FWD>(a, p, stream);
   if (rc) return rc;
   const int blocks = hd_blocks(v_pad, 4);
-  head_merge_kernel<<<blocks, 256, 0, stream>>>(p.part, p.tl, a->y, a->cw, p.splits, a->V, v_pad, a->lse2, sums);
+  head_merge_kernel<<<blocks, 256, 0, stream>>>(p.part, p.tl, a->y, a->cw, splits, a->V, v_pad, a->lse2, sums);
   sb_count_launch(1);
   return sb_head_total(sums, blocks, a->total, a->loss, a->den, stream);
 }
@@ -683,14 +658,6 @@ extern "C" int sb_head_total(const double* sums, int blocks, double* total, floa
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
-extern "C" int sb_head_weights(const SbHeadArgs* a, const float* gout, cudaStream_t stream) {
-  if (!a->lse2 || !a->y || !a->den || !a->g || !a->lse2g || !gout || a->V < 1) return SB_ERR_SHAPE;
-  const long long v_pad = pad128(a->V);
-  head_weights_kernel<<<hd_blocks(v_pad, 8), 256, 0, stream>>>(a->lse2, a->y, a->cw, gout, a->den, v_pad, a->g, a->lse2g);
-  sb_count_launch(1);
-  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
-}
-
 template <typename T>
 static void head_reduce(const float* ws, int slices, long long rows, long long rows_pad, int C, int ld, void* out,
                         cudaStream_t stream) {
@@ -698,45 +665,49 @@ static void head_reduce(const float* ws, int slices, long long rows, long long r
   sb_count_launch(1);
 }
 
-extern "C" int sb_head_dx(const SbHeadArgs* a, cudaStream_t stream) {
+// dx, dw and db (each optional) from gout and what the forward pass left; dw / db in fp32 when dw_kind / bias_kind is 2
+extern "C" int sb_head_backward(const SbHeadArgs* a, const float* gout, cudaStream_t stream) {
+  if (!shape_ok(a) || !a->x || !a->w || !a->y || !a->bias2 || !a->lse2 || !a->den || !a->g || !a->lse2g || !gout)
+    return SB_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(a->dx) | reinterpret_cast<uintptr_t>(a->dw) | reinterpret_cast<uintptr_t>(a->scratch)) & 15)
+    return SB_ERR_ALIGN;
+  if (a->scratch_floats < sb_head_scratch(a, 1)) return SB_ERR_TOO_LARGE;
+  const long long v_pad = pad(a->V);
+  head_weights_kernel<<<hd_blocks(v_pad, 8), 256, 0, stream>>>(a->lse2, a->y, a->cw, gout, a->den, v_pad, a->g, a->lse2g);
+  sb_count_launch(1);
+  if (wide(a)) return head_wide_backward(a, stream);
   HeadParams p;
-  int rc = head_geometry(a, HEAD_DX, p);
-  if (rc) return rc;
-  if (!a->x || !a->w || !a->y || !a->bias2 || !a->lse2 || !a->g || !a->dx) return SB_ERR_SHAPE;
-  if (reinterpret_cast<uintptr_t>(a->dx) & 15) return SB_ERR_ALIGN;
-  if (a->scratch_floats < sb_head_scratch(a, HEAD_DX)) return SB_ERR_TOO_LARGE;
-  p.colp = a->bias2;
-  p.rowp = a->lse2;
-  p.rowg = a->g;
-  p.rowy = a->y;
-  p.out = (__nv_bfloat16*)a->dx;
-  p.ws = a->scratch;
-  rc = head_launch<HEAD_DX>(a, p, stream);
-  if (rc || p.splits == 1) return rc;
-  head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a->dx, stream);
-  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
-}
-
-// dw (and db, optional): fp32 when w_kind / b_kind is 2, else bf16
-extern "C" int sb_head_dw(const SbHeadArgs* a, cudaStream_t stream) {
-  HeadParams p;
-  int rc = head_geometry(a, HEAD_DW, p);
-  if (rc) return rc;
-  if (!a->x || !a->w || !a->y || !a->bias2 || !a->lse2g || !a->g || !a->dw || !a->scratch) return SB_ERR_SHAPE;
-  if (a->scratch_floats < sb_head_scratch(a, HEAD_DW)) return SB_ERR_TOO_LARGE;
-  p.colp = a->lse2g;
-  p.colg = a->g;
-  p.coly = a->y;
-  p.rowp = a->bias2;
-  p.ws = a->scratch;
-  p.ws_b = a->scratch + (long long)p.splits * p.rows_pad * p.cpad;
-  rc = head_launch<HEAD_DW>(a, p, stream);
-  if (rc) return rc;
-  if (a->dw_kind == 2) head_reduce<float>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a->dw, stream);
-  else head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a->dw, stream);
-  if (a->db != nullptr) {
-    if (a->bias_kind == 2) head_reduce<float>(p.ws_b, 2 * p.splits, p.rows, p.rows_pad, 1, 1, a->db, stream);
-    else head_reduce<__nv_bfloat16>(p.ws_b, 2 * p.splits, p.rows, p.rows_pad, 1, 1, a->db, stream);
+  int rc = 0;
+  if (a->dx != nullptr) {
+    head_geometry(a, HEAD_DX, p);
+    p.colp = a->bias2;
+    p.rowp = a->lse2;
+    p.rowg = a->g;
+    p.rowy = a->y;
+    p.out = (__nv_bfloat16*)a->dx;
+    p.ws = a->scratch;
+    rc = head_launch<HEAD_DX>(a, p, stream);
+    if (rc) return rc;
+    if (p.splits > 1) head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a->dx, stream);
+  }
+  if (a->dw != nullptr || a->db != nullptr) {
+    head_geometry(a, HEAD_DW, p);
+    p.colp = a->lse2g;
+    p.colg = a->g;
+    p.coly = a->y;
+    p.rowp = a->bias2;
+    p.ws = a->scratch;
+    p.ws_b = a->scratch + p.splits * p.rows_pad * p.cpad;
+    rc = head_launch<HEAD_DW>(a, p, stream);
+    if (rc) return rc;
+    if (a->dw != nullptr) {
+      if (a->dw_kind == 2) head_reduce<float>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a->dw, stream);
+      else head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a->dw, stream);
+    }
+    if (a->db != nullptr) {
+      if (a->bias_kind == 2) head_reduce<float>(p.ws_b, 2 * p.splits, p.rows, p.rows_pad, 1, 1, a->db, stream);
+      else head_reduce<__nv_bfloat16>(p.ws_b, 2 * p.splits, p.rows, p.rows_pad, 1, 1, a->db, stream);
+    }
   }
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }

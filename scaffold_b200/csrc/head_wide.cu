@@ -1,0 +1,595 @@
+// Cross entropy of a head over features of more than 256 channels (head_loss.cuh): a tile of logits costs more on the
+// tensor cores than its exponentials, so the passes are matrix products with something fused into their epilogue, on SM
+// pairs (tcgen05 cta_group::2): a pair multiplies 256 rows by 256 columns, each CTA loads its own 128 rows and one half
+// of the columns (64 bytes a clock and SM out of L2, half of what one CTA alone would read).
+//   WIDE_LSE  rows = voxels, columns = classes: running maximum and sum of every row over the class tiles of a job
+//   WIDE_D    rows = classes, columns = voxels: D^T = g (p - [j = y]) in bf16, a piece of the classes by a piece of the
+//             voxels at a time (HW_PIECE elements: 64 MB, which stays in L2 until both products below have read it); db
+//   WIDE_OUT  dX = D W and dW = D^T X of the piece. D^T is read K-major for dW and MN-major for dX, W and X MN-major:
+//             nothing is transposed in memory. Long reductions are cut into slices that are added in order.
+// One thread holds a row of a tile, so a row's maximum, sum and db need no exchange.
+#include "head_loss.cuh"
+#include "pair.cuh"
+
+namespace sb {
+
+constexpr int HW_THREADS = 320;
+constexpr int HW_STAGES = 6;
+constexpr int HW_STAGE = 32768;  // 64 of K for 128 rows of A and 128 columns of B
+constexpr long long HW_PIECE = 32LL << 20;
+
+enum WideEpi { WIDE_LSE = 0, WIDE_D = 1, WIDE_OUT = 2 };
+
+struct WideParams {
+  CUtensorMap mapA, mapB;
+  int row_tiles, col_tiles;     // of 256
+  int splits, tiles_per_split;  // LSE / D: of the column tiles
+  int kc, kslices, kc_per_slice;
+  int cols;                     // real columns, for the last tile's width
+  long long rows_pad;
+  const int* y;                 // LSE: label of a row; D: of a column
+  const float* colp;            // LSE: bias2; D: lse2g
+  const float* colg;            // D: g
+  const float* rowp;            // D: bias2
+  int row0;                     // D: class of row 0
+  float2* part;
+  float* tl;
+  __nv_bfloat16* dl;            // D: [rows][ldd]
+  long long ldd;
+  float* ws_b;                  // D: [2 splits][rows_pad]
+  // OUT: [rows][C]; add: acc is added to the product; the sum goes to out16 / out32, or back to acc
+  long long rows;
+  float* acc;
+  int add;
+  __nv_bfloat16* out16;
+  float* out32;
+  float* slices;                // [kslices][rows][C] when kslices > 1
+  uint32_t* status;
+};
+
+// rows x C sums: v = (add ? acc : 0) + product, then to an output or back to acc; eight columns
+__device__ __forceinline__ void hw_sink(float* acc, int add, __nv_bfloat16* out16, float* out32, long long at,
+                                        float (&f)[8]) {
+  if (add) {
+    const float4 a = *reinterpret_cast<const float4*>(acc + at), b = *reinterpret_cast<const float4*>(acc + at + 4);
+    f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
+    f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+  }
+  if (out16 != nullptr) {
+    *reinterpret_cast<uint4*>(out16 + at) =
+        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+    return;
+  }
+  float* dst = out32 != nullptr ? out32 : acc;
+  *reinterpret_cast<float4*>(dst + at) = make_float4(f[0], f[1], f[2], f[3]);
+  *reinterpret_cast<float4*>(dst + at + 4) = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+template <int EPI, int A_MN, int B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
+    head_wide_kernel(const __grid_constant__ WideParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[HW_STAGES], empty[HW_STAGES], tfull[2], tempty[2];
+  __shared__ float s_m[128], s_s[128], s_t[128];
+  __shared__ uint32_t tmem_base_s, abort_s;
+  volatile uint32_t* abort_flag = &abort_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  // LSE and D: a job is a row tile and a run of column tiles; OUT: a row tile, a column tile and a slice of K
+  const int jobs = EPI == WIDE_OUT ? p.row_tiles * p.col_tiles * p.kslices : p.row_tiles * p.splits;
+
+  if (threadIdx.x == 0) {
+    abort_s = 0;
+    for (int i = 0; i < HW_STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], 16); }  // 8 epilogue warps, both CTAs
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem2_alloc(&tmem_base_s, 512);
+    tmem2_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers exist before any copy or arrive targets them
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+
+  struct Job {
+    int rt, t0, t1, k0, k1, sp;
+  };
+  auto job_at = [&](int job) {
+    Job j;
+    if (EPI == WIDE_OUT) {
+      j.rt = job % p.row_tiles;
+      const int t = job / p.row_tiles;
+      j.t0 = t % p.col_tiles;
+      j.t1 = j.t0 + 1;
+      j.sp = t / p.col_tiles;
+      j.k0 = j.sp * p.kc_per_slice;
+      j.k1 = j.k0 + p.kc_per_slice < p.kc ? j.k0 + p.kc_per_slice : p.kc;
+    } else {
+      j.rt = job % p.row_tiles;
+      j.sp = job / p.row_tiles;
+      j.t0 = j.sp * p.tiles_per_split;
+      j.t1 = j.t0 + p.tiles_per_split < p.col_tiles ? j.t0 + p.tiles_per_split : p.col_tiles;
+      j.k0 = 0;
+      j.k1 = p.kc;
+    }
+    return j;
+  };
+  auto cols_of = [&](int t) -> int {  // columns of tile t, up to a multiple of 32
+    const int left = p.cols - t * 256;
+    return left >= 256 ? 256 : (left + 31) / 32 * 32;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&p.mapA);
+      tma_prefetch_desc(&p.mapB);
+      uint32_t st = 0, ph = 0;
+      bool ok = true;
+      for (int job = pair; job < jobs && ok; job += npairs) {
+        const Job j = job_at(job);
+        const int row = j.rt * 256 + (int)rank * 128;
+        for (int t = j.t0; t < j.t1 && ok; ++t) {
+          const int nc = cols_of(t), col = t * 256 + (int)rank * (nc / 2);
+          const int nb = B_MN ? (nc / 2 + 63) / 64 : 0;
+          for (int k = j.k0; k < j.k1; ++k) {
+            if (!mbar_wait_cl(&empty[st], ph ^ 1u, abort_flag, p.status, 101)) { ok = false; break; }
+            const uint32_t bar = map_to_rank(smem_u32(&full[st]), 0);
+            if (rank == 0) mbar_expect_tx(&full[st], 2u * (16384u + (B_MN ? nb * 8192u : 16384u)));  // both CTAs' bytes
+            uint8_t* sa = smem + st * HW_STAGE;
+            uint8_t* sb = sa + 16384;
+            if (A_MN) {
+              for (int i = 0; i < 2; ++i) tma2_load_2d(sa + i * 8192, &p.mapA, bar, row + i * 64, k * 64);
+            } else {
+              tma2_load_2d(sa, &p.mapA, bar, k * 64, row);
+            }
+            if (B_MN) {
+              for (int i = 0; i < nb; ++i) tma2_load_2d(sb + i * 8192, &p.mapB, bar, col + i * 64, k * 64);
+            } else {
+              tma2_load_2d(sb, &p.mapB, bar, k * 64, col);
+            }
+            if (++st == HW_STAGES) { st = 0; ph ^= 1u; }
+          }
+        }
+      }
+      // every release of a stage that this CTA filled has arrived before the CTA may leave
+      for (int i = 0; i < HW_STAGES && ok; ++i) {
+        if (!mbar_wait_cl(&empty[st], ph ^ 1u, abort_flag, p.status, 102)) ok = false;
+        if (++st == HW_STAGES) { st = 0; ph ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool leader = elect_one();
+      const uint32_t hi = desc_hi(8u * 128u, 2u);
+      const uint32_t s0 = smem_u32(smem);
+      constexpr uint32_t A_STEP = A_MN ? 128u : 2u, B_STEP = B_MN ? 128u : 2u;  // 16 of K, in 16-byte units
+      uint32_t st = 0, ph = 0, b = 0, bph = 0;
+      bool ok = true;
+      for (int job = pair; job < jobs && ok; job += npairs) {
+        const Job j = job_at(job);
+        for (int t = j.t0; t < j.t1 && ok; ++t) {
+          if (!__all_sync(0xffffffffu, mbar_wait_cl(&tempty[b], bph ^ 1u, abort_flag, p.status, 103))) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t idesc = make_idesc_bf16(256, cols_of(t), A_MN, B_MN);
+          for (int k = j.k0; k < j.k1; ++k) {
+            if (!__all_sync(0xffffffffu, mbar_wait_cl(&full[st], ph, abort_flag, p.status, 104))) { ok = false; break; }
+            tc_fence_after();
+            if (leader) {
+              const uint32_t a_lo = desc_lo(s0 + st * HW_STAGE, A_MN ? 8192u : 16u);
+              const uint32_t b_lo = desc_lo(s0 + st * HW_STAGE + 16384u, B_MN ? 8192u : 16u);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                tc2_mma_bf16_pred(tmem + b * 256u, a_lo + i * A_STEP, hi, b_lo + i * B_STEP, hi, idesc,
+                                  k != j.k0 || i != 0 ? 1u : 0u);
+              tc2_commit_both(&empty[st]);
+            }
+            __syncwarp();
+            if (++st == HW_STAGES) { st = 0; ph ^= 1u; }
+          }
+          if (ok && leader) tc2_commit_both(&tfull[b]);
+          __syncwarp();
+          b ^= 1u;
+          if (b == 0) bph ^= 1u;
+        }
+      }
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16) + half * 128;
+    const uint32_t release[2] = {map_to_rank(smem_u32(&tempty[0]), 0), map_to_rank(smem_u32(&tempty[1]), 0)};
+    uint32_t b = 0, bph = 0;
+    bool ok = true;
+    for (int job = pair; job < jobs && ok; job += npairs) {
+      const Job j = job_at(job);
+      const long long r = (long long)j.rt * 256 + rank * 128 + row;
+      const int y = EPI == WIDE_LSE ? p.y[r] : 0;
+      const float rp = EPI == WIDE_D ? p.rowp[r] : 0.f;
+      float m = -INFINITY, s = 0.f, tl = 0.f, db = 0.f;
+      for (int t = j.t0; t < j.t1; ++t) {
+        if (!mbar_wait_cl(&tfull[b], bph, abort_flag, p.status, 105)) { ok = false; break; }
+        tc_fence_after();
+        const int nc = cols_of(t) - half * 128, c_abs = t * 256 + half * 128;
+        for (int c0 = 0; c0 < 128 && c0 < nc; c0 += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32(lane_base + b * 256 + c0, v);
+          tmem_ld_wait();
+          float f[32];
+          if (EPI != WIDE_OUT) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 cp = __ldg(reinterpret_cast<const float4*>(p.colp + c_abs + c0 + i));
+              const float cv[4] = {cp.x, cp.y, cp.z, cp.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                f[i + e] = fmaf(__uint_as_float(v[i + e]), HD_LOG2E, EPI == WIDE_LSE ? cv[e] : rp - cv[e]);
+            }
+          }
+          if (EPI == WIDE_LSE) {
+            const int at = y - (c_abs + c0);
+            if ((unsigned)at < 32u) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) tl = i == at ? f[i] : tl;
+            }
+            float mx = f[0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) mx = fmaxf(mx, f[i]);
+            if (mx > m) {
+              s *= hd_ex2(m - mx);
+              m = mx;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+            float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              a0 += hd_ex2(f[i] - base);
+              a1 += hd_ex2(f[i + 1] - base);
+              a2 += hd_ex2(f[i + 2] - base);
+              a3 += hd_ex2(f[i + 3] - base);
+            }
+            s += (a0 + a1) + (a2 + a3);
+          } else if (EPI == WIDE_D) {
+            float d0 = 0.f, d1 = 0.f, d2 = 0.f, d3 = 0.f;
+            const int cls = p.row0 + (int)r;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 cg = __ldg(reinterpret_cast<const float4*>(p.colg + c_abs + c0 + i));
+              const int4 cy = __ldg(reinterpret_cast<const int4*>(p.y + c_abs + c0 + i));
+              f[i] = hd_ex2(f[i]) - (cy.x == cls ? cg.x : 0.f);
+              f[i + 1] = hd_ex2(f[i + 1]) - (cy.y == cls ? cg.y : 0.f);
+              f[i + 2] = hd_ex2(f[i + 2]) - (cy.z == cls ? cg.z : 0.f);
+              f[i + 3] = hd_ex2(f[i + 3]) - (cy.w == cls ? cg.w : 0.f);
+              d0 += f[i]; d1 += f[i + 1]; d2 += f[i + 2]; d3 += f[i + 3];
+            }
+            db += (d0 + d1) + (d2 + d3);
+            uint4* dst = reinterpret_cast<uint4*>(p.dl + r * p.ldd + c_abs + c0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float* e = f + 16 * i;
+              st_global_v8(dst + 2 * i,
+                           make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
+                                      pack_bf16x2(e[6], e[7])),
+                           make_uint4(pack_bf16x2(e[8], e[9]), pack_bf16x2(e[10], e[11]), pack_bf16x2(e[12], e[13]),
+                                      pack_bf16x2(e[14], e[15])));
+            }
+          } else if (r < p.rows) {
+            float* acc = p.kslices > 1 ? p.slices + (long long)j.sp * p.rows * p.cols : p.acc;
+            const bool whole = p.kslices == 1;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int col = c_abs + c0 + g * 8;
+              if (col < p.cols) {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = __uint_as_float(v[g * 8 + i]);
+                hw_sink(acc, whole ? p.add : 0, whole ? p.out16 : nullptr, whole ? p.out32 : nullptr, r * p.cols + col, e);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(release[b]);
+        b ^= 1u;
+        if (b == 0) bph ^= 1u;
+      }
+      if (EPI == WIDE_LSE) {
+        if (half == 1) { s_m[row] = m; s_s[row] = s; s_t[row] = tl; }
+        ok = hd_epi_vote(ok);
+        if (half == 0 && ok) {
+          const float m1 = s_m[row], mm = fmaxf(m, m1);
+          const float base = mm == -INFINITY ? 0.f : mm;
+          p.part[(long long)j.sp * p.rows_pad + r] = make_float2(mm, s * hd_ex2(m - base) + s_s[row] * hd_ex2(m1 - base));
+          if (y >= j.t0 * 256 && y < j.t1 * 256) p.tl[r] = (y & 255) < 128 ? tl : s_t[row];
+        }
+        hd_epi_vote(true);  // the merge has read what the next job's will overwrite
+      }
+      if (EPI == WIDE_D && ok) p.ws_b[((long long)j.sp * 2 + half) * p.rows_pad + r] = db;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) __nanosleep(1000);
+    __syncthreads();
+  }
+  cluster_sync_all();  // the leader's MMAs read the peer's shared memory; arrives target the other CTA
+  if (warp == 0) {
+    __syncwarp();
+    tc_fence_after();
+    tmem2_dealloc(tmem, 512);
+  }
+}
+
+// [rows][C] = (add ? acc : 0) + the slices in order, to an output or back to acc (C a multiple of 8)
+__global__ void __launch_bounds__(256) head_slices_kernel(const float* __restrict__ slices, int n, long long elems,
+                                                          float* acc, int add, __nv_bfloat16* out16, float* out32) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < elems / 8; i += (long long)gridDim.x * 256) {
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < n; ++k) {
+      const float* src = slices + (long long)k * elems + i * 8;
+      const float4 a = __ldcs(reinterpret_cast<const float4*>(src)), b = __ldcs(reinterpret_cast<const float4*>(src + 4));
+      f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
+      f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+    }
+    hw_sink(acc, add, out16, out32, i * 8, f);
+  }
+}
+// the same for the bias's sums: slices [n][ld], rows of them
+__global__ void __launch_bounds__(256) head_slices_b_kernel(const float* __restrict__ slices, int n, long long ld,
+                                                            int rows, float* acc, int add, __nv_bfloat16* out16,
+                                                            float* out32) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows) return;
+  float f = 0.f;
+  for (int k = 0; k < n; ++k) f += slices[(long long)k * ld + i];
+  if (add) f += acc[i];
+  if (out16 != nullptr) out16[i] = __float2bfloat16(f);
+  else (out32 != nullptr ? out32 : acc)[i] = f;
+}
+
+static int g_hw_pairs = 0;
+template <int EPI, int A_MN, int B_MN>
+static int wide_setup() {
+  const int smem = 1024 + HW_STAGES * HW_STAGE;
+  if (cudaFuncSetAttribute(head_wide_kernel<EPI, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+      cudaSuccess)
+    return SB_ERR_DRIVER;
+  if (g_hw_pairs) return 0;
+  // SM pairs that can hold a cluster at the same time (a GPC with an odd SM count leaves one SM out)
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(148);
+  cfg.blockDim = dim3(HW_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  const bool known = cudaOccupancyMaxActiveClusters(&n, head_wide_kernel<EPI, A_MN, B_MN>, &cfg) == cudaSuccess;
+  cudaGetLastError();
+  g_hw_pairs = known && n > 0 && n < 74 ? n : 74;
+  return 0;
+}
+
+template <int EPI, int A_MN, int B_MN>
+static int wide_launch(WideParams& p, cudaStream_t stream) {
+  const int rc = wide_setup<EPI, A_MN, B_MN>();
+  if (rc) return rc;
+  const long long jobs = EPI == WIDE_OUT ? (long long)p.row_tiles * p.col_tiles * p.kslices : (long long)p.row_tiles * p.splits;
+  const int pairs = (int)(jobs < g_hw_pairs ? jobs : g_hw_pairs);
+  head_wide_kernel<EPI, A_MN, B_MN><<<2 * pairs, HW_THREADS, 1024 + HW_STAGES * HW_STAGE, stream>>>(p);
+  sb_count_launch(1);
+  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+}
+
+static int map_rows(CUtensorMap* m, const void* base, long long rows, long long inner, long long ld, int box_rows) {
+  const long long dims[2] = {inner, rows}, st[2] = {1, ld};
+  const int box[2] = {64, box_rows};
+  return make_map_bf16(m, base, 2, dims, st, box, 128);
+}
+static long long up(long long n, long long m) { return (n + m - 1) / m * m; }
+
+// Cuts of the column tiles of LSE / D: fewest rounds of (tiles per job + a quarter of one), fewest cuts first.
+static void wide_split(int row_tiles, int col_tiles, int* splits, int* per_out) {
+  long long best = -1;
+  for (int want = 1; want <= col_tiles && want <= 148; ++want) {
+    const int per = (col_tiles + want - 1) / want, s = (col_tiles + per - 1) / per;
+    const long long rounds = ((long long)row_tiles * s + 73) / 74, cost = rounds * (4 * per + 1);
+    if (best < 0 || cost < best) { best = cost; *splits = s; *per_out = per; }
+  }
+}
+// Slices of the reduction of a product rows x cols over kc blocks of 64: rounds of (blocks x 512 clocks + 1000), and the
+// slices' way through memory at some 3500 bytes a clock.
+static int wide_slices(long long rows, int C, int kc) {
+  const long long tiles = up(rows, 256) / 256 * (up(C, 256) / 256);
+  long long best = -1;
+  int pick = 1;
+  for (int s = 1; s <= 64 && s <= kc; ++s) {
+    const int per = (kc + s - 1) / s;
+    if ((kc + per - 1) / per != s) continue;
+    long long cost = (tiles * s + 73) / 74 * (per * 512LL + 1000);
+    if (s > 1) cost += 8LL * s * rows * C / 3500 + 4000;
+    if (best < 0 || cost < best) { best = cost; pick = s; }
+  }
+  return pick;
+}
+
+struct Pieces {
+  long long vc, kp;  // voxels and classes of a piece, multiples of 256
+  int nv, nk;
+  int sx, sw;        // slices of the two products
+  int d_splits, d_per;
+  long long dl, acc_x, acc_w, acc_b, ws_b, slices, total;  // offsets in floats
+};
+static Pieces wide_pieces(const SbHeadArgs* a) {
+  Pieces q;
+  const long long vp = up(a->V, 256), kp = up(a->K, 256);
+  if (kp * (vp < 16384 ? vp : 16384) <= HW_PIECE) {  // all classes, as many voxels as fit
+    q.kp = kp;
+    q.vc = HW_PIECE / kp / 256 * 256;
+    if (q.vc > vp) q.vc = vp;
+  } else {
+    q.vc = vp < 16384 ? vp : 16384;
+    q.kp = HW_PIECE / q.vc / 256 * 256;
+  }
+  q.nv = (int)((vp + q.vc - 1) / q.vc);
+  q.nk = (int)((kp + q.kp - 1) / q.kp);
+  q.vc = up((vp + q.nv - 1) / q.nv, 256);
+  q.kp = up((kp + q.nk - 1) / q.nk, 256);
+  q.sx = wide_slices(q.vc, a->C, (int)(q.kp / 64));
+  q.sw = wide_slices(q.kp, a->C, (int)(q.vc / 64));
+  wide_split((int)(q.kp / 256), (int)(q.vc / 256), &q.d_splits, &q.d_per);
+  long long at = 0;
+  auto take = [&](long long floats) { const long long o = at; at += up(floats, 64); return o; };
+  q.dl = take(q.kp * q.vc / 2);
+  q.acc_x = take(q.nk > 1 ? q.vc * a->C : 0);
+  q.acc_w = take(q.nv > 1 ? (long long)a->K * a->C : 0);
+  q.acc_b = take(q.nv > 1 ? a->K : 0);
+  q.ws_b = take(2LL * q.d_splits * q.kp);
+  const long long sx = q.sx > 1 ? q.sx * q.vc * a->C : 0, sw = q.sw > 1 ? q.sw * q.kp * a->C : 0;
+  q.slices = take(sx > sw ? sx : sw);
+  q.total = at;
+  return q;
+}
+
+long long head_wide_scratch(const SbHeadArgs* a) { return wide_pieces(a).total; }
+
+int head_wide_splits(long long V, int K) {
+  int s = 1, per = 1;
+  wide_split((int)(up(V, 256) / 256), (int)(up(K, 256) / 256), &s, &per);
+  return s;
+}
+
+int head_wide_forward(const SbHeadArgs* a, float2* part, float* tl, int, cudaStream_t stream) {
+  WideParams p;
+  memset(&p, 0, sizeof(p));
+  p.row_tiles = (int)(up(a->V, 256) / 256);
+  p.col_tiles = (int)(up(a->K, 256) / 256);
+  wide_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
+  p.kc = (a->C + 63) / 64;
+  p.cols = a->K;
+  p.rows_pad = up(a->V, HD_PAD);
+  p.y = a->y;
+  p.colp = a->bias2;
+  p.part = part;
+  p.tl = tl;
+  p.status = a->status;
+  int rc = map_rows(&p.mapA, a->x, a->V, a->C, a->C, 128);
+  if (rc) return rc;
+  rc = map_rows(&p.mapB, a->w, a->K, a->C, a->C, 128);
+  if (rc) return rc;
+  return wide_launch<WIDE_LSE, 0, 0>(p, stream);
+}
+
+// one product of a piece: rows x C over `kext` of the reduction
+template <int A_MN>
+static int wide_product(const SbHeadArgs* a, const void* dl, long long ldd, long long vext, long long kext, const void* b,
+                        long long b_rows, long long rows, int slices, float* ws, float* acc, int add, void* out16,
+                        void* out32, cudaStream_t stream) {
+  WideParams p;
+  memset(&p, 0, sizeof(p));
+  const long long ext = A_MN ? kext : vext;  // of the reduction
+  p.kc = (int)(ext / 64);
+  p.kslices = slices < p.kc ? slices : p.kc;
+  p.kc_per_slice = (p.kc + p.kslices - 1) / p.kslices;
+  p.kslices = (p.kc + p.kc_per_slice - 1) / p.kc_per_slice;
+  p.rows = rows;
+  p.row_tiles = (int)(up(rows, 256) / 256);
+  p.cols = a->C;
+  p.col_tiles = (a->C + 255) / 256;
+  p.acc = acc;
+  p.add = add;
+  p.out16 = (__nv_bfloat16*)out16;
+  p.out32 = (float*)out32;
+  p.slices = ws;
+  p.status = a->status;
+  int rc = map_rows(&p.mapA, dl, kext, vext, ldd, A_MN ? 64 : 128);
+  if (rc) return rc;
+  rc = map_rows(&p.mapB, b, b_rows, a->C, a->C, 64);
+  if (rc) return rc;
+  rc = wide_launch<WIDE_OUT, A_MN, 1>(p, stream);
+  if (rc || p.kslices == 1) return rc;
+  const long long elems = rows * a->C, blocks = (elems / 8 + 255) / 256;
+  head_slices_kernel<<<(int)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(ws, p.kslices, elems, acc, add,
+                                                                                    p.out16, p.out32);
+  sb_count_launch(1);
+  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+}
+
+int head_wide_backward(const SbHeadArgs* a, cudaStream_t stream) {
+  const Pieces q = wide_pieces(a);
+  if (a->scratch_floats < q.total) return SB_ERR_TOO_LARGE;
+  const __nv_bfloat16* x = (const __nv_bfloat16*)a->x;
+  const __nv_bfloat16* w = (const __nv_bfloat16*)a->w;
+  __nv_bfloat16* dl = (__nv_bfloat16*)(a->scratch + q.dl);
+  float* ws_b = a->scratch + q.ws_b;
+  for (int iv = 0; iv < q.nv; ++iv) {
+    const long long v0 = iv * q.vc, vrows = a->V - v0 < q.vc ? a->V - v0 : q.vc, vext = up(vrows, 256);
+    if (vrows <= 0) break;
+    const bool v_last = v0 + q.vc >= a->V;
+    for (int ik = 0; ik < q.nk; ++ik) {
+      const long long k0 = ik * q.kp, krows = a->K - k0 < q.kp ? a->K - k0 : q.kp, kext = up(krows, 256);
+      if (krows <= 0) break;
+      const bool k_last = k0 + q.kp >= a->K;
+      WideParams p;
+      memset(&p, 0, sizeof(p));
+      p.row_tiles = (int)(kext / 256);
+      p.col_tiles = (int)(vext / 256);
+      p.tiles_per_split = q.d_per;
+      p.splits = (p.col_tiles + q.d_per - 1) / q.d_per;
+      p.kc = (a->C + 63) / 64;
+      p.cols = (int)vext;
+      p.rows_pad = q.kp;
+      p.y = a->y + v0;
+      p.colp = a->lse2g + v0;
+      p.colg = a->g + v0;
+      p.rowp = a->bias2 + k0;
+      p.row0 = (int)k0;
+      p.dl = dl;
+      p.ldd = q.vc;
+      p.ws_b = ws_b;
+      p.status = a->status;
+      int rc = map_rows(&p.mapA, w + k0 * a->C, krows, a->C, a->C, 128);
+      if (rc) return rc;
+      rc = map_rows(&p.mapB, x + v0 * a->C, vrows, a->C, a->C, 128);
+      if (rc) return rc;
+      rc = wide_launch<WIDE_D, 0, 0>(p, stream);
+      if (rc) return rc;
+      if (a->db != nullptr) {
+        head_slices_b_kernel<<<(int)((krows + 255) / 256), 256, 0, stream>>>(
+            ws_b, 2 * p.splits, q.kp, (int)krows, a->scratch + q.acc_b + k0, iv > 0,
+            v_last && a->bias_kind == 0 ? (__nv_bfloat16*)a->db + k0 : nullptr,
+            v_last && a->bias_kind == 2 ? (float*)a->db + k0 : nullptr);
+        sb_count_launch(1);
+      }
+      if (a->dx != nullptr) {
+        rc = wide_product<1>(a, dl, q.vc, vext, kext, w + k0 * a->C, krows, vrows, q.sx, a->scratch + q.slices,
+                             a->scratch + q.acc_x, ik > 0, k_last ? (__nv_bfloat16*)a->dx + v0 * a->C : nullptr, nullptr,
+                             stream);
+        if (rc) return rc;
+      }
+      if (a->dw != nullptr) {
+        rc = wide_product<0>(a, dl, q.vc, vext, kext, x + v0 * a->C, vrows, krows, q.sw, a->scratch + q.slices,
+                             a->scratch + q.acc_w + k0 * a->C, iv > 0,
+                             v_last && a->dw_kind == 0 ? (__nv_bfloat16*)a->dw + k0 * a->C : nullptr,
+                             v_last && a->dw_kind == 2 ? (float*)a->dw + k0 * a->C : nullptr, stream);
+        if (rc) return rc;
+      }
+    }
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+}
+
+}  // namespace sb

@@ -208,8 +208,8 @@ int sb_gn8_apply(const SbGn8Args* a, cudaStream_t stream);
 int sb_gn8_bwd_partial(const SbGn8Args* a, cudaStream_t stream);
 int sb_gn8_bwd_dx(const SbGn8Args* a, cudaStream_t stream);
 
-// Cross entropy of a head of K classes over V voxels of C channels without its logits (head_loss.cu).
-// Arrays marked v / k are padded to a multiple of 128 voxels / classes.
+// Cross entropy of a head of K classes over V voxels of C channels without its logits (head_loss.cu, head_wide.cu).
+// Arrays marked v / k are padded to a multiple of 256 voxels / classes.
 typedef struct {
   const void* x;       // bf16 [V][C]
   const void* w;       // bf16 [K][C]
@@ -228,23 +228,20 @@ typedef struct {
   double* total;       // [2] forward out: sums of u nll and u
   float* loss;         // [1]
   float* den;          // [1]
-  float* g;            // v: sb_head_weights out
-  float* lse2g;        // v: sb_head_weights out
-  void* dx;            // bf16 [V][C]
-  void* dw;            // [K][C]
+  float* g;            // v: backward scratch, dL/d(nll) of a voxel
+  float* lse2g;        // v: backward scratch, lse2 - log2 g
+  void* dx;            // optional bf16 [V][C]
+  void* dw;            // optional [K][C]
   int dw_kind;         // 0 bf16, 2 fp32
   void* db;            // optional [K]
   float* scratch;      // sb_head_scratch() floats, 16-byte aligned
   long long scratch_floats;
   uint32_t* status;
 } SbHeadArgs;
-int sb_head_max_width(void);
-long long sb_head_scratch(const SbHeadArgs* a, int mode);  // 0 forward, 1 dx, 2 dw
+long long sb_head_scratch(const SbHeadArgs* a, int mode);  // 0 forward, 1 backward
 int sb_head_forward(const SbHeadArgs* a, cudaStream_t stream);
 int sb_head_total(const double* sums, int blocks, double* total, float* loss, float* den, cudaStream_t stream);
-int sb_head_weights(const SbHeadArgs* a, const float* gout, cudaStream_t stream);
-int sb_head_dx(const SbHeadArgs* a, cudaStream_t stream);
-int sb_head_dw(const SbHeadArgs* a, cudaStream_t stream);
+int sb_head_backward(const SbHeadArgs* a, const float* gout, cudaStream_t stream);
 
 // number of kernels this library launched so far in the process
 long long sb_launch_count(void);

@@ -225,14 +225,19 @@ SITES = {
     42: "gradient all-reduce: waiting for the peers' completion",
     61: "fused loss: a label outside [0, n_classes) (detail = label value, sample); the voxel was skipped",
     63: "head loss: a label outside [0, n_classes) (detail = label value, voxel); the voxel takes no part",
-    71: "head loss: producer waiting for a free tile",
-    72: "head loss: MMA waiting for a free accumulator",
-    73: "head loss: MMA waiting for the probabilities",
-    74: "head loss: MMA waiting for the resident tile",
-    75: "head loss: MMA waiting for a streamed tile",
-    76: "head loss: MMA waiting for a free tile of logits",
-    77: "head loss: epilogue waiting for the accumulator",
-    78: "head loss: epilogue waiting for a tile of logits",
+    91: "head loss: producer waiting for a free tile",
+    92: "head loss: MMA waiting for a free accumulator",
+    93: "head loss: MMA waiting for the probabilities",
+    94: "head loss: MMA waiting for the resident tile",
+    95: "head loss: MMA waiting for a streamed tile",
+    96: "head loss: MMA waiting for a free tile of logits",
+    97: "head loss: epilogue waiting for the accumulator",
+    98: "head loss: epilogue waiting for a tile of logits",
+    101: "wide head loss: producer waiting for a free stage",
+    102: "wide head loss: producer waiting for the last releases",
+    103: "wide head loss: MMA waiting for a free accumulator",
+    104: "wide head loss: MMA waiting for operands",
+    105: "wide head loss: epilogue waiting for an accumulator",
     62: "fused loss gradient: a label outside [0, n_classes) (detail = label value, sample); the voxel was skipped",
 }
 

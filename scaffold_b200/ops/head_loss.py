@@ -36,17 +36,14 @@ class SbHeadArgs(C.Structure):
     ]
 
 
-_lib.register("sb_head_max_width", [], C.c_int)
 _lib.register("sb_head_scratch", [C.POINTER(SbHeadArgs), C.c_int], C.c_longlong)
 _lib.register("sb_head_forward", [C.POINTER(SbHeadArgs), _P])
 _lib.register("sb_head_total", [_P, C.c_int, _P, _P, _P, _P])
-_lib.register("sb_head_weights", [C.POINTER(SbHeadArgs), _P, _P])
-_lib.register("sb_head_dx", [C.POINTER(SbHeadArgs), _P])
-_lib.register("sb_head_dw", [C.POINTER(SbHeadArgs), _P])
+_lib.register("sb_head_backward", [C.POINTER(SbHeadArgs), _P, _P])
 
 _LABEL_KIND = {torch.int16: 2, torch.int32: 4, torch.int64: 8}
 _KIND = {torch.bfloat16: 0, torch.float32: 2}
-MAX_WIDTH = 256  # HD_MAX_C of csrc/head_loss.cu
+MAX_WIDTH = 32768
 
 
 def head_supported(width: int) -> bool:
@@ -54,8 +51,8 @@ def head_supported(width: int) -> bool:
     return 8 <= width <= MAX_WIDTH and width % 8 == 0
 
 
-def _pad128(n: int) -> int:
-    return (n + 127) // 128 * 128
+def _pad(n: int) -> int:
+    return (n + 255) // 256 * 256
 
 
 def _scratch(a: SbHeadArgs, mode: int, dev):
@@ -88,7 +85,7 @@ class _HeadLossFn(torch.autograd.Function):
         a.labels, a.label_kind = labels.data_ptr(), _LABEL_KIND[labels.dtype]
         if ignore is not None:
             a.has_ignore, a.ignore = 1, ignore
-        vp, kp = _pad128(a.V), _pad128(a.K)
+        vp, kp = _pad(a.V), _pad(a.K)
         y = torch.empty(vp, dtype=torch.int32, device=dev)
         lse2 = torch.empty(vp, dtype=torch.float32, device=dev)
         bias2 = torch.empty(kp, dtype=torch.float32, device=dev)
@@ -112,29 +109,23 @@ class _HeadLossFn(torch.autograd.Function):
         x, w16, y, lse2, bias2, den, cw = ctx.saved_tensors
         dev = x.device
         w_type, b_type = ctx.like
-        L, st = _lib.lib(), _lib.stream_ptr()
         a = _args(x, w16, None, cw)
         g, lse2g = torch.empty_like(lse2), torch.empty_like(lse2)
         a.y, a.lse2, a.bias2, a.den, a.g, a.lse2g = (t.data_ptr() for t in (y, lse2, bias2, den, g, lse2g))
         gout = gout.float().contiguous()
-        _lib.check(L.sb_head_weights(C.byref(a), gout.data_ptr(), st), "sb_head_weights")
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
             dx = torch.empty_like(x)
             a.dx = dx.data_ptr()
-            keep = _scratch(a, 1, dev)
-            _lib.check(L.sb_head_dx(C.byref(a), st), "sb_head_dx")
-            del keep
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+        if ctx.needs_input_grad[1]:
             dw = torch.empty(w16.shape, dtype=w_type, device=dev)
             a.dw, a.dw_kind = dw.data_ptr(), _KIND[w_type]
-            if ctx.needs_input_grad[2]:
-                db = torch.empty(w16.shape[0], dtype=b_type, device=dev)
-                a.db, a.bias_kind = db.data_ptr(), _KIND[b_type]
-            keep = _scratch(a, 2, dev)
-            _lib.check(L.sb_head_dw(C.byref(a), st), "sb_head_dw")
-            del keep
-        return dx, dw if ctx.needs_input_grad[1] else None, db, None, None, None, None
+        if ctx.needs_input_grad[2]:
+            db = torch.empty(w16.shape[0], dtype=b_type, device=dev)
+            a.db, a.bias_kind = db.data_ptr(), _KIND[b_type]
+        keep = _scratch(a, 1, dev)  # noqa: F841
+        _lib.check(_lib.lib().sb_head_backward(C.byref(a), gout.data_ptr(), _lib.stream_ptr()), "sb_head_backward")
+        return dx, dw, db, None, None, None, None
 
 
 def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], labels: torch.Tensor,
@@ -178,7 +169,7 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
         raise ValueError(f"the kernels read features of 8 to {MAX_WIDTH} channels in multiples of 8; got {c}")
     if weight.dtype not in _KIND or (bias is not None and bias.dtype not in _KIND):
         raise TypeError("weight and bias must be bf16 or fp32")
-    if features.numel() // c > 2 ** 31 - 256:
+    if features.numel() // c > 2 ** 31 - 512:
         raise ValueError(f"{features.numel() // c} voxels are more than the kernels count")
     x = features.to(torch.bfloat16).reshape(-1, c)
     if not x.is_contiguous() or x.data_ptr() % 16:  # a tensor map starts on 16 bytes
