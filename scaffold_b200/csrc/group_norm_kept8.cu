@@ -20,6 +20,8 @@
 namespace sb {
 
 constexpr int GN8_THREADS = 256;
+constexpr int GN8_WAVE = 4, GN8_WAVE_SUMS = 3;  // blocks per SM: 64 registers a thread (the sums: 85)
+constexpr int GN8_U_APPLY = 4, GN8_U_SUMS = 4, GN8_U_DX = 2;  // voxels in flight per thread
 
 struct Gn8Params {
   const __nv_bfloat16* x;
@@ -60,7 +62,8 @@ __device__ __forceinline__ void gn8_values(uint2 q, float step, float (&f)[8]) {
   for (int i = 0; i < 4; ++i) { f[i] = lo[i] * step; f[4 + i] = hi[i] * step; }
 }
 
-__global__ void __launch_bounds__(GN8_THREADS, 3) gn8_apply_kernel(const Gn8Params p) {
+template <bool RELU>
+__global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE) gn8_apply_kernel(const Gn8Params p) {
   __shared__ float s_mean[256], s_rstd[256];
   const int n = blockIdx.y;
   for (int g = threadIdx.x; g < p.G; g += GN8_THREADS) {
@@ -83,42 +86,54 @@ __global__ void __launch_bounds__(GN8_THREADS, 3) gn8_apply_kernel(const Gn8Para
   }
   const long long base = (long long)n * p.S * p.C + oct * 8;
   // the loop is uniform over the block, for the shuffle: a thread without a voxel takes part with zeros
-  for (long long v0 = (long long)blockIdx.x * vpb; v0 < p.S; v0 += (long long)gridDim.x * vpb) {
-    const long long v = v0 + vl;
-    const bool live = vl < vpb && v < p.S;
-    const long long at = base + v * p.C;
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (live) raw = __ldg(reinterpret_cast<const uint4*>(p.x + at));
-    float f[8], t[8];
-    gn8_unpack(raw, f);
-    uint32_t amax = 0;
+  const long long stride = (long long)gridDim.x * vpb;
+  for (long long v0 = (long long)blockIdx.x * vpb; v0 < p.S; v0 += GN8_U_APPLY * stride) {
+    uint4 raw[GN8_U_APPLY];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    const uint32_t b = kept_exponent(amax);
-    const float step = kept_step(b), inv = b == 255u ? 0.f : kept_inv(b);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      t[i] = fmaf(f[i], inv, KEPT_MAGIC);
-      float yv = fmaf(f[i], a[i], c[i]);
-      if (p.relu) {
-        const bool on = yv > 0.f, kept_on = fmaf((t[i] - KEPT_MAGIC) * step, a[i], c[i]) > 0.f;
-        if (on != kept_on) t[i] += on == (a[i] > 0.f) ? 1.f : -1.f;
-        yv = yv <= 0.f ? 0.f : yv;  // NaN propagates
-      }
-      if (b >= KEPT_TOP_BF16) t[i] = b == 255u ? KEPT_MAGIC : kept_cap(t[i]);
-      f[i] = yv;
+    for (int u = 0; u < GN8_U_APPLY; ++u) {
+      const long long v = v0 + u * stride + vl;
+      raw[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (vl < vpb && v < p.S) raw[u] = __ldg(reinterpret_cast<const uint4*>(p.x + base + v * p.C));
     }
-    if (live) {
-      *reinterpret_cast<uint4*>(p.y + at) = gn8_pack(f);
-      *reinterpret_cast<uint2*>(p.q + at) =
-          make_uint2(kept_pack4(t[0], t[1], t[2], t[3]), kept_pack4(t[4], t[5], t[6], t[7]));
-      if ((oct & 1) == 0) p.exps[at / KEPT_BLOCK] = (uint8_t)b;
+#pragma unroll
+    for (int u = 0; u < GN8_U_APPLY; ++u) {
+      if (v0 + u * stride >= p.S) break;
+      const long long v = v0 + u * stride + vl, at = base + v * p.C;
+      float f[8], t[8];
+      gn8_unpack(raw[u], f);
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      const uint32_t b = kept_exponent(amax);
+      const float step = kept_step(b), inv = b == 255u ? 0.f : kept_inv(b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        t[i] = fmaf(f[i], inv, KEPT_MAGIC);
+        float yv = fmaf(f[i], a[i], c[i]);
+        if (RELU) {
+          const bool on = yv > 0.f, kept_on = fmaf((t[i] - KEPT_MAGIC) * step, a[i], c[i]) > 0.f;
+          if (on != kept_on) t[i] += on == (a[i] > 0.f) ? 1.f : -1.f;
+          yv = yv <= 0.f ? 0.f : yv;  // NaN propagates
+        }
+        f[i] = yv;
+      }
+      if (b >= KEPT_TOP_BF16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = b == 255u ? KEPT_MAGIC : kept_cap(t[i]);
+      }
+      if (vl < vpb && v < p.S) {
+        *reinterpret_cast<uint4*>(p.y + at) = gn8_pack(f);
+        *reinterpret_cast<uint2*>(p.q + at) =
+            make_uint2(kept_pack4(t[0], t[1], t[2], t[3]), kept_pack4(t[4], t[5], t[6], t[7]));
+        if ((oct & 1) == 0) p.exps[at / KEPT_BLOCK] = (uint8_t)b;
+      }
     }
   }
 }
 
-__global__ void __launch_bounds__(GN8_THREADS, 3) gn8_bwd_partial_kernel(const Gn8Params p) {
+template <int GP, bool RELU>  // GP: groups that eight consecutive channels cover
+__global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE_SUMS) gn8_bwd_partial_kernel(const Gn8Params p) {
   __shared__ float s_a[GN8_THREADS * 8], s_b[GN8_THREADS * 8];
   const int split = blockIdx.x, n = blockIdx.y;
   const int tpv = p.C / 8, vpb = GN8_THREADS / tpv;
@@ -127,31 +142,50 @@ __global__ void __launch_bounds__(GN8_THREADS, 3) gn8_bwd_partial_kernel(const G
   const long long chunk = (p.S + p.nsplit - 1) / p.nsplit;
   const long long v0 = (long long)split * chunk;
   const long long v1 = v0 + chunk < p.S ? v0 + chunk : p.S;
-  float a[8], c[8], A[8], B[8], mu[8];
+  float a[8], c[8], A[8], B[8], mu[GP];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int ch = oct * 8 + i, g = ch / cg;
-    mu[i] = p.mean[n * p.G + g];
+    const float m = p.mean[n * p.G + g];
+    if (i % (8 / GP) == 0) mu[i / (8 / GP)] = m;
     a[i] = p.rstd[n * p.G + g] * p.w[ch];
-    c[i] = p.b[ch] - mu[i] * a[i];
+    c[i] = p.b[ch] - m * a[i];
     A[i] = 0.f;
     B[i] = 0.f;
   }
   const long long base = (long long)n * p.S * p.C + oct * 8;
   if (vl < vpb) {
-    for (long long v = v0 + vl; v < v1; v += vpb) {
-      const long long at = base + v * p.C;
+    auto body = [&](const uint2 rq, uint32_t re, const uint4 rd) {
       float fx[8], fd[8];
-      gn8_values(__ldg(reinterpret_cast<const uint2*>(p.q + at)), kept_step(__ldg(p.exps + at / KEPT_BLOCK)), fx);
-      gn8_unpack(__ldg(reinterpret_cast<const uint4*>(p.dy + at)), fd);
+      gn8_values(rq, kept_step(re), fx);
+      gn8_unpack(rd, fd);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float d = fd[i];
-        if (p.relu && fmaf(fx[i], a[i], c[i]) <= 0.f) d = 0.f;
+        if (RELU && fmaf(fx[i], a[i], c[i]) <= 0.f) d = 0.f;
         A[i] += d;
-        B[i] = fmaf(d, fx[i] - mu[i], B[i]);
+        B[i] = fmaf(d, fx[i] - mu[i / (8 / GP)], B[i]);
       }
+    };
+    const long long row = (long long)vpb * p.C;
+    long long v = v0 + vl, at = base + v * p.C;
+    for (; v + (GN8_U_SUMS - 1) * vpb < v1; v += GN8_U_SUMS * vpb, at += GN8_U_SUMS * row) {
+      uint2 rq[GN8_U_SUMS];
+      uint32_t re[GN8_U_SUMS];
+      uint4 rd[GN8_U_SUMS];
+#pragma unroll
+      for (int u = 0; u < GN8_U_SUMS; ++u) {
+        const long long k = at + u * row;
+        rq[u] = __ldg(reinterpret_cast<const uint2*>(p.q + k));
+        re[u] = __ldg(p.exps + k / KEPT_BLOCK);
+        rd[u] = __ldg(reinterpret_cast<const uint4*>(p.dy + k));
+      }
+#pragma unroll
+      for (int u = 0; u < GN8_U_SUMS; ++u) body(rq[u], re[u], rd[u]);
     }
+    for (; v < v1; v += vpb, at += row)
+      body(__ldg(reinterpret_cast<const uint2*>(p.q + at)), __ldg(p.exps + at / KEPT_BLOCK),
+           __ldg(reinterpret_cast<const uint4*>(p.dy + at)));
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -172,7 +206,8 @@ __global__ void __launch_bounds__(GN8_THREADS, 3) gn8_bwd_partial_kernel(const G
   }
 }
 
-__global__ void __launch_bounds__(GN8_THREADS, 3) gn8_bwd_dx_kernel(const Gn8Params p) {
+template <int GP, bool RELU>
+__global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE) gn8_bwd_dx_kernel(const Gn8Params p) {
   __shared__ float s_c1[256], s_c2[256];
   const int n = blockIdx.y;
   const int tpv = p.C / 8, vpb = GN8_THREADS / tpv;
@@ -203,31 +238,51 @@ __global__ void __launch_bounds__(GN8_THREADS, 3) gn8_bwd_dx_kernel(const Gn8Par
   __syncthreads();
   if (vl >= vpb) return;
   // dx = rstd (d w - c1 - xhat c2) = d a + (x - mean) q + r
-  float a[8], c[8], mu[8], q[8], r[8];
+  float a[8], c[8], mu[GP], q[GP], r[GP];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int ch = oct * 8 + i, g = ch / cg;
-    const float rs = p.rstd[n * p.G + g];
-    mu[i] = p.mean[n * p.G + g];
+    const float rs = p.rstd[n * p.G + g], m = p.mean[n * p.G + g];
     a[i] = rs * p.w[ch];
-    c[i] = p.b[ch] - mu[i] * a[i];
-    q[i] = -rs * rs * s_c2[g];
-    r[i] = -rs * s_c1[g];
+    c[i] = p.b[ch] - m * a[i];
+    if (i % (8 / GP) == 0) {
+      mu[i / (8 / GP)] = m;
+      q[i / (8 / GP)] = -rs * rs * s_c2[g];
+      r[i / (8 / GP)] = -rs * s_c1[g];
+    }
   }
   const long long base = (long long)n * p.S * p.C + oct * 8;
-  for (long long v = (long long)blockIdx.x * vpb + vl; v < p.S; v += (long long)gridDim.x * vpb) {
-    const long long at = base + v * p.C;
+  auto body = [&](const uint2 rq, uint32_t re, const uint4 rd, long long at) {
     float fx[8], fd[8];
-    gn8_values(__ldg(reinterpret_cast<const uint2*>(p.q + at)), kept_step(__ldg(p.exps + at / KEPT_BLOCK)), fx);
-    gn8_unpack(__ldg(reinterpret_cast<const uint4*>(p.dy + at)), fd);
+    gn8_values(rq, kept_step(re), fx);
+    gn8_unpack(rd, fd);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float d = fd[i];
-      if (p.relu && fmaf(fx[i], a[i], c[i]) <= 0.f) d = 0.f;
-      fx[i] = fmaf(d, a[i], fmaf(fx[i] - mu[i], q[i], r[i]));
+      if (RELU && fmaf(fx[i], a[i], c[i]) <= 0.f) d = 0.f;
+      fx[i] = fmaf(d, a[i], fmaf(fx[i] - mu[i / (8 / GP)], q[i / (8 / GP)], r[i / (8 / GP)]));
     }
     *reinterpret_cast<uint4*>(p.y + at) = gn8_pack(fx);
+  };
+  const long long stride = (long long)gridDim.x * vpb, row = stride * p.C;
+  long long v = (long long)blockIdx.x * vpb + vl, at = base + v * p.C;
+  for (; v + (GN8_U_DX - 1) * stride < p.S; v += GN8_U_DX * stride, at += GN8_U_DX * row) {
+    uint2 rq[GN8_U_DX];
+    uint32_t re[GN8_U_DX];
+    uint4 rd[GN8_U_DX];
+#pragma unroll
+    for (int u = 0; u < GN8_U_DX; ++u) {
+      const long long k = at + u * row;
+      rq[u] = __ldg(reinterpret_cast<const uint2*>(p.q + k));
+      re[u] = __ldg(p.exps + k / KEPT_BLOCK);
+      rd[u] = __ldg(reinterpret_cast<const uint4*>(p.dy + k));
+    }
+#pragma unroll
+    for (int u = 0; u < GN8_U_DX; ++u) body(rq[u], re[u], rd[u], at + u * row);
   }
+  for (; v < p.S; v += stride, at += row)
+    body(__ldg(reinterpret_cast<const uint2*>(p.q + at)), __ldg(p.exps + at / KEPT_BLOCK),
+         __ldg(reinterpret_cast<const uint4*>(p.dy + at)), at);
 }
 
 static int gn8_fill(const SbGn8Args* a, Gn8Params& p) {
@@ -253,7 +308,7 @@ static int gn8_fill(const SbGn8Args* a, Gn8Params& p) {
 }
 static int gn8_blocks(const Gn8Params& p) {
   const int vpb = GN8_THREADS / (p.C / 8);
-  const long long need = (p.S + vpb - 1) / vpb, cap = 148LL * 3 / p.N;  // one wave
+  const long long need = (p.S + vpb - 1) / vpb, cap = 148LL * GN8_WAVE / p.N;  // one wave
   const long long b = need < cap ? need : cap;
   return (int)(b < 1 ? 1 : b);
 }
@@ -267,7 +322,9 @@ extern "C" int sb_gn8_apply(const SbGn8Args* a, cudaStream_t stream) {
   const int rc = gn8_fill(a, p);
   if (rc) return rc;
   if (p.x == nullptr || p.y == nullptr || p.fin == nullptr) return SB_ERR_SHAPE;
-  gn8_apply_kernel<<<dim3(gn8_blocks(p), p.N), GN8_THREADS, 0, stream>>>(p);
+  const dim3 grid(gn8_blocks(p), p.N);
+  if (p.relu) gn8_apply_kernel<true><<<grid, GN8_THREADS, 0, stream>>>(p);
+  else gn8_apply_kernel<false><<<grid, GN8_THREADS, 0, stream>>>(p);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
@@ -277,7 +334,11 @@ extern "C" int sb_gn8_bwd_partial(const SbGn8Args* a, cudaStream_t stream) {
   const int rc = gn8_fill(a, p);
   if (rc) return rc;
   if (p.dy == nullptr || p.part == nullptr || p.nsplit < 1) return SB_ERR_SHAPE;
-  gn8_bwd_partial_kernel<<<dim3(p.nsplit, p.N), GN8_THREADS, 0, stream>>>(p);
+  const dim3 grid(p.nsplit, p.N);
+  const int gp = p.C / p.G >= 8 ? 1 : 8 / (p.C / p.G);
+  if (gp == 1) p.relu ? gn8_bwd_partial_kernel<1, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_partial_kernel<1, false><<<grid, GN8_THREADS, 0, stream>>>(p);
+  else if (gp == 2) p.relu ? gn8_bwd_partial_kernel<2, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_partial_kernel<2, false><<<grid, GN8_THREADS, 0, stream>>>(p);
+  else p.relu ? gn8_bwd_partial_kernel<4, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_partial_kernel<4, false><<<grid, GN8_THREADS, 0, stream>>>(p);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
@@ -287,7 +348,11 @@ extern "C" int sb_gn8_bwd_dx(const SbGn8Args* a, cudaStream_t stream) {
   const int rc = gn8_fill(a, p);
   if (rc) return rc;
   if (p.dy == nullptr || p.y == nullptr || p.fin == nullptr || p.dw == nullptr || p.db == nullptr) return SB_ERR_SHAPE;
-  gn8_bwd_dx_kernel<<<dim3(gn8_blocks(p), p.N), GN8_THREADS, 0, stream>>>(p);
+  const dim3 grid(gn8_blocks(p), p.N);
+  const int gp = p.C / p.G >= 8 ? 1 : 8 / (p.C / p.G);
+  if (gp == 1) p.relu ? gn8_bwd_dx_kernel<1, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_dx_kernel<1, false><<<grid, GN8_THREADS, 0, stream>>>(p);
+  else if (gp == 2) p.relu ? gn8_bwd_dx_kernel<2, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_dx_kernel<2, false><<<grid, GN8_THREADS, 0, stream>>>(p);
+  else p.relu ? gn8_bwd_dx_kernel<4, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_dx_kernel<4, false><<<grid, GN8_THREADS, 0, stream>>>(p);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }

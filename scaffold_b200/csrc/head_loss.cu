@@ -3,47 +3,56 @@
 //   p_ij = exp(s_ij - lse_i),  D_ij = g_i (p_ij - [j = y_i]),  g_i = dL u_i / sum u
 //   dX = D W,  dW = D^T X,  db_j = sum_i D_ij
 // The logits (voxels x classes) are never written: each of the three kernels multiplies the tiles of X and W again, keeps
-// a 128 x 128 tile of s in tensor memory and uses it up there. Everything is counted in powers of two: t = s log2(e).
+// a 128 x 128 tile of s in tensor memory and uses it up there.
+//
+// Bias and log-sum-exp ride along the reduction: X and W have sixteen columns more (x16, w16), in which b_j, -lse_i and
+// log u_i stand as three bf16 each (24 bits) against ones of the other side, so the tensor cores hand over
+// s_ij + b_j - lse_i and an entry costs the epilogue a multiplication by log2(e) and an exponential. Column parameters
+// out of shared memory cost it a data-pipe cycle per warp and column each, more than the exponential unit's share.
 //
 // One kernel template, three modes. A CTA keeps 128 ROWS resident and walks 128-wide tiles of COLUMNS:
 //   HEAD_FWD  rows = voxels, columns = classes: running maximum and sum of every row (one row per thread, no exchange)
 //   HEAD_DX   rows = voxels, columns = classes: P = p - [j = y] in bf16 goes back to tensor memory over the tile of s it
 //             came from, and acc[128][C] += P W is the second MMA with P as its A operand (W's tile is the same shared
-//             memory, read MN-major)
-//   HEAD_DW   rows = classes, columns = voxels: the same with X and W exchanged, P = g (p - [j = y]); a row of P^T is a
-//             class, so db is a sum inside a thread
-// The target's one is taken off in fp32, before the rounding to bf16: behind it a confident voxel (p near 1) would keep
-// nothing but the rounding of p. Rounding: P has 8 significant bits, sums are fp32 everywhere.
+//             memory, read MN-major); the row's g multiplies the finished sum
+//   HEAD_DW   rows = classes, columns = voxels: the same with X and W exchanged, P = u (p - [j = y]); a row of P^T is a
+//             class, so db is a sum inside a thread; dL / sum u multiplies the finished sums
 //
-// Roles: warp 0 loads (TMA), warp 1 issues MMAs, warps 2-9 are two epilogue groups that share a tile's 128 rows and
-// take one half of its columns each. Column parameters (bias; log-sum-exp, weight and label of a voxel) travel with
-// their tile as bulk copies. All waits are bounded.
-#include "common.cuh"
+// Roundings. P has 8 significant bits, all sums are fp32. The target's one is taken off in fp32, before the rounding:
+// behind it a confident voxel (p near 1) would keep nothing but the rounding of p. Common factors stay out of P, so that
+// a target's entry is near -1 (exact when p is small) instead of -1 / V, whose rounding error all voxels would share.
+// Where one rounding can make up a result (LO: up to HD_FEW voxels; class weights in HEAD_DW, whose rounding the voxels
+// of a class share) P is kept as two bf16, value and remainder, and the second MMA runs once for each.
+//
+// Roles: warp 0 loads (TMA), warp 1 issues MMAs, warps 2-17 are the epilogue: four groups of four warps, a group takes
+// the even or the odd tiles and one half of their columns. In HEAD_DW the voxels' labels travel with their tile as bulk
+// copies. The first MMAs run ahead of the epilogue by all tiles of s that tensor memory holds; a tile's second MMA is
+// issued when the buffer is wanted again. All waits are bounded.
 #include "head_loss.cuh"
 
 namespace sb {
 
-constexpr int HD_THREADS = 320;
-constexpr int HD_EPI_WARPS = 8;
+constexpr int HD_EPI_WARPS = 16;
+constexpr int HD_THREADS = 64 + 32 * HD_EPI_WARPS;
 constexpr int HD_TILE = 128;
 constexpr int HD_BOX = HD_TILE * 128;  // bytes of a 128-row box of 64 channels
+constexpr int HD_BOX16 = HD_TILE * 32; // and of the sixteen columns more
 constexpr int HD_MAX_STAGES = 4;
 constexpr int HD_MAX_C = 256;          // TMEM: two or three tiles of s and the accumulator in 512 columns
+
 enum HeadMode { HEAD_FWD = 0, HEAD_DX = 1, HEAD_DW = 2 };
 
 struct HeadParams {
-  CUtensorMap mapR, mapQ;
-  const float* colp;    // [cols, padded to 128] FWD / DX: bias log2(e) (-inf behind the last class); DW: log2-sum-exp less log2 g
-  const float* colg;    // DW: g
+  CUtensorMap mapR, mapQ, mapR16, mapQ16;  // rows and columns, and their sixteen columns more
   const int* coly;      // DW: label (-1: none)
-  const float* rowp;    // DX: log2-sum-exp; DW: bias log2(e)
+  const float* roww;    // DW: class weight of a row, or null
   const float* rowg;    // DX: g
   const int* rowy;      // FWD / DX: label
   float2* part;         // FWD: [splits][rows padded] running maximum and sum
   float* tl;            // FWD: [rows padded] t at the label
   __nv_bfloat16* out;   // DX with one split: [rows][C]
   float* ws;            // DX / DW: [splits][rows padded][cpad]
-  float* ws_b;          // DW: [2 splits][rows padded]
+  float* ws_b;          // DW: [4 splits][rows padded]
   uint32_t* status;
   long long rows, cols, rows_pad;
   int C, cpad, kboxes, ksteps;
@@ -76,37 +85,54 @@ __device__ __forceinline__ void hd_bulk(void* dst, const void* src, uint32_t byt
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-template <int MODE>
+
+template <int MODE, bool LO>
 __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_constant__ HeadParams p) {
   constexpr int MAXB = 4;
-  constexpr int NPAR = MODE == HEAD_DW ? 3 : 1;  // column parameter arrays per tile
   const uint32_t NB = (uint32_t)p.bufs;          // tiles of s in tensor memory
   const uint32_t ACC = NB * HD_TILE;             // column of the accumulator
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t r_full[2], r_empty[2], q_full[HD_MAX_STAGES], q_empty[HD_MAX_STAGES], s_full[MAXB], s_done[MAXB],
       s_free[MAXB], acc_full, acc_empty;
-  __shared__ float s_m[HD_TILE], s_s[HD_TILE], s_t[HD_TILE];
+  __shared__ uint32_t s_hits[MODE == HEAD_DW ? HD_EPI_WARPS : 1][32];
+  __shared__ float s_fwd[MODE == HEAD_FWD ? 2 : 1][3][MODE == HEAD_FWD ? 4 : 1][HD_TILE];
   __shared__ uint32_t tmem_base_s, abort_s;
   volatile uint32_t* abort_flag = &abort_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int jobs = p.row_tiles * p.splits;
-  const uint32_t tile_bytes = (uint32_t)p.kboxes * HD_BOX;
+  const uint32_t box16 = (uint32_t)p.kboxes * HD_BOX;  // where the sixteen columns more are
+  const uint32_t tile_bytes = box16 + HD_BOX16;
   uint8_t* smem_r = smem;
   uint8_t* smem_q = smem + (size_t)p.rbufs * tile_bytes;
-  float* smem_p = reinterpret_cast<float*>(smem_q + (size_t)p.stages * tile_bytes);  // [stages][NPAR][128]
+  int* smem_y = reinterpret_cast<int*>(smem_q + (size_t)p.stages * tile_bytes);  // DW: [stages][128]
 
   if (threadIdx.x == 0) {
     abort_s = 0;
     for (int i = 0; i < 2; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], 1); }
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], MODE == HEAD_FWD ? 1 + HD_EPI_WARPS : 1);
+      mbar_init(&q_empty[i], MODE == HEAD_FWD ? 1 + HD_EPI_WARPS / 2 : 1);
     }
-    for (int i = 0; i < MAXB; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_done[i], HD_EPI_WARPS); mbar_init(&s_free[i], 1); }
+    for (int i = 0; i < MAXB; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_done[i], HD_EPI_WARPS / 2);
+      mbar_init(&s_free[i], 1);
+    }
     mbar_init(&acc_full, 1);
     mbar_init(&acc_empty, HD_EPI_WARPS);
     mbar_fence_init();
+  }
+  if (MODE == HEAD_FWD && threadIdx.x < HD_TILE) {
+    // the rows' columns more: ones against the three parts of the bias (32-byte rows, 16-byte halves exchanged in every
+    // second group of four rows: the 32-byte swizzle)
+    for (int b = 0; b < p.rbufs; ++b) {
+      uint4* at = reinterpret_cast<uint4*>(smem_r + b * tile_bytes + box16 + threadIdx.x * 32);
+      const int half = (threadIdx.x >> 2) & 1;
+      at[half] = make_uint4(0x3F803F80u, 0x00003F80u, 0u, 0u);
+      at[half ^ 1] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async();
   }
   if (warp == 0) {
     tmem_alloc(&tmem_base_s, 512);
@@ -132,21 +158,20 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         const int t0 = sp * p.tiles_per_split;
         const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
         if (!mbar_wait(&r_empty[rb], rph ^ 1u, abort_flag, p.status, 91)) break;
-        mbar_expect_tx(&r_full[rb], tile_bytes);
+        mbar_expect_tx(&r_full[rb], MODE == HEAD_FWD ? box16 : tile_bytes);
         for (int k = 0; k < p.kboxes; ++k)
           hd_tma_2d(smem_r + rb * tile_bytes + k * HD_BOX, &p.mapR, &r_full[rb], k * 64, rt * HD_TILE);
+        if (MODE != HEAD_FWD)
+          hd_tma_2d(smem_r + rb * tile_bytes + box16, &p.mapR16, &r_full[rb], 0, rt * HD_TILE);
         if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
         for (int t = t0; t < t1; ++t) {
           if (!mbar_wait(&q_empty[st], ph ^ 1u, abort_flag, p.status, 91)) { ok = false; break; }
-          mbar_expect_tx(&q_full[st], tile_bytes + NPAR * HD_TILE * 4);
+          mbar_expect_tx(&q_full[st], tile_bytes + (MODE == HEAD_DW ? HD_TILE * 4 : 0));
           for (int k = 0; k < p.kboxes; ++k)
             hd_tma_2d(smem_q + st * tile_bytes + k * HD_BOX, &p.mapQ, &q_full[st], k * 64, t * HD_TILE);
-          float* par = smem_p + st * NPAR * HD_TILE;
-          hd_bulk(par, p.colp + (long long)t * HD_TILE, HD_TILE * 4, &q_full[st]);
-          if (MODE == HEAD_DW) {
-            hd_bulk(par + HD_TILE, p.colg + (long long)t * HD_TILE, HD_TILE * 4, &q_full[st]);
-            hd_bulk(par + 2 * HD_TILE, p.coly + (long long)t * HD_TILE, HD_TILE * 4, &q_full[st]);
-          }
+          hd_tma_2d(smem_q + st * tile_bytes + box16, &p.mapQ16, &q_full[st], 0, t * HD_TILE);
+          if (MODE == HEAD_DW)
+            hd_bulk(smem_y + st * HD_TILE, p.coly + (long long)t * HD_TILE, HD_TILE * 4, &q_full[st]);
           if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
         }
       }
@@ -156,31 +181,41 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
     const uint32_t hi = desc_hi(8u * 128u, 2u);
     const uint32_t r0 = smem_u32(smem_r), q0 = smem_u32(smem_q);
     const uint32_t idesc2 = make_idesc_bf16(128, p.cpad, 0, 1);
+    const uint32_t ahead = NB < (uint32_t)p.stages ? NB : (uint32_t)p.stages;
     const uint32_t lbo = p.kboxes > 1 ? (uint32_t)HD_BOX : 0u;
+    const uint32_t hi16 = desc_hi(8u * 32u, 6u);
     uint32_t rb = 0, rph = 0, st = 0, ph = 0, b = 0, bph = 0, aph = 0;
-    // the tile whose P is still to be multiplied
-    bool have = false, prev_first = false, prev_last = false;
-    uint32_t prev_st = 0, prev_b = 0, prev_bph = 0;
-    int prev_cols = 0;
+    // tiles whose P is still to be multiplied, oldest first: stage and buffer (with its phase) follow those of the first
+    // MMAs, `flags` has two bits a tile (first, last of its job) and `cols` eight (columns / 16)
+    uint32_t waiting = 0, w_st = 0, w_b = 0, w_bph = 0, flags = 0, cols = 0;
     bool ok = true;
     auto second = [&]() -> bool {
-      if (prev_first) {
+      const bool first = flags & 1u, last = flags & 2u;
+      const int ksteps = (int)(cols & 255u);
+      if (first) {
         if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty, aph ^ 1u, abort_flag, p.status, 92))) return false;
         aph ^= 1u;
       }
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_done[prev_b], prev_bph, abort_flag, p.status, 93))) return false;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_done[w_b], w_bph, abort_flag, p.status, 93))) return false;
       tc_fence_after();
       if (leader) {
-        const uint32_t lo = desc_lo(q0 + prev_st * tile_bytes, lbo);
-        const uint32_t a = tmem + prev_b * HD_TILE;
-        for (int k = 0; k < prev_cols / 16; ++k)
-          hd_mma_ts(tmem + ACC, a + (k < 4 ? 8 * k : 32 + 8 * k), lo + k * 128u, hi, idesc2,
-                    prev_first && k == 0 ? 0u : 1u);
-        tc_commit(&q_empty[prev_st]);
-        tc_commit(&s_free[prev_b]);
-        if (prev_last) tc_commit(&acc_full);
+        const uint32_t lo = desc_lo(q0 + w_st * tile_bytes, lbo);
+        const uint32_t a = tmem + w_b * HD_TILE;
+#pragma unroll
+        for (int part = 0; part < (LO ? 2 : 1); ++part)
+          for (int k = 0; k < ksteps; ++k)
+            hd_mma_ts(tmem + ACC, a + 32 * (k >> 1) + 16 * part + 8 * (k & 1), lo + k * 128u, hi, idesc2,
+                      first && part == 0 && k == 0 ? 0u : 1u);
+        tc_commit(&q_empty[w_st]);
+        tc_commit(&s_free[w_b]);
+        if (last) tc_commit(&acc_full);
       }
       __syncwarp();
+      if (++w_st == (uint32_t)p.stages) w_st = 0;
+      if (++w_b == NB) { w_b = 0; w_bph ^= 1u; }
+      flags >>= 2;
+      cols >>= 8;
+      --waiting;
       return true;
     };
     for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
@@ -189,6 +224,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
       if (!__all_sync(0xffffffffu, mbar_wait(&r_full[rb], rph, abort_flag, p.status, 94))) { ok = false; break; }
       for (int t = t0; t < t1; ++t) {
+        // as many tiles as there are buffers (and stages) are on their way: the oldest one's second MMA frees both
+        if (MODE != HEAD_FWD && waiting == ahead && !second()) { ok = false; break; }
         if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95))) { ok = false; break; }
         // the buffer is free: read by the epilogue (FWD), or its P read by the second MMA that used it
         uint64_t* bar = MODE == HEAD_FWD ? &s_done[b] : &s_free[b];
@@ -197,34 +234,36 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         const int nc = cols_of(t);
         if (leader) {
           const uint32_t idesc = make_idesc_bf16(128, nc, 0, 0);
-          const uint32_t a_lo = desc_lo(r0 + rb * tile_bytes, 16u), b_lo = desc_lo(q0 + st * tile_bytes, 16u);
+          const uint32_t a0 = r0 + rb * tile_bytes, b0 = q0 + st * tile_bytes;
+          const uint32_t a_lo = desc_lo(a0, 16u), b_lo = desc_lo(b0, 16u);
           for (int k = 0; k < p.ksteps; ++k) {
             const uint32_t off = (uint32_t)(k >> 2) * (HD_BOX >> 4) + (uint32_t)(k & 3) * 2u;
             tc_mma_bf16_pred(tmem + b * HD_TILE, a_lo + off, hi, b_lo + off, hi, idesc, k != 0 ? 1u : 0u);
           }
+          tc_mma_bf16_pred(tmem + b * HD_TILE, desc_lo(a0 + box16, 16u), hi16, desc_lo(b0 + box16, 16u), hi16, idesc, 1u);
           tc_commit(&s_full[b]);
           if (MODE == HEAD_FWD) tc_commit(&q_empty[st]);
           if (t == t1 - 1) tc_commit(&r_empty[rb]);
         }
         __syncwarp();
         if (MODE != HEAD_FWD) {
-          if (have && !second()) { ok = false; break; }
-          have = true;
-          prev_first = t == t0;
-          prev_last = t == t1 - 1;
-          prev_st = st; prev_b = b; prev_bph = bph; prev_cols = nc;
+          flags |= ((t == t0 ? 1u : 0u) | (t == t1 - 1 ? 2u : 0u)) << (2 * waiting);
+          cols |= (uint32_t)(nc / 16) << (8 * waiting);
+          ++waiting;
         }
         if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
         if (++b == NB) { b = 0; bph ^= 1u; }
       }
       if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
     }
-    if (MODE != HEAD_FWD && ok && have) second();
+    if (MODE != HEAD_FWD)
+      while (ok && waiting > 0) ok = second();
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const int quad = warp & 3, group = (warp - 2) >> 2, half = group & 1;
+    const uint32_t par = group >> 1;
     const int row = quad * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    uint32_t st = 0, ph = 0, b = 0, bph = 0, aph = 0;
+    uint32_t st = 0, ph = 0, b = 0, bph = 0, aph = 0, tc = 0, jc = 0;
     bool ok = true, pending = false;
     int pend_rt = 0, pend_sp = 0;
     float pend_g = 0.f, pend_db = 0.f;
@@ -234,7 +273,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       aph ^= 1u;
       tc_fence_after();
       const long long r = (long long)pend_rt * HD_TILE + row;
-      for (int c0 = half * 16; c0 < p.cpad; c0 += 32) {
+      for (int c0 = group * 16; c0 < p.cpad; c0 += 64) {
         uint32_t v[16];
         tmem_ld_32x16(lane_base + ACC + c0, v);
         tmem_ld_wait();
@@ -261,129 +300,148 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
           for (int j = 0; j < 4; ++j) dst[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
         }
       }
-      if (MODE == HEAD_DW) p.ws_b[((long long)pend_sp * 2 + half) * p.rows_pad + r] = pend_db;
+      if (MODE == HEAD_DW) p.ws_b[((long long)pend_sp * 4 + group) * p.rows_pad + r] = pend_db;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty);
       return true;
     };
-    for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
+    // a row's own values; the next job's are read while this one runs
+    auto row_at = [&](int job) { return (long long)(job % p.row_tiles) * HD_TILE + row; };
+    int y_next = -1;
+    float g_next = 1.f;
+    auto fetch = [&](int job) {
+      if (job >= jobs) return;
+      const long long r = row_at(job);
+      if (MODE != HEAD_DW) y_next = __ldg(p.rowy + r);
+      if (MODE == HEAD_DX) g_next = __ldg(p.rowg + r);
+      if (MODE == HEAD_DW && p.roww != nullptr && r < p.rows) g_next = __ldg(p.roww + r);
+    };
+    fetch(blockIdx.x);
+    for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x, ++jc) {
       const int rt = job % p.row_tiles, sp = job / p.row_tiles;
       const int t0 = sp * p.tiles_per_split;
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
       const long long r = (long long)rt * HD_TILE + row;
-      int y = -1;
-      float rp = 0.f, g = 0.f, db = 0.f;
-      if (MODE != HEAD_DW) y = p.rowy[r];
-      if (MODE != HEAD_FWD) rp = p.rowp[r];
-      if (MODE == HEAD_DX) g = p.rowg[r];
-      float m = -INFINITY, s = 0.f, tl = 0.f;
-      for (int t = t0; t < t1; ++t) {
-        if (!mbar_wait(&q_full[st], ph, abort_flag, p.status, 98) ||
-            !mbar_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
-        tc_fence_after();
-        const float* par = smem_p + st * NPAR * HD_TILE + half * 64;
-        const int nc = cols_of(t) - half * 64;  // this group's columns: none, 32 or (64 and more) 64
-        const int c_abs = t * HD_TILE + half * 64;
+      const int y = y_next;
+      const float g = g_next;
+      fetch(job + gridDim.x);
+      float m = HD_LOWEST, s = 0.f, tl = 0.f, db = 0.f;
+      for (int t = t0; t < t1; ++t, ++tc) {
+        if ((tc & 1u) == par) {
+          if (!mbar_wait(&q_full[st], ph, abort_flag, p.status, 98) ||
+              !mbar_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
+          tc_fence_after();
+          const int nc = cols_of(t) - half * 64;  // this group's columns: none, 32 or (64 and more) 64
+          const int c_abs = t * HD_TILE + half * 64;
+          const uint32_t tile = lane_base + b * HD_TILE + half * 64;
 #pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 32) {
-          if (c0 >= nc) break;
-          uint32_t v[32];
-          tmem_ld_32x32(lane_base + b * HD_TILE + half * 64 + c0, v);
-          tmem_ld_wait();
-          float f[32];
+          for (int c0 = 0; c0 < 64; c0 += 32) {
+            if (c0 >= nc) break;
+            uint32_t v[32];
+            tmem_ld_32x32(tile + c0, v);
+            tmem_ld_wait();
+            float f[32];
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 cp = *reinterpret_cast<const float4*>(par + c0 + j);
-            const float cv[4] = {cp.x, cp.y, cp.z, cp.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float add = MODE == HEAD_FWD ? cv[i] : MODE == HEAD_DX ? cv[i] - rp : rp - cv[i];
-              f[j + i] = fmaf(__uint_as_float(v[j + i]), HD_LOG2E, add);
-            }
-          }
-          if (MODE == HEAD_FWD) {
-            const int at = y - (c_abs + c0);
-            if ((unsigned)at < 32u) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) tl = j == at ? f[j] : tl;
-            }
-            float mx = f[0];
-#pragma unroll
-            for (int j = 1; j < 32; ++j) mx = fmaxf(mx, f[j]);
-            if (mx > m) {
-              s *= hd_ex2(m - mx);  // m = -inf: 0 * 0
-              m = mx;
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              a0 += hd_ex2(f[j] - base);
-              a1 += hd_ex2(f[j + 1] - base);
-              a2 += hd_ex2(f[j + 2] - base);
-              a3 += hd_ex2(f[j + 3] - base);
-            }
-            s += (a0 + a1) + (a2 + a3);
-          } else {
-            uint32_t o[16];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = hd_ex2(f[j]);
-            if (MODE == HEAD_DX) {
+            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+            // bit j: column j is the row's label
+            uint32_t hits;
+            if (MODE != HEAD_DW) {
               const int at = y - (c_abs + c0);
-              if ((unsigned)at < 32u) {
+              hits = (unsigned)at < 32u ? 1u << at : 0u;
+            } else {
+              // lane c looks at the label of column c; the lanes of one label know each other's columns
+              const int rel = smem_y[st * HD_TILE + half * 64 + c0 + lane] - (int)(r - lane);
+              const uint32_t same = __match_any_sync(0xffffffffu, rel);
+              uint32_t* mine = s_hits[warp - 2];
+              mine[lane] = 0u;
+              __syncwarp();
+              if ((unsigned)rel < 32u) mine[rel] = same;
+              __syncwarp();
+              hits = mine[lane];
+              __syncwarp();
+            }
+            const bool any = __any_sync(0xffffffffu, hits != 0u);
+            if (MODE == HEAD_FWD) {
+              if (any) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                  if (j == at) f[j] -= 1.f;
+                  if (hits & (1u << j)) tl = f[j];
               }
+              float mx[4] = {f[0], f[1], f[2], f[3]};
+#pragma unroll
+              for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], f[j]);
+              const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+              if (top > m) {
+                s *= hd_ex2((m - top) * HD_LOG2E);
+                m = top;
+              }
+              const float base = -m * HD_LOG2E;
+              float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int j = 0; j < 32; ++j) a[j & 3] += hd_ex2(fmaf(f[j], HD_LOG2E, base));
+              s += (a[0] + a[1]) + (a[2] + a[3]);
             } else {
-              float d0 = 0.f, d1 = 0.f, d2 = 0.f, d3 = 0.f;
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 cg = *reinterpret_cast<const float4*>(par + HD_TILE + c0 + j);
-                const int4 cy = *reinterpret_cast<const int4*>(par + 2 * HD_TILE + c0 + j);
-                if (cy.x == (int)r) f[j] -= cg.x;
-                if (cy.y == (int)r) f[j + 1] -= cg.y;
-                if (cy.z == (int)r) f[j + 2] -= cg.z;
-                if (cy.w == (int)r) f[j + 3] -= cg.w;
-                d0 += f[j]; d1 += f[j + 1]; d2 += f[j + 2]; d3 += f[j + 3];
+              for (int j = 0; j < 32; ++j) f[j] = hd_ex2(f[j] * HD_LOG2E);
+              if (any) {
+                const float one = MODE == HEAD_DW ? g : 1.f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (hits & (1u << j)) f[j] -= one;
               }
-              db += (d0 + d1) + (d2 + d3);
-            }
+              if (MODE == HEAD_DW) {
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
-            // over the columns of s that this thread has read: the second chunk's are still behind them
-            hd_tmem_st_x16(lane_base + b * HD_TILE + half * 64 + c0 / 2, o);
+                for (int j = 0; j < 32; ++j) d[j & 3] += f[j];
+                db += (d[0] + d[1]) + (d[2] + d[3]);
+              }
+              uint32_t o[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+              // over the 32 columns of s that this thread has just read: 16 columns of P, 16 of its remainder
+              hd_tmem_st_x16(tile + c0, o);
+              if (LO) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  o[j] = pack_bf16x2(f[2 * j] - __uint_as_float(o[j] << 16),
+                                     f[2 * j + 1] - __uint_as_float(o[j] & 0xFFFF0000u));
+                hd_tmem_st_x16(tile + c0 + 16, o);
+              }
+            }
           }
-        }
-        if (MODE != HEAD_FWD) hd_tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&s_done[b]);
-          if (MODE == HEAD_FWD) mbar_arrive(&q_empty[st]);
+          if (MODE != HEAD_FWD) hd_tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&s_done[b]);
+            if (MODE == HEAD_FWD) mbar_arrive(&q_empty[st]);
+          }
+          if (MODE != HEAD_FWD && pending) {
+            if (!drain()) { ok = false; break; }
+            pending = false;
+          }
         }
         if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
         if (++b == NB) { b = 0; bph ^= 1u; }
-        if (MODE != HEAD_FWD && pending) {
-          if (!drain()) { ok = false; break; }
-          pending = false;
-        }
       }
       if (MODE == HEAD_FWD) {
-        // the two halves of the columns
-        if (half == 1) { s_m[row] = m; s_s[row] = s; s_t[row] = tl; }
-        ok = hd_epi_vote(ok);
-        if (half == 0 && ok) {
-          const float m1 = s_m[row], mm = fmaxf(m, m1);
-          const float base = mm == -INFINITY ? 0.f : mm;
-          const float ss = s * hd_ex2(m - base) + s_s[row] * hd_ex2(m1 - base);
-          p.part[(long long)sp * p.rows_pad + r] = make_float2(mm, ss);
-          const long long c_lo = (long long)t0 * HD_TILE, c_hi = (long long)t1 * HD_TILE;
-          if (y >= c_lo && y < c_hi) p.tl[r] = (y & (HD_TILE - 1)) < 64 ? tl : s_t[row];
+        // the four groups' shares of a row; two sets of buffers, so that a group that is a job ahead overwrites nothing
+        const int set = jc & 1;
+        s_fwd[set][0][group][row] = m;
+        s_fwd[set][1][group][row] = s;
+        s_fwd[set][2][group][row] = tl;
+        ok = hd_vote(1 + quad, 128, ok);
+        if (group == 0 && ok) {
+          for (int k = 1; k < 4; ++k) m = fmaxf(m, s_fwd[set][0][k][row]);
+          s = 0.f;
+          for (int k = 0; k < 4; ++k) s += s_fwd[set][1][k][row] * hd_ex2((s_fwd[set][0][k][row] - m) * HD_LOG2E);
+          for (int k = 1; k < 4; ++k) tl += s_fwd[set][2][k][row];  // one of them has met the label, the others hold 0
+          p.part[(long long)sp * p.rows_pad + r] = make_float2(m * HD_LOG2E, s);
+          if (y >= (long long)t0 * HD_TILE && y < (long long)t1 * HD_TILE) p.tl[r] = tl * HD_LOG2E;
         }
-        hd_epi_vote(true);  // the merge has read what the next job's will overwrite
       } else {
+        if (ok && pending) ok = drain();  // this job had no tile for this group
         pending = true;
         pend_rt = rt; pend_sp = sp; pend_g = g; pend_db = db;
       }
@@ -412,13 +470,27 @@ __device__ __forceinline__ long long hd_label(const void* labels, int kind, long
   return reinterpret_cast<const long long*>(labels)[i];
 }
 
+// a number as three bf16 that add up to it (two in the first word, one in the second)
+__device__ __forceinline__ uint2 hd_three(float v) {
+  const __nv_bfloat16 a = __float2bfloat16(v);
+  float rest = v - __bfloat162float(a);
+  if (!isfinite(rest)) rest = 0.f;  // an infinity or a NaN is all in the first
+  const __nv_bfloat16 b = __float2bfloat16(rest), c = __float2bfloat16(rest - __bfloat162float(b));
+  return make_uint2((uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16,
+                    (uint32_t)__bfloat16_as_ushort(c));
+}
+constexpr uint32_t HD_ONE = 0x3F80u;  // 1 in bf16
+
 // y[i]: the label, or -1 for a voxel that takes no part (the ignored label; one outside the classes, which is reported)
-// and behind the last voxel; bias2[j] = bias_j log2(e), -inf behind the last class
+// and behind the last voxel; bias2[j] = bias_j log2(e), -inf behind the last class. w16 (narrow heads): a class's sixteen
+// columns more, b in three parts against ones, then ones against -lse and (second array) log u. What is off stands as
+// HD_LOWEST instead of -inf: zeros of the other side must not make a NaN of it.
 __global__ void __launch_bounds__(256) head_prep_kernel(const void* __restrict__ labels, int kind, long long V,
                                                         long long v_pad, int K, int k_pad, int has_ignore,
                                                         long long ignore, int* __restrict__ y,
                                                         const void* __restrict__ bias, int bias_kind,
-                                                        float* __restrict__ bias2, uint32_t* __restrict__ status) {
+                                                        float* __restrict__ bias2, uint4* __restrict__ w16,
+                                                        uint32_t* __restrict__ status) {
   const long long n = v_pad > k_pad ? v_pad : k_pad;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     if (i < v_pad) {
@@ -436,9 +508,17 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const void* __restrict__
       float b = -INFINITY;
       if (i < K)
         b = bias == nullptr ? 0.f
-            : bias_kind == 0 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(bias)[i]) * HD_LOG2E
-                             : reinterpret_cast<const float*>(bias)[i] * HD_LOG2E;
-      bias2[i] = b;
+            : bias_kind == 0 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(bias)[i])
+                             : reinterpret_cast<const float*>(bias)[i];
+      bias2[i] = b * HD_LOG2E;
+      if (w16 != nullptr) {
+        const uint2 t = hd_three(b < HD_LOWEST ? HD_LOWEST : b);
+        for (int k = 0; k < 2; ++k) {
+          uint4* at = w16 + 2 * ((long long)k * k_pad + i);
+          at[0] = make_uint4(t.x, t.y | HD_ONE << 16, HD_ONE | HD_ONE << 16, k ? HD_ONE | HD_ONE << 16 : 0u);
+          at[1] = make_uint4(k ? HD_ONE : 0u, 0u, 0u, 0u);
+        }
+      }
     }
   }
 }
@@ -471,13 +551,14 @@ __global__ void __launch_bounds__(256) head_merge_kernel(const float2* __restric
     float l = INFINITY;
     if (i < V) {
       float m = -INFINITY, s = 0.f;
+#pragma unroll 4
       for (int k = 0; k < splits; ++k) {
         const float2 e = part[(long long)k * v_pad + i];
         const float mm = fmaxf(m, e.x), base = mm == -INFINITY ? 0.f : mm;
         s = s * hd_ex2(m - base) + e.y * hd_ex2(e.x - base);
         m = mm;
       }
-      l = m + log2f(s);
+      l = m < 0.1f * HD_LOWEST ? NAN : m + log2f(s);  // every class is off: 0 / 0
       const int c = y[i];
       if (c >= 0) {
         const float u = cw == nullptr ? 1.f : cw[c];
@@ -507,35 +588,56 @@ __global__ void __launch_bounds__(256) head_total_kernel(const double* __restric
   }
 }
 
-// g[i] = dL u_i / den and lse2 - log2 g (so that exp2(t - it) = g p), 0 and +inf where a voxel takes no part
-__global__ void __launch_bounds__(256) head_weights_kernel(const float* __restrict__ lse2, const int* __restrict__ y,
-                                                           const float* __restrict__ cw, const float* __restrict__ gout,
-                                                           const float* __restrict__ den, long long v_pad,
-                                                           float* __restrict__ g, float* __restrict__ lse2g) {
-  const float k = gout[0] / den[0];
+// what the backward passes need of a voxel; x16 (narrow heads): its sixteen columns more
+__global__ void __launch_bounds__(256) head_weights_kernel(HeadCall a, const float* __restrict__ gout, long long v_pad) {
+  const float k = gout[0] / a.den[0];
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.scale[0] = k;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < v_pad; i += (long long)gridDim.x * 256) {
-    const int c = y[i];
-    const float gi = c < 0 ? 0.f : k * (cw == nullptr ? 1.f : cw[c]);
-    g[i] = gi;
-    lse2g[i] = gi == 0.f ? INFINITY : lse2[i] - log2f(gi);
+    const int c = a.y[i];
+    const float u = c < 0 ? 0.f : a.cw == nullptr ? 1.f : a.cw[c], l = a.lse2[i];
+    a.g[i] = u == 0.f ? 0.f : k * u;
+    if (a.x16 == nullptr) {
+      a.u[i] = u;
+      a.lse2p[i] = u == 0.f ? INFINITY : l;
+    } else {
+      const uint2 t = hd_three(u == 0.f ? HD_LOWEST : -l * HD_LN2), v = hd_three(u == 0.f ? 0.f : logf(u));
+      uint4* at = a.x16 + 2 * i;
+      at[0] = make_uint4(HD_ONE | HD_ONE << 16, HD_ONE | t.x << 16, t.x >> 16 | t.y << 16, v.x);
+      at[1] = make_uint4(v.y, 0u, 0u, 0u);
+    }
   }
 }
 
-// out[r][c] = sum over the slices of ws[slice][rows_pad][ld], in slice order; r < rows, c < C
+// out[r][c] = scale * sum over the slices of ws[slice][rows_pad][ld], in slice order; r < rows, c < C. A block takes 32
+// neighbouring outputs, each of its eight warps every eighth slice: a thread that walks all slices waits an L2 trip for
+// a few of them at a time.
 template <typename T>
 __global__ void __launch_bounds__(256) head_reduce_kernel(const float* __restrict__ ws, int slices, long long rows,
-                                                          long long rows_pad, int C, int ld, T* __restrict__ out) {
-  const long long n = rows * C;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const long long r = i / C;
-    const int c = (int)(i - r * C);
-    const float* src = ws + r * ld + c;
+                                                          long long rows_pad, int C, int ld,
+                                                          const float* __restrict__ scale, T* __restrict__ out) {
+  __shared__ float s_part[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long n = rows * C, slice = rows_pad * ld;
+  const float k = scale != nullptr ? scale[0] : 1.f;
+  for (long long i0 = (long long)blockIdx.x * 32; i0 < n; i0 += (long long)gridDim.x * 32) {
+    const long long i = i0 + lane;
     float a = 0.f;
+    if (i < n) {
+      const float* src = ws + i / C * ld + i % C;
 #pragma unroll 4
-    for (int k = 0; k < slices; ++k) a += src[(long long)k * rows_pad * ld];
-    out[i] = hd_cast<T>(a);
+      for (int s = warp; s < slices; s += 8) a += src[s * slice];
+    }
+    s_part[warp][lane] = a;
+    __syncthreads();
+    if (warp == 0 && i < n) {
+      for (int w = 1; w < 8; ++w) a += s_part[w][lane];
+      out[i] = hd_cast<T>(a * k);
+    }
+    __syncthreads();
   }
 }
+
+static bool wide(const HeadCall& a) { return a.C > HD_MAX_C; }
 
 static int hd_blocks(long long n, int per_sm) {
   const long long b = (n + 255) / 256;
@@ -553,43 +655,147 @@ static void head_split(int row_tiles, int col_tiles, int* splits, int* tps) {
   }
 }
 
-static void head_geometry(const SbHeadArgs* a, int mode, HeadParams& p) {
+static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
   memset(&p, 0, sizeof(p));
-  p.C = a->C;
-  p.cpad = (a->C + 15) / 16 * 16;
-  p.kboxes = (a->C + 63) / 64;
+  p.C = a.C;
+  p.cpad = (a.C + 15) / 16 * 16;
+  p.kboxes = (a.C + 63) / 64;
   p.ksteps = p.cpad / 16;
-  p.rows = mode == HEAD_DW ? a->K : a->V;
-  p.cols = mode == HEAD_DW ? a->V : a->K;
+  p.rows = mode == HEAD_DW ? a.K : a.V;
+  p.cols = mode == HEAD_DW ? a.V : a.K;
   p.row_tiles = (int)((p.rows + HD_TILE - 1) / HD_TILE);
   p.col_tiles = (int)((p.cols + HD_TILE - 1) / HD_TILE);
-  p.rows_pad = (p.rows + HD_PAD - 1) / HD_PAD * HD_PAD;
+  p.rows_pad = hd_pad(p.rows);
   head_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
   p.bufs = mode == HEAD_FWD ? 4 : p.cpad <= 128 ? 3 : 2;
-  // shared memory: 12 boxes of 16 KB (kboxes per tile); one or two resident tiles and two to four in the ring
-  p.rbufs = p.kboxes <= 2 ? 2 : 1;
-  p.stages = 12 / p.kboxes - p.rbufs;
-  if (p.stages > HD_MAX_STAGES) p.stages = HD_MAX_STAGES;
-  p.status = a->status;
+  // shared memory: tiles of kboxes * 16 + 4 KB, one or two resident ones and two to four in the ring
+  p.rbufs = p.kboxes == 1 ? 2 : 1;
+  p.stages = p.kboxes <= 2 ? 4 : p.kboxes == 3 ? 3 : 2;
+  p.status = a.status;
 }
 
-template <int MODE>
-static int head_launch(const SbHeadArgs* a, HeadParams& p, cudaStream_t stream) {
-  const void* x = a->x;
-  const void* w = a->w;
-  const long long dv[2] = {a->C, a->V}, dk[2] = {a->C, a->K}, st[2] = {1, a->C};
+template <int MODE, bool LO>
+static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
+  const long long dv[2] = {a.C, a.V}, dk[2] = {a.C, a.K}, st[2] = {1, a.C};
   const int box[2] = {64, HD_TILE};
-  int rc = make_map_bf16(&p.mapR, MODE == HEAD_DW ? w : x, 2, MODE == HEAD_DW ? dk : dv, st, box, 128);
+  const bool dw = MODE == HEAD_DW;
+  int rc = make_map_bf16(&p.mapR, dw ? a.w : a.x, 2, dw ? dk : dv, st, box, 128);
   if (rc) return rc;
-  rc = make_map_bf16(&p.mapQ, MODE == HEAD_DW ? x : w, 2, MODE == HEAD_DW ? dv : dk, st, box, 128);
+  rc = make_map_bf16(&p.mapQ, dw ? a.x : a.w, 2, dw ? dv : dk, st, box, 128);
   if (rc) return rc;
-  const size_t smem = 1024 + (size_t)(p.rbufs + p.stages) * p.kboxes * HD_BOX + (size_t)p.stages * 3 * HD_TILE * 4;
-  if (cudaFuncSetAttribute(head_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 4096) !=
-      cudaSuccess)
+  const long long st16[2] = {1, 16}, xv[2] = {16, hd_pad(a.V)}, wk[2] = {16, hd_pad(a.K)};
+  const int box16[2] = {16, HD_TILE};
+  const uint4* w16 = a.w16 + (dw ? 2 * hd_pad(a.K) : 0);
+  rc = make_map_bf16(&p.mapR16, dw ? w16 : MODE == HEAD_FWD ? w16 : a.x16, 2, dw || MODE == HEAD_FWD ? wk : xv, st16, box16, 32);
+  if (rc) return rc;
+  rc = make_map_bf16(&p.mapQ16, dw ? a.x16 : w16, 2, dw ? xv : wk, st16, box16, 32);
+  if (rc) return rc;
+  constexpr int MOST = 4 * (3 * HD_BOX + HD_BOX16) + 1024 + 4 * HD_TILE * 4;  // three boxes, four tiles
+  const size_t smem = 1024 + (size_t)(p.rbufs + p.stages) * (p.kboxes * HD_BOX + HD_BOX16) + (size_t)p.stages * HD_TILE * 4;
+  if (cudaFuncSetAttribute(head_kernel<MODE, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess)
     return SB_ERR_DRIVER;
   const long long jobs = (long long)p.row_tiles * p.splits;
-  head_kernel<MODE><<<(int)(jobs < 148 ? jobs : 148), HD_THREADS, smem, stream>>>(p);
+  head_kernel<MODE, LO><<<(int)(jobs < 148 ? jobs : 148), HD_THREADS, smem, stream>>>(p);
   sb_count_launch(1);
+  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+}
+
+
+static bool shape_ok(long long V, int K, int C) {
+  return V >= 1 && V <= (1LL << 31) - 512 && K >= 1 && K <= (1 << 30) && C >= 8 && C % 8 == 0 && C <= 32768;
+}
+
+// The forward pass's state and the scratch of each pass, in the caller's memory (256-byte aligned).
+static long long head_state(HeadCall& a, void* base) {
+  char* at = (char*)base;
+  auto take = [&](long long bytes) { char* o = at; at += (bytes + 255) / 256 * 256; return o; };
+  char* head = take(32);
+  a.total = (double*)head;
+  a.den = (float*)(head + 16);
+  a.lse2 = (float*)take(4 * hd_pad(a.V));
+  a.y = (int*)take(4 * hd_pad(a.V));
+  a.bias2 = (float*)take(4 * hd_pad(a.K));
+  if (!wide(a)) a.w16 = (uint4*)take(64 * hd_pad(a.K));
+  return at - (char*)base;
+}
+struct HeadFwdScratch {
+  double* sums;
+  float2* part;
+  float* tl;
+};
+static long long head_fwd_scratch(const HeadCall& a, HeadFwdScratch& f, void* base) {
+  HeadParams p;
+  head_geometry(a, HEAD_FWD, p);
+  const long long splits = wide(a) ? head_wide_splits(a.V, a.K) : p.splits;
+  char* at = (char*)base;
+  auto take = [&](long long bytes) { char* o = at; at += (bytes + 255) / 256 * 256; return o; };
+  f.sums = (double*)take(16LL * HD_SUM_BLOCKS);
+  f.part = (float2*)take(8 * splits * p.rows_pad);
+  f.tl = (float*)take(4 * p.rows_pad);
+  return at - (char*)base;
+}
+static long long head_bwd_scratch(HeadCall& a, void* base) {
+  char* at = (char*)base;
+  auto take = [&](long long bytes) { char* o = at; at += (bytes + 255) / 256 * 256; return o; };
+  a.scale = (float*)take(4);
+  a.g = (float*)take(4 * hd_pad(a.V));
+  if (wide(a)) {
+    a.u = (float*)take(4 * hd_pad(a.V));
+    a.lse2p = (float*)take(4 * hd_pad(a.V));
+  } else {
+    a.x16 = (uint4*)take(32 * hd_pad(a.V));
+  }
+  a.scratch = (float*)at;
+  if (wide(a)) return at - (char*)base + 4 * head_wide_scratch(a);
+  HeadParams p;
+  head_geometry(a, HEAD_DX, p);
+  const long long dx = p.splits == 1 ? 0 : p.splits * p.rows_pad * p.cpad;
+  head_geometry(a, HEAD_DW, p);
+  const long long dw = p.splits * p.rows_pad * (p.cpad + 4);
+  return at - (char*)base + 4 * (dx > dw ? dx : dw);
+}
+
+template <typename T>
+static void head_reduce(const float* ws, int slices, long long rows, long long rows_pad, int C, int ld,
+                        const float* scale, void* out, cudaStream_t stream) {
+  const long long blocks = (rows * C + 31) / 32;
+  head_reduce_kernel<T><<<(int)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(ws, slices, rows, rows_pad, C, ld,
+                                                                                       scale, (T*)out);
+  sb_count_launch(1);
+}
+
+static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
+  HeadParams p;
+  int rc = 0;
+  const bool few = a.V <= HD_FEW;
+  if (a.dx != nullptr) {
+    head_geometry(a, HEAD_DX, p);
+    p.rowg = a.g;
+    p.rowy = a.y;
+    p.out = a.dx;
+    p.ws = a.scratch;
+    rc = few ? head_launch<HEAD_DX, true>(a, p, stream) : head_launch<HEAD_DX, false>(a, p, stream);
+    if (rc) return rc;
+    if (p.splits > 1)
+      head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, nullptr, a.dx, stream);
+  }
+  if (a.dw != nullptr || a.db != nullptr) {
+    head_geometry(a, HEAD_DW, p);
+    p.coly = a.y;
+    p.roww = a.cw;
+    p.ws = a.scratch;
+    p.ws_b = a.scratch + p.splits * p.rows_pad * p.cpad;
+    rc = few || a.cw != nullptr ? head_launch<HEAD_DW, true>(a, p, stream) : head_launch<HEAD_DW, false>(a, p, stream);
+    if (rc) return rc;
+    if (a.dw != nullptr) {
+      if (a.dw_kind == 2) head_reduce<float>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a.scale, a.dw, stream);
+      else head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a.scale, a.dw, stream);
+    }
+    if (a.db != nullptr) {
+      if (a.db_kind == 2) head_reduce<float>(p.ws_b, 4 * p.splits, p.rows, p.rows_pad, 1, 1, a.scale, a.db, stream);
+      else head_reduce<__nv_bfloat16>(p.ws_b, 4 * p.splits, p.rows, p.rows_pad, 1, 1, a.scale, a.db, stream);
+    }
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
@@ -597,117 +803,90 @@ static int head_launch(const SbHeadArgs* a, HeadParams& p, cudaStream_t stream) 
 
 using namespace sb;
 
-static long long pad(long long n) { return (n + HD_PAD - 1) / HD_PAD * HD_PAD; }
-static bool shape_ok(const SbHeadArgs* a) {
-  return a->V >= 1 && a->V <= (1LL << 31) - 512 && a->K >= 1 && a->K <= (1 << 30) && a->C >= 8 && a->C % 8 == 0 &&
-         a->C <= 32768;
-}
-static bool wide(const SbHeadArgs* a) { return a->C > HD_MAX_C; }
-constexpr int HD_SUM_BLOCKS = 148 * 4;
-
-// fp32 scratch of the forward (mode 0) and the backward pass (1); -1: outside the kernels' range
-extern "C" long long sb_head_scratch(const SbHeadArgs* a, int mode) {
-  if (mode < 0 || mode > 1 || !shape_ok(a)) return -1;
-  HeadParams p;
-  if (mode == 0) {
-    head_geometry(a, HEAD_FWD, p);
-    const int splits = wide(a) ? head_wide_splits(a->V, a->K) : p.splits;
-    return 4LL * HD_SUM_BLOCKS + (2LL * splits + 1) * p.rows_pad;
-  }
-  if (wide(a)) return head_wide_scratch(a);
-  head_geometry(a, HEAD_DX, p);
-  const long long dx = p.splits == 1 ? 0 : p.splits * p.rows_pad * p.cpad;
-  head_geometry(a, HEAD_DW, p);
-  const long long dw = p.splits * p.rows_pad * (p.cpad + 2);
-  return dx > dw ? dx : dw;
+// bytes of the state (0) and of the scratch of the forward (1) and the backward pass (2); -1: outside the range
+extern "C" long long sb_head_bytes(int what, long long V, int K, int C, int weighted) {
+  if (!shape_ok(V, K, C) || what < 0 || what > 2) return -1;
+  HeadCall a;
+  memset(&a, 0, sizeof(a));
+  a.V = V;
+  a.K = K;
+  a.C = C;
+  a.cw = weighted ? (const float*)1 : nullptr;  // looked at, not followed
+  HeadFwdScratch f;
+  return what == 0 ? head_state(a, nullptr) : what == 1 ? head_fwd_scratch(a, f, nullptr) : head_bwd_scratch(a, nullptr);
 }
 
-// labels, bias -> y, bias2, lse2, total, loss, den
-extern "C" int sb_head_forward(const SbHeadArgs* a, cudaStream_t stream) {
-  if (!shape_ok(a) || !a->x || !a->w || !a->labels || !a->y || !a->bias2 || !a->lse2 || !a->total || !a->loss ||
-      !a->den || !a->scratch)
-    return SB_ERR_SHAPE;
-  if (a->scratch_floats < sb_head_scratch(a, 0)) return SB_ERR_TOO_LARGE;
-  HeadParams p;
-  head_geometry(a, HEAD_FWD, p);
-  const long long v_pad = pad(a->V);
-  const int k_pad = (int)pad(a->K);
+extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, int bias_kind, const void* labels,
+                               int label_kind, int has_ignore, long long ignore, const float* cw, long long V, int K,
+                               int C, void* state, void* scratch, float* loss, uint32_t* status, cudaStream_t stream) {
+  if (!shape_ok(V, K, C) || !x || !w || !labels || !state || !scratch || !loss) return SB_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(state) | reinterpret_cast<uintptr_t>(scratch)) & 255) return SB_ERR_ALIGN;
+  HeadCall a;
+  memset(&a, 0, sizeof(a));
+  a.x = (const __nv_bfloat16*)x;
+  a.w = (const __nv_bfloat16*)w;
+  a.cw = cw;
+  a.V = V; a.K = K; a.C = C;
+  a.status = status;
+  head_state(a, state);
+  HeadFwdScratch f;
+  head_fwd_scratch(a, f, scratch);
+  const long long v_pad = hd_pad(V);
+  const int k_pad = (int)hd_pad(K);
   head_prep_kernel<<<hd_blocks(v_pad > k_pad ? v_pad : k_pad, 8), 256, 0, stream>>>(
-      a->labels, a->label_kind, a->V, v_pad, a->K, k_pad, a->has_ignore, a->ignore, a->y, a->bias, a->bias_kind, a->bias2,
-      a->status);
+      labels, label_kind, V, v_pad, K, k_pad, has_ignore, ignore, a.y, bias, bias_kind, a.bias2, a.w16, status);
   sb_count_launch(1);
-  // scratch: block sums (double), running maxima and sums, t at the labels
-  double* sums = (double*)a->scratch;
-  const int splits = wide(a) ? head_wide_splits(a->V, a->K) : p.splits;
-  p.part = (float2*)(a->scratch + 4LL * HD_SUM_BLOCKS);
-  p.tl = (float*)(p.part + splits * p.rows_pad);
-  p.colp = a->bias2;
-  p.rowy = a->y;
-  const int rc = wide(a) ? head_wide_forward(a, p.part, p.tl, splits, stream) : head_launch<HEAD_FWD>(a, p, stream);
+  int rc, splits;
+  if (wide(a)) {
+    splits = head_wide_splits(V, K);
+    rc = head_wide_forward(a, f.part, f.tl, stream);
+  } else {
+    HeadParams p;
+    head_geometry(a, HEAD_FWD, p);
+    p.part = f.part;
+    p.tl = f.tl;
+    p.rowy = a.y;
+    splits = p.splits;
+    rc = head_launch<HEAD_FWD, false>(a, p, stream);
+  }
   if (rc) return rc;
-  const int blocks = hd_blocks(v_pad, 4);
-  head_merge_kernel<<<blocks, 256, 0, stream>>>(p.part, p.tl, a->y, a->cw, splits, a->V, v_pad, a->lse2, sums);
-  sb_count_launch(1);
-  return sb_head_total(sums, blocks, a->total, a->loss, a->den, stream);
+  const int blocks = hd_blocks(v_pad, HD_SUM_BLOCKS / 148);
+  head_merge_kernel<<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, f.sums);
+  head_total_kernel<<<1, 256, 0, stream>>>(f.sums, blocks, a.total, loss, a.den);
+  sb_count_launch(2);
+  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
-extern "C" int sb_head_total(const double* sums, int blocks, double* total, float* loss, float* den,
-                             cudaStream_t stream) {
-  head_total_kernel<<<1, 256, 0, stream>>>(sums, blocks, total, loss, den);
+// the loss from the state's two sums (its first 16 bytes) after they were added over the shards
+extern "C" int sb_head_total(void* state, float* loss, cudaStream_t stream) {
+  if (!state || !loss) return SB_ERR_SHAPE;
+  double* total = (double*)state;
+  head_total_kernel<<<1, 256, 0, stream>>>(total, 1, total, loss, (float*)((char*)state + 16));
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
-template <typename T>
-static void head_reduce(const float* ws, int slices, long long rows, long long rows_pad, int C, int ld, void* out,
-                        cudaStream_t stream) {
-  head_reduce_kernel<T><<<hd_blocks(rows * C, 8), 256, 0, stream>>>(ws, slices, rows, rows_pad, C, ld, (T*)out);
+// dx, dw and db (each optional) from gout and the state; dw / db in fp32 when dw_kind / db_kind is 2, else bf16
+extern "C" int sb_head_backward(const void* x, const void* w, const float* cw, long long V, int K, int C, void* state,
+                                void* scratch, const float* gout, void* dx, void* dw, int dw_kind, void* db, int db_kind,
+                                uint32_t* status, cudaStream_t stream) {
+  if (!shape_ok(V, K, C) || !x || !w || !state || !scratch || !gout) return SB_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(state) | reinterpret_cast<uintptr_t>(scratch)) & 255) return SB_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15) return SB_ERR_ALIGN;
+  HeadCall a;
+  memset(&a, 0, sizeof(a));
+  a.x = (const __nv_bfloat16*)x;
+  a.w = (const __nv_bfloat16*)w;
+  a.cw = cw;
+  a.V = V; a.K = K; a.C = C;
+  a.status = status;
+  a.dx = (__nv_bfloat16*)dx;
+  a.dw = dw; a.dw_kind = dw_kind;
+  a.db = db; a.db_kind = db_kind;
+  head_state(a, state);
+  head_bwd_scratch(a, scratch);
+  const long long v_pad = hd_pad(V);
+  head_weights_kernel<<<hd_blocks(v_pad, 8), 256, 0, stream>>>(a, gout, v_pad);
   sb_count_launch(1);
-}
-
-// dx, dw and db (each optional) from gout and what the forward pass left; dw / db in fp32 when dw_kind / bias_kind is 2
-extern "C" int sb_head_backward(const SbHeadArgs* a, const float* gout, cudaStream_t stream) {
-  if (!shape_ok(a) || !a->x || !a->w || !a->y || !a->bias2 || !a->lse2 || !a->den || !a->g || !a->lse2g || !gout)
-    return SB_ERR_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(a->dx) | reinterpret_cast<uintptr_t>(a->dw) | reinterpret_cast<uintptr_t>(a->scratch)) & 15)
-    return SB_ERR_ALIGN;
-  if (a->scratch_floats < sb_head_scratch(a, 1)) return SB_ERR_TOO_LARGE;
-  const long long v_pad = pad(a->V);
-  head_weights_kernel<<<hd_blocks(v_pad, 8), 256, 0, stream>>>(a->lse2, a->y, a->cw, gout, a->den, v_pad, a->g, a->lse2g);
-  sb_count_launch(1);
-  if (wide(a)) return head_wide_backward(a, stream);
-  HeadParams p;
-  int rc = 0;
-  if (a->dx != nullptr) {
-    head_geometry(a, HEAD_DX, p);
-    p.colp = a->bias2;
-    p.rowp = a->lse2;
-    p.rowg = a->g;
-    p.rowy = a->y;
-    p.out = (__nv_bfloat16*)a->dx;
-    p.ws = a->scratch;
-    rc = head_launch<HEAD_DX>(a, p, stream);
-    if (rc) return rc;
-    if (p.splits > 1) head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a->dx, stream);
-  }
-  if (a->dw != nullptr || a->db != nullptr) {
-    head_geometry(a, HEAD_DW, p);
-    p.colp = a->lse2g;
-    p.colg = a->g;
-    p.coly = a->y;
-    p.rowp = a->bias2;
-    p.ws = a->scratch;
-    p.ws_b = a->scratch + p.splits * p.rows_pad * p.cpad;
-    rc = head_launch<HEAD_DW>(a, p, stream);
-    if (rc) return rc;
-    if (a->dw != nullptr) {
-      if (a->dw_kind == 2) head_reduce<float>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a->dw, stream);
-      else head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a->dw, stream);
-    }
-    if (a->db != nullptr) {
-      if (a->bias_kind == 2) head_reduce<float>(p.ws_b, 2 * p.splits, p.rows, p.rows_pad, 1, 1, a->db, stream);
-      else head_reduce<__nv_bfloat16>(p.ws_b, 2 * p.splits, p.rows, p.rows_pad, 1, 1, a->db, stream);
-    }
-  }
-  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  return wide(a) ? head_wide_backward(a, stream) : head_narrow_backward(a, stream);
 }

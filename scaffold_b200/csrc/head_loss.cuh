@@ -8,9 +8,43 @@ namespace sb {
 int make_map_bf16(CUtensorMap* m, const void* base, int rank, const long long* dims, const long long* strides,
                   const int* box, int rowb);
 
-constexpr int HD_PAD = 256;  // per-voxel and per-class arrays are padded to a multiple of this
+constexpr int HD_PAD = 256;         // per-voxel and per-class arrays are padded to a multiple of this
+constexpr int HD_FEW = 128;         // up to this many voxels, D's entries are kept in two bf16 (head_loss.cu)
+constexpr int HD_SUM_BLOCKS = 592;  // blocks of the loss's sums at most
 constexpr float HD_LOG2E = 1.4426950408889634f;
 constexpr float HD_LN2 = 0.6931471805599453f;
+constexpr float HD_LOWEST = -1e30f;
+
+static inline long long hd_pad(long long n) { return (n + HD_PAD - 1) / HD_PAD * HD_PAD; }
+
+// What a call works on; arrays of voxels / classes are padded to HD_PAD.
+struct HeadCall {
+  const __nv_bfloat16* x;  // [V][C]
+  const __nv_bfloat16* w;  // [K][C]
+  const float* cw;         // optional class weights
+  long long V;
+  int K, C;
+  // what the forward pass leaves for the backward pass
+  double* total;  // [2] sums of u nll and of u
+  float* den;     // [1] the second one, at least eps
+  float* lse2;    // voxels: log2 of the sum of exponentials, +inf behind the last
+  int* y;         // voxels: label, -1 where a voxel takes no part
+  float* bias2;   // classes: bias log2(e), -inf behind the last
+  uint4* w16;     // narrow heads, classes, twice: sixteen columns more of w
+  // of the backward pass
+  float* scale;   // [1] dL / den
+  float* g;       // voxels: scale u, u the class weight of the label, 0 where a voxel takes no part
+  uint4* x16;     // narrow heads, voxels: sixteen columns more of x
+  float* u;       // wide heads, voxels: u
+  float* lse2p;   // wide heads, voxels: lse2, +inf where u is 0
+  __nv_bfloat16* dx;
+  void* dw;
+  int dw_kind;    // 0 bf16, 2 fp32
+  void* db;
+  int db_kind;
+  float* scratch;
+  uint32_t* status;
+};
 
 __device__ __forceinline__ float hd_ex2(float x) {
   float y;
@@ -23,28 +57,27 @@ __device__ __forceinline__ void hd_tma_2d(void* dst, const CUtensorMap* m, uint6
       ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
       : "memory");
 }
-// barrier of the 256 threads of the epilogue warps; the same answer in all of them: whether every one said `ok`
-__device__ __forceinline__ bool hd_epi_vote(bool ok) {
+// named barrier `id` of `threads` threads; the same answer in all of them: whether every one said `ok`
+__device__ __forceinline__ bool hd_vote(int id, int threads, bool ok) {
   uint32_t all;
   asm volatile(
       "{\n\t.reg .pred a, q;\n\t"
       "setp.ne.u32 a, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 256, a;\n\t"
+      "barrier.cta.red.and.pred q, %2, %3, a;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(all)
-      : "r"(ok ? 1u : 0u)
+      : "r"(ok ? 1u : 0u), "r"(id), "r"(threads)
       : "memory");
   return all != 0;
 }
-
 template <typename T> __device__ __forceinline__ T hd_cast(float v);
 template <> __device__ __forceinline__ float hd_cast<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 hd_cast<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
 
 // head_wide.cu
 int head_wide_splits(long long V, int K);
-int head_wide_forward(const SbHeadArgs* a, float2* part, float* tl, int splits, cudaStream_t stream);
-long long head_wide_scratch(const SbHeadArgs* a);
-int head_wide_backward(const SbHeadArgs* a, cudaStream_t stream);
+int head_wide_forward(const HeadCall& a, float2* part, float* tl, cudaStream_t stream);
+long long head_wide_scratch(const HeadCall& a);  // floats
+int head_wide_backward(const HeadCall& a, cudaStream_t stream);
 
 }  // namespace sb

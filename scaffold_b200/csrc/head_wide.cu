@@ -3,10 +3,13 @@
 // pairs (tcgen05 cta_group::2): a pair multiplies 256 rows by 256 columns, each CTA loads its own 128 rows and one half
 // of the columns (64 bytes a clock and SM out of L2, half of what one CTA alone would read).
 //   WIDE_LSE  rows = voxels, columns = classes: running maximum and sum of every row over the class tiles of a job
-//   WIDE_D    rows = classes, columns = voxels: D^T = g (p - [j = y]) in bf16, a piece of the classes by a piece of the
+//   WIDE_D    rows = classes, columns = voxels: P^T = p - [j = y] in bf16, a piece of the classes by a piece of the
 //             voxels at a time (HW_PIECE elements: 64 MB, which stays in L2 until both products below have read it); db
-//   WIDE_OUT  dX = D W and dW = D^T X of the piece. D^T is read K-major for dW and MN-major for dX, W and X MN-major:
-//             nothing is transposed in memory. Long reductions are cut into slices that are added in order.
+//   WIDE_OUT  dX = g P W and dW = P^T (u X) of the piece (head_loss.cu for g and u). P^T is read K-major for dW and
+//             MN-major for dX, W and X MN-major: nothing is transposed in memory. Long reductions are cut into slices
+//             that are added in order.
+// Roundings as in head_loss.cu; here the class weights go into a copy of X (whose roundings are independent of one
+// another) and up to HD_FEW voxels P^T is followed by its remainder, along which the products' reductions go on.
 // One thread holds a row of a tile, so a row's maximum, sum and db need no exchange.
 #include "head_loss.cuh"
 #include "pair.cuh"
@@ -28,16 +31,20 @@ struct WideParams {
   int cols;                     // real columns, for the last tile's width
   long long rows_pad;
   const int* y;                 // LSE: label of a row; D: of a column
-  const float* colp;            // LSE: bias2; D: lse2g
-  const float* colg;            // D: g
+  const float* colp;            // LSE: bias2; D: lse2p
+  const float* colg;            // D: u
   const float* rowp;            // D: bias2
   int row0;                     // D: class of row 0
   float2* part;
   float* tl;
-  __nv_bfloat16* dl;            // D: [rows][ldd]
+  __nv_bfloat16* dl;            // D: [rows][ldd]; the remainder lo_rows rows further
   long long ldd;
+  int lo_rows;                  // 0: no remainder
   float* ws_b;                  // D: [2 splits][rows_pad]
-  // OUT: [rows][C]; add: acc is added to the product; the sum goes to out16 / out32, or back to acc
+  // OUT: [rows][C]; add: acc is added to the product; the sum goes, scaled, to out16 / out32, or back to acc
+  int kc0;                      // blocks of the reduction behind which the remainder's begin
+  const float* row_scale;       // of a row (0: the result is 0), or
+  const float* scale;           // of all
   long long rows;
   float* acc;
   int add;
@@ -47,13 +54,18 @@ struct WideParams {
   uint32_t* status;
 };
 
-// rows x C sums: v = (add ? acc : 0) + product, then to an output or back to acc; eight columns
-__device__ __forceinline__ void hw_sink(float* acc, int add, __nv_bfloat16* out16, float* out32, long long at,
+// rows x C sums: v = (add ? acc : 0) + product, then scaled to an output or back to acc; eight columns
+__device__ __forceinline__ void hw_sink(float* acc, int add, __nv_bfloat16* out16, float* out32, float scale, long long at,
                                         float (&f)[8]) {
   if (add) {
     const float4 a = *reinterpret_cast<const float4*>(acc + at), b = *reinterpret_cast<const float4*>(acc + at + 4);
     f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
     f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+  }
+  if (out16 != nullptr || out32 != nullptr) {
+    // a voxel that takes no part has no gradient, whatever its features hold
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = scale == 0.f ? 0.f : f[i] * scale;
   }
   if (out16 != nullptr) {
     *reinterpret_cast<uint4*>(out16 + at) =
@@ -142,15 +154,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
             if (rank == 0) mbar_expect_tx(&full[st], 2u * (16384u + (B_MN ? nb * 8192u : 16384u)));  // both CTAs' bytes
             uint8_t* sa = smem + st * HW_STAGE;
             uint8_t* sb = sa + 16384;
+            // behind block kc0 the reduction runs over the remainder, against the same B
+            const bool lo = EPI == WIDE_OUT && k >= p.kc0;
+            const int at = (lo ? k - p.kc0 : k) * 64, down = lo ? p.lo_rows : 0;
             if (A_MN) {
-              for (int i = 0; i < 2; ++i) tma2_load_2d(sa + i * 8192, &p.mapA, bar, row + i * 64, k * 64);
+              for (int i = 0; i < 2; ++i) tma2_load_2d(sa + i * 8192, &p.mapA, bar, row + i * 64, at + down);
             } else {
-              tma2_load_2d(sa, &p.mapA, bar, k * 64, row);
+              tma2_load_2d(sa, &p.mapA, bar, at, row + down);
             }
             if (B_MN) {
-              for (int i = 0; i < nb; ++i) tma2_load_2d(sb + i * 8192, &p.mapB, bar, col + i * 64, k * 64);
+              for (int i = 0; i < nb; ++i) tma2_load_2d(sb + i * 8192, &p.mapB, bar, col + i * 64, at);
             } else {
-              tma2_load_2d(sb, &p.mapB, bar, k * 64, col);
+              tma2_load_2d(sb, &p.mapB, bar, at, col);
             }
             if (++st == HW_STAGES) { st = 0; ph ^= 1u; }
           }
@@ -254,32 +269,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
             }
             s += (a0 + a1) + (a2 + a3);
           } else if (EPI == WIDE_D) {
-            float d0 = 0.f, d1 = 0.f, d2 = 0.f, d3 = 0.f;
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
             const int cls = p.row0 + (int)r;
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              const float4 cg = __ldg(reinterpret_cast<const float4*>(p.colg + c_abs + c0 + i));
+              const float4 cu = __ldg(reinterpret_cast<const float4*>(p.colg + c_abs + c0 + i));
               const int4 cy = __ldg(reinterpret_cast<const int4*>(p.y + c_abs + c0 + i));
-              f[i] = hd_ex2(f[i]) - (cy.x == cls ? cg.x : 0.f);
-              f[i + 1] = hd_ex2(f[i + 1]) - (cy.y == cls ? cg.y : 0.f);
-              f[i + 2] = hd_ex2(f[i + 2]) - (cy.z == cls ? cg.z : 0.f);
-              f[i + 3] = hd_ex2(f[i + 3]) - (cy.w == cls ? cg.w : 0.f);
-              d0 += f[i]; d1 += f[i + 1]; d2 += f[i + 2]; d3 += f[i + 3];
+              f[i] = hd_ex2(f[i]) - (cy.x == cls ? 1.f : 0.f);
+              f[i + 1] = hd_ex2(f[i + 1]) - (cy.y == cls ? 1.f : 0.f);
+              f[i + 2] = hd_ex2(f[i + 2]) - (cy.z == cls ? 1.f : 0.f);
+              f[i + 3] = hd_ex2(f[i + 3]) - (cy.w == cls ? 1.f : 0.f);
+              d[0] = fmaf(cu.x, f[i], d[0]);
+              d[1] = fmaf(cu.y, f[i + 1], d[1]);
+              d[2] = fmaf(cu.z, f[i + 2], d[2]);
+              d[3] = fmaf(cu.w, f[i + 3], d[3]);
             }
-            db += (d0 + d1) + (d2 + d3);
+            db += (d[0] + d[1]) + (d[2] + d[3]);
+            uint32_t o[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
             uint4* dst = reinterpret_cast<uint4*>(p.dl + r * p.ldd + c_abs + c0);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float* e = f + 16 * i;
-              st_global_v8(dst + 2 * i,
-                           make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
-                                      pack_bf16x2(e[6], e[7])),
-                           make_uint4(pack_bf16x2(e[8], e[9]), pack_bf16x2(e[10], e[11]), pack_bf16x2(e[12], e[13]),
-                                      pack_bf16x2(e[14], e[15])));
+            for (int i = 0; i < 2; ++i)
+              st_global_v8(dst + 2 * i, make_uint4(o[8 * i], o[8 * i + 1], o[8 * i + 2], o[8 * i + 3]),
+                           make_uint4(o[8 * i + 4], o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]));
+            if (p.lo_rows) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                o[i] = pack_bf16x2(f[2 * i] - __uint_as_float(o[i] << 16), f[2 * i + 1] - __uint_as_float(o[i] & 0xFFFF0000u));
+              dst = reinterpret_cast<uint4*>(p.dl + (r + p.lo_rows) * p.ldd + c_abs + c0);
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                st_global_v8(dst + 2 * i, make_uint4(o[8 * i], o[8 * i + 1], o[8 * i + 2], o[8 * i + 3]),
+                             make_uint4(o[8 * i + 4], o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]));
             }
           } else if (r < p.rows) {
             float* acc = p.kslices > 1 ? p.slices + (long long)j.sp * p.rows * p.cols : p.acc;
             const bool whole = p.kslices == 1;
+            const float scale = p.row_scale != nullptr ? __ldg(p.row_scale + r) : p.scale != nullptr ? __ldg(p.scale) : 1.f;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               const int col = c_abs + c0 + g * 8;
@@ -287,7 +314,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
                 float e[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) e[i] = __uint_as_float(v[g * 8 + i]);
-                hw_sink(acc, whole ? p.add : 0, whole ? p.out16 : nullptr, whole ? p.out32 : nullptr, r * p.cols + col, e);
+                hw_sink(acc, whole ? p.add : 0, whole ? p.out16 : nullptr, whole ? p.out32 : nullptr, scale,
+                        r * p.cols + col, e);
               }
             }
           }
@@ -300,14 +328,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
       }
       if (EPI == WIDE_LSE) {
         if (half == 1) { s_m[row] = m; s_s[row] = s; s_t[row] = tl; }
-        ok = hd_epi_vote(ok);
+        ok = hd_vote(1, 256, ok);
         if (half == 0 && ok) {
           const float m1 = s_m[row], mm = fmaxf(m, m1);
           const float base = mm == -INFINITY ? 0.f : mm;
           p.part[(long long)j.sp * p.rows_pad + r] = make_float2(mm, s * hd_ex2(m - base) + s_s[row] * hd_ex2(m1 - base));
           if (y >= j.t0 * 256 && y < j.t1 * 256) p.tl[r] = (y & 255) < 128 ? tl : s_t[row];
         }
-        hd_epi_vote(true);  // the merge has read what the next job's will overwrite
+        hd_vote(1, 256, true);  // the merge has read what the next job's will overwrite
       }
       if (EPI == WIDE_D && ok) p.ws_b[((long long)j.sp * 2 + half) * p.rows_pad + r] = db;
     }
@@ -328,31 +356,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
   }
 }
 
-// [rows][C] = (add ? acc : 0) + the slices in order, to an output or back to acc (C a multiple of 8)
-__global__ void __launch_bounds__(256) head_slices_kernel(const float* __restrict__ slices, int n, long long elems,
-                                                          float* acc, int add, __nv_bfloat16* out16, float* out32) {
+// [rows][C] = (add ? acc : 0) + the slices in order, scaled to an output or back to acc (C a multiple of 8)
+__global__ void __launch_bounds__(256) head_slices_kernel(const float* __restrict__ slices, int n, long long elems, int C,
+                                                          float* acc, int add, __nv_bfloat16* out16, float* out32,
+                                                          const float* __restrict__ row_scale,
+                                                          const float* __restrict__ scale) {
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < elems / 8; i += (long long)gridDim.x * 256) {
     float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int k = 0; k < n; ++k) {
       const float* src = slices + (long long)k * elems + i * 8;
       const float4 a = __ldcs(reinterpret_cast<const float4*>(src)), b = __ldcs(reinterpret_cast<const float4*>(src + 4));
       f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
       f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
     }
-    hw_sink(acc, add, out16, out32, i * 8, f);
+    hw_sink(acc, add, out16, out32, row_scale != nullptr ? row_scale[i * 8 / C] : scale != nullptr ? scale[0] : 1.f, i * 8, f);
   }
 }
 // the same for the bias's sums: slices [n][ld], rows of them
 __global__ void __launch_bounds__(256) head_slices_b_kernel(const float* __restrict__ slices, int n, long long ld,
                                                             int rows, float* acc, int add, __nv_bfloat16* out16,
-                                                            float* out32) {
+                                                            float* out32, const float* __restrict__ scale) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= rows) return;
   float f = 0.f;
+#pragma unroll 8
   for (int k = 0; k < n; ++k) f += slices[(long long)k * ld + i];
   if (add) f += acc[i];
-  if (out16 != nullptr) out16[i] = __float2bfloat16(f);
-  else (out32 != nullptr ? out32 : acc)[i] = f;
+  if (out16 != nullptr) out16[i] = __float2bfloat16(f * scale[0]);
+  else if (out32 != nullptr) out32[i] = f * scale[0];
+  else acc[i] = f;
+}
+// out = u x, eight channels a thread (zeros for a voxel that takes no part, whatever its features hold)
+__global__ void __launch_bounds__(256) head_weigh_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__ u,
+                                                         long long octets, int C, __nv_bfloat16* __restrict__ out) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < octets; i += (long long)gridDim.x * 256) {
+    const float k = u[i * 8 / C];
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x) + i);
+    const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] = k == 0.f ? 0u : pack_bf16x2(k * __uint_as_float(v[j] << 16), k * __uint_as_float(v[j] & 0xFFFF0000u));
+    reinterpret_cast<uint4*>(out)[i] = make_uint4(o[0], o[1], o[2], o[3]);
+  }
 }
 
 static int g_hw_pairs = 0;
@@ -401,12 +448,12 @@ static int map_rows(CUtensorMap* m, const void* base, long long rows, long long 
 }
 static long long up(long long n, long long m) { return (n + m - 1) / m * m; }
 
-// Cuts of the column tiles of LSE / D: fewest rounds of (tiles per job + a quarter of one), fewest cuts first.
+// Cuts of the column tiles of LSE / D: fewest rounds of (tiles per job + a sixteenth of one), fewest cuts first.
 static void wide_split(int row_tiles, int col_tiles, int* splits, int* per_out) {
   long long best = -1;
   for (int want = 1; want <= col_tiles && want <= 148; ++want) {
     const int per = (col_tiles + want - 1) / want, s = (col_tiles + per - 1) / per;
-    const long long rounds = ((long long)row_tiles * s + 73) / 74, cost = rounds * (4 * per + 1);
+    const long long rounds = ((long long)row_tiles * s + 73) / 74, cost = rounds * (16 * per + 1);
     if (best < 0 || cost < best) { best = cost; *splits = s; *per_out = per; }
   }
 }
@@ -431,11 +478,12 @@ struct Pieces {
   int nv, nk;
   int sx, sw;        // slices of the two products
   int d_splits, d_per;
-  long long dl, acc_x, acc_w, acc_b, ws_b, slices, total;  // offsets in floats
+  int lo;            // P^T has a remainder
+  long long dl, xu, acc_x, acc_w, acc_b, ws_b, slices, total;  // offsets in floats
 };
-static Pieces wide_pieces(const SbHeadArgs* a) {
+static Pieces wide_pieces(const HeadCall& a) {
   Pieces q;
-  const long long vp = up(a->V, 256), kp = up(a->K, 256);
+  const long long vp = up(a.V, 256), kp = up(a.K, 256);
   if (kp * (vp < 16384 ? vp : 16384) <= HW_PIECE) {  // all classes, as many voxels as fit
     q.kp = kp;
     q.vc = HW_PIECE / kp / 256 * 256;
@@ -448,23 +496,25 @@ static Pieces wide_pieces(const SbHeadArgs* a) {
   q.nk = (int)((kp + q.kp - 1) / q.kp);
   q.vc = up((vp + q.nv - 1) / q.nv, 256);
   q.kp = up((kp + q.nk - 1) / q.nk, 256);
-  q.sx = wide_slices(q.vc, a->C, (int)(q.kp / 64));
-  q.sw = wide_slices(q.kp, a->C, (int)(q.vc / 64));
+  q.lo = a.V <= HD_FEW;
+  q.sx = wide_slices(q.vc, a.C, (int)(q.kp / 64) * (1 + q.lo));
+  q.sw = wide_slices(q.kp, a.C, (int)(q.vc / 64) * (1 + q.lo));
   wide_split((int)(q.kp / 256), (int)(q.vc / 256), &q.d_splits, &q.d_per);
   long long at = 0;
   auto take = [&](long long floats) { const long long o = at; at += up(floats, 64); return o; };
-  q.dl = take(q.kp * q.vc / 2);
-  q.acc_x = take(q.nk > 1 ? q.vc * a->C : 0);
-  q.acc_w = take(q.nv > 1 ? (long long)a->K * a->C : 0);
-  q.acc_b = take(q.nv > 1 ? a->K : 0);
+  q.dl = take(q.kp * q.vc / 2 * (1 + q.lo));
+  q.xu = take(a.cw != nullptr ? q.vc * a.C / 2 : 0);
+  q.acc_x = take(q.nk > 1 ? q.vc * a.C : 0);
+  q.acc_w = take(q.nv > 1 ? (long long)a.K * a.C : 0);
+  q.acc_b = take(q.nv > 1 ? a.K : 0);
   q.ws_b = take(2LL * q.d_splits * q.kp);
-  const long long sx = q.sx > 1 ? q.sx * q.vc * a->C : 0, sw = q.sw > 1 ? q.sw * q.kp * a->C : 0;
+  const long long sx = q.sx > 1 ? q.sx * q.vc * a.C : 0, sw = q.sw > 1 ? q.sw * q.kp * a.C : 0;
   q.slices = take(sx > sw ? sx : sw);
   q.total = at;
   return q;
 }
 
-long long head_wide_scratch(const SbHeadArgs* a) { return wide_pieces(a).total; }
+long long head_wide_scratch(const HeadCall& a) { return wide_pieces(a).total; }
 
 int head_wide_splits(long long V, int K) {
   int s = 1, per = 1;
@@ -472,119 +522,131 @@ int head_wide_splits(long long V, int K) {
   return s;
 }
 
-int head_wide_forward(const SbHeadArgs* a, float2* part, float* tl, int, cudaStream_t stream) {
+int head_wide_forward(const HeadCall& a, float2* part, float* tl, cudaStream_t stream) {
   WideParams p;
   memset(&p, 0, sizeof(p));
-  p.row_tiles = (int)(up(a->V, 256) / 256);
-  p.col_tiles = (int)(up(a->K, 256) / 256);
+  p.row_tiles = (int)(up(a.V, 256) / 256);
+  p.col_tiles = (int)(up(a.K, 256) / 256);
   wide_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
-  p.kc = (a->C + 63) / 64;
-  p.cols = a->K;
-  p.rows_pad = up(a->V, HD_PAD);
-  p.y = a->y;
-  p.colp = a->bias2;
+  p.kc = (a.C + 63) / 64;
+  p.cols = a.K;
+  p.rows_pad = up(a.V, HD_PAD);
+  p.y = a.y;
+  p.colp = a.bias2;
   p.part = part;
   p.tl = tl;
-  p.status = a->status;
-  int rc = map_rows(&p.mapA, a->x, a->V, a->C, a->C, 128);
+  p.status = a.status;
+  int rc = map_rows(&p.mapA, a.x, a.V, a.C, a.C, 128);
   if (rc) return rc;
-  rc = map_rows(&p.mapB, a->w, a->K, a->C, a->C, 128);
+  rc = map_rows(&p.mapB, a.w, a.K, a.C, a.C, 128);
   if (rc) return rc;
   return wide_launch<WIDE_LSE, 0, 0>(p, stream);
 }
 
 // one product of a piece: rows x C over `kext` of the reduction
 template <int A_MN>
-static int wide_product(const SbHeadArgs* a, const void* dl, long long ldd, long long vext, long long kext, const void* b,
-                        long long b_rows, long long rows, int slices, float* ws, float* acc, int add, void* out16,
-                        void* out32, cudaStream_t stream) {
+static int wide_product(const HeadCall& a, const void* dl, long long ldd, long long vext, long long kext, int lo_rows,
+                        const void* b, long long b_rows, long long rows, int slices, float* ws, float* acc, int add,
+                        const float* row_scale, const float* scale, void* out16, void* out32, cudaStream_t stream) {
   WideParams p;
   memset(&p, 0, sizeof(p));
   const long long ext = A_MN ? kext : vext;  // of the reduction
-  p.kc = (int)(ext / 64);
+  p.kc0 = (int)(ext / 64);
+  p.kc = lo_rows ? 2 * p.kc0 : p.kc0;
+  p.lo_rows = lo_rows;
+  p.row_scale = row_scale;
+  p.scale = scale;
   p.kslices = slices < p.kc ? slices : p.kc;
   p.kc_per_slice = (p.kc + p.kslices - 1) / p.kslices;
   p.kslices = (p.kc + p.kc_per_slice - 1) / p.kc_per_slice;
   p.rows = rows;
   p.row_tiles = (int)(up(rows, 256) / 256);
-  p.cols = a->C;
-  p.col_tiles = (a->C + 255) / 256;
+  p.cols = a.C;
+  p.col_tiles = (a.C + 255) / 256;
   p.acc = acc;
   p.add = add;
   p.out16 = (__nv_bfloat16*)out16;
   p.out32 = (float*)out32;
   p.slices = ws;
-  p.status = a->status;
-  int rc = map_rows(&p.mapA, dl, kext, vext, ldd, A_MN ? 64 : 128);
+  p.status = a.status;
+  int rc = map_rows(&p.mapA, dl, lo_rows + kext, vext, ldd, A_MN ? 64 : 128);
   if (rc) return rc;
-  rc = map_rows(&p.mapB, b, b_rows, a->C, a->C, 64);
+  rc = map_rows(&p.mapB, b, b_rows, a.C, a.C, 64);
   if (rc) return rc;
   rc = wide_launch<WIDE_OUT, A_MN, 1>(p, stream);
   if (rc || p.kslices == 1) return rc;
-  const long long elems = rows * a->C, blocks = (elems / 8 + 255) / 256;
-  head_slices_kernel<<<(int)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(ws, p.kslices, elems, acc, add,
-                                                                                    p.out16, p.out32);
+  const long long elems = rows * a.C, blocks = (elems / 8 + 255) / 256;
+  head_slices_kernel<<<(int)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(
+      ws, p.kslices, elems, a.C, acc, add, p.out16, p.out32, row_scale, scale);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
-int head_wide_backward(const SbHeadArgs* a, cudaStream_t stream) {
+int head_wide_backward(const HeadCall& a, cudaStream_t stream) {
   const Pieces q = wide_pieces(a);
-  if (a->scratch_floats < q.total) return SB_ERR_TOO_LARGE;
-  const __nv_bfloat16* x = (const __nv_bfloat16*)a->x;
-  const __nv_bfloat16* w = (const __nv_bfloat16*)a->w;
-  __nv_bfloat16* dl = (__nv_bfloat16*)(a->scratch + q.dl);
-  float* ws_b = a->scratch + q.ws_b;
+  __nv_bfloat16* dl = (__nv_bfloat16*)(a.scratch + q.dl);
+  __nv_bfloat16* xu = (__nv_bfloat16*)(a.scratch + q.xu);
+  float* ws_b = a.scratch + q.ws_b;
   for (int iv = 0; iv < q.nv; ++iv) {
-    const long long v0 = iv * q.vc, vrows = a->V - v0 < q.vc ? a->V - v0 : q.vc, vext = up(vrows, 256);
+    const long long v0 = iv * q.vc, vrows = a.V - v0 < q.vc ? a.V - v0 : q.vc, vext = up(vrows, 256);
     if (vrows <= 0) break;
-    const bool v_last = v0 + q.vc >= a->V;
+    const bool v_last = v0 + q.vc >= a.V;
+    const __nv_bfloat16* xv = a.x + v0 * a.C;
+    const __nv_bfloat16* xw = xv;
+    if (a.cw != nullptr && a.dw != nullptr) {
+      const long long octets = vrows * a.C / 8, blocks = (octets + 255) / 256;
+      head_weigh_kernel<<<(int)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(xv, a.u + v0, octets, a.C, xu);
+      sb_count_launch(1);
+      xw = xu;
+    }
     for (int ik = 0; ik < q.nk; ++ik) {
-      const long long k0 = ik * q.kp, krows = a->K - k0 < q.kp ? a->K - k0 : q.kp, kext = up(krows, 256);
+      const long long k0 = ik * q.kp, krows = a.K - k0 < q.kp ? a.K - k0 : q.kp, kext = up(krows, 256);
       if (krows <= 0) break;
-      const bool k_last = k0 + q.kp >= a->K;
+      const bool k_last = k0 + q.kp >= a.K;
+      const __nv_bfloat16* wk = a.w + k0 * a.C;
       WideParams p;
       memset(&p, 0, sizeof(p));
       p.row_tiles = (int)(kext / 256);
       p.col_tiles = (int)(vext / 256);
       p.tiles_per_split = q.d_per;
       p.splits = (p.col_tiles + q.d_per - 1) / q.d_per;
-      p.kc = (a->C + 63) / 64;
+      p.kc = (a.C + 63) / 64;
       p.cols = (int)vext;
       p.rows_pad = q.kp;
-      p.y = a->y + v0;
-      p.colp = a->lse2g + v0;
-      p.colg = a->g + v0;
-      p.rowp = a->bias2 + k0;
+      p.y = a.y + v0;
+      p.colp = a.lse2p + v0;
+      p.colg = a.u + v0;
+      p.rowp = a.bias2 + k0;
       p.row0 = (int)k0;
       p.dl = dl;
       p.ldd = q.vc;
+      p.lo_rows = q.lo ? (int)q.kp : 0;
       p.ws_b = ws_b;
-      p.status = a->status;
-      int rc = map_rows(&p.mapA, w + k0 * a->C, krows, a->C, a->C, 128);
+      p.status = a.status;
+      int rc = map_rows(&p.mapA, wk, krows, a.C, a.C, 128);
       if (rc) return rc;
-      rc = map_rows(&p.mapB, x + v0 * a->C, vrows, a->C, a->C, 128);
+      rc = map_rows(&p.mapB, xv, vrows, a.C, a.C, 128);
       if (rc) return rc;
       rc = wide_launch<WIDE_D, 0, 0>(p, stream);
       if (rc) return rc;
-      if (a->db != nullptr) {
+      if (a.db != nullptr) {
         head_slices_b_kernel<<<(int)((krows + 255) / 256), 256, 0, stream>>>(
-            ws_b, 2 * p.splits, q.kp, (int)krows, a->scratch + q.acc_b + k0, iv > 0,
-            v_last && a->bias_kind == 0 ? (__nv_bfloat16*)a->db + k0 : nullptr,
-            v_last && a->bias_kind == 2 ? (float*)a->db + k0 : nullptr);
+            ws_b, 2 * p.splits, q.kp, (int)krows, a.scratch + q.acc_b + k0, iv > 0,
+            v_last && a.db_kind == 0 ? (__nv_bfloat16*)a.db + k0 : nullptr,
+            v_last && a.db_kind == 2 ? (float*)a.db + k0 : nullptr, a.scale);
         sb_count_launch(1);
       }
-      if (a->dx != nullptr) {
-        rc = wide_product<1>(a, dl, q.vc, vext, kext, w + k0 * a->C, krows, vrows, q.sx, a->scratch + q.slices,
-                             a->scratch + q.acc_x, ik > 0, k_last ? (__nv_bfloat16*)a->dx + v0 * a->C : nullptr, nullptr,
-                             stream);
+      if (a.dx != nullptr) {
+        rc = wide_product<1>(a, dl, q.vc, vext, kext, p.lo_rows, wk, krows, vrows, q.sx, a.scratch + q.slices,
+                             a.scratch + q.acc_x, ik > 0, a.g + v0, nullptr,
+                             k_last ? a.dx + v0 * a.C : nullptr, nullptr, stream);
         if (rc) return rc;
       }
-      if (a->dw != nullptr) {
-        rc = wide_product<0>(a, dl, q.vc, vext, kext, x + v0 * a->C, vrows, krows, q.sw, a->scratch + q.slices,
-                             a->scratch + q.acc_w + k0 * a->C, iv > 0,
-                             v_last && a->dw_kind == 0 ? (__nv_bfloat16*)a->dw + k0 * a->C : nullptr,
-                             v_last && a->dw_kind == 2 ? (float*)a->dw + k0 * a->C : nullptr, stream);
+      if (a.dw != nullptr) {
+        rc = wide_product<0>(a, dl, q.vc, vext, kext, p.lo_rows, xw, vrows, krows, q.sw, a.scratch + q.slices,
+                             a.scratch + q.acc_w + k0 * a.C, iv > 0, nullptr, a.scale,
+                             v_last && a.dw_kind == 0 ? (__nv_bfloat16*)a.dw + k0 * a.C : nullptr,
+                             v_last && a.dw_kind == 2 ? (float*)a.dw + k0 * a.C : nullptr, stream);
         if (rc) return rc;
       }
     }

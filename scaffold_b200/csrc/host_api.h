@@ -209,39 +209,18 @@ int sb_gn8_bwd_partial(const SbGn8Args* a, cudaStream_t stream);
 int sb_gn8_bwd_dx(const SbGn8Args* a, cudaStream_t stream);
 
 // Cross entropy of a head of K classes over V voxels of C channels without its logits (head_loss.cu, head_wide.cu).
-// Arrays marked v / k are padded to a multiple of 256 voxels / classes.
-typedef struct {
-  const void* x;       // bf16 [V][C]
-  const void* w;       // bf16 [K][C]
-  const void* bias;    // optional [K]
-  int bias_kind;       // of bias and db: 0 bf16, 2 fp32
-  const void* labels;  // [V]
-  int label_kind;      // 2 int16, 4 int32, 8 int64
-  int has_ignore;
-  long long ignore;    // label of voxels that take no part
-  const float* cw;     // optional class weights [K], not negative
-  long long V;
-  int K, C;
-  int* y;              // v: forward out: label, -1 takes no part
-  float* bias2;        // k: forward out
-  float* lse2;         // v: forward out: log2 of the sum of exponentials
-  double* total;       // [2] forward out: sums of u nll and u
-  float* loss;         // [1]
-  float* den;          // [1]
-  float* g;            // v: backward scratch, dL/d(nll) of a voxel
-  float* lse2g;        // v: backward scratch, lse2 - log2 g
-  void* dx;            // optional bf16 [V][C]
-  void* dw;            // optional [K][C]
-  int dw_kind;         // 0 bf16, 2 fp32
-  void* db;            // optional [K]
-  float* scratch;      // sb_head_scratch() floats, 16-byte aligned
-  long long scratch_floats;
-  uint32_t* status;
-} SbHeadArgs;
-long long sb_head_scratch(const SbHeadArgs* a, int mode);  // 0 forward, 1 backward
-int sb_head_forward(const SbHeadArgs* a, cudaStream_t stream);
-int sb_head_total(const double* sums, int blocks, double* total, float* loss, float* den, cudaStream_t stream);
-int sb_head_backward(const SbHeadArgs* a, const float* gout, cudaStream_t stream);
+// x bf16 [V][C], w bf16 [K][C], bias optional [K] (bias_kind 0 bf16, 2 fp32), labels [V] (label_kind 2 int16, 4 int32,
+// 8 int64; `ignore`, if has_ignore, takes no part), cw optional class weights [K], not negative. The forward pass fills
+// `state` for the backward pass; its first 16 bytes are the sums of u nll and of u. state and scratch: sb_head_bytes()
+// bytes, 256-byte aligned. Backward: dx bf16 [V][C], dw [K][C] and db [K] (kind 0 bf16, 2 fp32) are each optional.
+long long sb_head_bytes(int what, long long V, int K, int C, int weighted);  // 0 state, 1 / 2 scratch forward / backward
+int sb_head_forward(const void* x, const void* w, const void* bias, int bias_kind, const void* labels, int label_kind,
+                    int has_ignore, long long ignore, const float* cw, long long V, int K, int C, void* state,
+                    void* scratch, float* loss, uint32_t* status, cudaStream_t stream);
+int sb_head_total(void* state, float* loss, cudaStream_t stream);  // the loss from sums that were added over shards
+int sb_head_backward(const void* x, const void* w, const float* cw, long long V, int K, int C, void* state, void* scratch,
+                     const float* gout, void* dx, void* dw, int dw_kind, void* db, int db_kind, uint32_t* status,
+                     cudaStream_t stream);
 
 // number of kernels this library launched so far in the process
 long long sb_launch_count(void);

@@ -16,6 +16,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import gn_kernels as gk
 from .layout import direct_grad_target, from_vm, notify_grad_written, to_vm, use_cuda_kernels
@@ -79,6 +80,7 @@ class _Gn8Fn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gy):
         kept, w32, b32, mean, rstd = ctx.saved_tensors
         groups, relu = ctx.cfg

@@ -11,6 +11,7 @@ tile by tile, once for the loss and once for each gradient; other tensors take t
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
@@ -22,24 +23,12 @@ from .layout import use_cuda_kernels
 _P = C.c_void_p
 
 
-class SbHeadArgs(C.Structure):
-    _fields_ = [
-        ("x", _P), ("w", _P), ("bias", _P), ("bias_kind", C.c_int),
-        ("labels", _P), ("label_kind", C.c_int), ("has_ignore", C.c_int), ("ignore", C.c_longlong),
-        ("cw", _P),
-        ("V", C.c_longlong), ("K", C.c_int), ("C", C.c_int),
-        ("y", _P), ("bias2", _P), ("lse2", _P), ("total", _P), ("loss", _P), ("den", _P),
-        ("g", _P), ("lse2g", _P),
-        ("dx", _P), ("dw", _P), ("dw_kind", C.c_int), ("db", _P),
-        ("scratch", _P), ("scratch_floats", C.c_longlong),
-        ("status", _P),
-    ]
-
-
-_lib.register("sb_head_scratch", [C.POINTER(SbHeadArgs), C.c_int], C.c_longlong)
-_lib.register("sb_head_forward", [C.POINTER(SbHeadArgs), _P])
-_lib.register("sb_head_total", [_P, C.c_int, _P, _P, _P, _P])
-_lib.register("sb_head_backward", [C.POINTER(SbHeadArgs), _P, _P])
+_lib.register("sb_head_bytes", [C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int], C.c_longlong)
+_lib.register("sb_head_forward", [_P, _P, _P, C.c_int, _P, C.c_int, C.c_int, C.c_longlong, _P, C.c_longlong, C.c_int,
+                                  C.c_int, _P, _P, _P, _P, _P])
+_lib.register("sb_head_total", [_P, _P, _P])
+_lib.register("sb_head_backward", [_P, _P, _P, C.c_longlong, C.c_int, C.c_int, _P, _P, _P, _P, _P, C.c_int, _P, C.c_int,
+                                   _P, _P])
 
 _LABEL_KIND = {torch.int16: 2, torch.int32: 4, torch.int64: 8}
 _KIND = {torch.bfloat16: 0, torch.float32: 2}
@@ -51,28 +40,13 @@ def head_supported(width: int) -> bool:
     return 8 <= width <= MAX_WIDTH and width % 8 == 0
 
 
-def _pad(n: int) -> int:
-    return (n + 255) // 256 * 256
-
-
-def _scratch(a: SbHeadArgs, mode: int, dev):
-    n = _lib.lib().sb_head_scratch(C.byref(a), mode)
-    if n < 0:
-        raise _lib.NativeError(f"sb_head_scratch refused {a.V} voxels, {a.K} classes, width {a.C}")
-    t = torch.empty(n, dtype=torch.float32, device=dev) if n else None
-    a.scratch, a.scratch_floats = _lib.ptr(t), n
-    return t
-
-
-def _args(x, w16, bias, cw) -> SbHeadArgs:
-    a = SbHeadArgs()
-    a.V, a.C = x.shape
-    a.K = w16.shape[0]
-    a.x, a.w, a.cw = x.data_ptr(), w16.data_ptr(), _lib.ptr(cw)
-    if bias is not None:
-        a.bias, a.bias_kind = bias.data_ptr(), _KIND[bias.dtype]
-    a.status = _lib.status_tensor(x.device).data_ptr()
-    return a
+@functools.lru_cache(maxsize=256)
+def _bytes(v: int, k: int, c: int, weighted: bool):
+    """Bytes of the state, of the forward pass's scratch and of the backward pass's."""
+    out = tuple(_lib.lib().sb_head_bytes(what, v, k, c, weighted) for what in range(3))
+    if min(out) < 0:
+        raise _lib.NativeError(f"sb_head_bytes refused {v} voxels, {k} classes, width {c}")
+    return out
 
 
 class _HeadLossFn(torch.autograd.Function):
@@ -80,51 +54,44 @@ class _HeadLossFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, labels, cw, ignore, spatial):
         """x [V, C] bf16, weight [K, C], both contiguous."""
         dev = x.device
-        w16 = weight.to(torch.bfloat16)
-        a = _args(x, w16, bias, cw)
-        a.labels, a.label_kind = labels.data_ptr(), _LABEL_KIND[labels.dtype]
-        if ignore is not None:
-            a.has_ignore, a.ignore = 1, ignore
-        vp, kp = _pad(a.V), _pad(a.K)
-        y = torch.empty(vp, dtype=torch.int32, device=dev)
-        lse2 = torch.empty(vp, dtype=torch.float32, device=dev)
-        bias2 = torch.empty(kp, dtype=torch.float32, device=dev)
-        total = torch.empty(2, dtype=torch.float64, device=dev)
+        w16 = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
+        v, c = x.shape
+        k = w16.shape[0]
+        n_state, n_scratch, _ = _bytes(v, k, c, cw is not None)
+        state = torch.empty(n_state, dtype=torch.uint8, device=dev)
+        scratch = torch.empty(n_scratch, dtype=torch.uint8, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        den = torch.empty(1, dtype=torch.float32, device=dev)
-        a.y, a.lse2, a.bias2, a.total, a.loss, a.den = (t.data_ptr() for t in (y, lse2, bias2, total, loss, den))
-        keep = _scratch(a, 0, dev)  # noqa: F841  (freed in stream order)
-        _lib.check(_lib.lib().sb_head_forward(C.byref(a), _lib.stream_ptr()), "sb_head_forward")
+        st = _lib.stream_ptr()
+        _lib.check(_lib.lib().sb_head_forward(
+            x.data_ptr(), w16.data_ptr(), _lib.ptr(bias), 0 if bias is None else _KIND[bias.dtype], labels.data_ptr(),
+            _LABEL_KIND[labels.dtype], ignore is not None, ignore or 0, _lib.ptr(cw), v, k, c, state.data_ptr(),
+            scratch.data_ptr(), loss.data_ptr(), _lib.status_tensor(dev).data_ptr(), st), "sb_head_forward")
         if spatial is not None and spatial.size > 1:
-            spatial.all_reduce_sum(total)
-            _lib.check(_lib.lib().sb_head_total(total.data_ptr(), 1, total.data_ptr(), loss.data_ptr(), den.data_ptr(),
-                                                _lib.stream_ptr()), "sb_head_total")
-        ctx.save_for_backward(x, w16, y, lse2, bias2, den, cw)
-        ctx.like = weight.dtype, None if bias is None else bias.dtype
+            spatial.all_reduce_sum(state[:16].view(torch.float64))
+            _lib.check(_lib.lib().sb_head_total(state.data_ptr(), loss.data_ptr(), st), "sb_head_total")
+        ctx.save_for_backward(x, w16, state, cw)
+        ctx.types = weight.dtype, None if bias is None else bias.dtype
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        x, w16, y, lse2, bias2, den, cw = ctx.saved_tensors
+        x, w16, state, cw = ctx.saved_tensors
         dev = x.device
-        w_type, b_type = ctx.like
-        a = _args(x, w16, None, cw)
-        g, lse2g = torch.empty_like(lse2), torch.empty_like(lse2)
-        a.y, a.lse2, a.bias2, a.den, a.g, a.lse2g = (t.data_ptr() for t in (y, lse2, bias2, den, g, lse2g))
-        gout = gout.float().contiguous()
-        dx = dw = db = None
-        if ctx.needs_input_grad[0]:
-            dx = torch.empty_like(x)
-            a.dx = dx.data_ptr()
-        if ctx.needs_input_grad[1]:
-            dw = torch.empty(w16.shape, dtype=w_type, device=dev)
-            a.dw, a.dw_kind = dw.data_ptr(), _KIND[w_type]
-        if ctx.needs_input_grad[2]:
-            db = torch.empty(w16.shape[0], dtype=b_type, device=dev)
-            a.db, a.bias_kind = db.data_ptr(), _KIND[b_type]
-        keep = _scratch(a, 1, dev)  # noqa: F841
-        _lib.check(_lib.lib().sb_head_backward(C.byref(a), gout.data_ptr(), _lib.stream_ptr()), "sb_head_backward")
+        v, c = x.shape
+        k = w16.shape[0]
+        w_type, b_type = ctx.types
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        gout = gout.float()
+        with torch.cuda.device(dev):
+            dx = torch.empty_like(x) if want_x else None
+            dw = torch.empty((k, c), dtype=w_type, device=dev) if want_w else None
+            db = torch.empty(k, dtype=b_type, device=dev) if want_b else None
+            scratch = torch.empty(_bytes(v, k, c, cw is not None)[2], dtype=torch.uint8, device=dev)
+            _lib.check(_lib.lib().sb_head_backward(
+                x.data_ptr(), w16.data_ptr(), _lib.ptr(cw), v, k, c, state.data_ptr(), scratch.data_ptr(), gout.data_ptr(),
+                _lib.ptr(dx), _lib.ptr(dw), _KIND[w_type], _lib.ptr(db), _KIND[b_type] if want_b else 0,
+                _lib.status_tensor(dev).data_ptr(), _lib.stream_ptr()), "sb_head_backward")
         return dx, dw, db, None, None, None, None
 
 
