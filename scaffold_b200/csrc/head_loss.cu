@@ -24,20 +24,24 @@
 // Where one rounding can make up a result (LO: up to HD_FEW voxels; class weights in HEAD_DW, whose rounding the voxels
 // of a class share) P is kept as two bf16, value and remainder, and the second MMA runs once for each.
 //
-// Roles: warp 0 loads (TMA), warp 1 issues MMAs, warps 2-17 are the epilogue: four groups of four warps, a group takes
-// the even or the odd tiles and one half of their columns. In HEAD_DW the voxels' labels travel with their tile as bulk
-// copies. The first MMAs run ahead of the epilogue by all tiles of s that tensor memory holds; a tile's second MMA is
-// issued when the buffer is wanted again. All waits are bounded.
+// Roles: warp 0 loads (TMA), warps 1 and 2 issue MMAs, warps 3-18 are the epilogue: four groups of four warps, a group
+// takes the even or the odd tiles and one half of their columns. In HEAD_DW the voxels' labels travel with their tile as
+// bulk copies. All waits are bounded.
+// Two issuing warps: one is never more than about an MMA ahead of the tensor pipe and loses some 100 clocks at each wait
+// and some 300 at each commit, during which only the other one's MMAs can run. HEAD_DX / HEAD_DW: warp 1 the first MMAs
+// (as many tiles ahead as tensor memory holds), warp 2 the second ones; HEAD_FWD: the even and the odd tiles. One warp
+// for everything took 2150 clocks a tile at 64 channels, the exponentials left out or not.
 #include "head_loss.cuh"
 
 namespace sb {
 
 constexpr int HD_EPI_WARPS = 16;
-constexpr int HD_THREADS = 64 + 32 * HD_EPI_WARPS;
+constexpr int HD_FIRST_EPI = 3;
+constexpr int HD_THREADS = 32 * (HD_FIRST_EPI + HD_EPI_WARPS);
 constexpr int HD_TILE = 128;
 constexpr int HD_BOX = HD_TILE * 128;  // bytes of a 128-row box of 64 channels
 constexpr int HD_BOX16 = HD_TILE * 32; // and of the sixteen columns more
-constexpr int HD_MAX_STAGES = 4;
+constexpr int HD_MAX_STAGES = 8;
 constexpr int HD_MAX_C = 256;          // TMEM: two or three tiles of s and the accumulator in 512 columns
 
 enum HeadMode { HEAD_FWD = 0, HEAD_DX = 1, HEAD_DW = 2 };
@@ -80,6 +84,17 @@ __device__ __forceinline__ void hd_tmem_st_x16(uint32_t taddr, const uint32_t* v
       : "memory");
 }
 __device__ __forceinline__ void hd_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// where `bits & bit`: v -= d, or v = d; predicated, never a branch
+__device__ __forceinline__ void hd_sub_if(float& v, float d, uint32_t bits, uint32_t bit) {
+  asm("{\n\t.reg .pred q;\n\t.reg .b32 t;\n\tand.b32 t, %2, %3;\n\tsetp.ne.u32 q, t, 0;\n\t@q sub.f32 %0, %0, %1;\n\t}"
+      : "+f"(v)
+      : "f"(d), "r"(bits), "r"(bit));
+}
+__device__ __forceinline__ void hd_set_if(float& v, float d, uint32_t bits, uint32_t bit) {
+  asm("{\n\t.reg .pred q;\n\t.reg .b32 t;\n\tand.b32 t, %2, %3;\n\tsetp.ne.u32 q, t, 0;\n\t@q mov.f32 %0, %1;\n\t}"
+      : "+f"(v)
+      : "f"(d), "r"(bits), "r"(bit));
+}
 __device__ __forceinline__ void hd_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
@@ -94,7 +109,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t r_full[2], r_empty[2], q_full[HD_MAX_STAGES], q_empty[HD_MAX_STAGES], s_full[MAXB], s_done[MAXB],
-      s_free[MAXB], acc_full, acc_empty;
+      acc_full, acc_empty;
   __shared__ uint32_t s_hits[MODE == HEAD_DW ? HD_EPI_WARPS : 1][32];
   __shared__ float s_fwd[MODE == HEAD_FWD ? 2 : 1][3][MODE == HEAD_FWD ? 4 : 1][HD_TILE];
   __shared__ uint32_t tmem_base_s, abort_s;
@@ -109,15 +124,14 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
 
   if (threadIdx.x == 0) {
     abort_s = 0;
-    for (int i = 0; i < 2; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], MODE == HEAD_FWD ? 2 : 1); }
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], MODE == HEAD_FWD ? 1 + HD_EPI_WARPS / 2 : 1);
+      mbar_init(&q_empty[i], 1);
     }
     for (int i = 0; i < MAXB; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_done[i], HD_EPI_WARPS / 2);
-      mbar_init(&s_free[i], 1);
     }
     mbar_init(&acc_full, 1);
     mbar_init(&acc_empty, HD_EPI_WARPS);
@@ -176,90 +190,97 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || (MODE == HEAD_FWD && warp == 2)) {
+    // s = R Q^T of a tile: R's and Q's channels, then the sixteen columns more
     const bool leader = elect_one();
-    const uint32_t hi = desc_hi(8u * 128u, 2u);
+    const uint32_t hi = desc_hi(8u * 128u, 2u), hi16 = desc_hi(8u * 32u, 6u);
     const uint32_t r0 = smem_u32(smem_r), q0 = smem_u32(smem_q);
-    const uint32_t idesc2 = make_idesc_bf16(128, p.cpad, 0, 1);
-    const uint32_t ahead = NB < (uint32_t)p.stages ? NB : (uint32_t)p.stages;
-    const uint32_t lbo = p.kboxes > 1 ? (uint32_t)HD_BOX : 0u;
-    const uint32_t hi16 = desc_hi(8u * 32u, 6u);
-    uint32_t rb = 0, rph = 0, st = 0, ph = 0, b = 0, bph = 0, aph = 0;
-    // tiles whose P is still to be multiplied, oldest first: stage and buffer (with its phase) follow those of the first
-    // MMAs, `flags` has two bits a tile (first, last of its job) and `cols` eight (columns / 16)
-    uint32_t waiting = 0, w_st = 0, w_b = 0, w_bph = 0, flags = 0, cols = 0;
+    uint32_t rb = 0, rph = 0, st = 0, ph = 0, b = 0, bph = 0, tc = 0;
+    uint32_t old_st = 0, old_ph = 0;  // the tile that had this one's buffer
     bool ok = true;
-    auto second = [&]() -> bool {
-      const bool first = flags & 1u, last = flags & 2u;
-      const int ksteps = (int)(cols & 255u);
-      if (first) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty, aph ^ 1u, abort_flag, p.status, 92))) return false;
-        aph ^= 1u;
-      }
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_done[w_b], w_bph, abort_flag, p.status, 93))) return false;
-      tc_fence_after();
-      if (leader) {
-        const uint32_t lo = desc_lo(q0 + w_st * tile_bytes, lbo);
-        const uint32_t a = tmem + w_b * HD_TILE;
-#pragma unroll
-        for (int part = 0; part < (LO ? 2 : 1); ++part)
-          for (int k = 0; k < ksteps; ++k)
-            hd_mma_ts(tmem + ACC, a + 32 * (k >> 1) + 16 * part + 8 * (k & 1), lo + k * 128u, hi, idesc2,
-                      first && part == 0 && k == 0 ? 0u : 1u);
-        tc_commit(&q_empty[w_st]);
-        tc_commit(&s_free[w_b]);
-        if (last) tc_commit(&acc_full);
-      }
-      __syncwarp();
-      if (++w_st == (uint32_t)p.stages) w_st = 0;
-      if (++w_b == NB) { w_b = 0; w_bph ^= 1u; }
-      flags >>= 2;
-      cols >>= 8;
-      --waiting;
-      return true;
-    };
     for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
       const int sp = job / p.row_tiles;
       const int t0 = sp * p.tiles_per_split;
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
       if (!__all_sync(0xffffffffu, mbar_wait(&r_full[rb], rph, abort_flag, p.status, 94))) { ok = false; break; }
-      for (int t = t0; t < t1; ++t) {
-        // as many tiles as there are buffers (and stages) are on their way: the oldest one's second MMA frees both
-        if (MODE != HEAD_FWD && waiting == ahead && !second()) { ok = false; break; }
-        if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95))) { ok = false; break; }
-        // the buffer is free: read by the epilogue (FWD), or its P read by the second MMA that used it
-        uint64_t* bar = MODE == HEAD_FWD ? &s_done[b] : &s_free[b];
-        if (!__all_sync(0xffffffffu, mbar_wait(bar, bph ^ 1u, abort_flag, p.status, 96))) { ok = false; break; }
-        tc_fence_after();
-        const int nc = cols_of(t);
-        if (leader) {
+      bool used = false;
+      for (int t = t0; t < t1; ++t, ++tc) {
+        if (MODE != HEAD_FWD || (tc & 1u) == (uint32_t)(warp - 1)) {
+          const int nc = cols_of(t);
           const uint32_t idesc = make_idesc_bf16(128, nc, 0, 0);
           const uint32_t a0 = r0 + rb * tile_bytes, b0 = q0 + st * tile_bytes;
           const uint32_t a_lo = desc_lo(a0, 16u), b_lo = desc_lo(b0, 16u);
-          for (int k = 0; k < p.ksteps; ++k) {
-            const uint32_t off = (uint32_t)(k >> 2) * (HD_BOX >> 4) + (uint32_t)(k & 3) * 2u;
-            tc_mma_bf16_pred(tmem + b * HD_TILE, a_lo + off, hi, b_lo + off, hi, idesc, k != 0 ? 1u : 0u);
+          const uint32_t a16 = desc_lo(a0 + box16, 16u), b16 = desc_lo(b0 + box16, 16u);
+          // the buffer is free: read by the epilogue (FWD), or its P read by the second MMA that used it
+          if (MODE == HEAD_FWD) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&s_done[b], bph ^ 1u, abort_flag, p.status, 96))) { ok = false; break; }
+          } else if (tc >= NB) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[old_st], old_ph, abort_flag, p.status, 96))) { ok = false; break; }
+            if (++old_st == (uint32_t)p.stages) { old_st = 0; old_ph ^= 1u; }
           }
-          tc_mma_bf16_pred(tmem + b * HD_TILE, desc_lo(a0 + box16, 16u), hi16, desc_lo(b0 + box16, 16u), hi16, idesc, 1u);
-          tc_commit(&s_full[b]);
-          if (MODE == HEAD_FWD) tc_commit(&q_empty[st]);
-          if (t == t1 - 1) tc_commit(&r_empty[rb]);
-        }
-        __syncwarp();
-        if (MODE != HEAD_FWD) {
-          flags |= ((t == t0 ? 1u : 0u) | (t == t1 - 1 ? 2u : 0u)) << (2 * waiting);
-          cols |= (uint32_t)(nc / 16) << (8 * waiting);
-          ++waiting;
+          if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95))) { ok = false; break; }
+          tc_fence_after();
+          if (leader) {
+            tc_mma_bf16_pred(tmem + b * HD_TILE, a16, hi16, b16, hi16, idesc, 0u);
+            for (int k = 0; k < p.ksteps; ++k) {
+              const uint32_t off = (uint32_t)(k >> 2) * (HD_BOX >> 4) + (uint32_t)(k & 3) * 2u;
+              tc_mma_bf16_pred(tmem + b * HD_TILE, a_lo + off, hi, b_lo + off, hi, idesc, 1u);
+            }
+            tc_commit(&s_full[b]);
+            if (MODE == HEAD_FWD) tc_commit(&q_empty[st]);
+          }
+          __syncwarp();
+          used = true;
         }
         if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
         if (++b == NB) { b = 0; bph ^= 1u; }
       }
+      if (ok && leader) {  // this warp is done with the resident tile
+        if (used) tc_commit(&r_empty[rb]);
+        else mbar_arrive(&r_empty[rb]);
+      }
+      __syncwarp();
       if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
     }
-    if (MODE != HEAD_FWD)
-      while (ok && waiting > 0) ok = second();
+  } else if (warp == 2) {
+    // acc += P Q of a tile, P out of the buffer of s
+    const bool leader = elect_one();
+    const uint32_t hi = desc_hi(8u * 128u, 2u);
+    const uint32_t q0 = smem_u32(smem_q);
+    const uint32_t idesc = make_idesc_bf16(128, p.cpad, 0, 1);
+    const uint32_t lbo = p.kboxes > 1 ? (uint32_t)HD_BOX : 0u;
+    uint32_t st = 0, ph = 0, b = 0, bph = 0, aph = 0;
+    bool ok = true;
+    for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
+      const int sp = job / p.row_tiles;
+      const int t0 = sp * p.tiles_per_split;
+      const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty, aph ^ 1u, abort_flag, p.status, 92))) { ok = false; break; }
+      aph ^= 1u;
+      for (int t = t0; t < t1; ++t) {
+        const int ksteps = cols_of(t) / 16;
+        const uint32_t lo = desc_lo(q0 + st * tile_bytes, lbo);
+        const uint32_t a = tmem + b * HD_TILE;
+        // (the other issuing warp has waited for the tile's loads; this one has to see them too)
+        if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95) &&
+                                         mbar_wait(&s_done[b], bph, abort_flag, p.status, 93))) { ok = false; break; }
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int part = 0; part < (LO ? 2 : 1); ++part)
+            for (int k = 0; k < ksteps; ++k)
+              hd_mma_ts(tmem + ACC, a + 32 * (k >> 1) + 16 * part + 8 * (k & 1), lo + k * 128u, hi, idesc,
+                        t == t0 && part == 0 && k == 0 ? 0u : 1u);
+          tc_commit(&q_empty[st]);
+          if (t == t1 - 1) tc_commit(&acc_full);
+        }
+        __syncwarp();
+        if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
+        if (++b == NB) { b = 0; bph ^= 1u; }
+      }
+    }
   } else {
-    const int quad = warp & 3, group = (warp - 2) >> 2, half = group & 1;
+    const int quad = warp & 3, group = (warp - HD_FIRST_EPI) >> 2, half = group & 1;
     const uint32_t par = group >> 1;
     const int row = quad * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
@@ -329,7 +350,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       float m = HD_LOWEST, s = 0.f, tl = 0.f, db = 0.f;
       for (int t = t0; t < t1; ++t, ++tc) {
         if ((tc & 1u) == par) {
-          if (!mbar_wait(&q_full[st], ph, abort_flag, p.status, 98) ||
+          // (HEAD_DW reads the labels that came with the tile: their copy is seen through its own barrier)
+          if ((MODE == HEAD_DW && !mbar_wait(&q_full[st], ph, abort_flag, p.status, 98)) ||
               !mbar_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
           tc_fence_after();
           const int nc = cols_of(t) - half * 64;  // this group's columns: none, 32 or (64 and more) 64
@@ -353,7 +375,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
               // lane c looks at the label of column c; the lanes of one label know each other's columns
               const int rel = smem_y[st * HD_TILE + half * 64 + c0 + lane] - (int)(r - lane);
               const uint32_t same = __match_any_sync(0xffffffffu, rel);
-              uint32_t* mine = s_hits[warp - 2];
+              uint32_t* mine = s_hits[warp - HD_FIRST_EPI];
               mine[lane] = 0u;
               __syncwarp();
               if ((unsigned)rel < 32u) mine[rel] = same;
@@ -365,8 +387,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
             if (MODE == HEAD_FWD) {
               if (any) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (hits & (1u << j)) tl = f[j];
+                for (int j = 0; j < 32; ++j) hd_set_if(tl, f[j], hits, 1u << j);
               }
               float mx[4] = {f[0], f[1], f[2], f[3]};
 #pragma unroll
@@ -387,8 +408,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
               if (any) {
                 const float one = MODE == HEAD_DW ? g : 1.f;
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (hits & (1u << j)) f[j] -= one;
+                for (int j = 0; j < 32; ++j) hd_sub_if(f[j], one, hits, 1u << j);
               }
               if (MODE == HEAD_DW) {
                 float d[4] = {0.f, 0.f, 0.f, 0.f};
@@ -413,10 +433,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
           if (MODE != HEAD_FWD) hd_tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&s_done[b]);
-            if (MODE == HEAD_FWD) mbar_arrive(&q_empty[st]);
-          }
+          if (lane == 0) mbar_arrive(&s_done[b]);
           if (MODE != HEAD_FWD && pending) {
             if (!drain()) { ok = false; break; }
             pending = false;
@@ -668,9 +685,11 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
   p.rows_pad = hd_pad(p.rows);
   head_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
   p.bufs = mode == HEAD_FWD ? 4 : p.cpad <= 128 ? 3 : 2;
-  // shared memory: tiles of kboxes * 16 + 4 KB, one or two resident ones and two to four in the ring
+  // Shared memory: tiles of kboxes * 16 + 4 KB, one or two resident ones, the rest in the ring. In HEAD_DX and HEAD_DW a
+  // tile stays until its second MMA, which is `bufs` tiles later, and only what is left then hides the latency of a load
+  // (a ring of four for three tiles of s, 64 channels: 2500 clocks a tile, with exponentials or without).
   p.rbufs = p.kboxes == 1 ? 2 : 1;
-  p.stages = p.kboxes <= 2 ? 4 : p.kboxes == 3 ? 3 : 2;
+  p.stages = p.kboxes == 1 ? 8 : p.kboxes == 2 ? (mode == HEAD_FWD ? 4 : 5) : p.kboxes == 3 ? 3 : 2;
   p.status = a.status;
 }
 
@@ -690,7 +709,7 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
   if (rc) return rc;
   rc = make_map_bf16(&p.mapQ16, dw ? a.x16 : w16, 2, dw ? xv : wk, st16, box16, 32);
   if (rc) return rc;
-  constexpr int MOST = 4 * (3 * HD_BOX + HD_BOX16) + 1024 + 4 * HD_TILE * 4;  // three boxes, four tiles
+  constexpr int MOST = (MODE == HEAD_FWD ? 214 : 221) * 1024;  // beside 12 and 3 KB that are static
   const size_t smem = 1024 + (size_t)(p.rbufs + p.stages) * (p.kboxes * HD_BOX + HD_BOX16) + (size_t)p.stages * HD_TILE * 4;
   if (cudaFuncSetAttribute(head_kernel<MODE, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess)
     return SB_ERR_DRIVER;
