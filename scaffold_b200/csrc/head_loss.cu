@@ -25,8 +25,7 @@
 // of a class share) P is kept as two bf16, value and remainder, and the second MMA runs once for each.
 //
 // Roles: warp 0 loads (TMA), warps 1 and 2 issue MMAs, warps 3-18 are the epilogue: four groups of four warps, a group
-// takes the even or the odd tiles and one half of their columns. In HEAD_DW the voxels' labels travel with their tile as
-// bulk copies. All waits are bounded.
+// takes the even or the odd tiles and one half of their columns. All waits are bounded.
 // Two issuing warps: one is never more than about an MMA ahead of the tensor pipe and loses some 100 clocks at each wait
 // and some 300 at each commit, during which only the other one's MMAs can run. HEAD_DX / HEAD_DW: warp 1 the first MMAs
 // (as many tiles ahead as tensor memory holds), warp 2 the second ones; HEAD_FWD: the even and the odd tiles. One warp
@@ -61,7 +60,7 @@ struct HeadParams {
   long long rows, cols, rows_pad;
   int C, cpad, kboxes, ksteps;
   int row_tiles, col_tiles, splits, tiles_per_split;
-  int stages, rbufs, bufs;
+  int stages, rbufs, bufs, accs;
 };
 
 // D[tmem] (+)= A[tmem] * B[smem]: A holds two bf16 of K per 32-bit column, one row per lane
@@ -84,33 +83,22 @@ __device__ __forceinline__ void hd_tmem_st_x16(uint32_t taddr, const uint32_t* v
       : "memory");
 }
 __device__ __forceinline__ void hd_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// where `bits & bit`: v -= d, or v = d; predicated, never a branch
+// where `bits & bit`: v -= d; predicated, never a branch
 __device__ __forceinline__ void hd_sub_if(float& v, float d, uint32_t bits, uint32_t bit) {
   asm("{\n\t.reg .pred q;\n\t.reg .b32 t;\n\tand.b32 t, %2, %3;\n\tsetp.ne.u32 q, t, 0;\n\t@q sub.f32 %0, %0, %1;\n\t}"
       : "+f"(v)
       : "f"(d), "r"(bits), "r"(bit));
 }
-__device__ __forceinline__ void hd_set_if(float& v, float d, uint32_t bits, uint32_t bit) {
-  asm("{\n\t.reg .pred q;\n\t.reg .b32 t;\n\tand.b32 t, %2, %3;\n\tsetp.ne.u32 q, t, 0;\n\t@q mov.f32 %0, %1;\n\t}"
-      : "+f"(v)
-      : "f"(d), "r"(bits), "r"(bit));
-}
-__device__ __forceinline__ void hd_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 template <int MODE, bool LO>
 __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_constant__ HeadParams p) {
   constexpr int MAXB = 4;
   const uint32_t NB = (uint32_t)p.bufs;          // tiles of s in tensor memory
-  const uint32_t ACC = NB * HD_TILE;             // column of the accumulator
+  const uint32_t ACC = NB * HD_TILE;             // column of the accumulators
+  const uint32_t naccs = (uint32_t)p.accs;       // one or two, 64 columns apart: a job goes on while the last one's is read
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t r_full[2], r_empty[2], q_full[HD_MAX_STAGES], q_empty[HD_MAX_STAGES], s_full[MAXB], s_done[MAXB],
-      acc_full, acc_empty;
-  __shared__ uint32_t s_hits[MODE == HEAD_DW ? HD_EPI_WARPS : 1][32];
+      acc_full[2], acc_empty[2];
   __shared__ float s_fwd[MODE == HEAD_FWD ? 2 : 1][3][MODE == HEAD_FWD ? 4 : 1][HD_TILE];
   __shared__ uint32_t tmem_base_s, abort_s;
   volatile uint32_t* abort_flag = &abort_s;
@@ -120,7 +108,6 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
   const uint32_t tile_bytes = box16 + HD_BOX16;
   uint8_t* smem_r = smem;
   uint8_t* smem_q = smem + (size_t)p.rbufs * tile_bytes;
-  int* smem_y = reinterpret_cast<int*>(smem_q + (size_t)p.stages * tile_bytes);  // DW: [stages][128]
 
   if (threadIdx.x == 0) {
     abort_s = 0;
@@ -133,8 +120,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       mbar_init(&s_full[i], 1);
       mbar_init(&s_done[i], HD_EPI_WARPS / 2);
     }
-    mbar_init(&acc_full, 1);
-    mbar_init(&acc_empty, HD_EPI_WARPS);
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], HD_EPI_WARPS); }
     mbar_fence_init();
   }
   if (MODE == HEAD_FWD && threadIdx.x < HD_TILE) {
@@ -156,10 +142,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
-  auto cols_of = [&](int t) -> int {  // columns of tile t, up to a multiple of 32
-    const long long left = p.cols - (long long)t * HD_TILE;
-    return left >= HD_TILE ? HD_TILE : (int)(left + 31) / 32 * 32;
-  };
+  const int last_cols = ((int)(p.cols - (long long)(p.col_tiles - 1) * HD_TILE) + 31) & ~31;
+  auto cols_of = [&](int t) -> int { return t + 1 < p.col_tiles ? HD_TILE : last_cols; };  // up to a multiple of 32
 
   if (warp == 0) {
     if (lane == 0) {
@@ -180,12 +164,10 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
         for (int t = t0; t < t1; ++t) {
           if (!mbar_wait(&q_empty[st], ph ^ 1u, abort_flag, p.status, 91)) { ok = false; break; }
-          mbar_expect_tx(&q_full[st], tile_bytes + (MODE == HEAD_DW ? HD_TILE * 4 : 0));
+          mbar_expect_tx(&q_full[st], tile_bytes);
           for (int k = 0; k < p.kboxes; ++k)
             hd_tma_2d(smem_q + st * tile_bytes + k * HD_BOX, &p.mapQ, &q_full[st], k * 64, t * HD_TILE);
           hd_tma_2d(smem_q + st * tile_bytes + box16, &p.mapQ16, &q_full[st], 0, t * HD_TILE);
-          if (MODE == HEAD_DW)
-            hd_bulk(smem_y + st * HD_TILE, p.coly + (long long)t * HD_TILE, HD_TILE * 4, &q_full[st]);
           if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
         }
       }
@@ -249,14 +231,14 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
     const uint32_t q0 = smem_u32(smem_q);
     const uint32_t idesc = make_idesc_bf16(128, p.cpad, 0, 1);
     const uint32_t lbo = p.kboxes > 1 ? (uint32_t)HD_BOX : 0u;
-    uint32_t st = 0, ph = 0, b = 0, bph = 0, aph = 0;
+    uint32_t st = 0, ph = 0, b = 0, bph = 0, ab = 0, aph = 0;
     bool ok = true;
     for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
       const int sp = job / p.row_tiles;
       const int t0 = sp * p.tiles_per_split;
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
-      if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty, aph ^ 1u, abort_flag, p.status, 92))) { ok = false; break; }
-      aph ^= 1u;
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[ab], aph ^ 1u, abort_flag, p.status, 92))) { ok = false; break; }
+      const uint32_t acc = tmem + ACC + ab * 64u;
       for (int t = t0; t < t1; ++t) {
         const int ksteps = cols_of(t) / 16;
         const uint32_t lo = desc_lo(q0 + st * tile_bytes, lbo);
@@ -269,34 +251,39 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
 #pragma unroll
           for (int part = 0; part < (LO ? 2 : 1); ++part)
             for (int k = 0; k < ksteps; ++k)
-              hd_mma_ts(tmem + ACC, a + 32 * (k >> 1) + 16 * part + 8 * (k & 1), lo + k * 128u, hi, idesc,
+              hd_mma_ts(acc, a + 32 * (k >> 1) + 16 * part + 8 * (k & 1), lo + k * 128u, hi, idesc,
                         t == t0 && part == 0 && k == 0 ? 0u : 1u);
           tc_commit(&q_empty[st]);
-          if (t == t1 - 1) tc_commit(&acc_full);
+          if (t == t1 - 1) tc_commit(&acc_full[ab]);
         }
         __syncwarp();
         if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
         if (++b == NB) { b = 0; bph ^= 1u; }
       }
+      if (++ab == naccs) { ab = 0; aph ^= 1u; }
     }
   } else {
     const int quad = warp & 3, group = (warp - HD_FIRST_EPI) >> 2, half = group & 1;
     const uint32_t par = group >> 1;
     const int row = quad * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    uint32_t st = 0, ph = 0, b = 0, bph = 0, aph = 0, tc = 0, jc = 0;
+    uint32_t b = par, bph = 0, ab = 0, aph = 0, tc = 0, jc = 0;  // b: buffer of this group's next tile (two or more there are)
     bool ok = true, pending = false;
     int pend_rt = 0, pend_sp = 0;
     float pend_g = 0.f, pend_db = 0.f;
+    uint32_t rank_bits[5];  // HEAD_DW: all ones where the lane's number has a zero
+    if (MODE == HEAD_DW) {
+#pragma unroll
+      for (int k = 0; k < 5; ++k) rank_bits[k] = lane >> k & 1 ? 0u : ~0u;
+    }
     // the accumulator of a finished job
     auto drain = [&]() -> bool {
-      if (!mbar_wait(&acc_full, aph, abort_flag, p.status, 97)) return false;
-      aph ^= 1u;
+      if (!mbar_wait(&acc_full[ab], aph, abort_flag, p.status, 97)) return false;
       tc_fence_after();
       const long long r = (long long)pend_rt * HD_TILE + row;
       for (int c0 = group * 16; c0 < p.cpad; c0 += 64) {
         uint32_t v[16];
-        tmem_ld_32x16(lane_base + ACC + c0, v);
+        tmem_ld_32x16(lane_base + ACC + ab * 64u + c0, v);
         tmem_ld_wait();
         float f[16];
 #pragma unroll
@@ -324,35 +311,50 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       if (MODE == HEAD_DW) p.ws_b[((long long)pend_sp * 4 + group) * p.rows_pad + r] = pend_db;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty);
+      if (lane == 0) mbar_arrive(&acc_empty[ab]);
+      if (++ab == naccs) { ab = 0; aph ^= 1u; }
       return true;
     };
     // a row's own values; the next job's are read while this one runs
-    auto row_at = [&](int job) { return (long long)(job % p.row_tiles) * HD_TILE + row; };
     int y_next = -1;
     float g_next = 1.f;
-    auto fetch = [&](int job) {
-      if (job >= jobs) return;
-      const long long r = row_at(job);
+    auto fetch = [&](int rt) {
+      const long long r = (long long)rt * HD_TILE + row;
       if (MODE != HEAD_DW) y_next = __ldg(p.rowy + r);
       if (MODE == HEAD_DX) g_next = __ldg(p.rowg + r);
       if (MODE == HEAD_DW && p.roww != nullptr && r < p.rows) g_next = __ldg(p.roww + r);
     };
-    fetch(blockIdx.x);
-    for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x, ++jc) {
-      const int rt = job % p.row_tiles, sp = job / p.row_tiles;
+    int rt = blockIdx.x % p.row_tiles, sp = blockIdx.x / p.row_tiles;
+    fetch(rt);
+    while (sp < p.splits && ok) {
       const int t0 = sp * p.tiles_per_split;
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
       const long long r = (long long)rt * HD_TILE + row;
       const int y = y_next;
       const float g = g_next;
-      fetch(job + gridDim.x);
+      int next_rt = rt + gridDim.x, next_sp = sp;
+      if (next_rt >= p.row_tiles) {
+        next_sp += next_rt / p.row_tiles;
+        next_rt %= p.row_tiles;
+      }
+      if (next_sp < p.splits) fetch(next_rt);
       float m = HD_LOWEST, s = 0.f, tl = 0.f, db = 0.f;
-      for (int t = t0; t < t1; ++t, ++tc) {
-        if ((tc & 1u) == par) {
-          // (HEAD_DW reads the labels that came with the tile: their copy is seen through its own barrier)
-          if ((MODE == HEAD_DW && !mbar_wait(&q_full[st], ph, abort_flag, p.status, 98)) ||
-              !mbar_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
+      // this group's tiles of the job: every second one over all jobs
+      int t = t0 + (int)((tc ^ par) & 1u);
+      tc += t1 - t0;
+      const int* labels = MODE == HEAD_DW ? p.coly + half * 64 + lane : nullptr;
+      int label[2] = {-1, -1};  // HEAD_DW: of the tile's column `lane`, and 32 further; a tile ahead
+      if (MODE == HEAD_DW && t < t1) {
+        label[0] = __ldg(labels + (long long)t * HD_TILE);
+        label[1] = __ldg(labels + (long long)t * HD_TILE + 32);
+      }
+      for (; t < t1; t += 2) {
+          if (!mbar_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
+          int rel[2] = {label[0] - (int)(r - lane), label[1] - (int)(r - lane)};
+          if (MODE == HEAD_DW && t + 2 < t1) {
+            label[0] = __ldg(labels + (long long)(t + 2) * HD_TILE);
+            label[1] = __ldg(labels + (long long)(t + 2) * HD_TILE + 32);
+          }
           tc_fence_after();
           const int nc = cols_of(t) - half * 64;  // this group's columns: none, 32 or (64 and more) 64
           const int c_abs = t * HD_TILE + half * 64;
@@ -372,22 +374,24 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
               const int at = y - (c_abs + c0);
               hits = (unsigned)at < 32u ? 1u << at : 0u;
             } else {
-              // lane c looks at the label of column c; the lanes of one label know each other's columns
-              const int rel = smem_y[st * HD_TILE + half * 64 + c0 + lane] - (int)(r - lane);
-              const uint32_t same = __match_any_sync(0xffffffffu, rel);
-              uint32_t* mine = s_hits[warp - HD_FIRST_EPI];
-              mine[lane] = 0u;
-              __syncwarp();
-              if ((unsigned)rel < 32u) mine[rel] = same;
-              __syncwarp();
-              hits = mine[lane];
-              __syncwarp();
+              // lane c has the label of column c; a row's columns are those whose label has the row's five bits
+              hits = __ballot_sync(0xffffffffu, (unsigned)rel[c0 / 32] < 32u);
+#pragma unroll
+              for (int k = 0; k < 5; ++k)
+                hits &= __ballot_sync(0xffffffffu, rel[c0 / 32] >> k & 1) ^ rank_bits[k];
             }
             const bool any = __any_sync(0xffffffffu, hits != 0u);
             if (MODE == HEAD_FWD) {
-              if (any) {
+              if (any) {  // f[at], by halves
+                const int at = y - (c_abs + c0);
+                float h[16];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) hd_set_if(tl, f[j], hits, 1u << j);
+                for (int j = 0; j < 16; ++j) h[j] = at & 16 ? f[16 + j] : f[j];
+#pragma unroll
+                for (int n = 8; n > 0; n >>= 1)
+#pragma unroll
+                  for (int j = 0; j < n; ++j) h[j] = at & n ? h[n + j] : h[j];
+                if (hits) tl = h[0];
               }
               float mx[4] = {f[0], f[1], f[2], f[3]};
 #pragma unroll
@@ -438,9 +442,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
             if (!drain()) { ok = false; break; }
             pending = false;
           }
-        }
-        if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
-        if (++b == NB) { b = 0; bph ^= 1u; }
+          b += 2;
+          if (b >= NB) { b -= NB; bph ^= 1u; }
       }
       if (MODE == HEAD_FWD) {
         // the four groups' shares of a row; two sets of buffers, so that a group that is a job ahead overwrites nothing
@@ -449,11 +452,12 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         s_fwd[set][1][group][row] = s;
         s_fwd[set][2][group][row] = tl;
         ok = hd_vote(1 + quad, 128, ok);
-        if (group == 0 && ok) {
+        if (group == (int)(jc & 3u) && ok) {
+          m = s_fwd[set][0][0][row];
           for (int k = 1; k < 4; ++k) m = fmaxf(m, s_fwd[set][0][k][row]);
-          s = 0.f;
+          s = tl = 0.f;
           for (int k = 0; k < 4; ++k) s += s_fwd[set][1][k][row] * hd_ex2((s_fwd[set][0][k][row] - m) * HD_LOG2E);
-          for (int k = 1; k < 4; ++k) tl += s_fwd[set][2][k][row];  // one of them has met the label, the others hold 0
+          for (int k = 0; k < 4; ++k) tl += s_fwd[set][2][k][row];  // one of them has met the label, the others hold 0
           p.part[(long long)sp * p.rows_pad + r] = make_float2(m * HD_LOG2E, s);
           if (y >= (long long)t0 * HD_TILE && y < (long long)t1 * HD_TILE) p.tl[r] = tl * HD_LOG2E;
         }
@@ -462,6 +466,9 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         pending = true;
         pend_rt = rt; pend_sp = sp; pend_g = g; pend_db = db;
       }
+      rt = next_rt;
+      sp = next_sp;
+      ++jc;
     }
     if (MODE != HEAD_FWD && ok && pending) drain();
   }
@@ -685,6 +692,7 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
   p.rows_pad = hd_pad(p.rows);
   head_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
   p.bufs = mode == HEAD_FWD ? 4 : p.cpad <= 128 ? 3 : 2;
+  p.accs = p.cpad <= 64 ? 2 : 1;
   // Shared memory: tiles of kboxes * 16 + 4 KB, one or two resident ones, the rest in the ring. In HEAD_DX and HEAD_DW a
   // tile stays until its second MMA, which is `bufs` tiles later, and only what is left then hides the latency of a load
   // (a ring of four for three tiles of s, 64 channels: 2500 clocks a tile, with exponentials or without).
@@ -710,7 +718,7 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
   rc = make_map_bf16(&p.mapQ16, dw ? a.x16 : w16, 2, dw ? xv : wk, st16, box16, 32);
   if (rc) return rc;
   constexpr int MOST = (MODE == HEAD_FWD ? 214 : 221) * 1024;  // beside 12 and 3 KB that are static
-  const size_t smem = 1024 + (size_t)(p.rbufs + p.stages) * (p.kboxes * HD_BOX + HD_BOX16) + (size_t)p.stages * HD_TILE * 4;
+  const size_t smem = 1024 + (size_t)(p.rbufs + p.stages) * (p.kboxes * HD_BOX + HD_BOX16);
   if (cudaFuncSetAttribute(head_kernel<MODE, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess)
     return SB_ERR_DRIVER;
   const long long jobs = (long long)p.row_tiles * p.splits;
