@@ -285,26 +285,20 @@ __global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE) gn8_bwd_dx_kernel(const
          __ldg(reinterpret_cast<const uint4*>(p.dy + at)), at);
 }
 
-static int gn8_fill(const SbGn8Args* a, Gn8Params& p) {
-  if (!sb_gn_supported(a->C, a->G) || a->C % KEPT_BLOCK || a->N < 1 || a->N > 65535 || a->S < 1) return SB_ERR_SHAPE;
-  if (a->w == nullptr || a->b == nullptr || a->kept == nullptr || a->mean == nullptr || a->rstd == nullptr)
-    return SB_ERR_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->dy) | reinterpret_cast<uintptr_t>(a->y) |
-       reinterpret_cast<uintptr_t>(a->kept)) & 15)
-    return SB_ERR_ALIGN;
+static bool gn8_ok(int N, long long S, int C, int G) {
+  return sb_gn_supported(C, G) && C % KEPT_BLOCK == 0 && N >= 1 && N <= 65535 && S >= 1;
+}
+static void gn8_fill(Gn8Params& p, void* kept, const float* w, const float* b, float* stats, int N, long long S, int C,
+                     int G, int relu) {
   memset(&p, 0, sizeof(p));
-  p.x = (const __nv_bfloat16*)a->x;
-  p.dy = (const __nv_bfloat16*)a->dy;
-  p.y = (__nv_bfloat16*)a->y;
-  p.q = (uint8_t*)a->kept;
-  p.exps = p.q + (long long)a->N * a->S * a->C;
-  p.w = a->w; p.b = a->b; p.mean = a->mean; p.rstd = a->rstd;
-  p.fin = a->fin; p.part = a->part; p.dw = a->dw; p.db = a->db;
-  p.N = a->N; p.C = a->C; p.G = a->G; p.S = a->S;
-  p.nsplit = a->nsplit; p.relu = a->relu; p.accumulate = a->accumulate;
-  p.eps = a->eps;
-  p.group_elems = (float)((double)a->S * (a->C / a->G));
-  return 0;
+  p.q = (uint8_t*)kept;
+  p.exps = p.q + (long long)N * S * C;
+  p.w = w; p.b = b;
+  p.mean = stats;
+  p.rstd = stats + (long long)N * G;
+  p.N = N; p.C = C; p.G = G; p.S = S;
+  p.relu = relu;
+  p.group_elems = (float)((double)S * (C / G));
 }
 static int gn8_blocks(const Gn8Params& p) {
   const int vpb = GN8_THREADS / (p.C / 8);
@@ -317,42 +311,81 @@ static int gn8_blocks(const Gn8Params& p) {
 
 using namespace sb;
 
-extern "C" int sb_gn8_apply(const SbGn8Args* a, cudaStream_t stream) {
+static long long gn8_floats(long long n) { return (n + 63) / 64 * 64; }
+
+// fp32 scratch of the forward (0) and the backward pass (1); -1: outside the kernels' range
+extern "C" long long sb_gn8_scratch(int backward, int N, long long S, int C, int G) {
+  if (!gn8_ok(N, S, C, G)) return -1;
+  if (backward) return gn8_floats((long long)N * sb_gn_bwd_nsplit(N, S, C) * C * 2) + gn8_floats((long long)N * C * 2);
+  return gn8_floats((long long)N * sb_gn_nsplit(N, S, C) * G * 3) + gn8_floats((long long)N * G * 3);
+}
+
+// fin: the statistics when the tensor's producer has them, else null; hand_over: the statistics kernel's last block
+// collapses its partials (not inside a captured graph, see gn_kernels.py)
+extern "C" int sb_gn8_forward(const void* x, const float* w, const float* b, int N, long long S, int C, int G, float eps,
+                              int relu, const float* fin, int hand_over, void* y, void* kept, float* stats,
+                              float* scratch, cudaStream_t stream) {
+  if (!gn8_ok(N, S, C, G) || !x || !w || !b || !y || !kept || !stats || (!fin && !scratch)) return SB_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(kept)) & 15)
+    return SB_ERR_ALIGN;
+  if (fin == nullptr) {
+    SbGnArgs a;
+    memset(&a, 0, sizeof(a));
+    a.x = x; a.w = w; a.b = b;
+    a.N = N; a.C = C; a.G = G; a.S = a.S_total = S;
+    a.eps = eps; a.relu = relu;
+    a.nsplit = sb_gn_nsplit(N, S, C);
+    a.part = scratch;
+    a.parts[0] = scratch;
+    a.n_parts = 1;
+    float* own = scratch + gn8_floats((long long)N * a.nsplit * G * 3);
+    if (hand_over) a.fin = own;
+    int rc = sb_gn_stats(&a, stream);
+    if (rc == 0 && !hand_over) rc = sb_gn_stats_finalize(scratch, own, N, G, a.nsplit, stream);
+    if (rc) return rc;
+    fin = own;
+  }
   Gn8Params p;
-  const int rc = gn8_fill(a, p);
-  if (rc) return rc;
-  if (p.x == nullptr || p.y == nullptr || p.fin == nullptr) return SB_ERR_SHAPE;
+  gn8_fill(p, kept, w, b, stats, N, S, C, G, relu);
+  p.x = (const __nv_bfloat16*)x;
+  p.y = (__nv_bfloat16*)y;
+  p.fin = fin;
+  p.eps = eps;
   const dim3 grid(gn8_blocks(p), p.N);
-  if (p.relu) gn8_apply_kernel<true><<<grid, GN8_THREADS, 0, stream>>>(p);
+  if (relu) gn8_apply_kernel<true><<<grid, GN8_THREADS, 0, stream>>>(p);
   else gn8_apply_kernel<false><<<grid, GN8_THREADS, 0, stream>>>(p);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
-extern "C" int sb_gn8_bwd_partial(const SbGn8Args* a, cudaStream_t stream) {
-  Gn8Params p;
-  const int rc = gn8_fill(a, p);
+template <int GP, bool RELU>
+static int gn8_backward(Gn8Params& p, float* fin, cudaStream_t stream) {
+  gn8_bwd_partial_kernel<GP, RELU><<<dim3(p.nsplit, p.N), GN8_THREADS, 0, stream>>>(p);
+  sb_count_launch(1);
+  const int rc = sb_gn_bwd_finalize(p.part, fin, p.N, p.C, p.nsplit, stream);
   if (rc) return rc;
-  if (p.dy == nullptr || p.part == nullptr || p.nsplit < 1) return SB_ERR_SHAPE;
-  const dim3 grid(p.nsplit, p.N);
-  const int gp = p.C / p.G >= 8 ? 1 : 8 / (p.C / p.G);
-  if (gp == 1) p.relu ? gn8_bwd_partial_kernel<1, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_partial_kernel<1, false><<<grid, GN8_THREADS, 0, stream>>>(p);
-  else if (gp == 2) p.relu ? gn8_bwd_partial_kernel<2, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_partial_kernel<2, false><<<grid, GN8_THREADS, 0, stream>>>(p);
-  else p.relu ? gn8_bwd_partial_kernel<4, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_partial_kernel<4, false><<<grid, GN8_THREADS, 0, stream>>>(p);
+  p.fin = fin;
+  gn8_bwd_dx_kernel<GP, RELU><<<dim3(gn8_blocks(p), p.N), GN8_THREADS, 0, stream>>>(p);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 
-extern "C" int sb_gn8_bwd_dx(const SbGn8Args* a, cudaStream_t stream) {
+extern "C" int sb_gn8_backward(const void* dy, const void* kept, const float* w, const float* b, const float* stats, int N,
+                               long long S, int C, int G, int relu, void* dx, float* dw, float* db, int accumulate,
+                               float* scratch, cudaStream_t stream) {
+  if (!gn8_ok(N, S, C, G) || !dy || !kept || !w || !b || !stats || !dx || !dw || !db || !scratch) return SB_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(kept)) & 15)
+    return SB_ERR_ALIGN;
   Gn8Params p;
-  const int rc = gn8_fill(a, p);
-  if (rc) return rc;
-  if (p.dy == nullptr || p.y == nullptr || p.fin == nullptr || p.dw == nullptr || p.db == nullptr) return SB_ERR_SHAPE;
-  const dim3 grid(gn8_blocks(p), p.N);
-  const int gp = p.C / p.G >= 8 ? 1 : 8 / (p.C / p.G);
-  if (gp == 1) p.relu ? gn8_bwd_dx_kernel<1, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_dx_kernel<1, false><<<grid, GN8_THREADS, 0, stream>>>(p);
-  else if (gp == 2) p.relu ? gn8_bwd_dx_kernel<2, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_dx_kernel<2, false><<<grid, GN8_THREADS, 0, stream>>>(p);
-  else p.relu ? gn8_bwd_dx_kernel<4, true><<<grid, GN8_THREADS, 0, stream>>>(p) : gn8_bwd_dx_kernel<4, false><<<grid, GN8_THREADS, 0, stream>>>(p);
-  sb_count_launch(1);
-  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  gn8_fill(p, const_cast<void*>(kept), w, b, const_cast<float*>(stats), N, S, C, G, relu);
+  p.dy = (const __nv_bfloat16*)dy;
+  p.y = (__nv_bfloat16*)dx;
+  p.dw = dw; p.db = db;
+  p.accumulate = accumulate;
+  p.nsplit = sb_gn_bwd_nsplit(N, S, C);
+  p.part = scratch;
+  float* fin = scratch + gn8_floats((long long)N * p.nsplit * C * 2);
+  const int gp = C / G >= 8 ? 1 : 8 / (C / G);
+  if (relu) return gp == 1 ? gn8_backward<1, true>(p, fin, stream) : gp == 2 ? gn8_backward<2, true>(p, fin, stream) : gn8_backward<4, true>(p, fin, stream);
+  return gp == 1 ? gn8_backward<1, false>(p, fin, stream) : gp == 2 ? gn8_backward<2, false>(p, fin, stream) : gn8_backward<4, false>(p, fin, stream);
 }

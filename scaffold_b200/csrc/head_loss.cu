@@ -30,6 +30,8 @@
 // and some 300 at each commit, during which only the other one's MMAs can run. HEAD_DX / HEAD_DW: warp 1 the first MMAs
 // (as many tiles ahead as tensor memory holds), warp 2 the second ones; HEAD_FWD: the even and the odd tiles. One warp
 // for everything took 2150 clocks a tile at 64 channels, the exponentials left out or not.
+#include <atomic>
+
 #include "head_loss.cuh"
 
 namespace sb {
@@ -565,11 +567,23 @@ __device__ __forceinline__ HeadSum hd_block_sum(HeadSum a) {
   return t;
 }
 
-// lse2[i] from the splits' running maxima and sums, merged in split order; block sums of u nll and u in double
+// loss = num / max(den, eps), den the clamped denominator
+__device__ __forceinline__ void hd_loss(const HeadSum& a, double* total, float* loss, float* den) {
+  const double eps = 1.1920928955078125e-7, d = a.den < eps ? eps : a.den;  // NaN stays
+  total[0] = a.num;
+  total[1] = a.den;
+  loss[0] = (float)(a.num / d);
+  den[0] = (float)d;
+}
+
+// lse2[i] from the splits' running maxima and sums, merged in split order; block sums of u nll and u in double (a single
+// block goes on to the loss)
 __global__ void __launch_bounds__(256) head_merge_kernel(const float2* __restrict__ part, const float* __restrict__ tl,
                                                          const int* __restrict__ y, const float* __restrict__ cw,
                                                          int splits, long long V, long long v_pad,
-                                                         float* __restrict__ lse2, double* __restrict__ sums) {
+                                                         float* __restrict__ lse2, double* __restrict__ sums,
+                                                         double* __restrict__ total, float* __restrict__ loss,
+                                                         float* __restrict__ den) {
   HeadSum a{0.0, 0.0};
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < v_pad; i += (long long)gridDim.x * 256) {
     float l = INFINITY;
@@ -593,23 +607,20 @@ __global__ void __launch_bounds__(256) head_merge_kernel(const float2* __restric
     lse2[i] = l;
   }
   a = hd_block_sum(a);
-  if (threadIdx.x == 0) { sums[2 * blockIdx.x] = a.num; sums[2 * blockIdx.x + 1] = a.den; }
+  if (threadIdx.x == 0) {
+    if (gridDim.x == 1) hd_loss(a, total, loss, den);
+    else { sums[2 * blockIdx.x] = a.num; sums[2 * blockIdx.x + 1] = a.den; }
+  }
 }
 
-// total[2] = the blocks' sums in order; loss = num / max(den, eps), den the clamped denominator
+// total[2] = the blocks' sums in order, and the loss
 __global__ void __launch_bounds__(256) head_total_kernel(const double* __restrict__ sums, int blocks,
                                                          double* __restrict__ total, float* __restrict__ loss,
                                                          float* __restrict__ den) {
   HeadSum a{0.0, 0.0};
   for (int i = threadIdx.x; i < blocks; i += 256) { a.num += sums[2 * i]; a.den += sums[2 * i + 1]; }
   a = hd_block_sum(a);
-  if (threadIdx.x == 0) {
-    const double eps = 1.1920928955078125e-7, d = a.den < eps ? eps : a.den;  // NaN stays
-    total[0] = a.num;
-    total[1] = a.den;
-    loss[0] = (float)(a.num / d);
-    den[0] = (float)d;
-  }
+  if (threadIdx.x == 0) hd_loss(a, total, loss, den);
 }
 
 // what the backward passes need of a voxel; x16 (narrow heads): its sixteen columns more
@@ -632,30 +643,38 @@ __global__ void __launch_bounds__(256) head_weights_kernel(HeadCall a, const flo
   }
 }
 
-// out[r][c] = scale * sum over the slices of ws[slice][rows_pad][ld], in slice order; r < rows, c < C. A block takes 32
-// neighbouring outputs, each of its eight warps every eighth slice: a thread that walks all slices waits an L2 trip for
-// a few of them at a time.
-template <typename T>
-__global__ void __launch_bounds__(256) head_reduce_kernel(const float* __restrict__ ws, int slices, long long rows,
-                                                          long long rows_pad, int C, int ld,
-                                                          const float* __restrict__ scale, T* __restrict__ out) {
+// One sum over slices: out[r][c] = scale * sum of ws[slice][rows_pad][ld] in slice order, r < rows, c < C.
+struct HeadReduce {
+  const float* ws;
+  int slices, C, ld, kind, blocks;  // kind of out: 0 bf16, 2 fp32
+  long long rows, rows_pad;
+  void* out;
+};
+// The first a.blocks blocks take a, the others b (dw and db). A block takes 32 neighbouring outputs, each of its eight
+// warps every eighth slice: a thread that walks all slices waits an L2 trip for a few of them at a time.
+__global__ void __launch_bounds__(256) head_reduce_kernel(const HeadReduce a, const HeadReduce b,
+                                                          const float* __restrict__ scale) {
   __shared__ float s_part[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long n = rows * C, slice = rows_pad * ld;
+  const bool first = (int)blockIdx.x < a.blocks;
+  const HeadReduce& p = first ? a : b;
+  const long long n = p.rows * p.C, slice = p.rows_pad * p.ld;
   const float k = scale != nullptr ? scale[0] : 1.f;
-  for (long long i0 = (long long)blockIdx.x * 32; i0 < n; i0 += (long long)gridDim.x * 32) {
+  for (long long i0 = (long long)(first ? blockIdx.x : blockIdx.x - a.blocks) * 32; i0 < n; i0 += (long long)p.blocks * 32) {
     const long long i = i0 + lane;
-    float a = 0.f;
+    float sum = 0.f;
     if (i < n) {
-      const float* src = ws + i / C * ld + i % C;
+      const float* src = p.ws + i / p.C * p.ld + i % p.C;
 #pragma unroll 4
-      for (int s = warp; s < slices; s += 8) a += src[s * slice];
+      for (int s = warp; s < p.slices; s += 8) sum += src[s * slice];
     }
-    s_part[warp][lane] = a;
+    s_part[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && i < n) {
-      for (int w = 1; w < 8; ++w) a += s_part[w][lane];
-      out[i] = hd_cast<T>(a * k);
+      for (int w = 1; w < 8; ++w) sum += s_part[w][lane];
+      sum *= k;
+      if (p.kind == 2) reinterpret_cast<float*>(p.out)[i] = sum;
+      else reinterpret_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16(sum);
     }
     __syncthreads();
   }
@@ -719,8 +738,14 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
   if (rc) return rc;
   constexpr int MOST = (MODE == HEAD_FWD ? 214 : 221) * 1024;  // beside 12 and 3 KB that are static
   const size_t smem = 1024 + (size_t)(p.rbufs + p.stages) * (p.kboxes * HD_BOX + HD_BOX16);
-  if (cudaFuncSetAttribute(head_kernel<MODE, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess)
-    return SB_ERR_DRIVER;
+  static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have that much
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return SB_ERR_DRIVER;
+  if (dev > 63 || !(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
+    if (cudaFuncSetAttribute(head_kernel<MODE, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess)
+      return SB_ERR_DRIVER;
+    if (dev <= 63) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   const long long jobs = (long long)p.row_tiles * p.splits;
   head_kernel<MODE, LO><<<(int)(jobs < 148 ? jobs : 148), HD_THREADS, smem, stream>>>(p);
   sb_count_launch(1);
@@ -782,12 +807,16 @@ static long long head_bwd_scratch(HeadCall& a, void* base) {
   return at - (char*)base + 4 * (dx > dw ? dx : dw);
 }
 
-template <typename T>
-static void head_reduce(const float* ws, int slices, long long rows, long long rows_pad, int C, int ld,
-                        const float* scale, void* out, cudaStream_t stream) {
-  const long long blocks = (rows * C + 31) / 32;
-  head_reduce_kernel<T><<<(int)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(ws, slices, rows, rows_pad, C, ld,
-                                                                                       scale, (T*)out);
+static HeadReduce reduce_of(const float* ws, int slices, const HeadParams& p, int C, int ld, int kind, void* out) {
+  HeadReduce r;
+  r.ws = ws; r.slices = slices; r.C = C; r.ld = ld; r.kind = kind; r.out = out;
+  r.rows = p.rows; r.rows_pad = p.rows_pad;
+  const long long blocks = out == nullptr ? 0 : (p.rows * C + 31) / 32;
+  r.blocks = (int)(blocks < 148 * 8 ? blocks : 148 * 8);
+  return r;
+}
+static void head_reduce(const HeadReduce& a, const HeadReduce& b, const float* scale, cudaStream_t stream) {
+  head_reduce_kernel<<<a.blocks + b.blocks, 256, 0, stream>>>(a, b, scale);
   sb_count_launch(1);
 }
 
@@ -804,7 +833,8 @@ static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
     rc = few ? head_launch<HEAD_DX, true>(a, p, stream) : head_launch<HEAD_DX, false>(a, p, stream);
     if (rc) return rc;
     if (p.splits > 1)
-      head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, nullptr, a.dx, stream);
+      head_reduce(reduce_of(p.ws, p.splits, p, p.C, p.cpad, 0, a.dx), reduce_of(nullptr, 0, p, 1, 1, 0, nullptr), nullptr,
+                  stream);
   }
   if (a.dw != nullptr || a.db != nullptr) {
     head_geometry(a, HEAD_DW, p);
@@ -814,14 +844,8 @@ static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
     p.ws_b = a.scratch + p.splits * p.rows_pad * p.cpad;
     rc = few || a.cw != nullptr ? head_launch<HEAD_DW, true>(a, p, stream) : head_launch<HEAD_DW, false>(a, p, stream);
     if (rc) return rc;
-    if (a.dw != nullptr) {
-      if (a.dw_kind == 2) head_reduce<float>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a.scale, a.dw, stream);
-      else head_reduce<__nv_bfloat16>(p.ws, p.splits, p.rows, p.rows_pad, p.C, p.cpad, a.scale, a.dw, stream);
-    }
-    if (a.db != nullptr) {
-      if (a.db_kind == 2) head_reduce<float>(p.ws_b, 4 * p.splits, p.rows, p.rows_pad, 1, 1, a.scale, a.db, stream);
-      else head_reduce<__nv_bfloat16>(p.ws_b, 4 * p.splits, p.rows, p.rows_pad, 1, 1, a.scale, a.db, stream);
-    }
+    head_reduce(reduce_of(p.ws, p.splits, p, p.C, p.cpad, a.dw_kind, a.dw),
+                reduce_of(p.ws_b, 4 * p.splits, p, 1, 1, a.db_kind, a.db), a.scale, stream);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
@@ -877,10 +901,11 @@ extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, i
     rc = head_launch<HEAD_FWD, false>(a, p, stream);
   }
   if (rc) return rc;
-  const int blocks = hd_blocks(v_pad, HD_SUM_BLOCKS / 148);
-  head_merge_kernel<<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, f.sums);
-  head_total_kernel<<<1, 256, 0, stream>>>(f.sums, blocks, a.total, loss, a.den);
-  sb_count_launch(2);
+  const int blocks = v_pad <= 4096 ? 1 : hd_blocks(v_pad, HD_SUM_BLOCKS / 148);  // 16 rounds cost less than a launch
+  head_merge_kernel<<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, f.sums, a.total, loss,
+                                                a.den);
+  if (blocks > 1) head_total_kernel<<<1, 256, 0, stream>>>(f.sums, blocks, a.total, loss, a.den);
+  sb_count_launch(blocks > 1 ? 2 : 1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 

@@ -70,10 +70,6 @@ __device__ __forceinline__ bool hd_vote(int id, int threads, bool ok) {
       : "memory");
   return all != 0;
 }
-template <typename T> __device__ __forceinline__ T hd_cast(float v);
-template <> __device__ __forceinline__ float hd_cast<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 hd_cast<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
-
 // head_wide.cu
 int head_wide_splits(long long V, int K);
 int head_wide_forward(const HeadCall& a, float2* part, float* tl, cudaStream_t stream);

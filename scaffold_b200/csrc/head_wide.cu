@@ -11,6 +11,8 @@
 // Roundings as in head_loss.cu; here the class weights go into a copy of X (whose roundings are independent of one
 // another) and up to HD_FEW voxels P^T is followed by its remainder, along which the products' reductions go on.
 // One thread holds a row of a tile, so a row's maximum, sum and db need no exchange.
+#include <atomic>
+
 #include "head_loss.cuh"
 #include "pair.cuh"
 
@@ -402,15 +404,17 @@ __global__ void __launch_bounds__(256) head_weigh_kernel(const __nv_bfloat16* __
   }
 }
 
-static int g_hw_pairs = 0;
+// SM pairs that can hold a cluster at the same time (a GPC with an odd SM count leaves one SM out)
 template <int EPI, int A_MN, int B_MN>
-static int wide_setup() {
+static int wide_setup(int* pairs) {
+  static std::atomic<int> known[64];  // by device; 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return SB_ERR_DRIVER;
+  if (dev < 64 && (*pairs = known[dev].load(std::memory_order_relaxed)) > 0) return 0;
   const int smem = 1024 + HW_STAGES * HW_STAGE;
   if (cudaFuncSetAttribute(head_wide_kernel<EPI, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
       cudaSuccess)
     return SB_ERR_DRIVER;
-  if (g_hw_pairs) return 0;
-  // SM pairs that can hold a cluster at the same time (a GPC with an odd SM count leaves one SM out)
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(148);
@@ -424,18 +428,20 @@ static int wide_setup() {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   int n = 0;
-  const bool known = cudaOccupancyMaxActiveClusters(&n, head_wide_kernel<EPI, A_MN, B_MN>, &cfg) == cudaSuccess;
+  const bool ok = cudaOccupancyMaxActiveClusters(&n, head_wide_kernel<EPI, A_MN, B_MN>, &cfg) == cudaSuccess;
   cudaGetLastError();
-  g_hw_pairs = known && n > 0 && n < 74 ? n : 74;
+  *pairs = ok && n > 0 && n < 74 ? n : 74;
+  if (dev < 64) known[dev].store(*pairs, std::memory_order_relaxed);
   return 0;
 }
 
 template <int EPI, int A_MN, int B_MN>
 static int wide_launch(WideParams& p, cudaStream_t stream) {
-  const int rc = wide_setup<EPI, A_MN, B_MN>();
+  int most = 0;
+  const int rc = wide_setup<EPI, A_MN, B_MN>(&most);
   if (rc) return rc;
   const long long jobs = EPI == WIDE_OUT ? (long long)p.row_tiles * p.col_tiles * p.kslices : (long long)p.row_tiles * p.splits;
-  const int pairs = (int)(jobs < g_hw_pairs ? jobs : g_hw_pairs);
+  const int pairs = (int)(jobs < most ? jobs : most);
   head_wide_kernel<EPI, A_MN, B_MN><<<2 * pairs, HW_THREADS, 1024 + HW_STAGES * HW_STAGE, stream>>>(p);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;

@@ -180,33 +180,16 @@ long long sb_kept8_bytes(long long n);
 int sb_keep8(const void* x, int kind, long long n, void* kept, cudaStream_t stream);
 int sb_restore8(const void* kept, int kind, long long n, void* y, cudaStream_t stream);
 
-// GroupNorm (+ReLU) with an 8-bit copy of its input for the backward pass (group_norm_kept8.cu); C a multiple of 16.
-// `kept` is the copy of x as one row of N S C elements. Forward: x, fin (the [N][G][3] block of sb_gn_stats) -> y, kept,
-// mean, rstd. Backward: dy, kept, mean, rstd -> part [N][nsplit][C][2]; sb_gn_bwd_finalize makes fin [N][C][2] of it,
-// which sb_gn8_bwd_dx turns into y (= dx), dw and db.
-typedef struct {
-  const void* x;
-  const void* dy;
-  void* y;
-  void* kept;
-  const float* w;
-  const float* b;
-  float* mean;
-  float* rstd;
-  const float* fin;
-  float* part;
-  float* dw;
-  float* db;
-  int N, C, G;
-  long long S;
-  int nsplit;
-  float eps;
-  int relu;
-  int accumulate;  // add to dw / db instead of overwriting them
-} SbGn8Args;
-int sb_gn8_apply(const SbGn8Args* a, cudaStream_t stream);
-int sb_gn8_bwd_partial(const SbGn8Args* a, cudaStream_t stream);
-int sb_gn8_bwd_dx(const SbGn8Args* a, cudaStream_t stream);
+// GroupNorm (+ReLU) with an 8-bit copy of its input for the backward pass (group_norm_kept8.cu); C a multiple of 16,
+// tensors [N][S][C], `kept` the copy of x as one row of N S C elements, stats [2][N][G] (mean, rstd), scratch of
+// sb_gn8_scratch() floats. fin (optional): the [N][G][3] block of sb_gn_stats; hand_over: see SbGnArgs.fin.
+long long sb_gn8_scratch(int backward, int N, long long S, int C, int G);
+int sb_gn8_forward(const void* x, const float* w, const float* b, int N, long long S, int C, int G, float eps, int relu,
+                   const float* fin, int hand_over, void* y, void* kept, float* stats, float* scratch,
+                   cudaStream_t stream);
+int sb_gn8_backward(const void* dy, const void* kept, const float* w, const float* b, const float* stats, int N,
+                    long long S, int C, int G, int relu, void* dx, float* dw, float* db, int accumulate, float* scratch,
+                    cudaStream_t stream);
 
 // Cross entropy of a head of K classes over V voxels of C channels without its logits (head_loss.cu, head_wide.cu).
 // x bf16 [V][C], w bf16 [K][C], bias optional [K] (bias_kind 0 bf16, 2 fp32), labels [V] (label_kind 2 int16, 4 int32,
@@ -228,6 +211,9 @@ void sb_count_launch(int n);
 
 int sb_gn_supported(int C, int G);
 int sb_gn_nsplit(int N, long long S, int C);
+int sb_gn_bwd_nsplit(int N, long long S, int C);
+int sb_gn_stats_finalize(const float* part, float* fin, int N, int G, int nsplit, cudaStream_t stream);
+int sb_gn_bwd_finalize(const float* part, float* fin, int N, int C, int nsplit, cudaStream_t stream);
 int sb_gn_stats(const SbGnArgs* a, cudaStream_t stream);
 int sb_gn_apply(const SbGnArgs* a, cudaStream_t stream);
 int sb_gn_bwd_partial(const SbGnArgs* a, cudaStream_t stream);

@@ -8,6 +8,7 @@ result equals the unsharded normalisation.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 from typing import Optional, Sequence
 
@@ -214,24 +215,12 @@ def gn_backward(dy, x, w, b, mean, rstd, groups: int, eps: float = 1e-5, relu: b
 
 
 # -- with an 8-bit copy of the input for the backward pass ------------------------------------------------------------------
-class SbGn8Args(C.Structure):
-    _fields_ = [
-        ("x", C.c_void_p), ("dy", C.c_void_p), ("y", C.c_void_p), ("kept", C.c_void_p),
-        ("w", C.c_void_p), ("b", C.c_void_p),
-        ("mean", C.c_void_p), ("rstd", C.c_void_p),
-        ("fin", C.c_void_p), ("part", C.c_void_p),
-        ("dw", C.c_void_p), ("db", C.c_void_p),
-        ("N", C.c_int), ("C", C.c_int), ("G", C.c_int),
-        ("S", C.c_longlong),
-        ("nsplit", C.c_int),
-        ("eps", C.c_float),
-        ("relu", C.c_int),
-        ("accumulate", C.c_int),
-    ]
-
-
-for _n in ("sb_gn8_apply", "sb_gn8_bwd_partial", "sb_gn8_bwd_dx"):
-    _lib.register(_n, [C.POINTER(SbGn8Args), C.c_void_p], C.c_int)
+_P = C.c_void_p
+_lib.register("sb_gn8_scratch", [C.c_int, C.c_int, C.c_longlong, C.c_int, C.c_int], C.c_longlong)
+_lib.register("sb_gn8_forward", [_P, _P, _P, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_float, C.c_int, _P, C.c_int, _P, _P,
+                                 _P, _P, _P])
+_lib.register("sb_gn8_backward", [_P, _P, _P, _P, _P, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int, _P, _P, _P, C.c_int,
+                                  _P, _P])
 
 
 def supported_kept8(channels: int, groups: int) -> bool:
@@ -239,49 +228,36 @@ def supported_kept8(channels: int, groups: int) -> bool:
     return channels % KEPT_BLOCK == 0 and supported(channels, groups)
 
 
-def _base8(shape, w, b, mean, rstd, kept, groups: int, relu: bool) -> SbGn8Args:
-    a = SbGn8Args()
-    n, d, h, wd, c = shape
-    a.N, a.C, a.G, a.S = n, c, groups, d * h * wd
-    a.w, a.b, a.mean, a.rstd, a.kept = (t.data_ptr() for t in (w, b, mean, rstd, kept))
-    a.relu = 1 if relu else 0
-    return a
+@functools.lru_cache(maxsize=256)
+def _scratch8(backward: int, n: int, s: int, c: int, groups: int) -> int:
+    return int(_lib.lib().sb_gn8_scratch(backward, n, s, c, groups))
 
 
 def gn8_forward(x, w, b, groups: int, eps: float = 1e-5, relu: bool = True, fin: Optional[torch.Tensor] = None):
-    """(y, 8-bit copy of x, mean, rstd); ``fin`` as in :func:`gn_forward`."""
-    if fin is None:
-        fin = gn_stats(x, w, b, groups, eps, relu)
-    n, c = x.shape[0], x.shape[4]
+    """(y, 8-bit copy of x, statistics [2, N, G]: mean and rstd); ``fin`` as in :func:`gn_forward`."""
+    n, d, h, wd, c = x.shape
+    s = d * h * wd
+    dev = x.device
     y = torch.empty_like(x)
-    kept = torch.empty(kept_bytes(x.numel()), dtype=torch.uint8, device=x.device)
-    mean = torch.empty((n, groups), dtype=torch.float32, device=x.device)
-    rstd = torch.empty((n, groups), dtype=torch.float32, device=x.device)
-    a = _base8(x.shape, w, b, mean, rstd, kept, groups, relu)
-    a.x, a.y, a.fin, a.eps = x.data_ptr(), y.data_ptr(), fin.data_ptr(), eps
-    _lib.check(_lib.lib().sb_gn8_apply(C.byref(a), _lib.stream_ptr()), "sb_gn8_apply")
-    return y, kept, mean, rstd
+    kept = torch.empty(kept_bytes(n * s * c), dtype=torch.uint8, device=dev)
+    stats = torch.empty((2, n, groups), dtype=torch.float32, device=dev)
+    scratch = torch.empty(_scratch8(0, n, s, c, groups), dtype=torch.float32, device=dev) if fin is None else None
+    _lib.check(_lib.lib().sb_gn8_forward(
+        x.data_ptr(), w.data_ptr(), b.data_ptr(), n, s, c, groups, eps, relu, _lib.ptr(fin),
+        fin is None and _fused_finalize(n * groups), y.data_ptr(), kept.data_ptr(), stats.data_ptr(), _lib.ptr(scratch),
+        _lib.stream_ptr()), "sb_gn8_forward")
+    return y, kept, stats
 
 
-def gn8_backward(dy, kept, w, b, mean, rstd, groups: int, relu: bool = True, into=None):
+def gn8_backward(dy, kept, w, b, stats, groups: int, relu: bool = True, into=None):
     """(dx, dw, db) from the 8-bit copy; ``into`` as in :func:`gn_bwd_dx`."""
     n, d, h, wd, c = dy.shape
-    L, st = _lib.lib(), _lib.stream_ptr()
-    a = _base8(dy.shape, w, b, mean, rstd, kept, groups, relu)
-    a.dy = dy.data_ptr()
-    a.nsplit = L.sb_gn_bwd_nsplit(n, d * h * wd, c)
-    part = torch.empty((n, a.nsplit, c, 2), dtype=torch.float32, device=dy.device)
-    fin = torch.empty((n, c, 2), dtype=torch.float32, device=dy.device)
-    a.part = part.data_ptr()
-    _lib.check(L.sb_gn8_bwd_partial(C.byref(a), st), "sb_gn8_bwd_partial")
-    _lib.check(L.sb_gn_bwd_finalize(part.data_ptr(), fin.data_ptr(), n, c, a.nsplit, st), "sb_gn_bwd_finalize")
+    s = d * h * wd
+    dev = dy.device
     dx = torch.empty_like(dy)
-    if into is not None:
-        dw, db = into
-        a.accumulate = 1
-    else:
-        dw = torch.empty(c, dtype=torch.float32, device=dy.device)
-        db = torch.empty(c, dtype=torch.float32, device=dy.device)
-    a.fin, a.y, a.dw, a.db = fin.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr()
-    _lib.check(L.sb_gn8_bwd_dx(C.byref(a), st), "sb_gn8_bwd_dx")
+    dw, db = into if into is not None else (torch.empty(c, dtype=torch.float32, device=dev) for _ in range(2))
+    scratch = torch.empty(_scratch8(1, n, s, c, groups), dtype=torch.float32, device=dev)
+    _lib.check(_lib.lib().sb_gn8_backward(
+        dy.data_ptr(), kept.data_ptr(), w.data_ptr(), b.data_ptr(), stats.data_ptr(), n, s, c, groups, relu, dx.data_ptr(),
+        dw.data_ptr(), db.data_ptr(), into is not None, scratch.data_ptr(), _lib.stream_ptr()), "sb_gn8_backward")
     return dx, dw, db

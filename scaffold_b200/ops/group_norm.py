@@ -19,7 +19,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from . import gn_kernels as gk
-from .layout import direct_grad_target, from_vm, notify_grad_written, to_vm, use_cuda_kernels
+from .layout import direct_grad_target, from_vm, notify_grad_written, on_device, to_vm, use_cuda_kernels
 
 
 class _GnFn(torch.autograd.Function):
@@ -67,14 +67,14 @@ class _Gn8Fn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, relu, partials):
-        w32, b32 = weight.detach().float().contiguous(), bias.detach().float().contiguous()
+        w32, b32 = _fp32(weight), _fp32(bias)
         fin = None
         if partials is not None:
             part, splits, pg = partials
             if pg == groups and part.numel() == x.shape[0] * splits * groups * 3:
                 fin = gk.gn_finalize(part, x.shape[0], groups, splits)
-        y, kept, mean, rstd = gk.gn8_forward(x, w32, b32, groups, eps, relu, fin=fin)
-        ctx.save_for_backward(kept, w32, b32, mean, rstd)
+        y, kept, stats = gk.gn8_forward(x, w32, b32, groups, eps, relu, fin=fin)
+        ctx.save_for_backward(kept, w32, b32, stats)
         ctx.cfg = (groups, relu)
         ctx.params = (weight, bias)
         return y
@@ -82,19 +82,24 @@ class _Gn8Fn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        kept, w32, b32, mean, rstd = ctx.saved_tensors
+        kept, w32, b32, stats = ctx.saved_tensors
         groups, relu = ctx.cfg
         into = None
         if ctx.needs_input_grad[1] and ctx.needs_input_grad[2]:
             into = tuple(direct_grad_target(p, ctx) for p in ctx.params)
             if any(t is None for t in into):
                 into = None
-        dx, dw, db = gk.gn8_backward(gy.contiguous(), kept, w32, b32, mean, rstd, groups, relu, into=into)
+        with on_device(gy.device):
+            dx, dw, db = gk.gn8_backward(gy.contiguous(), kept, w32, b32, stats, groups, relu, into=into)
         if into is not None:
             dw = db = None
             for p in ctx.params:
                 notify_grad_written(p)
         return dx, dw, db, None, None, None, None
+
+
+def _fp32(p: torch.Tensor) -> torch.Tensor:
+    return p if p.dtype == torch.float32 and p.is_contiguous() else p.detach().float().contiguous()
 
 
 def group_norm_kept8(x: torch.Tensor, num_groups: int, weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-5,
@@ -119,7 +124,7 @@ def group_norm_kept8(x: torch.Tensor, num_groups: int, weight: torch.Tensor, bia
         raise ValueError(f"weight and bias must be [{c}] on {x.device}")
     if x.numel() == 0:
         raise ValueError(f"group_norm_kept8 has no statistics of an empty tensor {tuple(x.shape)}")
-    with torch.cuda.device(x.device):
+    with on_device(x.device):
         return from_vm(_Gn8Fn.apply(to_vm(x), weight, bias, num_groups, eps, activation == "relu", None))
 
 

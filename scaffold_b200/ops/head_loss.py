@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .layout import use_cuda_kernels
+from .layout import on_device, use_cuda_kernels
 
 _P = C.c_void_p
 
@@ -83,7 +83,7 @@ class _HeadLossFn(torch.autograd.Function):
         w_type, b_type = ctx.types
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         gout = gout.float()
-        with torch.cuda.device(dev):
+        with on_device(dev):
             dx = torch.empty_like(x) if want_x else None
             dw = torch.empty((k, c), dtype=w_type, device=dev) if want_w else None
             db = torch.empty(k, dtype=b_type, device=dev) if want_b else None
@@ -149,7 +149,7 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
     if x.shape[0] == 0:  # a shard without voxels: its terms are zero, the other shards' sums are not
         return _formula(x.float(), weight.float(), None if bias is None else bias.float(), labels.reshape(-1),
                         class_weights, ignore_label, spatial)
-    with torch.cuda.device(features.device):
+    with on_device(features.device):
         return _HeadLossFn.apply(x, weight, None if bias is None else bias.contiguous(), labels.reshape(-1).contiguous(),
                                  class_weights, ignore_label, spatial)
 

@@ -20,6 +20,7 @@ from typing import NamedTuple, Tuple
 import torch
 
 from . import _lib
+from .layout import on_device
 
 _lib.register("sb_kept8_bytes", [C.c_longlong], C.c_longlong)
 _lib.register("sb_keep8", [C.c_void_p, C.c_int, C.c_longlong, C.c_void_p, C.c_void_p])
@@ -77,16 +78,15 @@ def keep8(x: torch.Tensor) -> Kept8:
         raise TypeError(f"keep8 takes bf16, fp16 or fp32; got {x.dtype}")
     if x.layout != torch.strided or x.is_conj() or x.is_neg():
         raise TypeError("keep8 takes plain strided tensors")
-    x = x.detach()
     if not _dense(x):
-        x = x.contiguous()
+        x = x.detach().contiguous()
     n = x.numel()
-    flat = x.as_strided((n,), (1,), x.storage_offset())
     if not x.is_cuda:
-        return Kept8(_keep_formula(flat), tuple(x.shape), x.stride(), x.dtype)
-    with torch.cuda.device(x.device):
-        data = torch.empty(kept_bytes(n), dtype=torch.uint8, device=x.device)
-        _lib.check(_lib.lib().sb_keep8(flat.data_ptr(), KINDS[x.dtype], n, data.data_ptr(), _lib.stream_ptr()), "sb_keep8")
+        return Kept8(_keep_formula(x.detach().as_strided((n,), (1,), x.storage_offset())), tuple(x.shape), x.stride(), x.dtype)
+    dev = x.device
+    with on_device(dev):
+        data = torch.empty(kept_bytes(n), dtype=torch.uint8, device=dev)
+        _lib.check(_lib.lib().sb_keep8(x.data_ptr(), KINDS[x.dtype], n, data.data_ptr(), _lib.stream_ptr()), "sb_keep8")
     return Kept8(data, tuple(x.shape), x.stride(), x.dtype)
 
 
@@ -99,13 +99,14 @@ def restore8(kept: Kept8) -> torch.Tensor:
     if data.dtype != torch.uint8 or data.numel() != kept_bytes(n) or not data.is_contiguous():
         raise ValueError(f"an 8-bit copy of {n} elements is {kept_bytes(n)} contiguous bytes; got "
                          f"{data.numel()} of {data.dtype}")
-    y = torch.empty_strided(kept.shape, kept.stride, dtype=kept.dtype, device=data.device)
+    dev = data.device
+    y = torch.empty_strided(kept.shape, kept.stride, dtype=kept.dtype, device=dev)
     if not _dense(y):
         raise ValueError(f"strides {kept.stride} of shape {kept.shape} do not cover one run of memory")
     if not data.is_cuda:
         y.as_strided((n,), (1,)).copy_(_restore_formula(data, n, kept.dtype))
         return y
-    with torch.cuda.device(data.device):
+    with on_device(dev):
         _lib.check(_lib.lib().sb_restore8(data.data_ptr(), KINDS[kept.dtype], n, y.data_ptr(), _lib.stream_ptr()),
                    "sb_restore8")
     return y

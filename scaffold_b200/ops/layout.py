@@ -37,6 +37,22 @@ def use_cuda_kernels(x: torch.Tensor) -> bool:
     return torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16
 
 
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one (free of charge when it is already)."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
 def to_vm(x: torch.Tensor, pad16: bool = False, pad_to: int = 16) -> torch.Tensor:
     """NCDHW-shaped tensor -> contiguous voxel-major bf16 ``[N, D, H, W, C]``."""
     if (pad16 and x.is_cuda and x.dim() == 5 and x.shape[1] < 16 and x.is_contiguous()

@@ -49,7 +49,8 @@ SHAPES = [((1, 1, 1, 1, 16), 1), ((2, 1, 1, 1, 16), 2), ((1, 3, 5, 7, 16), 8), (
 def test_forward_and_gradients(shape, groups, relu):
     x, gy, w, b = _inputs(shape, sum(shape))
     eps = 1e-5
-    y, kept, mean, rstd = gk.gn8_forward(x, w, b, groups, eps, relu)
+    y, kept, stats = gk.gn8_forward(x, w, b, groups, eps, relu)
+    mean, rstd = stats
     ordinary = gk.gn_forward(x, w, b, groups, eps, relu)
     # statistics and result: those of the ordinary kernels, to the bit
     assert torch.equal(y, ordinary[0]) and torch.equal(mean, ordinary[1]) and torch.equal(rstd, ordinary[2])
@@ -67,7 +68,7 @@ def test_forward_and_gradients(shape, groups, relu):
         assert (side(xk) == side(x))[~near].all()
     # bf16 result: half a step, 2^-8 of the value, with the fp32 error of statistics and affine (a few 2^-24 of values below 50)
     assert ((y.double().reshape(ry.shape) - ry).abs() <= 2 ** -8 * ry.abs() + 1e-4 * (rstd.max() + 1)).all()
-    dx, dw, db = gk.gn8_backward(gy, kept, w, b, mean, rstd, groups, relu)
+    dx, dw, db = gk.gn8_backward(gy, kept, w, b, stats, groups, relu)
     # dx: half a step of bf16 (2^-8 of the value), and terms of the size of rstd * max|gy w| in fp32 with the errors of
     # mean and rstd (fp32 sums in a tree: 1e-5 of the terms is far above them); a value nearer to the ReLU's border
     # than fp32 resolves may take the other mask
@@ -86,8 +87,8 @@ def test_the_gradient_is_that_of_the_function_to_the_step_of_the_copy():
     copy's step, 1/126 of a block's largest value."""
     shape, groups = (2, 4, 6, 5, 32), 8
     x, gy, w, b = _inputs(shape, 3)
-    y, kept, mean, rstd = gk.gn8_forward(x, w, b, groups, 1e-5, False)
-    dx, dw, db = gk.gn8_backward(gy, kept, w, b, mean, rstd, groups, False)
+    y, kept, stats = gk.gn8_forward(x, w, b, groups, 1e-5, False)
+    dx, dw, db = gk.gn8_backward(gy, kept, w, b, stats, groups, False)
 
     def loss(xx, ww, bb):
         n, c = shape[0], shape[-1]
@@ -112,15 +113,15 @@ def test_statistics_of_nothing_but_equal_values_and_values_that_are_not_finite()
     shape = (2, 2, 4, 4, 32)
     x, gy, w, b = _inputs(shape, 1)
     x[0] = 1.5
-    y, kept, mean, rstd = gk.gn8_forward(x, w, b, 8, 1e-5, True)
+    y, kept, stats = gk.gn8_forward(x, w, b, 8, 1e-5, True)
     assert torch.equal(y, gk.gn_forward(x, w, b, 8, 1e-5, True)[0])
-    dx, dw, db = gk.gn8_backward(gy, kept, w, b, mean, rstd, 8, True)
+    dx, dw, db = gk.gn8_backward(gy, kept, w, b, stats, 8, True)
     assert dx.isfinite().all() and dw.isfinite().all() and db.isfinite().all()
     x[1, 0, 0, 0, 5] = float("inf")  # group 1 of sample 1
-    y, kept, mean, rstd = gk.gn8_forward(x, w, b, 8, 1e-5, True)
+    y, kept, stats = gk.gn8_forward(x, w, b, 8, 1e-5, True)
     want = gk.gn_forward(x, w, b, 8, 1e-5, True)
     assert torch.equal(y.nan_to_num(), want[0].nan_to_num()) and torch.equal(y.isnan(), want[0].isnan())
-    dx, *_ = gk.gn8_backward(gy, kept, w, b, mean, rstd, 8, True)
+    dx, *_ = gk.gn8_backward(gy, kept, w, b, stats, 8, True)
     assert dx[1, ..., 4:8].isnan().all()
     # the block of 16 channels around the infinity is NaN, the rest of the sample and the other sample are not
     assert dx[0].isfinite().all() and dx[1, ..., 16:].isfinite().all()
@@ -185,8 +186,8 @@ def test_a_captured_pass_is_replayed_on_new_values():
             x.copy_(nx)
             gy.copy_(ng)
         graph.replay()
-        ey, kept, mean, rstd = gk.gn8_forward(nx, w.detach(), b.detach(), 8, 1e-5, True)
-        want = gk.gn8_backward(ng, kept, w.detach(), b.detach(), mean, rstd, 8, True)
+        ey, kept, stats = gk.gn8_forward(nx, w.detach(), b.detach(), 8, 1e-5, True)
+        want = gk.gn8_backward(ng, kept, w.detach(), b.detach(), stats, 8, True)
         assert torch.equal(y.permute(0, 2, 3, 4, 1), ey) and torch.equal(grads[0].permute(0, 2, 3, 4, 1), want[0])
         assert torch.equal(grads[1], want[1]) and torch.equal(grads[2], want[2])
 
