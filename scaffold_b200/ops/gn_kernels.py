@@ -223,6 +223,7 @@ _lib.register("sb_gn8_backward", [_P, _P, _P, _P, _P, C.c_int, C.c_longlong, C.c
                                   _P, _P])
 
 
+@functools.lru_cache(maxsize=256)
 def supported_kept8(channels: int, groups: int) -> bool:
     """What the kernels with an 8-bit copy cover: a voxel is a whole number of 16-element blocks."""
     return channels % KEPT_BLOCK == 0 and supported(channels, groups)
@@ -233,12 +234,14 @@ def _scratch8(backward: int, n: int, s: int, c: int, groups: int) -> int:
     return int(_lib.lib().sb_gn8_scratch(backward, n, s, c, groups))
 
 
-def gn8_forward(x, w, b, groups: int, eps: float = 1e-5, relu: bool = True, fin: Optional[torch.Tensor] = None):
-    """(y, 8-bit copy of x, statistics [2, N, G]: mean and rstd); ``fin`` as in :func:`gn_forward`."""
+def gn8_forward(x, w, b, groups: int, eps: float = 1e-5, relu: bool = True, fin: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None):
+    """(y, 8-bit copy of x, statistics [2, N, G]: mean and rstd); ``fin`` as in :func:`gn_forward`. ``out``: a tensor over
+    the same memory layout for y, whatever its shape."""
     n, d, h, wd, c = x.shape
     s = d * h * wd
     dev = x.device
-    y = torch.empty_like(x)
+    y = torch.empty_like(x) if out is None else out
     kept = torch.empty(kept_bytes(n * s * c), dtype=torch.uint8, device=dev)
     stats = torch.empty((2, n, groups), dtype=torch.float32, device=dev)
     scratch = torch.empty(_scratch8(0, n, s, c, groups), dtype=torch.float32, device=dev) if fin is None else None
@@ -249,12 +252,12 @@ def gn8_forward(x, w, b, groups: int, eps: float = 1e-5, relu: bool = True, fin:
     return y, kept, stats
 
 
-def gn8_backward(dy, kept, w, b, stats, groups: int, relu: bool = True, into=None):
-    """(dx, dw, db) from the 8-bit copy; ``into`` as in :func:`gn_bwd_dx`."""
+def gn8_backward(dy, kept, w, b, stats, groups: int, relu: bool = True, into=None, out: Optional[torch.Tensor] = None):
+    """(dx, dw, db) from the 8-bit copy; ``into`` as in :func:`gn_bwd_dx`, ``out`` (for dx) as in :func:`gn8_forward`."""
     n, d, h, wd, c = dy.shape
     s = d * h * wd
     dev = dy.device
-    dx = torch.empty_like(dy)
+    dx = torch.empty_like(dy) if out is None else out
     dw, db = into if into is not None else (torch.empty(c, dtype=torch.float32, device=dev) for _ in range(2))
     scratch = torch.empty(_scratch8(1, n, s, c, groups), dtype=torch.float32, device=dev)
     _lib.check(_lib.lib().sb_gn8_backward(

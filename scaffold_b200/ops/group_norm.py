@@ -63,17 +63,20 @@ class _GnFn(torch.autograd.Function):
 
 
 class _Gn8Fn(torch.autograd.Function):
-    """:class:`_GnFn` that keeps an 8-bit copy of ``x`` for its backward pass instead of ``x``."""
+    """:class:`_GnFn` of an NCDHW-shaped ``x`` that keeps an 8-bit copy of it for its backward pass instead of ``x``."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, relu, partials):
+        shape, x = x.shape, to_vm(x)
         w32, b32 = _fp32(weight), _fp32(bias)
         fin = None
         if partials is not None:
             part, splits, pg = partials
             if pg == groups and part.numel() == x.shape[0] * splits * groups * 3:
                 fin = gk.gn_finalize(part, x.shape[0], groups, splits)
-        y, kept, stats = gk.gn8_forward(x, w32, b32, groups, eps, relu, fin=fin)
+        # (no view of another tensor: autograd keeps a record of such a result's base)
+        y = torch.empty(shape, dtype=x.dtype, device=x.device, memory_format=torch.channels_last_3d)
+        _, kept, stats = gk.gn8_forward(x, w32, b32, groups, eps, relu, fin=fin, out=y)
         ctx.save_for_backward(kept, w32, b32, stats)
         ctx.cfg = (groups, relu)
         ctx.params = (weight, bias)
@@ -90,7 +93,8 @@ class _Gn8Fn(torch.autograd.Function):
             if any(t is None for t in into):
                 into = None
         with on_device(gy.device):
-            dx, dw, db = gk.gn8_backward(gy.contiguous(), kept, w32, b32, stats, groups, relu, into=into)
+            dx = torch.empty(gy.shape, dtype=torch.bfloat16, device=gy.device, memory_format=torch.channels_last_3d)
+            _, dw, db = gk.gn8_backward(to_vm(gy), kept, w32, b32, stats, groups, relu, into=into, out=dx)
         if into is not None:
             dw = db = None
             for p in ctx.params:
@@ -116,16 +120,16 @@ def group_norm_kept8(x: torch.Tensor, num_groups: int, weight: torch.Tensor, bia
     if x.dim() != 5 or x.dtype != torch.bfloat16 or not x.is_cuda:
         raise ValueError(f"group_norm_kept8 takes bf16 CUDA tensors [N, C, D, H, W]; got {x.dtype} {tuple(x.shape)} on "
                          f"{x.device}")
-    c = x.shape[1]
+    c, dev = x.shape[1], x.device
     if not gk.supported_kept8(c, num_groups):
         raise ValueError(f"{c} channels in {num_groups} groups are outside the kernels' range: a multiple of 16 up to "
                          "2048, and groups of whole octets (or of 2 or 4 channels)")
-    if weight.shape != (c,) or bias.shape != (c,) or weight.device != x.device or bias.device != x.device:
-        raise ValueError(f"weight and bias must be [{c}] on {x.device}")
+    if weight.shape != (c,) or bias.shape != (c,) or weight.device != dev or bias.device != dev:
+        raise ValueError(f"weight and bias must be [{c}] on {dev}")
     if x.numel() == 0:
         raise ValueError(f"group_norm_kept8 has no statistics of an empty tensor {tuple(x.shape)}")
-    with on_device(x.device):
-        return from_vm(_Gn8Fn.apply(to_vm(x), weight, bias, num_groups, eps, activation == "relu", None))
+    with on_device(dev):
+        return _Gn8Fn.apply(x, weight, bias, num_groups, eps, activation == "relu", None)
 
 
 class GroupNorm(nn.GroupNorm):
@@ -164,9 +168,9 @@ class GroupNorm(nn.GroupNorm):
         if use_cuda_kernels(x) and x.dim() == 5 and self.kernel_supported():
             partials = getattr(x, "_sb_gn_partials", None)  # left by the convolution that produced x, if it could
             if self.keeps8():
-                y = _Gn8Fn.apply(to_vm(x), self.weight, self.bias, self.num_groups, self.eps, relu, partials)
-            else:
-                y = _GnFn.apply(to_vm(x), self.weight, self.bias, self.num_groups, self.eps, relu, self._spatial, partials)
+                return _Gn8Fn.apply(x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16), self.weight, self.bias,
+                                    self.num_groups, self.eps, relu, partials)
+            y = _GnFn.apply(to_vm(x), self.weight, self.bias, self.num_groups, self.eps, relu, self._spatial, partials)
             return from_vm(y)
         if x.is_cuda and use_cuda_kernels(x) and not self._warned:
             self._warned = True

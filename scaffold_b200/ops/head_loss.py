@@ -111,47 +111,51 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
     The kernels read bf16: an fp32 ``weight`` is rounded, its gradient comes back in fp32. Gradients: features in bf16,
     weight and bias in their own types.
     """
-    if features.dim() < 1 or labels.shape != features.shape[:-1]:
-        raise ValueError(f"features {tuple(features.shape)} need labels {tuple(features.shape[:-1])}; "
-                         f"got {tuple(labels.shape)}")
-    c = features.shape[-1]
-    if weight.dim() < 2 or weight.shape[1] != c or weight.numel() != weight.shape[0] * c or weight.shape[0] < 1:
+    shape, dev = features.shape, features.device
+    if not shape or labels.shape != shape[:-1]:
+        raise ValueError(f"features {tuple(shape)} need labels {tuple(shape[:-1])}; got {tuple(labels.shape)}")
+    c, k = shape[-1], weight.shape[0] if weight.dim() else 0
+    if weight.dim() < 2 or k < 1 or weight.shape[1] != c or weight.numel() != k * c:
         raise ValueError(f"weight must be [classes, {c}] (or [classes, {c}, 1, 1, 1]); got {tuple(weight.shape)}")
-    k = weight.shape[0]
-    if bias is not None and bias.shape != (k,):
-        raise ValueError(f"bias must be [{k}]; got {tuple(bias.shape)}")
-    if class_weights is not None and class_weights.shape != (k,):
-        raise ValueError(f"class_weights must be [{k}]; got {tuple(class_weights.shape)}")
     if labels.dtype not in _LABEL_KIND:
         raise TypeError(f"labels must be int16, int32 or int64; got {labels.dtype}")
+    for name, t in (("bias", bias), ("class_weights", class_weights)):
+        if t is not None and t.shape != (k,):
+            raise ValueError(f"{name} must be [{k}]; got {tuple(t.shape)}")
     for name, t in (("weight", weight), ("bias", bias), ("labels", labels), ("class_weights", class_weights)):
-        if t is not None and t.device != features.device:
-            raise ValueError(f"{name} is on {t.device}, the features are on {features.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the features are on {dev}")
     if ignore_label is not None and not -2 ** 63 <= ignore_label < 2 ** 63:
         raise ValueError(f"ignore_label {ignore_label} is no 64-bit number")
-    weight = weight.reshape(k, c)
+    if weight.dim() > 2:
+        weight = weight.reshape(k, c)
     if not use_cuda_kernels(features):
         return _formula(features, weight, bias, labels, class_weights, ignore_label, spatial)
     if not head_supported(c):
         raise ValueError(f"the kernels read features of 8 to {MAX_WIDTH} channels in multiples of 8; got {c}")
     if weight.dtype not in _KIND or (bias is not None and bias.dtype not in _KIND):
         raise TypeError("weight and bias must be bf16 or fp32")
-    if features.numel() // c > 2 ** 31 - 512:
-        raise ValueError(f"{features.numel() // c} voxels are more than the kernels count")
-    x = features.to(torch.bfloat16).reshape(-1, c)
+    n = features.numel() // c
+    if n > 2 ** 31 - 512:
+        raise ValueError(f"{n} voxels are more than the kernels count")
+    x = features if features.dtype == torch.bfloat16 else features.to(torch.bfloat16)
+    if x.dim() != 2:
+        x = x.reshape(n, c)
     if not x.is_contiguous() or x.data_ptr() % 16:  # a tensor map starts on 16 bytes
         x = x.clone(memory_format=torch.contiguous_format)
-    weight = weight.contiguous()
-    if weight.dtype == torch.bfloat16 and weight.data_ptr() % 16:
-        weight = weight.clone()
-    if class_weights is not None:
+    if not weight.is_contiguous() or (weight.dtype == torch.bfloat16 and weight.data_ptr() % 16):
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    if labels.dim() != 1 or not labels.is_contiguous():
+        labels = labels.reshape(-1).contiguous()
+    if class_weights is not None and (class_weights.dtype != torch.float32 or class_weights.requires_grad
+                                      or not class_weights.is_contiguous()):
         class_weights = class_weights.detach().float().contiguous()
-    if x.shape[0] == 0:  # a shard without voxels: its terms are zero, the other shards' sums are not
-        return _formula(x.float(), weight.float(), None if bias is None else bias.float(), labels.reshape(-1),
-                        class_weights, ignore_label, spatial)
-    with on_device(features.device):
-        return _HeadLossFn.apply(x, weight, None if bias is None else bias.contiguous(), labels.reshape(-1).contiguous(),
-                                 class_weights, ignore_label, spatial)
+    if n == 0:  # a shard without voxels: its terms are zero, the other shards' sums are not
+        return _formula(x.float(), weight.float(), None if bias is None else bias.float(), labels, class_weights,
+                        ignore_label, spatial)
+    with on_device(dev):
+        return _HeadLossFn.apply(x, weight, None if bias is None else bias.contiguous(), labels, class_weights,
+                                 ignore_label, spatial)
 
 
 def _formula(features, weight, bias, labels, class_weights, ignore_label, spatial):
