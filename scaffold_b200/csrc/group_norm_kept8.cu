@@ -20,7 +20,7 @@
 namespace sb {
 
 constexpr int GN8_THREADS = 256;
-constexpr int GN8_WAVE = 4, GN8_WAVE_SUMS = 3;  // blocks per SM: 64 registers a thread (the sums: 85)
+constexpr int GN8_WAVE_APPLY = 3, GN8_WAVE_SUMS = 3, GN8_WAVE_DX = 4;  // blocks per SM: 64 registers a thread (85)
 constexpr int GN8_U_APPLY = 4, GN8_U_SUMS = 4, GN8_U_DX = 2;  // voxels in flight per thread
 
 struct Gn8Params {
@@ -61,9 +61,23 @@ __device__ __forceinline__ void gn8_values(uint2 q, float step, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) { f[i] = lo[i] * step; f[4 + i] = hi[i] * step; }
 }
+// The value's whole number t (plus KEPT_MAGIC) one step further towards the value where its kept form xq lies on the
+// other side of the ReLU: y = x a + c there, and a step in the direction of a's sign makes y grow.
+__device__ __forceinline__ void gn8_keep_side(float& t, float y, float xq, float a, float c) {
+  // (predicated: half of the warps have such a value among a thread's eight)
+  asm("{\n\t.reg .pred on, other;\n\t.reg .f32 k, d;\n\t"
+      "fma.rn.f32 k, %2, %3, %4;\n\t"
+      "setp.gt.f32 on, %1, 0f00000000;\n\t"
+      "setp.gt.xor.f32 other, k, 0f00000000, on;\n\t"
+      "copysign.f32 d, %3, 0f3F800000;\n\t"
+      "@!on neg.f32 d, d;\n\t"
+      "@other add.f32 %0, %0, d;\n\t}"
+      : "+f"(t)
+      : "f"(y), "f"(xq), "f"(a), "f"(c));
+}
 
 template <bool RELU>
-__global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE) gn8_apply_kernel(const Gn8Params p) {
+__global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE_APPLY) gn8_apply_kernel(const Gn8Params p) {
   __shared__ float s_mean[256], s_rstd[256];
   const int n = blockIdx.y;
   for (int g = threadIdx.x; g < p.G; g += GN8_THREADS) {
@@ -84,37 +98,34 @@ __global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE) gn8_apply_kernel(const 
     a[i] = s_rstd[g] * p.w[ch];
     c[i] = p.b[ch] - s_mean[g] * a[i];
   }
-  const long long base = (long long)n * p.S * p.C + oct * 8;
-  // the loop is uniform over the block, for the shuffle: a thread without a voxel takes part with zeros
-  const long long stride = (long long)gridDim.x * vpb;
-  for (long long v0 = (long long)blockIdx.x * vpb; v0 < p.S; v0 += GN8_U_APPLY * stride) {
+  // The loop is uniform over the block, for the shuffle: a thread without a voxel takes part with zeros. A thread counts
+  // the voxels it has left and moves on by `row` elements a voxel (below 2^31: a row of voxels of the whole grid).
+  const long long stride = (long long)gridDim.x * vpb, first = (long long)blockIdx.x * vpb;
+  const int row = (int)(stride * p.C);
+  int left = vl < vpb && first + vl < p.S ? (int)((p.S - first - vl + stride - 1) / stride) : 0;
+  long long at = (long long)n * p.S * p.C + (first + vl) * p.C + oct * 8;
+  for (int rounds = (int)((p.S - first + GN8_U_APPLY * stride - 1) / (GN8_U_APPLY * stride)); rounds > 0; --rounds) {
     uint4 raw[GN8_U_APPLY];
 #pragma unroll
     for (int u = 0; u < GN8_U_APPLY; ++u) {
-      const long long v = v0 + u * stride + vl;
       raw[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (vl < vpb && v < p.S) raw[u] = __ldg(reinterpret_cast<const uint4*>(p.x + base + v * p.C));
+      if (u < left) raw[u] = __ldg(reinterpret_cast<const uint4*>(p.x + at + u * row));
     }
 #pragma unroll
     for (int u = 0; u < GN8_U_APPLY; ++u) {
-      if (v0 + u * stride >= p.S) break;
-      const long long v = v0 + u * stride + vl, at = base + v * p.C;
+      uint32_t m2 = kept_max2(kept_max2(raw[u].x, raw[u].y), kept_max2(raw[u].z, raw[u].w));
+      m2 = kept_max2(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
+      const uint32_t b = kept_exponent(max(m2 << 16 & 0x7FFF0000u, m2 & 0x7FFF0000u));
+      const float step = kept_step(b), inv = b == 255u ? 0.f : kept_inv(b);
       float f[8], t[8];
       gn8_unpack(raw[u], f);
-      uint32_t amax = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      const uint32_t b = kept_exponent(amax);
-      const float step = kept_step(b), inv = b == 255u ? 0.f : kept_inv(b);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         t[i] = fmaf(f[i], inv, KEPT_MAGIC);
         float yv = fmaf(f[i], a[i], c[i]);
         if (RELU) {
-          const bool on = yv > 0.f, kept_on = fmaf((t[i] - KEPT_MAGIC) * step, a[i], c[i]) > 0.f;
-          if (on != kept_on) t[i] += on == (a[i] > 0.f) ? 1.f : -1.f;
-          yv = yv <= 0.f ? 0.f : yv;  // NaN propagates
+          gn8_keep_side(t[i], yv, (t[i] - KEPT_MAGIC) * step, a[i], c[i]);
+          asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(yv));  // NaN propagates
         }
         f[i] = yv;
       }
@@ -122,13 +133,15 @@ __global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE) gn8_apply_kernel(const 
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[i] = b == 255u ? KEPT_MAGIC : kept_cap(t[i]);
       }
-      if (vl < vpb && v < p.S) {
+      if (u < left) {
         *reinterpret_cast<uint4*>(p.y + at) = gn8_pack(f);
         *reinterpret_cast<uint2*>(p.q + at) =
             make_uint2(kept_pack4(t[0], t[1], t[2], t[3]), kept_pack4(t[4], t[5], t[6], t[7]));
         if ((oct & 1) == 0) p.exps[at / KEPT_BLOCK] = (uint8_t)b;
       }
+      at += row;
     }
+    left -= GN8_U_APPLY;
   }
 }
 
@@ -161,10 +174,19 @@ __global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE_SUMS) gn8_bwd_partial_ke
       gn8_unpack(rd, fd);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float d = fd[i];
-        if (RELU && fmaf(fx[i], a[i], c[i]) <= 0.f) d = 0.f;
-        A[i] += d;
-        B[i] = fmaf(d, fx[i] - mu[i / (8 / GP)], B[i]);
+        const float dev = fx[i] - mu[i / (8 / GP)];
+        if (RELU) {  // two predicated sums instead of a selection in front of them
+          asm("{\n\t.reg .pred off;\n\t.reg .f32 y;\n\t"
+              "fma.rn.f32 y, %2, %3, %4;\n\t"
+              "setp.le.f32 off, y, 0f00000000;\n\t"
+              "@!off add.f32 %0, %0, %5;\n\t"
+              "@!off fma.rn.f32 %1, %5, %6, %1;\n\t}"
+              : "+f"(A[i]), "+f"(B[i])
+              : "f"(fx[i]), "f"(a[i]), "f"(c[i]), "f"(fd[i]), "f"(dev));
+        } else {
+          A[i] += fd[i];
+          B[i] = fmaf(fd[i], dev, B[i]);
+        }
       }
     };
     const long long row = (long long)vpb * p.C;
@@ -207,7 +229,7 @@ __global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE_SUMS) gn8_bwd_partial_ke
 }
 
 template <int GP, bool RELU>
-__global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE) gn8_bwd_dx_kernel(const Gn8Params p) {
+__global__ void __launch_bounds__(GN8_THREADS, GN8_WAVE_DX) gn8_bwd_dx_kernel(const Gn8Params p) {
   __shared__ float s_c1[256], s_c2[256];
   const int n = blockIdx.y;
   const int tpv = p.C / 8, vpb = GN8_THREADS / tpv;
@@ -300,9 +322,9 @@ static void gn8_fill(Gn8Params& p, void* kept, const float* w, const float* b, f
   p.relu = relu;
   p.group_elems = (float)((double)S * (C / G));
 }
-static int gn8_blocks(const Gn8Params& p) {
+static int gn8_blocks(const Gn8Params& p, int wave) {
   const int vpb = GN8_THREADS / (p.C / 8);
-  const long long need = (p.S + vpb - 1) / vpb, cap = 148LL * GN8_WAVE / p.N;  // one wave
+  const long long need = (p.S + vpb - 1) / vpb, cap = 148LL * wave / p.N;  // one wave
   const long long b = need < cap ? need : cap;
   return (int)(b < 1 ? 1 : b);
 }
@@ -351,7 +373,7 @@ extern "C" int sb_gn8_forward(const void* x, const float* w, const float* b, int
   p.y = (__nv_bfloat16*)y;
   p.fin = fin;
   p.eps = eps;
-  const dim3 grid(gn8_blocks(p), p.N);
+  const dim3 grid(gn8_blocks(p, GN8_WAVE_APPLY), p.N);
   if (relu) gn8_apply_kernel<true><<<grid, GN8_THREADS, 0, stream>>>(p);
   else gn8_apply_kernel<false><<<grid, GN8_THREADS, 0, stream>>>(p);
   sb_count_launch(1);
@@ -365,7 +387,7 @@ static int gn8_backward(Gn8Params& p, float* fin, cudaStream_t stream) {
   const int rc = sb_gn_bwd_finalize(p.part, fin, p.N, p.C, p.nsplit, stream);
   if (rc) return rc;
   p.fin = fin;
-  gn8_bwd_dx_kernel<GP, RELU><<<dim3(gn8_blocks(p), p.N), GN8_THREADS, 0, stream>>>(p);
+  gn8_bwd_dx_kernel<GP, RELU><<<dim3(gn8_blocks(p, GN8_WAVE_DX), p.N), GN8_THREADS, 0, stream>>>(p);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }

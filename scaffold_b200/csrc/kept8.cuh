@@ -43,4 +43,11 @@ __device__ __forceinline__ void kept_unpack4(uint32_t w, float (&f)[4]) {
   for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540 + i)) - 8388736.f;
 }
 
+// the larger magnitude of each half of two pairs of bf16 (a NaN is the largest); the signs mean nothing
+__device__ __forceinline__ uint32_t kept_max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 }  // namespace sb
