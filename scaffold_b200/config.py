@@ -91,6 +91,12 @@ def _choice(*allowed: str) -> Callable[[str, Any], str]:
     return conv
 
 
+def _activation_bits(name: str, v: Any) -> int:
+    if isinstance(v, bool) or v not in (8, 16):
+        raise ValueError(f"{name} must be 8 or 16; got {v!r}")
+    return int(v)
+
+
 SCHEMA: List[Key] = [
     Key("base_run_dir", _REQUIRED, conv=_path),
     Key("dataset_dir", "datasets/", conv=_path),
@@ -136,6 +142,8 @@ SCHEMA: List[Key] = [
     # --- superset keys (not in the reference schema) ---
     Key("unet_base_width", 64, scalar=True, conv=require_positive_int),
     Key("n_channels", 3, scalar=True, conv=require_positive_int),
+    Key("activation_bits", 16, scalar=True, conv=_activation_bits),  # of what is kept for the backward pass
+    Key("loss", "ce_dice", conv=_choice("ce_dice", "ce")),  # "ce": cross entropy alone, without keeping the logits
     Key("gn_stats", "global", conv=_choice("global", "per_shard")),
     Key("grad_allreduce", "fused", conv=_choice("fused", "nccl")),
     Key("grad_overlap", True, conv=_flag),

@@ -12,6 +12,7 @@
 //
 // One kernel template, three modes. A CTA keeps 128 ROWS resident and walks 128-wide tiles of COLUMNS:
 //   HEAD_FWD  rows = voxels, columns = classes: running maximum and sum of every row (one row per thread, no exchange)
+//   HEAD_ARG  the same with the largest logit and its class (the lowest of several) in their place
 //   HEAD_DX   rows = voxels, columns = classes: P = p - [j = y] in bf16 goes back to tensor memory over the tile of s it
 //             came from, and acc[128][C] += P W is the second MMA with P as its A operand (W's tile is the same shared
 //             memory, read MN-major); the row's g multiplies the finished sum
@@ -30,6 +31,8 @@
 // and some 300 at each commit, during which only the other one's MMAs can run. HEAD_DX / HEAD_DW: warp 1 the first MMAs
 // (as many tiles ahead as tensor memory holds), warp 2 the second ones; HEAD_FWD: the even and the odd tiles. One warp
 // for everything took 2150 clocks a tile at 64 channels, the exponentials left out or not.
+#include <limits.h>
+
 #include <atomic>
 
 #include "head_loss.cuh"
@@ -45,7 +48,7 @@ constexpr int HD_BOX16 = HD_TILE * 32; // and of the sixteen columns more
 constexpr int HD_MAX_STAGES = 8;
 constexpr int HD_MAX_C = 256;          // TMEM: two or three tiles of s and the accumulator in 512 columns
 
-enum HeadMode { HEAD_FWD = 0, HEAD_DX = 1, HEAD_DW = 2 };
+enum HeadMode { HEAD_FWD = 0, HEAD_DX = 1, HEAD_DW = 2, HEAD_ARG = 3 };
 
 struct HeadParams {
   CUtensorMap mapR, mapQ, mapR16, mapQ16;  // rows and columns, and their sixteen columns more
@@ -94,6 +97,7 @@ __device__ __forceinline__ void hd_sub_if(float& v, float d, uint32_t bits, uint
 template <int MODE, bool LO>
 __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_constant__ HeadParams p) {
   constexpr int MAXB = 4;
+  constexpr bool FWD = MODE == HEAD_FWD || MODE == HEAD_ARG;
   const uint32_t NB = (uint32_t)p.bufs;          // tiles of s in tensor memory
   const uint32_t ACC = NB * HD_TILE;             // column of the accumulators
   const uint32_t naccs = (uint32_t)p.accs;       // one or two, 64 columns apart: a job goes on while the last one's is read
@@ -101,7 +105,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t r_full[2], r_empty[2], q_full[HD_MAX_STAGES], q_empty[HD_MAX_STAGES], s_full[MAXB], s_done[MAXB],
       acc_full[2], acc_empty[2];
-  __shared__ float s_fwd[MODE == HEAD_FWD ? 2 : 1][3][MODE == HEAD_FWD ? 4 : 1][HD_TILE];
+  __shared__ float s_fwd[FWD ? 2 : 1][3][FWD ? 4 : 1][HD_TILE];
   __shared__ uint32_t tmem_base_s, abort_s;
   volatile uint32_t* abort_flag = &abort_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -113,7 +117,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
 
   if (threadIdx.x == 0) {
     abort_s = 0;
-    for (int i = 0; i < 2; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], MODE == HEAD_FWD ? 2 : 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], FWD ? 2 : 1); }
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
@@ -125,7 +129,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
     for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], HD_EPI_WARPS); }
     mbar_fence_init();
   }
-  if (MODE == HEAD_FWD && threadIdx.x < HD_TILE) {
+  if (FWD && threadIdx.x < HD_TILE) {
     // the rows' columns more: ones against the three parts of the bias (32-byte rows, 16-byte halves exchanged in every
     // second group of four rows: the 32-byte swizzle)
     for (int b = 0; b < p.rbufs; ++b) {
@@ -158,10 +162,10 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         const int t0 = sp * p.tiles_per_split;
         const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
         if (!mbar_wait(&r_empty[rb], rph ^ 1u, abort_flag, p.status, 91)) break;
-        mbar_expect_tx(&r_full[rb], MODE == HEAD_FWD ? box16 : tile_bytes);
+        mbar_expect_tx(&r_full[rb], FWD ? box16 : tile_bytes);
         for (int k = 0; k < p.kboxes; ++k)
           hd_tma_2d(smem_r + rb * tile_bytes + k * HD_BOX, &p.mapR, &r_full[rb], k * 64, rt * HD_TILE);
-        if (MODE != HEAD_FWD)
+        if (!FWD)
           hd_tma_2d(smem_r + rb * tile_bytes + box16, &p.mapR16, &r_full[rb], 0, rt * HD_TILE);
         if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
         for (int t = t0; t < t1; ++t) {
@@ -174,7 +178,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         }
       }
     }
-  } else if (warp == 1 || (MODE == HEAD_FWD && warp == 2)) {
+  } else if (warp == 1 || (FWD && warp == 2)) {
     // s = R Q^T of a tile: R's and Q's channels, then the sixteen columns more
     const bool leader = elect_one();
     const uint32_t hi = desc_hi(8u * 128u, 2u), hi16 = desc_hi(8u * 32u, 6u);
@@ -189,14 +193,14 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       if (!__all_sync(0xffffffffu, mbar_wait(&r_full[rb], rph, abort_flag, p.status, 94))) { ok = false; break; }
       bool used = false;
       for (int t = t0; t < t1; ++t, ++tc) {
-        if (MODE != HEAD_FWD || (tc & 1u) == (uint32_t)(warp - 1)) {
+        if (!FWD || (tc & 1u) == (uint32_t)(warp - 1)) {
           const int nc = cols_of(t);
           const uint32_t idesc = make_idesc_bf16(128, nc, 0, 0);
           const uint32_t a0 = r0 + rb * tile_bytes, b0 = q0 + st * tile_bytes;
           const uint32_t a_lo = desc_lo(a0, 16u), b_lo = desc_lo(b0, 16u);
           const uint32_t a16 = desc_lo(a0 + box16, 16u), b16 = desc_lo(b0 + box16, 16u);
           // the buffer is free: read by the epilogue (FWD), or its P read by the second MMA that used it
-          if (MODE == HEAD_FWD) {
+          if (FWD) {
             if (!__all_sync(0xffffffffu, mbar_wait(&s_done[b], bph ^ 1u, abort_flag, p.status, 96))) { ok = false; break; }
           } else if (tc >= NB) {
             if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[old_st], old_ph, abort_flag, p.status, 96))) { ok = false; break; }
@@ -211,7 +215,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
               tc_mma_bf16_pred(tmem + b * HD_TILE, a_lo + off, hi, b_lo + off, hi, idesc, 1u);
             }
             tc_commit(&s_full[b]);
-            if (MODE == HEAD_FWD) tc_commit(&q_empty[st]);
+            if (FWD) tc_commit(&q_empty[st]);
           }
           __syncwarp();
           used = true;
@@ -322,7 +326,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
     float g_next = 1.f;
     auto fetch = [&](int rt) {
       const long long r = (long long)rt * HD_TILE + row;
-      if (MODE != HEAD_DW) y_next = __ldg(p.rowy + r);
+      if (MODE == HEAD_FWD || MODE == HEAD_DX) y_next = __ldg(p.rowy + r);
       if (MODE == HEAD_DX) g_next = __ldg(p.rowg + r);
       if (MODE == HEAD_DW && p.roww != nullptr && r < p.rows) g_next = __ldg(p.roww + r);
     };
@@ -340,7 +344,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         next_rt %= p.row_tiles;
       }
       if (next_sp < p.splits) fetch(next_rt);
-      float m = HD_LOWEST, s = 0.f, tl = 0.f, db = 0.f;
+      float m = MODE == HEAD_ARG ? -INFINITY : HD_LOWEST, s = 0.f, tl = 0.f, db = 0.f;
+      int best = INT_MAX;
       // this group's tiles of the job: every second one over all jobs
       int t = t0 + (int)((tc ^ par) & 1u);
       tc += t1 - t0;
@@ -372,7 +377,9 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
             for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
             // bit j: column j is the row's label
             uint32_t hits;
-            if (MODE != HEAD_DW) {
+            if (MODE == HEAD_ARG) {
+              hits = 0u;
+            } else if (MODE != HEAD_DW) {
               const int at = y - (c_abs + c0);
               hits = (unsigned)at < 32u ? 1u << at : 0u;
             } else {
@@ -383,7 +390,11 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
                 hits &= __ballot_sync(0xffffffffu, rel[c0 / 32] >> k & 1) ^ rank_bits[k];
             }
             const bool any = __any_sync(0xffffffffu, hits != 0u);
-            if (MODE == HEAD_FWD) {
+            if (MODE == HEAD_ARG) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (f[j] > m || (f[j] != f[j] && m == m)) { m = f[j]; best = c_abs + c0 + j; }
+            } else if (FWD) {
               if (any) {  // f[at], by halves
                 const int at = y - (c_abs + c0);
                 float h[16];
@@ -436,25 +447,30 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
               }
             }
           }
-          if (MODE != HEAD_FWD) hd_tmem_st_wait();
+          if (!FWD) hd_tmem_st_wait();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_done[b]);
-          if (MODE != HEAD_FWD && pending) {
+          if (!FWD && pending) {
             if (!drain()) { ok = false; break; }
             pending = false;
           }
           b += 2;
           if (b >= NB) { b -= NB; bph ^= 1u; }
       }
-      if (MODE == HEAD_FWD) {
+      if (FWD) {
         // the four groups' shares of a row; two sets of buffers, so that a group that is a job ahead overwrites nothing
         const int set = jc & 1;
         s_fwd[set][0][group][row] = m;
-        s_fwd[set][1][group][row] = s;
+        s_fwd[set][1][group][row] = MODE == HEAD_ARG ? __int_as_float(best) : s;
         s_fwd[set][2][group][row] = tl;
         ok = hd_vote(1 + quad, 128, ok);
-        if (group == (int)(jc & 3u) && ok) {
+        if (MODE == HEAD_ARG && group == (int)(jc & 3u) && ok) {
+          m = s_fwd[set][0][0][row];
+          best = __float_as_int(s_fwd[set][1][0][row]);
+          for (int k = 1; k < 4; ++k) hd_better(m, best, s_fwd[set][0][k][row], __float_as_int(s_fwd[set][1][k][row]));
+          p.part[(long long)sp * p.rows_pad + r] = make_float2(m, __int_as_float(best));
+        } else if (group == (int)(jc & 3u) && ok) {
           m = s_fwd[set][0][0][row];
           for (int k = 1; k < 4; ++k) m = fmaxf(m, s_fwd[set][0][k][row]);
           s = tl = 0.f;
@@ -472,7 +488,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       sp = next_sp;
       ++jc;
     }
-    if (MODE != HEAD_FWD && ok && pending) drain();
+    if (!FWD && ok && pending) drain();
   }
 
   tc_fence_before();
@@ -519,7 +535,7 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const void* __restrict__
                                                         uint32_t* __restrict__ status) {
   const long long n = v_pad > k_pad ? v_pad : k_pad;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    if (i < v_pad) {
+    if (i < v_pad && y != nullptr) {
       int v = -1;
       if (i < V) {
         const long long raw = hd_label(labels, kind, i);
@@ -546,6 +562,20 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const void* __restrict__
         }
       }
     }
+  }
+}
+
+// the class of a voxel's largest logit, from the splits' in their order
+__global__ void __launch_bounds__(256) head_arg_kernel(const float2* __restrict__ part, int splits, long long V,
+                                                       long long v_pad, long long* __restrict__ out) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < V; i += (long long)gridDim.x * 256) {
+    float m = -INFINITY;
+    int best = INT_MAX;
+    for (int k = 0; k < splits; ++k) {
+      const float2 e = part[(long long)k * v_pad + i];
+      hd_better(m, best, e.x, __float_as_int(e.y));
+    }
+    out[i] = best == INT_MAX ? 0 : best;  // nothing above -inf
   }
 }
 
@@ -710,13 +740,13 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
   p.col_tiles = (int)((p.cols + HD_TILE - 1) / HD_TILE);
   p.rows_pad = hd_pad(p.rows);
   head_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
-  p.bufs = mode == HEAD_FWD ? 4 : p.cpad <= 128 ? 3 : 2;
+  p.bufs = mode == HEAD_FWD || mode == HEAD_ARG ? 4 : p.cpad <= 128 ? 3 : 2;
   p.accs = p.cpad <= 64 ? 2 : 1;
   // Shared memory: tiles of kboxes * 16 + 4 KB, one or two resident ones, the rest in the ring. In HEAD_DX and HEAD_DW a
   // tile stays until its second MMA, which is `bufs` tiles later, and only what is left then hides the latency of a load
   // (a ring of four for three tiles of s, 64 channels: 2500 clocks a tile, with exponentials or without).
   p.rbufs = p.kboxes == 1 ? 2 : 1;
-  p.stages = p.kboxes == 1 ? 8 : p.kboxes == 2 ? (mode == HEAD_FWD ? 4 : 5) : p.kboxes == 3 ? 3 : 2;
+  p.stages = p.kboxes == 1 ? 8 : p.kboxes == 2 ? (mode == HEAD_FWD || mode == HEAD_ARG ? 4 : 5) : p.kboxes == 3 ? 3 : 2;
   p.status = a.status;
 }
 
@@ -725,6 +755,7 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
   const long long dv[2] = {a.C, a.V}, dk[2] = {a.C, a.K}, st[2] = {1, a.C};
   const int box[2] = {64, HD_TILE};
   const bool dw = MODE == HEAD_DW;
+  constexpr bool FWD = MODE == HEAD_FWD || MODE == HEAD_ARG;
   int rc = make_map_bf16(&p.mapR, dw ? a.w : a.x, 2, dw ? dk : dv, st, box, 128);
   if (rc) return rc;
   rc = make_map_bf16(&p.mapQ, dw ? a.x : a.w, 2, dw ? dv : dk, st, box, 128);
@@ -732,11 +763,11 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
   const long long st16[2] = {1, 16}, xv[2] = {16, hd_pad(a.V)}, wk[2] = {16, hd_pad(a.K)};
   const int box16[2] = {16, HD_TILE};
   const uint4* w16 = a.w16 + (dw ? 2 * hd_pad(a.K) : 0);
-  rc = make_map_bf16(&p.mapR16, dw ? w16 : MODE == HEAD_FWD ? w16 : a.x16, 2, dw || MODE == HEAD_FWD ? wk : xv, st16, box16, 32);
+  rc = make_map_bf16(&p.mapR16, dw || FWD ? w16 : a.x16, 2, dw || FWD ? wk : xv, st16, box16, 32);
   if (rc) return rc;
   rc = make_map_bf16(&p.mapQ16, dw ? a.x16 : w16, 2, dw ? xv : wk, st16, box16, 32);
   if (rc) return rc;
-  constexpr int MOST = (MODE == HEAD_FWD ? 214 : 221) * 1024;  // beside 12 and 3 KB that are static
+  constexpr int MOST = (FWD ? 214 : 221) * 1024;  // beside 12 and 3 KB that are static
   const size_t smem = 1024 + (size_t)(p.rbufs + p.stages) * (p.kboxes * HD_BOX + HD_BOX16);
   static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have that much
   int dev = 0;
@@ -906,6 +937,50 @@ extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, i
                                                 a.den);
   if (blocks > 1) head_total_kernel<<<1, 256, 0, stream>>>(f.sums, blocks, a.total, loss, a.den);
   sb_count_launch(blocks > 1 ? 2 : 1);
+  return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+}
+
+// scratch bytes of sb_head_predict; -1: outside the range
+extern "C" long long sb_head_predict_bytes(long long V, int K, int C) {
+  if (!shape_ok(V, K, C)) return -1;
+  HeadCall a;
+  memset(&a, 0, sizeof(a));
+  a.V = V; a.K = K; a.C = C;
+  HeadFwdScratch f;
+  return head_state(a, nullptr) + head_fwd_scratch(a, f, nullptr);
+}
+
+// out [V]: the class of the largest logit, the lowest of several; a NaN is the largest
+extern "C" int sb_head_predict(const void* x, const void* w, const void* bias, int bias_kind, long long V, int K, int C,
+                               void* scratch, long long* out, uint32_t* status, cudaStream_t stream) {
+  if (!shape_ok(V, K, C) || !x || !w || !scratch || !out) return SB_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(scratch) & 255) return SB_ERR_ALIGN;
+  HeadCall a;
+  memset(&a, 0, sizeof(a));
+  a.x = (const __nv_bfloat16*)x;
+  a.w = (const __nv_bfloat16*)w;
+  a.V = V; a.K = K; a.C = C;
+  a.status = status;
+  HeadFwdScratch f;
+  head_fwd_scratch(a, f, (char*)scratch + head_state(a, scratch));
+  const int k_pad = (int)hd_pad(K);
+  head_prep_kernel<<<hd_blocks(k_pad, 8), 256, 0, stream>>>(nullptr, 4, V, 0, K, k_pad, 0, 0, nullptr, bias, bias_kind,
+                                                            a.bias2, a.w16, status);
+  sb_count_launch(1);
+  int rc, splits;
+  if (wide(a)) {
+    splits = head_wide_splits(V, K);
+    rc = head_wide_predict(a, f.part, stream);
+  } else {
+    HeadParams p;
+    head_geometry(a, HEAD_ARG, p);
+    p.part = f.part;
+    splits = p.splits;
+    rc = head_launch<HEAD_ARG, false>(a, p, stream);
+  }
+  if (rc) return rc;
+  head_arg_kernel<<<hd_blocks(V, 8), 256, 0, stream>>>(f.part, splits, V, hd_pad(V), out);
+  sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
 

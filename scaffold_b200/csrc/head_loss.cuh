@@ -70,9 +70,16 @@ __device__ __forceinline__ bool hd_vote(int id, int threads, bool ok) {
       : "memory");
   return all != 0;
 }
+// (v, i) in the place of (m, best) if it comes before it: NaN before numbers, larger ones first, then lower classes
+__device__ __forceinline__ void hd_better(float& m, int& best, float v, int i) {
+  const bool a = v != v, b = m != m;
+  if ((a && !b) || (a == b && (v > m || ((v == m || a) && i < best)))) { m = v; best = i; }
+}
+
 // head_wide.cu
 int head_wide_splits(long long V, int K);
 int head_wide_forward(const HeadCall& a, float2* part, float* tl, cudaStream_t stream);
+int head_wide_predict(const HeadCall& a, float2* part, cudaStream_t stream);
 long long head_wide_scratch(const HeadCall& a);  // floats
 int head_wide_backward(const HeadCall& a, cudaStream_t stream);
 

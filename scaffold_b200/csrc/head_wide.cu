@@ -3,6 +3,7 @@
 // pairs (tcgen05 cta_group::2): a pair multiplies 256 rows by 256 columns, each CTA loads its own 128 rows and one half
 // of the columns (64 bytes a clock and SM out of L2, half of what one CTA alone would read).
 //   WIDE_LSE  rows = voxels, columns = classes: running maximum and sum of every row over the class tiles of a job
+//   WIDE_ARG  the same with the largest logit and its class in their place
 //   WIDE_D    rows = classes, columns = voxels: P^T = p - [j = y] in bf16, a piece of the classes by a piece of the
 //             voxels at a time (HW_PIECE elements: 64 MB, which stays in L2 until both products below have read it); db
 //   WIDE_OUT  dX = g P W and dW = P^T (u X) of the piece (head_loss.cu for g and u). P^T is read K-major for dW and
@@ -11,6 +12,8 @@
 // Roundings as in head_loss.cu; here the class weights go into a copy of X (whose roundings are independent of one
 // another) and up to HD_FEW voxels P^T is followed by its remainder, along which the products' reductions go on.
 // One thread holds a row of a tile, so a row's maximum, sum and db need no exchange.
+#include <limits.h>
+
 #include <atomic>
 
 #include "head_loss.cuh"
@@ -23,7 +26,7 @@ constexpr int HW_STAGES = 6;
 constexpr int HW_STAGE = 32768;  // 64 of K for 128 rows of A and 128 columns of B
 constexpr long long HW_PIECE = 32LL << 20;
 
-enum WideEpi { WIDE_LSE = 0, WIDE_D = 1, WIDE_OUT = 2 };
+enum WideEpi { WIDE_LSE = 0, WIDE_D = 1, WIDE_OUT = 2, WIDE_ARG = 3 };
 
 struct WideParams {
   CUtensorMap mapA, mapB;
@@ -228,6 +231,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
       const int y = EPI == WIDE_LSE ? p.y[r] : 0;
       const float rp = EPI == WIDE_D ? p.rowp[r] : 0.f;
       float m = -INFINITY, s = 0.f, tl = 0.f, db = 0.f;
+      int best = INT_MAX;
       for (int t = j.t0; t < j.t1; ++t) {
         if (!mbar_wait_cl(&tfull[b], bph, abort_flag, p.status, 105)) { ok = false; break; }
         tc_fence_after();
@@ -244,10 +248,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
               const float cv[4] = {cp.x, cp.y, cp.z, cp.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                f[i + e] = fmaf(__uint_as_float(v[i + e]), HD_LOG2E, EPI == WIDE_LSE ? cv[e] : rp - cv[e]);
+                f[i + e] = fmaf(__uint_as_float(v[i + e]), HD_LOG2E, EPI == WIDE_D ? rp - cv[e] : cv[e]);
             }
           }
-          if (EPI == WIDE_LSE) {
+          if (EPI == WIDE_ARG) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (f[i] > m || (f[i] != f[i] && m == m)) { m = f[i]; best = c_abs + c0 + i; }
+          } else if (EPI == WIDE_LSE) {
             const int at = y - (c_abs + c0);
             if ((unsigned)at < 32u) {
 #pragma unroll
@@ -327,6 +335,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
         if (lane == 0) mbar_arrive_remote(release[b]);
         b ^= 1u;
         if (b == 0) bph ^= 1u;
+      }
+      if (EPI == WIDE_ARG) {
+        if (half == 1) { s_m[row] = m; s_s[row] = __int_as_float(best); }
+        ok = hd_vote(1, 256, ok);
+        if (half == 0 && ok) {
+          hd_better(m, best, s_m[row], __float_as_int(s_s[row]));
+          p.part[(long long)j.sp * p.rows_pad + r] = make_float2(m, __int_as_float(best));
+        }
+        hd_vote(1, 256, true);
       }
       if (EPI == WIDE_LSE) {
         if (half == 1) { s_m[row] = m; s_s[row] = s; s_t[row] = tl; }
@@ -528,7 +545,8 @@ int head_wide_splits(long long V, int K) {
   return s;
 }
 
-int head_wide_forward(const HeadCall& a, float2* part, float* tl, cudaStream_t stream) {
+template <int EPI>
+static int wide_rows(const HeadCall& a, float2* part, float* tl, cudaStream_t stream) {
   WideParams p;
   memset(&p, 0, sizeof(p));
   p.row_tiles = (int)(up(a.V, 256) / 256);
@@ -546,7 +564,14 @@ int head_wide_forward(const HeadCall& a, float2* part, float* tl, cudaStream_t s
   if (rc) return rc;
   rc = map_rows(&p.mapB, a.w, a.K, a.C, a.C, 128);
   if (rc) return rc;
-  return wide_launch<WIDE_LSE, 0, 0>(p, stream);
+  return wide_launch<EPI, 0, 0>(p, stream);
+}
+
+int head_wide_forward(const HeadCall& a, float2* part, float* tl, cudaStream_t stream) {
+  return wide_rows<WIDE_LSE>(a, part, tl, stream);
+}
+int head_wide_predict(const HeadCall& a, float2* part, cudaStream_t stream) {
+  return wide_rows<WIDE_ARG>(a, part, nullptr, stream);
 }
 
 // one product of a piece: rows x C over `kext` of the reduction

@@ -204,6 +204,10 @@ int sb_head_total(void* state, float* loss, cudaStream_t stream);  // the loss f
 int sb_head_backward(const void* x, const void* w, const float* cw, long long V, int K, int C, void* state, void* scratch,
                      const float* gout, void* dx, void* dw, int dw_kind, void* db, int db_kind, uint32_t* status,
                      cudaStream_t stream);
+// out [V]: the class of the largest logit (the lowest of several), without the logits; scratch 256-byte aligned
+long long sb_head_predict_bytes(long long V, int K, int C);
+int sb_head_predict(const void* x, const void* w, const void* bias, int bias_kind, long long V, int K, int C,
+                    void* scratch, long long* out, uint32_t* status, cudaStream_t stream);
 
 // number of kernels this library launched so far in the process
 long long sb_launch_count(void);

@@ -222,3 +222,17 @@ class UNet(nn.Module):
 
     def use_checkpointing(self) -> None:
         self.checkpointing = True
+
+    def keep_activations(self, bits: int) -> None:
+        """What the backward pass needs of a layer's input is kept in ``bits`` = 8 or 16 (the ordinary form) until then.
+
+        With 8, convolutions save an 8-bit copy for their weight gradient and every GroupNorm works on one in its
+        backward pass (:mod:`scaffold_b200.ops.kept8`): about half of the memory between the passes, the result of the
+        forward pass unchanged, gradients at the kept values. Kernel path only; convolutions and GroupNorms that exchange
+        with other shards keep 16 bits.
+        """
+        if bits not in (8, 16):
+            raise ValueError(f"activations are kept in 8 or 16 bits; got {bits!r}")
+        for m in self.modules():
+            if isinstance(m, (Conv3d, ConvTranspose3d, GroupNorm)):
+                m.keep_bits = bits

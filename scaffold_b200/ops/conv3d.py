@@ -27,6 +27,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import conv_kernels as ck
+from .kept8 import Kept8, keep8, restore8
 from .layout import (EPOCH_CELL_ATTR, direct_grad_target, from_vm, notify_grad_written, to_vm, use_cuda_kernels,
                      weights_epoch)
 
@@ -227,6 +228,23 @@ def _bias_grad(ctx, gy: torch.Tensor, n_out: int, bias) -> Optional[torch.Tensor
     return None
 
 
+def _save(ctx, mod, weight, xs) -> None:
+    """Save a layer's inputs for its weight gradient, as 8-bit copies where the layer was told to (``keep_bits``)."""
+    ctx.kept = None
+    if mod.keep_bits == 8 and ctx.needs_input_grad[0]:
+        kept = [keep8(x) for x in xs]
+        xs = [k.data for k in kept]
+        ctx.kept = [tuple(k)[1:] for k in kept]
+    ctx.save_for_backward(weight, *xs)
+
+
+def _saved_inputs(ctx, saved):
+    """The inputs that :func:`_save` saved, from ``ctx.saved_tensors[1:]`` (where the weight's gradient is wanted)."""
+    if ctx.kept is None:
+        return list(saved)
+    return [restore8(Kept8(d, *how)) for d, how in zip(saved, ctx.kept)]
+
+
 class _ConvSameFn(torch.autograd.Function):
     """k in {1,3} stride-1 'same' conv over voxel-major bf16 sources."""
 
@@ -265,7 +283,7 @@ class _ConvSameFn(torch.autograd.Function):
         ctx.src_c, ctx.real_c = src_c, real_c
         ctx.tap_swap = ts
         ctx.has_bias = bias is not None
-        ctx.save_for_backward(weight, *xs)
+        _save(ctx, mod, weight, xs)
         return y
 
     @staticmethod
@@ -291,6 +309,7 @@ class _ConvSameFn(torch.autograd.Function):
                     gxs[i] = o
         gw = gb = None
         if ctx.needs_input_grad[0]:
+            xs = _saved_inputs(ctx, xs)
             direct = direct_grad_target(ctx.wparam, ctx) if list(src_c) == list(real_c) else None
             if direct is not None:
                 # the ordered split-K reduce adds straight into the parameter's slice of the flat gradient buffer
@@ -331,15 +350,16 @@ class _StemFn(torch.autograd.Function):
         (y,) = ck.conv_same([xs], wf, 3, [cout_pad], bias=bpad, gn_groups=gn, gn_sink=sink, stem=True)
         mod._gn_partials = sink[0] if sink else None
         ctx.wparam, ctx.bparam = weight, bias
-        ctx.save_for_backward(weight, xs)
+        _save(ctx, mod, weight, [xs])
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        weight, xs = ctx.saved_tensors
+        weight, *xs = ctx.saved_tensors
         gy = gy.contiguous()
         gw = gb = None
         if ctx.needs_input_grad[0]:
+            (xs,) = _saved_inputs(ctx, xs)
             direct = direct_grad_target(ctx.wparam, ctx)
             if direct is not None:
                 ck.conv_wgrad(gy, [xs], 3, direct, accumulate=True, stem=True)
@@ -408,6 +428,8 @@ class _ConvHaloFn(torch.autograd.Function):
 
 class Conv3d(nn.Conv3d):
     """3-D convolution; drop-in for ``nn.Conv3d`` (k=1 or k=3 'same', stride 1 on the CUDA path)."""
+
+    keep_bits = 16  # 8: the kernel path saves an 8-bit copy of its input for the weight gradient (ops/kept8.py)
 
     def __init__(self, *args, **kwargs):
         super().__init__(*args, **kwargs)
@@ -518,19 +540,21 @@ class _ConvTFn(torch.autograd.Function):
         ctx.mod = mod
         ctx.wparam, ctx.bparam = weight, bias
         ctx.has_bias = bias is not None
-        ctx.save_for_backward(weight, x)
+        ctx.in_channels = x.shape[4]
+        _save(ctx, mod, weight, [x])
         return y
 
     @staticmethod
     def backward(ctx, gy):
-        weight, x = ctx.saved_tensors
+        weight, *x = ctx.saved_tensors
         mod = ctx.mod
         gy = gy.contiguous()
         gx = gw = gb = None
         if ctx.needs_input_grad[3]:
             wd = mod._cache.get(weight, "both", lambda w: ck.pack_convT(w, True, True))[1]
-            gx = ck.convT_dgrad(gy, wd, x.shape[4])
+            gx = ck.convT_dgrad(gy, wd, ctx.in_channels)
         if ctx.needs_input_grad[0]:
+            (x,) = _saved_inputs(ctx, x)
             direct = direct_grad_target(ctx.wparam, ctx)
             if direct is not None:
                 ck.conv_wgrad(gy, [x], 2, direct, accumulate=True)
@@ -545,6 +569,8 @@ class _ConvTFn(torch.autograd.Function):
 
 class ConvTranspose3d(nn.ConvTranspose3d):
     """k=2, s=2 transposed convolution (the U-Net upsampler); drop-in for ``nn.ConvTranspose3d``."""
+
+    keep_bits = 16  # as Conv3d.keep_bits
 
     def __init__(self, *args, **kwargs):
         super().__init__(*args, **kwargs)

@@ -30,6 +30,9 @@ _lib.register("sb_head_total", [_P, _P, _P])
 _lib.register("sb_head_backward", [_P, _P, _P, C.c_longlong, C.c_int, C.c_int, _P, _P, _P, _P, _P, C.c_int, _P, C.c_int,
                                    _P, _P])
 
+_lib.register("sb_head_predict_bytes", [C.c_longlong, C.c_int, C.c_int], C.c_longlong)
+_lib.register("sb_head_predict", [_P, _P, _P, C.c_int, C.c_longlong, C.c_int, C.c_int, _P, _P, _P, _P])
+
 _LABEL_KIND = {torch.int16: 2, torch.int32: 4, torch.int64: 8}
 _KIND = {torch.bfloat16: 0, torch.float32: 2}
 MAX_WIDTH = 32768
@@ -111,26 +114,74 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
     The kernels read bf16: an fp32 ``weight`` is rounded, its gradient comes back in fp32. Gradients: features in bf16,
     weight and bias in their own types.
     """
-    shape, dev = features.shape, features.device
+    shape = features.shape
     if not shape or labels.shape != shape[:-1]:
         raise ValueError(f"features {tuple(shape)} need labels {tuple(shape[:-1])}; got {tuple(labels.shape)}")
-    c, k = shape[-1], weight.shape[0] if weight.dim() else 0
-    if weight.dim() < 2 or k < 1 or weight.shape[1] != c or weight.numel() != k * c:
-        raise ValueError(f"weight must be [classes, {c}] (or [classes, {c}, 1, 1, 1]); got {tuple(weight.shape)}")
     if labels.dtype not in _LABEL_KIND:
         raise TypeError(f"labels must be int16, int32 or int64; got {labels.dtype}")
-    for name, t in (("bias", bias), ("class_weights", class_weights)):
-        if t is not None and t.shape != (k,):
-            raise ValueError(f"{name} must be [{k}]; got {tuple(t.shape)}")
-    for name, t in (("weight", weight), ("bias", bias), ("labels", labels), ("class_weights", class_weights)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the features are on {dev}")
     if ignore_label is not None and not -2 ** 63 <= ignore_label < 2 ** 63:
         raise ValueError(f"ignore_label {ignore_label} is no 64-bit number")
-    if weight.dim() > 2:
-        weight = weight.reshape(k, c)
+    weight = _check(features, weight, bias=bias, class_weights=class_weights, labels=labels)
     if not use_cuda_kernels(features):
         return _formula(features, weight, bias, labels, class_weights, ignore_label, spatial)
+    x, weight = _operands(features, weight, bias)
+    if labels.dim() != 1 or not labels.is_contiguous():
+        labels = labels.reshape(-1).contiguous()
+    if class_weights is not None and (class_weights.dtype != torch.float32 or class_weights.requires_grad
+                                      or not class_weights.is_contiguous()):
+        class_weights = class_weights.detach().float().contiguous()
+    if x.shape[0] == 0:  # a shard without voxels: its terms are zero, the other shards' sums are not
+        return _formula(x.float(), weight.float(), None if bias is None else bias.float(), labels, class_weights,
+                        ignore_label, spatial)
+    with on_device(x.device):
+        return _HeadLossFn.apply(x, weight, None if bias is None else bias.contiguous(), labels, class_weights,
+                                 ignore_label, spatial)
+
+
+def head_predict(features: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The class of the largest of the logits ``features @ weight.T + bias`` (the lowest of several; a NaN is the
+    largest), as int64 ``[...]``, without the logits. Arguments as for :func:`head_cross_entropy`; no gradients."""
+    if not features.shape:
+        raise ValueError("features need a channel axis")
+    weight = _check(features, weight, bias=bias)
+    with torch.no_grad():
+        if not use_cuda_kernels(features):
+            return _logits(features.reshape(-1, features.shape[-1]), weight, bias).argmax(1).view(features.shape[:-1])
+        x, weight = _operands(features, weight, bias)
+        out = torch.empty(features.shape[:-1], dtype=torch.int64, device=x.device)
+        (v, c), k = x.shape, weight.shape[0]
+        if v == 0:
+            return out
+        with on_device(x.device):
+            w16 = weight.to(torch.bfloat16)
+            bias = None if bias is None else bias.contiguous()
+            scratch = torch.empty(_lib.lib().sb_head_predict_bytes(v, k, c), dtype=torch.uint8, device=x.device)
+            _lib.check(_lib.lib().sb_head_predict(
+                x.data_ptr(), w16.data_ptr(), _lib.ptr(bias), 0 if bias is None else _KIND[bias.dtype], v, k, c,
+                scratch.data_ptr(), out.data_ptr(), _lib.status_tensor(x.device).data_ptr(), _lib.stream_ptr()),
+                "sb_head_predict")
+    return out
+
+
+def _check(features, weight, **others) -> torch.Tensor:
+    """The weight as [classes, channels], after checks of shapes and devices."""
+    c, dev = features.shape[-1], features.device
+    k = weight.shape[0] if weight.dim() else 0
+    if weight.dim() < 2 or k < 1 or weight.shape[1] != c or weight.numel() != k * c:
+        raise ValueError(f"weight must be [classes, {c}] (or [classes, {c}, 1, 1, 1]); got {tuple(weight.shape)}")
+    if weight.device != dev:
+        raise ValueError(f"weight is on {weight.device}, the features are on {dev}")
+    for name, t in others.items():
+        if t is not None and name != "labels" and t.shape != (k,):
+            raise ValueError(f"{name} must be [{k}]; got {tuple(t.shape)}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the features are on {dev}")
+    return weight if weight.dim() == 2 else weight.reshape(k, c)
+
+
+def _operands(features, weight, bias):
+    """(features [V, C] in bf16, weight) as the kernels read them: contiguous, on 16 bytes (a tensor map starts there)."""
+    c = features.shape[-1]
     if not head_supported(c):
         raise ValueError(f"the kernels read features of 8 to {MAX_WIDTH} channels in multiples of 8; got {c}")
     if weight.dtype not in _KIND or (bias is not None and bias.dtype not in _KIND):
@@ -141,21 +192,17 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
     x = features if features.dtype == torch.bfloat16 else features.to(torch.bfloat16)
     if x.dim() != 2:
         x = x.reshape(n, c)
-    if not x.is_contiguous() or x.data_ptr() % 16:  # a tensor map starts on 16 bytes
+    if not x.is_contiguous() or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     if not weight.is_contiguous() or (weight.dtype == torch.bfloat16 and weight.data_ptr() % 16):
         weight = weight.clone(memory_format=torch.contiguous_format)
-    if labels.dim() != 1 or not labels.is_contiguous():
-        labels = labels.reshape(-1).contiguous()
-    if class_weights is not None and (class_weights.dtype != torch.float32 or class_weights.requires_grad
-                                      or not class_weights.is_contiguous()):
-        class_weights = class_weights.detach().float().contiguous()
-    if n == 0:  # a shard without voxels: its terms are zero, the other shards' sums are not
-        return _formula(x.float(), weight.float(), None if bias is None else bias.float(), labels, class_weights,
-                        ignore_label, spatial)
-    with on_device(dev):
-        return _HeadLossFn.apply(x, weight, None if bias is None else bias.contiguous(), labels, class_weights,
-                                 ignore_label, spatial)
+    return x, weight
+
+
+def _logits(x, weight, bias):
+    kind = torch.promote_types(torch.promote_types(x.dtype, weight.dtype), torch.float32)
+    logits = x.to(kind) @ weight.to(kind).T
+    return logits if bias is None else logits + bias.to(kind)
 
 
 def _formula(features, weight, bias, labels, class_weights, ignore_label, spatial):
@@ -167,10 +214,8 @@ def _formula(features, weight, bias, labels, class_weights, ignore_label, spatia
     if ignore_label is not None:
         live &= y != ignore_label
     x, y = features.reshape(-1, features.shape[-1])[live], y[live]
-    kind = torch.promote_types(torch.promote_types(x.dtype, weight.dtype), torch.float32)
-    logits = x.to(kind) @ weight.to(kind).T
-    if bias is not None:
-        logits = logits + bias.to(kind)
+    logits = _logits(x, weight, bias)
+    kind = logits.dtype
     u = torch.ones(len(y), dtype=kind, device=y.device) if class_weights is None else class_weights.to(kind)[y]
     nll = torch.logsumexp(logits, 1) - logits.gather(1, y[:, None])[:, 0]
     total = spatial_all_reduce(torch.stack([(u * nll).sum(), u.sum()]), spatial)

@@ -182,3 +182,17 @@ def hard_dice_fused(logits_vm: torch.Tensor, labels: torch.Tensor, n_classes: in
 def hard_dice_reference(logits: torch.Tensor, labels: torch.Tensor, n_classes: int, spatial=None) -> torch.Tensor:
     pred = F.one_hot(logits.argmax(dim=1), n_classes).permute(0, 4, 1, 2, 3).float()
     return sharded_dice(pred, labels_to_onehot(labels, n_classes), spatial)
+
+
+def hard_dice_of_prediction(pred: torch.Tensor, labels: torch.Tensor, n_classes: int, spatial=None) -> torch.Tensor:
+    """Dice per (sample, class) of predicted classes ``[B, D, H, W]`` (:func:`scaffold_b200.ops.head_loss.head_predict`),
+    as :func:`hard_dice_reference` has it of the logits, from counts. A label outside the classes belongs to none."""
+    b = pred.shape[0]
+    pred, labels = pred.reshape(b, -1).long(), labels.reshape(b, -1).long()
+    valid = (labels >= 0) & (labels < n_classes)
+    labels = torch.where(valid, labels, 0)
+    count = lambda at, w: torch.zeros((b, n_classes), dtype=torch.int64, device=at.device).scatter_add_(1, at, w.long())  # noqa: E731
+    inter, sets = count(pred, (pred == labels) & valid), count(pred, torch.ones_like(pred)) + count(labels, valid)
+    packed = torch.stack([2 * inter, sets]).float()
+    packed = spatial_all_reduce(packed, spatial)
+    return dice_from_sums(packed[0], packed[1])

@@ -85,6 +85,8 @@ def worker(run_dict: Dict[str, Any]) -> Dict[str, Any]:
         model = model.to(device=device, memory_format=torch.channels_last_3d)
         if config.activation_checkpointing:
             model.use_checkpointing()
+        if config.activation_bits != 16:
+            model.keep_activations(config.activation_bits)
         layout = ParallelLayout(config.dc_num_shards, config.dc_shard_dims, world, rank)
         spatial = SpatialContext(layout, gn_stats=config.gn_stats, halo_backend=config.halo_exchange)
         attach_spatial(model, spatial if layout.spatial_size > 1 else None)

@@ -15,6 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..ops import loss as L
+from ..ops.head_loss import head_cross_entropy, head_predict
 from ..ops.layout import AMP_DTYPE
 from ..ops.optim import FusedClipAdam
 from ..parallel.ddp import GradReducer
@@ -25,7 +26,13 @@ from .step_graph import StepGraphs, remember_functions
 class TrainEngine:
     def __init__(self, model, optimizer, n_classes: int, device, layout=None, spatial=None,
                  class_weights: Optional[torch.Tensor] = None, amp: bool = True, grad_backend: str = "nccl",
-                 max_norm: float = 1.0, grad_overlap: bool = False, allow_fallback: bool = False):
+                 max_norm: float = 1.0, grad_overlap: bool = False, allow_fallback: bool = False, loss: str = "ce_dice"):
+        """``loss="ce"`` trains on the class-weighted cross entropy alone, taken from the features in front of the head:
+        the logits of a head with many classes are never kept (:mod:`scaffold_b200.ops.head_loss`). ``last_dice`` is NaN
+        then."""
+        if loss not in ("ce_dice", "ce"):
+            raise ValueError(f"loss must be 'ce_dice' or 'ce'; got {loss!r}")
+        self.loss = loss
         self.model, self.optimizer = model, optimizer
         self.n_classes = n_classes
         self.device = torch.device(device)
@@ -35,7 +42,7 @@ class TrainEngine:
         self.max_norm = max_norm
         self.cuda = self.device.type == "cuda"
         # the fused loss kernels keep one voxel's classes in registers (at most 32); wider heads use the PyTorch formula
-        self.fused_loss = self.cuda and self.amp and L.fused_supported(n_classes)
+        self.fused_loss = self.cuda and self.amp and L.fused_supported(n_classes) and loss == "ce_dice"
         self.flat = optimizer.attach() if isinstance(optimizer, FusedClipAdam) else None
         params = [p for p in model.parameters() if p.requires_grad]
         self.reducer = GradReducer(layout, flat=self.flat, params=params, backend=grad_backend, overlap=grad_overlap,
@@ -64,8 +71,25 @@ class TrainEngine:
         return torch.autocast(self.device.type, dtype=AMP_DTYPE)
 
     # -- forward + loss ---------------------------------------------------------
+    def _forward_ce(self, images: torch.Tensor, masks: torch.Tensor):
+        """(loss, loss, NaN, (features, masks)) of ``loss="ce"``, features and masks in kernel space."""
+        with region("predict"), self._autocast():
+            features = self.model.features(images)
+        with region("calculate_loss"):
+            if self.spatial is not None and self.spatial.lead_swap is not None:
+                masks = self.spatial.to_kernel_space(masks, first_spatial=1).contiguous()
+            if masks.dtype not in (torch.int16, torch.int32, torch.int64):
+                masks = masks.long()
+            head = self.model.up_list[-1].conv
+            with self._autocast():
+                ce = head_cross_entropy(features.permute(0, 2, 3, 4, 1), head.weight, head.bias, masks,
+                                        self.class_weights, spatial=self.spatial)
+        return ce, ce, torch.full_like(ce.detach(), float("nan")), (features, masks)
+
     def forward_loss(self, images: torch.Tensor, masks: torch.Tensor):
         """Returns (loss, ce, foreground soft dice, logits-or-None)."""
+        if self.loss == "ce":
+            return self._forward_ce(images, masks)
         with region("predict"):
             fused = self.fused_loss
             with self._autocast():
@@ -165,7 +189,13 @@ class TrainEngine:
 
     def _eval_pass(self, images: torch.Tensor, masks: torch.Tensor):
         loss, ce, fg, logits = self.forward_loss(images, masks)
-        if self.fused_loss:
+        if self.loss == "ce":
+            features, masks = logits
+            head = self.model.up_list[-1].conv
+            with self._autocast():
+                pred = head_predict(features.permute(0, 2, 3, 4, 1), head.weight, head.bias)
+            dice = L.hard_dice_of_prediction(pred, masks, self.n_classes, self.spatial)
+        elif self.fused_loss:
             logits, masks = logits  # kernel-space pair of the fused path
             dice = L.hard_dice_fused(logits, masks, self.n_classes, self.spatial)
         else:

@@ -197,7 +197,8 @@ class Trainer:
                                   spatial=self.spatial, class_weights=self.ce_class_weights,
                                   amp=bool(cfg.torch_amp), grad_backend=getattr(cfg, "grad_allreduce", "nccl"),
                                   grad_overlap=bool(getattr(cfg, "grad_overlap", False)),
-                                  allow_fallback=bool(getattr(cfg, "allow_fallback", False)))
+                                  allow_fallback=bool(getattr(cfg, "allow_fallback", False)),
+                                  loss=getattr(cfg, "loss", "ce_dice"))
         self._log_kernel_selection()
 
     def _log_kernel_selection(self) -> None:

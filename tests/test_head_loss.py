@@ -339,6 +339,35 @@ def test_nothing_is_written_beside_the_gradients(v, c, k):
     assert torch.equal(db[0][margin:-margin], bs.grad)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("v,c,k", [(1, 8, 1), (1, 64, 5000), (300, 64, 147), (1000, 16, 33), (129, 256, 1000), (257, 320, 513),
+                                   (30, 1024, 3000), (70000, 32, 34)])
+def test_the_predicted_class(v, c, k):
+    """Whole numbers make every logit exact: the class is torch's, with many ties (the lowest wins)."""
+    g = torch.Generator(device="cuda").manual_seed(v + k)
+    x = torch.randint(-1, 2, (v, c), generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.randint(-1, 2, (k, c), generator=g, device="cuda").to(torch.bfloat16)
+    b = torch.randint(-2, 3, (k,), generator=g, device="cuda").to(torch.bfloat16)
+    logits = x.double() @ w.double().T + b.double()
+    got = H.head_predict(x, w, b)
+    assert got.dtype == torch.int64 and torch.equal(got, logits.argmax(1))
+    assert torch.equal(H.head_predict(x.view(1, v, 1, c), w.view(k, c, 1, 1, 1)), (x.double() @ w.double().T).argmax(1).view(1, v, 1))
+    if k > 2:
+        b[1] = float("inf")
+        b[0] = float("-inf")
+        assert (H.head_predict(x, w, b) == 1).all()
+        x[0, 0] = float("nan")  # every logit of the voxel: the first one
+        assert int(H.head_predict(x, w)[0]) == 0
+    assert H.head_predict(x[:0], w).shape == (0,)
+
+
+def test_the_predicted_class_on_the_cpu():
+    x, w, b, *_ = _inputs(50, 16, 9, dev="cpu")
+    assert torch.equal(H.head_predict(x, w, b), (x.float() @ w.float().T + b.float()).argmax(1))
+    with pytest.raises(ValueError, match="weight"):
+        H.head_predict(x, w[:, :8], b)
+
+
 def test_the_formula_on_the_cpu_and_its_gradients():
     x, w, b, y, cw = _inputs(60, 24, 40, ignored=0.2, weighted=True, dev="cpu")
     xs, ws, bs = (t.double().requires_grad_() for t in (x, w, b))
