@@ -10,14 +10,14 @@
 // s_ij + b_j - lse_i and an entry costs the epilogue a multiplication by log2(e) and an exponential. Column parameters
 // out of shared memory cost it a data-pipe cycle per warp and column each, more than the exponential unit's share.
 //
-// One kernel template, three modes. A CTA keeps 128 ROWS resident and walks 128-wide tiles of COLUMNS:
-//   HEAD_FWD  rows = voxels, columns = classes: running maximum and sum of every row (one row per thread, no exchange)
-//   HEAD_ARG  the same with the largest logit and its class (the lowest of several) in their place
-//   HEAD_DX   rows = voxels, columns = classes: P = p - [j = y] in bf16 goes back to tensor memory over the tile of s it
-//             came from, and acc[128][C] += P W is the second MMA with P as its A operand (W's tile is the same shared
-//             memory, read MN-major); the row's g multiplies the finished sum
-//   HEAD_DW   rows = classes, columns = voxels: the same with X and W exchanged, P = u (p - [j = y]); a row of P^T is a
-//             class, so db is a sum inside a thread; dL / sum u multiplies the finished sums
+// A CTA keeps tiles of 128 ROWS resident and walks 128-wide tiles of COLUMNS, two kernels:
+//   head_rows_kernel  rows = voxels, columns = classes: running maximum and sum of every row (one row per thread, no
+//                     exchange between threads), or (ARG) the largest logit and its class
+//   head_grad_kernel  HEAD_DX  rows = voxels, columns = classes: P = p - [j = y] in bf16 goes back to tensor memory over
+//                     the tile of s it came from, and acc[128][C] += P W is the second MMA with P as its A operand (W's
+//                     tile is the same shared memory, read MN-major); the row's g multiplies the finished sum
+//                     HEAD_DW  rows = classes, columns = voxels: the same with X and W exchanged, P = u (p - [j = y]); a
+//                     row of P^T is a class, so db is a sum inside a thread; dL / sum u multiplies the finished sums
 //
 // Roundings. P has 8 significant bits, all sums are fp32. The target's one is taken off in fp32, before the rounding:
 // behind it a confident voxel (p near 1) would keep nothing but the rounding of p. Common factors stay out of P, so that
@@ -25,12 +25,12 @@
 // Where one rounding can make up a result (LO: up to HD_FEW voxels; class weights in HEAD_DW, whose rounding the voxels
 // of a class share) P is kept as two bf16, value and remainder, and the second MMA runs once for each.
 //
-// Roles: warp 0 loads (TMA), warps 1 and 2 issue MMAs, warps 3-18 are the epilogue: four groups of four warps, a group
-// takes the even or the odd tiles and one half of their columns. All waits are bounded.
+// Roles: warp 0 loads (TMA), warps 1 and 2 issue MMAs, warps 3-18 are the epilogue, four groups of four warps (a row per
+// thread). All waits are bounded.
 // Two issuing warps: one is never more than about an MMA ahead of the tensor pipe and loses some 100 clocks at each wait
-// and some 300 at each commit, during which only the other one's MMAs can run. HEAD_DX / HEAD_DW: warp 1 the first MMAs
-// (as many tiles ahead as tensor memory holds), warp 2 the second ones; HEAD_FWD: the even and the odd tiles. One warp
-// for everything took 2150 clocks a tile at 64 channels, the exponentials left out or not.
+// and some 300 at each commit, during which only the other one's MMAs can run. head_grad_kernel: warp 1 the first MMAs
+// (as many tiles ahead as tensor memory holds), warp 2 the second ones; head_rows_kernel: two groups' tiles each. One
+// warp for everything took 2150 clocks a tile at 64 channels, the exponentials left out or not.
 #include <limits.h>
 
 #include <atomic>
@@ -48,16 +48,16 @@ constexpr int HD_BOX16 = HD_TILE * 32; // and of the sixteen columns more
 constexpr int HD_MAX_STAGES = 8;
 constexpr int HD_MAX_C = 256;          // TMEM: two or three tiles of s and the accumulator in 512 columns
 
-enum HeadMode { HEAD_FWD = 0, HEAD_DX = 1, HEAD_DW = 2, HEAD_ARG = 3 };
+enum HeadMode { HEAD_ROWS = 0, HEAD_DX = 1, HEAD_DW = 2 };
 
 struct HeadParams {
   CUtensorMap mapR, mapQ, mapR16, mapQ16;  // rows and columns, and their sixteen columns more
   const int* coly;      // DW: label (-1: none)
   const float* roww;    // DW: class weight of a row, or null
   const float* rowg;    // DX: g
-  const int* rowy;      // FWD / DX: label
-  float2* part;         // FWD: [splits][rows padded] running maximum and sum
-  float* tl;            // FWD: [rows padded] t at the label
+  const int* rowy;      // ROWS / DX: label
+  float2* part;         // ROWS: [splits, times four with `together` 1][rows padded] running maximum and sum
+  float* tl;            // ROWS: [rows padded] s log2(e) at the label
   __nv_bfloat16* out;   // DX with one split: [rows][C]
   float* ws;            // DX / DW: [splits][rows padded][cpad]
   float* ws_b;          // DW: [4 splits][rows padded]
@@ -66,6 +66,7 @@ struct HeadParams {
   int C, cpad, kboxes, ksteps;
   int row_tiles, col_tiles, splits, tiles_per_split;
   int stages, rbufs, bufs, accs;
+  int together;         // ROWS: row tiles of a job, 4 or 1
 };
 
 // D[tmem] (+)= A[tmem] * B[smem]: A holds two bf16 of K per 32-bit column, one row per lane
@@ -94,42 +95,54 @@ __device__ __forceinline__ void hd_sub_if(float& v, float d, uint32_t bits, uint
       : "+f"(v)
       : "f"(d), "r"(bits), "r"(bit));
 }
-template <int MODE, bool LO>
-__global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_constant__ HeadParams p) {
-  constexpr int MAXB = 4;
-  constexpr bool FWD = MODE == HEAD_FWD || MODE == HEAD_ARG;
-  const uint32_t NB = (uint32_t)p.bufs;          // tiles of s in tensor memory
-  const uint32_t ACC = NB * HD_TILE;             // column of the accumulators
-  const uint32_t naccs = (uint32_t)p.accs;       // one or two, 64 columns apart: a job goes on while the last one's is read
+// s = R Q^T of a tile: the sixteen columns more, then the channels
+__device__ __forceinline__ void hd_first_mma(uint32_t d, uint32_t r, uint32_t q, uint32_t box16, int cols, int ksteps) {
+  const uint32_t hi = desc_hi(8u * 128u, 2u), hi16 = desc_hi(8u * 32u, 6u);
+  const uint32_t idesc = make_idesc_bf16(128, cols, 0, 0);
+  const uint32_t a_lo = desc_lo(r, 16u), b_lo = desc_lo(q, 16u);
+  tc_mma_bf16_pred(d, desc_lo(r + box16, 16u), hi16, desc_lo(q + box16, 16u), hi16, idesc, 0u);
+  for (int k = 0; k < ksteps; ++k) {
+    const uint32_t off = (uint32_t)(k >> 2) * (HD_BOX >> 4) + (uint32_t)(k & 3) * 2u;
+    tc_mma_bf16_pred(d, a_lo + off, hi, b_lo + off, hi, idesc, 1u);
+  }
+}
+
+// Log-sum-exp of the rows (or ARG: their largest logit). Tensor memory holds four tiles of s, one for each epilogue group.
+//   together = 4: a job is four row tiles by a run of column tiles; group g has row tile g all along, so a column tile is
+//                 loaded once for 512 rows and a row's statistics stay in one thread: nothing is merged in the CTA
+//   together = 1: a job is one row tile; group g takes every fourth column tile and leaves statistics of its own
+// The second one is for calls that have no four row tiles for every SM, and for tiles of which shared memory holds few.
+// Bound: the exponential unit, 1024 clocks a tile of 128 x 128. Merging two halves of a tile's columns over two groups by
+// tile parity instead (a barrier and an exchange in every job): 631 us for 2 x 128^3 voxels, 64 channels and 257 classes.
+template <bool ARG>
+__global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_constant__ HeadParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t r_full[2], r_empty[2], q_full[HD_MAX_STAGES], q_empty[HD_MAX_STAGES], s_full[MAXB], s_done[MAXB],
-      acc_full[2], acc_empty[2];
-  __shared__ float s_fwd[FWD ? 2 : 1][3][FWD ? 4 : 1][HD_TILE];
+  __shared__ uint64_t r_full[4], r_empty[4], q_full[HD_MAX_STAGES], q_empty[HD_MAX_STAGES], s_full[4], s_done[4];
   __shared__ uint32_t tmem_base_s, abort_s;
   volatile uint32_t* abort_flag = &abort_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int jobs = p.row_tiles * p.splits;
-  const uint32_t box16 = (uint32_t)p.kboxes * HD_BOX;  // where the sixteen columns more are
-  const uint32_t tile_bytes = box16 + HD_BOX16;
+  const bool four = p.together == 4;
+  const int row_jobs = four ? (p.row_tiles + 3) / 4 : p.row_tiles, jobs = row_jobs * p.splits;
+  const uint32_t box16 = (uint32_t)p.kboxes * HD_BOX, tile_bytes = box16 + HD_BOX16;
   uint8_t* smem_r = smem;
   uint8_t* smem_q = smem + (size_t)p.rbufs * tile_bytes;
 
   if (threadIdx.x == 0) {
     abort_s = 0;
-    for (int i = 0; i < 2; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], FWD ? 2 : 1); }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&r_full[i], 1);
+      mbar_init(&r_empty[i], four ? 1 : 2);  // a row tile of several is one issuing warp's, a single one both warps'
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_done[i], HD_EPI_WARPS / 4);
+    }
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
+      mbar_init(&q_empty[i], four ? 2 : 1);
     }
-    for (int i = 0; i < MAXB; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_done[i], HD_EPI_WARPS / 2);
-    }
-    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], HD_EPI_WARPS); }
     mbar_fence_init();
   }
-  if (FWD && threadIdx.x < HD_TILE) {
+  if (threadIdx.x < HD_TILE) {
     // the rows' columns more: ones against the three parts of the bias (32-byte rows, 16-byte halves exchanged in every
     // second group of four rows: the 32-byte swizzle)
     for (int b = 0; b < p.rbufs; ++b) {
@@ -158,15 +171,237 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       uint32_t rb = 0, rph = 0, st = 0, ph = 0;
       bool ok = true;
       for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
+        const int rt = job % row_jobs * p.together, sp = job / row_jobs;
+        const int t0 = sp * p.tiles_per_split;
+        const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
+        for (int t = t0; t < t1 && ok; ++t) {
+          // the column tile, and in front of the first one the row tiles (each as soon as its last one is done with)
+          for (int g = 0; t == t0 && g < p.together; ++g) {
+            if (!mbar_wait(&r_empty[rb], rph ^ 1u, abort_flag, p.status, 91)) { ok = false; break; }
+            mbar_expect_tx(&r_full[rb], box16);
+            for (int k = 0; k < p.kboxes; ++k)
+              hd_tma_2d(smem_r + rb * tile_bytes + k * HD_BOX, &p.mapR, &r_full[rb], k * 64, (rt + g) * HD_TILE);
+            if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
+          }
+          if (!ok || !mbar_wait(&q_empty[st], ph ^ 1u, abort_flag, p.status, 91)) { ok = false; break; }
+          mbar_expect_tx(&q_full[st], tile_bytes);
+          for (int k = 0; k < p.kboxes; ++k)
+            hd_tma_2d(smem_q + st * tile_bytes + k * HD_BOX, &p.mapQ, &q_full[st], k * 64, t * HD_TILE);
+          hd_tma_2d(smem_q + st * tile_bytes + box16, &p.mapQ16, &q_full[st], 0, t * HD_TILE);
+          if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
+        }
+      }
+    }
+  } else if (warp <= 2) {
+    const bool leader = elect_one();
+    const uint32_t mine = (uint32_t)warp - 1u;
+    const uint32_t r0 = smem_u32(smem_r), q0 = smem_u32(smem_q);
+    uint32_t rb = 0, rph = 0, st = 0, ph = 0, fi = 0;  // fi: column tiles so far (together = 1)
+    uint32_t uses[2] = {0u, 0u};                       // of this warp's two tiles of s
+    bool ok = true;
+    // one tile into buffer g: rows out of r_slot, columns out of the current stage
+    auto tile = [&](uint32_t g, uint32_t r_slot, int t) -> bool {
+      const uint32_t u = uses[g >> 1]++;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_done[g], (u & 1u) ^ 1u, abort_flag, p.status, 96))) return false;
+      tc_fence_after();
+      if (leader) {
+        hd_first_mma(tmem + g * HD_TILE, r0 + r_slot * tile_bytes, q0 + st * tile_bytes, box16, cols_of(t), p.ksteps);
+        tc_commit(&s_full[g]);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
+      const int sp = job / row_jobs;
+      const int t0 = sp * p.tiles_per_split;
+      const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
+      bool used = false;
+      if (!four && !__all_sync(0xffffffffu, mbar_wait(&r_full[rb], rph, abort_flag, p.status, 94))) break;
+      for (int t = t0; t < t1 && ok; ++t, ++fi) {
+        if (four || (fi & 1u) == mine) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95))) { ok = false; break; }
+          if (four) {
+            for (uint32_t g = mine; g < 4u && ok; g += 2u) {
+              if (t == t0) ok = __all_sync(0xffffffffu, mbar_wait(&r_full[g], rph, abort_flag, p.status, 94));
+              ok = ok && tile(g, g, t);
+              if (ok && leader && t == t1 - 1) tc_commit(&r_empty[g]);
+              __syncwarp();
+            }
+          } else {
+            ok = tile(fi & 3u, rb, t);
+            used = true;
+          }
+          if (ok && leader) tc_commit(&q_empty[st]);
+          __syncwarp();
+        }
+        if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
+      }
+      if (four) {
+        rph ^= 1u;
+      } else {
+        if (ok && leader) {  // this warp is done with the resident tile
+          if (used) tc_commit(&r_empty[rb]);
+          else mbar_arrive(&r_empty[rb]);
+        }
+        __syncwarp();
+        if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
+      }
+    }
+  } else {
+    const int quad = warp & 3, group = (warp - HD_FIRST_EPI) >> 2;
+    const uint32_t tile = tmem + ((uint32_t)(quad * 32) << 16) + group * HD_TILE;
+    uint32_t uses = 0, fi = 0;
+    bool ok = true;
+    int rt = blockIdx.x % row_jobs, sp = blockIdx.x / row_jobs;
+    auto row_of = [&](int j) { return ((long long)(four ? j * 4 + group : j)) * HD_TILE + quad * 32 + lane; };
+    auto label_of = [&](int j) { return !ARG && row_of(j) < p.rows_pad ? __ldg(p.rowy + row_of(j)) : -1; };
+    int y_next = label_of(rt);
+    while (sp < p.splits && ok) {
+      const int t0 = sp * p.tiles_per_split;
+      const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
+      const long long r = row_of(rt);
+      const int y = y_next, slot = four ? sp : sp * 4 + group;
+      rt += gridDim.x;
+      if (rt >= row_jobs) {
+        sp += rt / row_jobs;
+        rt %= row_jobs;
+      }
+      if (sp < p.splits) y_next = label_of(rt);
+      float m = ARG ? -INFINITY : HD_LOWEST, s = 0.f, tl = 0.f;
+      bool met = false;
+      int best = INT_MAX;
+      int t = four ? t0 : t0 + (int)((group - fi) & 3u);
+      fi += t1 - t0;
+      for (; t < t1; t += four ? 1 : 4, ++uses) {
+        if (!mbar_wait(&s_full[group], uses & 1u, abort_flag, p.status, 98)) { ok = false; break; }
+        tc_fence_after();
+        const int nc = cols_of(t), c_abs = t * HD_TILE;
+#pragma unroll 1
+        for (int c0 = 0; c0 < nc; c0 += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32(tile + c0, v);
+          tmem_ld_wait();
+          if (c0 + 32 >= nc) {  // read to the end: the next tile may come
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_done[group]);
+          }
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+          if (ARG) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (f[j] > m || (f[j] != f[j] && m == m)) { m = f[j]; best = c_abs + c0 + j; }
+          } else {
+            const int at = y - (c_abs + c0);
+            const bool hit = (unsigned)at < 32u;
+            if (__any_sync(0xffffffffu, hit)) {  // f[at], by halves
+              float h[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) h[j] = at & 16 ? f[16 + j] : f[j];
+#pragma unroll
+              for (int n = 8; n > 0; n >>= 1)
+#pragma unroll
+                for (int j = 0; j < n; ++j) h[j] = at & n ? h[n + j] : h[j];
+              if (hit) { tl = h[0]; met = true; }
+            }
+            float mx[4] = {f[0], f[1], f[2], f[3]};
+#pragma unroll
+            for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], f[j]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (top > m) {
+              s *= hd_ex2((m - top) * HD_LOG2E);
+              m = top;
+            }
+            const float base = -m * HD_LOG2E;
+            float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a[j & 3] += hd_ex2(fmaf(f[j], HD_LOG2E, base));
+            s += (a[0] + a[1]) + (a[2] + a[3]);
+          }
+        }
+      }
+      if (ok && r < p.rows_pad) {
+        p.part[(long long)slot * p.rows_pad + r] = ARG ? make_float2(m, __int_as_float(best)) : make_float2(m * HD_LOG2E, s);
+        if (!ARG && met) p.tl[r] = tl * HD_LOG2E;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 0) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int MODE, bool LO>
+__global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_constant__ HeadParams p) {
+  constexpr int MAXB = 3;
+  const uint32_t NB = (uint32_t)p.bufs;          // tiles of s in tensor memory
+  const uint32_t ACC = NB * HD_TILE;             // column of the accumulators
+  const uint32_t naccs = (uint32_t)p.accs;       // one or two, 64 columns apart: a job goes on while the last one's is read
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t r_full[2], r_empty[2], q_full[HD_MAX_STAGES], q_empty[HD_MAX_STAGES], s_full[MAXB], s_done[MAXB],
+      acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_base_s, abort_s;
+  volatile uint32_t* abort_flag = &abort_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int jobs = p.row_tiles * p.splits;
+  const uint32_t box16 = (uint32_t)p.kboxes * HD_BOX;  // where the sixteen columns more are
+  const uint32_t tile_bytes = box16 + HD_BOX16;
+  uint8_t* smem_r = smem;
+  uint8_t* smem_q = smem + (size_t)p.rbufs * tile_bytes;
+
+  if (threadIdx.x == 0) {
+    abort_s = 0;
+    for (int i = 0; i < 2; ++i) { mbar_init(&r_full[i], 1); mbar_init(&r_empty[i], 1); }
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < MAXB; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_done[i], HD_EPI_WARPS / 2);
+    }
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], HD_EPI_WARPS); }
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&tmem_base_s, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+  const int last_cols = ((int)(p.cols - (long long)(p.col_tiles - 1) * HD_TILE) + 31) & ~31;
+  auto cols_of = [&](int t) -> int { return t + 1 < p.col_tiles ? HD_TILE : last_cols; };  // up to a multiple of 32
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&p.mapR);
+      tma_prefetch_desc(&p.mapQ);
+      uint32_t rb = 0, rph = 0, st = 0, ph = 0;
+      bool ok = true;
+      for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
         const int rt = job % p.row_tiles, sp = job / p.row_tiles;
         const int t0 = sp * p.tiles_per_split;
         const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
         if (!mbar_wait(&r_empty[rb], rph ^ 1u, abort_flag, p.status, 91)) break;
-        mbar_expect_tx(&r_full[rb], FWD ? box16 : tile_bytes);
+        mbar_expect_tx(&r_full[rb], tile_bytes);
         for (int k = 0; k < p.kboxes; ++k)
           hd_tma_2d(smem_r + rb * tile_bytes + k * HD_BOX, &p.mapR, &r_full[rb], k * 64, rt * HD_TILE);
-        if (!FWD)
-          hd_tma_2d(smem_r + rb * tile_bytes + box16, &p.mapR16, &r_full[rb], 0, rt * HD_TILE);
+        hd_tma_2d(smem_r + rb * tile_bytes + box16, &p.mapR16, &r_full[rb], 0, rt * HD_TILE);
         if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
         for (int t = t0; t < t1; ++t) {
           if (!mbar_wait(&q_empty[st], ph ^ 1u, abort_flag, p.status, 91)) { ok = false; break; }
@@ -178,12 +413,10 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         }
       }
     }
-  } else if (warp == 1 || (FWD && warp == 2)) {
-    // s = R Q^T of a tile: R's and Q's channels, then the sixteen columns more
+  } else if (warp == 1) {
     const bool leader = elect_one();
-    const uint32_t hi = desc_hi(8u * 128u, 2u), hi16 = desc_hi(8u * 32u, 6u);
     const uint32_t r0 = smem_u32(smem_r), q0 = smem_u32(smem_q);
-    uint32_t rb = 0, rph = 0, st = 0, ph = 0, b = 0, bph = 0, tc = 0;
+    uint32_t rb = 0, rph = 0, st = 0, ph = 0, b = 0, tc = 0;
     uint32_t old_st = 0, old_ph = 0;  // the tile that had this one's buffer
     bool ok = true;
     for (int job = blockIdx.x; job < jobs && ok; job += gridDim.x) {
@@ -191,43 +424,23 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
       const int t0 = sp * p.tiles_per_split;
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
       if (!__all_sync(0xffffffffu, mbar_wait(&r_full[rb], rph, abort_flag, p.status, 94))) { ok = false; break; }
-      bool used = false;
       for (int t = t0; t < t1; ++t, ++tc) {
-        if (!FWD || (tc & 1u) == (uint32_t)(warp - 1)) {
-          const int nc = cols_of(t);
-          const uint32_t idesc = make_idesc_bf16(128, nc, 0, 0);
-          const uint32_t a0 = r0 + rb * tile_bytes, b0 = q0 + st * tile_bytes;
-          const uint32_t a_lo = desc_lo(a0, 16u), b_lo = desc_lo(b0, 16u);
-          const uint32_t a16 = desc_lo(a0 + box16, 16u), b16 = desc_lo(b0 + box16, 16u);
-          // the buffer is free: read by the epilogue (FWD), or its P read by the second MMA that used it
-          if (FWD) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&s_done[b], bph ^ 1u, abort_flag, p.status, 96))) { ok = false; break; }
-          } else if (tc >= NB) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[old_st], old_ph, abort_flag, p.status, 96))) { ok = false; break; }
-            if (++old_st == (uint32_t)p.stages) { old_st = 0; old_ph ^= 1u; }
-          }
-          if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95))) { ok = false; break; }
-          tc_fence_after();
-          if (leader) {
-            tc_mma_bf16_pred(tmem + b * HD_TILE, a16, hi16, b16, hi16, idesc, 0u);
-            for (int k = 0; k < p.ksteps; ++k) {
-              const uint32_t off = (uint32_t)(k >> 2) * (HD_BOX >> 4) + (uint32_t)(k & 3) * 2u;
-              tc_mma_bf16_pred(tmem + b * HD_TILE, a_lo + off, hi, b_lo + off, hi, idesc, 1u);
-            }
-            tc_commit(&s_full[b]);
-            if (FWD) tc_commit(&q_empty[st]);
-          }
-          __syncwarp();
-          used = true;
+        // the buffer is free: its P was read by the second MMA that used it
+        if (tc >= NB) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[old_st], old_ph, abort_flag, p.status, 96))) { ok = false; break; }
+          if (++old_st == (uint32_t)p.stages) { old_st = 0; old_ph ^= 1u; }
         }
+        if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95))) { ok = false; break; }
+        tc_fence_after();
+        if (leader) {
+          hd_first_mma(tmem + b * HD_TILE, r0 + rb * tile_bytes, q0 + st * tile_bytes, box16, cols_of(t), p.ksteps);
+          tc_commit(&s_full[b]);
+          if (t == t1 - 1) tc_commit(&r_empty[rb]);
+        }
+        __syncwarp();
         if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
-        if (++b == NB) { b = 0; bph ^= 1u; }
+        if (++b == NB) b = 0;
       }
-      if (ok && leader) {  // this warp is done with the resident tile
-        if (used) tc_commit(&r_empty[rb]);
-        else mbar_arrive(&r_empty[rb]);
-      }
-      __syncwarp();
       if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
     }
   } else if (warp == 2) {
@@ -273,7 +486,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
     const uint32_t par = group >> 1;
     const int row = quad * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    uint32_t b = par, bph = 0, ab = 0, aph = 0, tc = 0, jc = 0;  // b: buffer of this group's next tile (two or more there are)
+    uint32_t b = par, bph = 0, ab = 0, aph = 0, tc = 0;  // b: buffer of this group's next tile (two or more there are)
     bool ok = true, pending = false;
     int pend_rt = 0, pend_sp = 0;
     float pend_g = 0.f, pend_db = 0.f;
@@ -326,8 +539,10 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
     float g_next = 1.f;
     auto fetch = [&](int rt) {
       const long long r = (long long)rt * HD_TILE + row;
-      if (MODE == HEAD_FWD || MODE == HEAD_DX) y_next = __ldg(p.rowy + r);
-      if (MODE == HEAD_DX) g_next = __ldg(p.rowg + r);
+      if (MODE == HEAD_DX) {
+        y_next = __ldg(p.rowy + r);
+        g_next = __ldg(p.rowg + r);
+      }
       if (MODE == HEAD_DW && p.roww != nullptr && r < p.rows) g_next = __ldg(p.roww + r);
     };
     int rt = blockIdx.x % p.row_tiles, sp = blockIdx.x / p.row_tiles;
@@ -344,8 +559,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
         next_rt %= p.row_tiles;
       }
       if (next_sp < p.splits) fetch(next_rt);
-      float m = MODE == HEAD_ARG ? -INFINITY : HD_LOWEST, s = 0.f, tl = 0.f, db = 0.f;
-      int best = INT_MAX;
+      float db = 0.f;
       // this group's tiles of the job: every second one over all jobs
       int t = t0 + (int)((tc ^ par) & 1u);
       tc += t1 - t0;
@@ -377,9 +591,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
             for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
             // bit j: column j is the row's label
             uint32_t hits;
-            if (MODE == HEAD_ARG) {
-              hits = 0u;
-            } else if (MODE != HEAD_DW) {
+            if (MODE == HEAD_DX) {
               const int at = y - (c_abs + c0);
               hits = (unsigned)at < 32u ? 1u << at : 0u;
             } else {
@@ -390,36 +602,6 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
                 hits &= __ballot_sync(0xffffffffu, rel[c0 / 32] >> k & 1) ^ rank_bits[k];
             }
             const bool any = __any_sync(0xffffffffu, hits != 0u);
-            if (MODE == HEAD_ARG) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (f[j] > m || (f[j] != f[j] && m == m)) { m = f[j]; best = c_abs + c0 + j; }
-            } else if (FWD) {
-              if (any) {  // f[at], by halves
-                const int at = y - (c_abs + c0);
-                float h[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) h[j] = at & 16 ? f[16 + j] : f[j];
-#pragma unroll
-                for (int n = 8; n > 0; n >>= 1)
-#pragma unroll
-                  for (int j = 0; j < n; ++j) h[j] = at & n ? h[n + j] : h[j];
-                if (hits) tl = h[0];
-              }
-              float mx[4] = {f[0], f[1], f[2], f[3]};
-#pragma unroll
-              for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], f[j]);
-              const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-              if (top > m) {
-                s *= hd_ex2((m - top) * HD_LOG2E);
-                m = top;
-              }
-              const float base = -m * HD_LOG2E;
-              float a[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int j = 0; j < 32; ++j) a[j & 3] += hd_ex2(fmaf(f[j], HD_LOG2E, base));
-              s += (a[0] + a[1]) + (a[2] + a[3]);
-            } else {
 #pragma unroll
               for (int j = 0; j < 32; ++j) f[j] = hd_ex2(f[j] * HD_LOG2E);
               if (any) {
@@ -445,50 +627,25 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_kernel(const __grid_consta
                                      f[2 * j + 1] - __uint_as_float(o[j] & 0xFFFF0000u));
                 hd_tmem_st_x16(tile + c0 + 16, o);
               }
-            }
           }
-          if (!FWD) hd_tmem_st_wait();
+          hd_tmem_st_wait();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_done[b]);
-          if (!FWD && pending) {
+          if (pending) {
             if (!drain()) { ok = false; break; }
             pending = false;
           }
           b += 2;
           if (b >= NB) { b -= NB; bph ^= 1u; }
       }
-      if (FWD) {
-        // the four groups' shares of a row; two sets of buffers, so that a group that is a job ahead overwrites nothing
-        const int set = jc & 1;
-        s_fwd[set][0][group][row] = m;
-        s_fwd[set][1][group][row] = MODE == HEAD_ARG ? __int_as_float(best) : s;
-        s_fwd[set][2][group][row] = tl;
-        ok = hd_vote(1 + quad, 128, ok);
-        if (MODE == HEAD_ARG && group == (int)(jc & 3u) && ok) {
-          m = s_fwd[set][0][0][row];
-          best = __float_as_int(s_fwd[set][1][0][row]);
-          for (int k = 1; k < 4; ++k) hd_better(m, best, s_fwd[set][0][k][row], __float_as_int(s_fwd[set][1][k][row]));
-          p.part[(long long)sp * p.rows_pad + r] = make_float2(m, __int_as_float(best));
-        } else if (group == (int)(jc & 3u) && ok) {
-          m = s_fwd[set][0][0][row];
-          for (int k = 1; k < 4; ++k) m = fmaxf(m, s_fwd[set][0][k][row]);
-          s = tl = 0.f;
-          for (int k = 0; k < 4; ++k) s += s_fwd[set][1][k][row] * hd_ex2((s_fwd[set][0][k][row] - m) * HD_LOG2E);
-          for (int k = 0; k < 4; ++k) tl += s_fwd[set][2][k][row];  // one of them has met the label, the others hold 0
-          p.part[(long long)sp * p.rows_pad + r] = make_float2(m * HD_LOG2E, s);
-          if (y >= (long long)t0 * HD_TILE && y < (long long)t1 * HD_TILE) p.tl[r] = tl * HD_LOG2E;
-        }
-      } else {
-        if (ok && pending) ok = drain();  // this job had no tile for this group
-        pending = true;
-        pend_rt = rt; pend_sp = sp; pend_g = g; pend_db = db;
-      }
+      if (ok && pending) ok = drain();  // this job had no tile for this group
+      pending = true;
+      pend_rt = rt; pend_sp = sp; pend_g = g; pend_db = db;
       rt = next_rt;
       sp = next_sp;
-      ++jc;
     }
-    if (!FWD && ok && pending) drain();
+    if (ok && pending) drain();
   }
 
   tc_fence_before();
@@ -739,23 +896,42 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
   p.row_tiles = (int)((p.rows + HD_TILE - 1) / HD_TILE);
   p.col_tiles = (int)((p.cols + HD_TILE - 1) / HD_TILE);
   p.rows_pad = hd_pad(p.rows);
-  head_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
-  p.bufs = mode == HEAD_FWD || mode == HEAD_ARG ? 4 : p.cpad <= 128 ? 3 : 2;
-  p.accs = p.cpad <= 64 ? 2 : 1;
-  // Shared memory: tiles of kboxes * 16 + 4 KB, one or two resident ones, the rest in the ring. In HEAD_DX and HEAD_DW a
-  // tile stays until its second MMA, which is `bufs` tiles later, and only what is left then hides the latency of a load
-  // (a ring of four for three tiles of s, 64 channels: 2500 clocks a tile, with exponentials or without).
-  p.rbufs = p.kboxes == 1 ? 2 : 1;
-  p.stages = p.kboxes == 1 ? 8 : p.kboxes == 2 ? (mode == HEAD_FWD || mode == HEAD_ARG ? 4 : 5) : p.kboxes == 3 ? 3 : 2;
   p.status = a.status;
+  head_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
+  // shared memory holds 54 boxes of 4 KB, a tile of rows or columns is 4 kboxes + 1 of them
+  if (mode == HEAD_ROWS) {
+    // with four row tiles a job the rounds have four tiles for each of theirs; with one, four of a job's tiles run side by
+    // side, so one with fewer is as long
+    p.together = 1;
+    if (p.kboxes <= 2) {
+      int s4 = 1, per4 = 1;
+      const int rows4 = (p.row_tiles + 3) / 4;
+      head_split(rows4, p.col_tiles, &s4, &per4);
+      const long long cost4 = (((long long)rows4 * s4 + 147) / 148) * (4 * per4 + 2);
+      const long long cost1 = (((long long)p.row_tiles * p.splits + 147) / 148) * ((p.tiles_per_split > 4 ? p.tiles_per_split : 4) + 2);
+      if (cost4 <= cost1) {
+        p.together = 4;
+        p.splits = s4;
+        p.tiles_per_split = per4;
+      }
+    }
+    p.rbufs = p.together == 4 ? 4 : p.kboxes <= 2 ? 2 : 1;
+    p.stages = p.kboxes == 1 ? (p.together == 4 ? 6 : 8) : p.kboxes == 2 ? (p.together == 4 ? 2 : 4) : p.kboxes == 3 ? 3 : 2;
+    return;
+  }
+  p.bufs = p.cpad <= 128 ? 3 : 2;
+  p.accs = p.cpad <= 64 ? 2 : 1;
+  // One or two resident tiles, the rest in the ring. A tile stays until its second MMA, which is `bufs` tiles later, and
+  // only what is left then hides the latency of a load.
+  p.rbufs = p.kboxes == 1 ? 2 : 1;
+  p.stages = p.kboxes == 1 ? 8 : p.kboxes == 2 ? 5 : p.kboxes == 3 ? 3 : 2;
 }
 
-template <int MODE, bool LO>
+template <int MODE, bool FLAG>
 static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
+  constexpr bool rows = MODE == HEAD_ROWS, dw = MODE == HEAD_DW;
   const long long dv[2] = {a.C, a.V}, dk[2] = {a.C, a.K}, st[2] = {1, a.C};
   const int box[2] = {64, HD_TILE};
-  const bool dw = MODE == HEAD_DW;
-  constexpr bool FWD = MODE == HEAD_FWD || MODE == HEAD_ARG;
   int rc = make_map_bf16(&p.mapR, dw ? a.w : a.x, 2, dw ? dk : dv, st, box, 128);
   if (rc) return rc;
   rc = make_map_bf16(&p.mapQ, dw ? a.x : a.w, 2, dw ? dv : dk, st, box, 128);
@@ -763,29 +939,34 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
   const long long st16[2] = {1, 16}, xv[2] = {16, hd_pad(a.V)}, wk[2] = {16, hd_pad(a.K)};
   const int box16[2] = {16, HD_TILE};
   const uint4* w16 = a.w16 + (dw ? 2 * hd_pad(a.K) : 0);
-  rc = make_map_bf16(&p.mapR16, dw || FWD ? w16 : a.x16, 2, dw || FWD ? wk : xv, st16, box16, 32);
-  if (rc) return rc;
+  if (!rows) {
+    rc = make_map_bf16(&p.mapR16, dw ? w16 : a.x16, 2, dw ? wk : xv, st16, box16, 32);
+    if (rc) return rc;
+  }
   rc = make_map_bf16(&p.mapQ16, dw ? a.x16 : w16, 2, dw ? xv : wk, st16, box16, 32);
   if (rc) return rc;
-  constexpr int MOST = (FWD ? 214 : 221) * 1024;  // beside 12 and 3 KB that are static
+  void (*kernel)(HeadParams) = nullptr;
+  if constexpr (rows) kernel = head_rows_kernel<FLAG>;
+  else kernel = head_grad_kernel<MODE, FLAG>;
   const size_t smem = 1024 + (size_t)(p.rbufs + p.stages) * (p.kboxes * HD_BOX + HD_BOX16);
-  static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have that much
+  static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have as much as it can need
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return SB_ERR_DRIVER;
   if (dev > 63 || !(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
-    if (cudaFuncSetAttribute(head_kernel<MODE, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + 54 * HD_BOX16) != cudaSuccess)
       return SB_ERR_DRIVER;
     if (dev <= 63) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  const long long jobs = (long long)p.row_tiles * p.splits;
-  head_kernel<MODE, LO><<<(int)(jobs < 148 ? jobs : 148), HD_THREADS, smem, stream>>>(p);
+  const long long jobs = (long long)(rows && p.together == 4 ? (p.row_tiles + 3) / 4 : p.row_tiles) * p.splits;
+  kernel<<<(int)(jobs < 148 ? jobs : 148), HD_THREADS, smem, stream>>>(p);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
-
+// statistics that head_rows_kernel leaves of a row
+static int head_shares(const HeadParams& p) { return p.splits * (p.together == 4 ? 1 : 4); }
 
 static bool shape_ok(long long V, int K, int C) {
-  return V >= 1 && V <= (1LL << 31) - 512 && K >= 1 && K <= (1 << 30) && C >= 8 && C % 8 == 0 && C <= 32768;
+  return V >= 1 && V <= (1LL << 31) - 1024 && K >= 1 && K <= (1 << 30) && C >= 8 && C % 8 == 0 && C <= 32768;
 }
 
 // The forward pass's state and the scratch of each pass, in the caller's memory (256-byte aligned).
@@ -808,8 +989,8 @@ struct HeadFwdScratch {
 };
 static long long head_fwd_scratch(const HeadCall& a, HeadFwdScratch& f, void* base) {
   HeadParams p;
-  head_geometry(a, HEAD_FWD, p);
-  const long long splits = wide(a) ? head_wide_splits(a.V, a.K) : p.splits;
+  head_geometry(a, HEAD_ROWS, p);
+  const long long splits = wide(a) ? head_wide_splits(a.V, a.K) : head_shares(p);
   char* at = (char*)base;
   auto take = [&](long long bytes) { char* o = at; at += (bytes + 255) / 256 * 256; return o; };
   f.sums = (double*)take(16LL * HD_SUM_BLOCKS);
@@ -924,12 +1105,12 @@ extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, i
     rc = head_wide_forward(a, f.part, f.tl, stream);
   } else {
     HeadParams p;
-    head_geometry(a, HEAD_FWD, p);
+    head_geometry(a, HEAD_ROWS, p);
     p.part = f.part;
     p.tl = f.tl;
     p.rowy = a.y;
-    splits = p.splits;
-    rc = head_launch<HEAD_FWD, false>(a, p, stream);
+    splits = head_shares(p);
+    rc = head_launch<HEAD_ROWS, false>(a, p, stream);
   }
   if (rc) return rc;
   const int blocks = v_pad <= 4096 ? 1 : hd_blocks(v_pad, HD_SUM_BLOCKS / 148);  // 16 rounds cost less than a launch
@@ -973,10 +1154,10 @@ extern "C" int sb_head_predict(const void* x, const void* w, const void* bias, i
     rc = head_wide_predict(a, f.part, stream);
   } else {
     HeadParams p;
-    head_geometry(a, HEAD_ARG, p);
+    head_geometry(a, HEAD_ROWS, p);
     p.part = f.part;
-    splits = p.splits;
-    rc = head_launch<HEAD_ARG, false>(a, p, stream);
+    splits = head_shares(p);
+    rc = head_launch<HEAD_ROWS, true>(a, p, stream);
   }
   if (rc) return rc;
   head_arg_kernel<<<hd_blocks(V, 8), 256, 0, stream>>>(f.part, splits, V, hd_pad(V), out);

@@ -187,7 +187,7 @@ def _operands(features, weight, bias):
     if weight.dtype not in _KIND or (bias is not None and bias.dtype not in _KIND):
         raise TypeError("weight and bias must be bf16 or fp32")
     n = features.numel() // c
-    if n > 2 ** 31 - 512:
+    if n > 2 ** 31 - 1024:
         raise ValueError(f"{n} voxels are more than the kernels count")
     x = features if features.dtype == torch.bfloat16 else features.to(torch.bfloat16)
     if x.dim() != 2:
