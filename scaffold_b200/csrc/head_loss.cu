@@ -89,6 +89,28 @@ __device__ __forceinline__ void hd_tmem_st_x16(uint32_t taddr, const uint32_t* v
       : "memory");
 }
 __device__ __forceinline__ void hd_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// two fp32 in one instruction
+__device__ __forceinline__ float2 hd_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 hd_add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float hd_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // where `bits & bit`: v -= d; predicated, never a branch
 __device__ __forceinline__ void hd_sub_if(float& v, float d, uint32_t bits, uint32_t bit) {
   asm("{\n\t.reg .pred q;\n\t.reg .b32 t;\n\tand.b32 t, %2, %3;\n\tsetp.ne.u32 q, t, 0;\n\t@q sub.f32 %0, %0, %1;\n\t}"
@@ -306,19 +328,28 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
                 for (int j = 0; j < n; ++j) h[j] = at & n ? h[n + j] : h[j];
               if (hit) { tl = h[0]; met = true; }
             }
-            float mx[4] = {f[0], f[1], f[2], f[3]};
+            float mx[4];
 #pragma unroll
-            for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], f[j]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            for (int j = 0; j < 4; ++j) {
+              mx[j] = hd_max3(f[8 * j], f[8 * j + 1], f[8 * j + 2]);
+              mx[j] = hd_max3(mx[j], f[8 * j + 3], f[8 * j + 4]);
+              mx[j] = hd_max3(mx[j], f[8 * j + 5], f[8 * j + 6]);
+              mx[j] = fmaxf(mx[j], f[8 * j + 7]);
+            }
+            const float top = hd_max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
             if (top > m) {
               s *= hd_ex2((m - top) * HD_LOG2E);
               m = top;
             }
-            const float base = -m * HD_LOG2E;
-            float a[4] = {0.f, 0.f, 0.f, 0.f};
+            const float2 scale = make_float2(HD_LOG2E, HD_LOG2E), base = make_float2(-m * HD_LOG2E, -m * HD_LOG2E);
+            float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) a[j & 3] += hd_ex2(fmaf(f[j], HD_LOG2E, base));
-            s += (a[0] + a[1]) + (a[2] + a[3]);
+            for (int j = 0; j < 32; j += 2) {
+              const float2 t = hd_fma2(make_float2(f[j], f[j + 1]), scale, base);
+              a[j / 2 & 1] = hd_add2(a[j / 2 & 1], make_float2(hd_ex2(t.x), hd_ex2(t.y)));
+            }
+            a[0] = hd_add2(a[0], a[1]);
+            s += a[0].x + a[0].y;
           }
         }
       }
@@ -603,17 +634,22 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
             }
             const bool any = __any_sync(0xffffffffu, hits != 0u);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) f[j] = hd_ex2(f[j] * HD_LOG2E);
+              for (int j = 0; j < 32; j += 2) {
+                const float2 t = hd_fma2(make_float2(f[j], f[j + 1]), make_float2(HD_LOG2E, HD_LOG2E), make_float2(0.f, 0.f));
+                f[j] = hd_ex2(t.x);
+                f[j + 1] = hd_ex2(t.y);
+              }
               if (any) {
                 const float one = MODE == HEAD_DW ? g : 1.f;
 #pragma unroll
                 for (int j = 0; j < 32; ++j) hd_sub_if(f[j], one, hits, 1u << j);
               }
               if (MODE == HEAD_DW) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                float2 d[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int j = 0; j < 32; ++j) d[j & 3] += f[j];
-                db += (d[0] + d[1]) + (d[2] + d[3]);
+                for (int j = 0; j < 32; j += 2) d[j / 2 & 1] = hd_add2(d[j / 2 & 1], make_float2(f[j], f[j + 1]));
+                d[0] = hd_add2(d[0], d[1]);
+                db += d[0].x + d[0].y;
               }
               uint32_t o[16];
 #pragma unroll
