@@ -758,17 +758,57 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const void* __restrict__
   }
 }
 
-// the class of a voxel's largest logit, from the splits' in their order
-__global__ void __launch_bounds__(256) head_arg_kernel(const float2* __restrict__ part, int splits, long long V,
+// Shares of a row's statistics, merged. TEAM 1: by one thread, in order; TEAM 32: by a warp, each lane every 32nd one and
+// then in a fixed tree: few voxels have many shares, and a thread would wait an L2 trip for a few of them at a time (512
+// shares of one voxel: 45 us by one thread).
+template <int TEAM>
+__device__ __forceinline__ void hd_merge_best(const float2* part, int shares, long long v_pad, long long i, int lane,
+                                              float& m, int& best) {
+  m = -INFINITY;
+  best = INT_MAX;
+#pragma unroll 4
+  for (int k = lane; k < shares; k += TEAM) {
+    const float2 e = part[(long long)k * v_pad + i];
+    hd_better(m, best, e.x, __float_as_int(e.y));
+  }
+#pragma unroll
+  for (int o = TEAM / 2; o > 0; o >>= 1) {
+    const float v = __shfl_xor_sync(0xffffffffu, m, o);
+    const int j = __shfl_xor_sync(0xffffffffu, best, o);
+    hd_better(m, best, v, j);
+  }
+}
+template <int TEAM>
+__device__ __forceinline__ float2 hd_merge_sums(const float2* part, int shares, long long v_pad, long long i, int lane) {
+  float m = -INFINITY, s = 0.f;
+#pragma unroll 4
+  for (int k = lane; k < shares; k += TEAM) {
+    const float2 e = part[(long long)k * v_pad + i];
+    const float mm = fmaxf(m, e.x), base = mm == -INFINITY ? 0.f : mm;
+    s = s * hd_ex2(m - base) + e.y * hd_ex2(e.x - base);
+    m = mm;
+  }
+#pragma unroll
+  for (int o = TEAM / 2; o > 0; o >>= 1) {
+    const float v = __shfl_xor_sync(0xffffffffu, m, o), t = __shfl_xor_sync(0xffffffffu, s, o);
+    const float mm = fmaxf(m, v), base = mm == -INFINITY ? 0.f : mm;
+    const float x = s * hd_ex2(m - base), y = t * hd_ex2(v - base);
+    s = x + y;  // the same in both lanes
+    m = mm;
+  }
+  return make_float2(m, s);
+}
+
+// the class of a voxel's largest logit
+template <int TEAM>
+__global__ void __launch_bounds__(256) head_arg_kernel(const float2* __restrict__ part, int shares, long long V,
                                                        long long v_pad, long long* __restrict__ out) {
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < V; i += (long long)gridDim.x * 256) {
-    float m = -INFINITY;
-    int best = INT_MAX;
-    for (int k = 0; k < splits; ++k) {
-      const float2 e = part[(long long)k * v_pad + i];
-      hd_better(m, best, e.x, __float_as_int(e.y));
-    }
-    out[i] = best == INT_MAX ? 0 : best;  // nothing above -inf
+  const int lane = threadIdx.x % TEAM;
+  for (long long i = (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM; i < V; i += (long long)gridDim.x * (256 / TEAM)) {
+    float m;
+    int best;
+    hd_merge_best<TEAM>(part, shares, v_pad, i, lane, m, best);
+    if (lane == 0) out[i] = best == INT_MAX ? 0 : best;  // nothing above -inf
   }
 }
 
@@ -799,35 +839,30 @@ __device__ __forceinline__ void hd_loss(const HeadSum& a, double* total, float* 
   den[0] = (float)d;
 }
 
-// lse2[i] from the splits' running maxima and sums, merged in split order; block sums of u nll and u in double (a single
-// block goes on to the loss)
+// lse2[i] from the shares of its statistics; block sums of u nll and u in double (a single block goes on to the loss)
+template <int TEAM>
 __global__ void __launch_bounds__(256) head_merge_kernel(const float2* __restrict__ part, const float* __restrict__ tl,
                                                          const int* __restrict__ y, const float* __restrict__ cw,
-                                                         int splits, long long V, long long v_pad,
+                                                         int shares, long long V, long long v_pad,
                                                          float* __restrict__ lse2, double* __restrict__ sums,
                                                          double* __restrict__ total, float* __restrict__ loss,
                                                          float* __restrict__ den) {
   HeadSum a{0.0, 0.0};
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < v_pad; i += (long long)gridDim.x * 256) {
+  const int lane = threadIdx.x % TEAM;
+  for (long long i = (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM; i < v_pad;
+       i += (long long)gridDim.x * (256 / TEAM)) {
     float l = INFINITY;
-    if (i < V) {
-      float m = -INFINITY, s = 0.f;
-#pragma unroll 4
-      for (int k = 0; k < splits; ++k) {
-        const float2 e = part[(long long)k * v_pad + i];
-        const float mm = fmaxf(m, e.x), base = mm == -INFINITY ? 0.f : mm;
-        s = s * hd_ex2(m - base) + e.y * hd_ex2(e.x - base);
-        m = mm;
-      }
-      l = m < 0.1f * HD_LOWEST ? NAN : m + log2f(s);  // every class is off: 0 / 0
+    if (i < V) {  // (the same in a team's lanes)
+      const float2 e = hd_merge_sums<TEAM>(part, shares, v_pad, i, lane);
+      l = e.x < 0.1f * HD_LOWEST ? NAN : e.x + log2f(e.y);  // every class is off: 0 / 0
       const int c = y[i];
-      if (c >= 0) {
+      if (c >= 0 && lane == 0) {
         const float u = cw == nullptr ? 1.f : cw[c];
         a.num += (double)u * ((double)(l - tl[i]) * (double)HD_LN2);
         a.den += (double)u;
       }
     }
-    lse2[i] = l;
+    if (lane == 0) lse2[i] = l;
   }
   a = hd_block_sum(a);
   if (threadIdx.x == 0) {
@@ -1149,9 +1184,15 @@ extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, i
     rc = head_launch<HEAD_ROWS, false>(a, p, stream);
   }
   if (rc) return rc;
-  const int blocks = v_pad <= 4096 ? 1 : hd_blocks(v_pad, HD_SUM_BLOCKS / 148);  // 16 rounds cost less than a launch
-  head_merge_kernel<<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, f.sums, a.total, loss,
-                                                a.den);
+  const bool team = splits > 4;
+  // one block, which goes on to the loss, where its rounds cost less than another launch
+  const int blocks = v_pad <= (team ? 256 : 4096) ? 1 : hd_blocks(team ? v_pad * 32 : v_pad, HD_SUM_BLOCKS / 148);
+  if (team)
+    head_merge_kernel<32><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, f.sums, a.total,
+                                                      loss, a.den);
+  else
+    head_merge_kernel<1><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, f.sums, a.total,
+                                                     loss, a.den);
   if (blocks > 1) head_total_kernel<<<1, 256, 0, stream>>>(f.sums, blocks, a.total, loss, a.den);
   sb_count_launch(blocks > 1 ? 2 : 1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
@@ -1196,7 +1237,8 @@ extern "C" int sb_head_predict(const void* x, const void* w, const void* bias, i
     rc = head_launch<HEAD_ROWS, true>(a, p, stream);
   }
   if (rc) return rc;
-  head_arg_kernel<<<hd_blocks(V, 8), 256, 0, stream>>>(f.part, splits, V, hd_pad(V), out);
+  if (splits > 4) head_arg_kernel<32><<<hd_blocks(V * 32, 8), 256, 0, stream>>>(f.part, splits, V, hd_pad(V), out);
+  else head_arg_kernel<1><<<hd_blocks(V, 8), 256, 0, stream>>>(f.part, splits, V, hd_pad(V), out);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }

@@ -10,7 +10,7 @@ int make_map_bf16(CUtensorMap* m, const void* base, int rank, const long long* d
 
 constexpr int HD_PAD = 256;         // per-voxel and per-class arrays are padded to a multiple of this
 constexpr int HD_FEW = 128;         // up to this many voxels, D's entries are kept in two bf16 (head_loss.cu)
-constexpr int HD_SUM_BLOCKS = 592;  // blocks of the loss's sums at most
+constexpr int HD_SUM_BLOCKS = 1184;  // blocks of the loss's sums at most
 constexpr float HD_LOG2E = 1.4426950408889634f;
 constexpr float HD_LN2 = 0.6931471805599453f;
 constexpr float HD_LOWEST = -1e30f;

@@ -5,7 +5,7 @@
 //   WIDE_LSE  rows = voxels, columns = classes: running maximum and sum of every row over the class tiles of a job
 //   WIDE_ARG  the same with the largest logit and its class in their place
 //   WIDE_D    rows = classes, columns = voxels: P^T = p - [j = y] in bf16, a piece of the classes by a piece of the
-//             voxels at a time (HW_PIECE elements: 64 MB, which stays in L2 until both products below have read it); db
+//             voxels at a time (HW_PIECE elements); db
 //   WIDE_OUT  dX = g P W and dW = P^T (u X) of the piece (head_loss.cu for g and u). P^T is read K-major for dW and
 //             MN-major for dX, W and X MN-major: nothing is transposed in memory. Long reductions are cut into slices
 //             that are added in order.
@@ -24,7 +24,10 @@ namespace sb {
 constexpr int HW_THREADS = 320;
 constexpr int HW_STAGES = 6;
 constexpr int HW_STAGE = 32768;  // 64 of K for 128 rows of A and 128 columns of B
-constexpr long long HW_PIECE = 32LL << 20;
+// 128 MB of P^T at a time. Larger pieces have fewer tails and fewer sums to carry on, smaller ones stay in L2: the gradients
+// of 40000 voxels x 512 channels x 8000 classes take 2.02 ms with 64 MB, 1.87 with 128, 1.72 with 192; those of 8192 x 1024 x
+// 32771 2.06, 1.96 and 1.89. The memory counts here: half of the last step for two thirds of its size.
+constexpr long long HW_PIECE = 64LL << 20;
 
 enum WideEpi { WIDE_LSE = 0, WIDE_D = 1, WIDE_OUT = 2, WIDE_ARG = 3 };
 
@@ -59,27 +62,26 @@ struct WideParams {
   uint32_t* status;
 };
 
-// rows x C sums: v = (add ? acc : 0) + product, then scaled to an output or back to acc; eight columns
+constexpr int HW_STRIDE = 20;  // floats of a staged row of 16
+
+// rows x C sums: v = (add ? acc : 0) + product, then scaled to an output or back to acc; four columns
 __device__ __forceinline__ void hw_sink(float* acc, int add, __nv_bfloat16* out16, float* out32, float scale, long long at,
-                                        float (&f)[8]) {
+                                        float4 f) {
   if (add) {
-    const float4 a = *reinterpret_cast<const float4*>(acc + at), b = *reinterpret_cast<const float4*>(acc + at + 4);
-    f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
-    f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+    const float4 a = *reinterpret_cast<const float4*>(acc + at);
+    f.x += a.x; f.y += a.y; f.z += a.z; f.w += a.w;
   }
   if (out16 != nullptr || out32 != nullptr) {
     // a voxel that takes no part has no gradient, whatever its features hold
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = scale == 0.f ? 0.f : f[i] * scale;
+    f.x = scale == 0.f ? 0.f : f.x * scale;
+    f.y = scale == 0.f ? 0.f : f.y * scale;
+    f.z = scale == 0.f ? 0.f : f.z * scale;
+    f.w = scale == 0.f ? 0.f : f.w * scale;
   }
-  if (out16 != nullptr) {
-    *reinterpret_cast<uint4*>(out16 + at) =
-        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-    return;
-  }
-  float* dst = out32 != nullptr ? out32 : acc;
-  *reinterpret_cast<float4*>(dst + at) = make_float4(f[0], f[1], f[2], f[3]);
-  *reinterpret_cast<float4*>(dst + at + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  if (out16 != nullptr)
+    *reinterpret_cast<uint2*>(out16 + at) = make_uint2(pack_bf16x2(f.x, f.y), pack_bf16x2(f.z, f.w));
+  else
+    *reinterpret_cast<float4*>((out32 != nullptr ? out32 : acc) + at) = f;
 }
 
 template <int EPI, int A_MN, int B_MN>
@@ -88,7 +90,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[HW_STAGES], empty[HW_STAGES], tfull[2], tempty[2];
-  __shared__ float s_m[128], s_s[128], s_t[128];
+  __shared__ float s_m[EPI == WIDE_OUT ? 1 : 128], s_s[EPI == WIDE_OUT ? 1 : 128], s_t[EPI == WIDE_OUT ? 1 : 128];
+  __shared__ __align__(16) float s_stage[EPI == WIDE_OUT ? 8 : 1][EPI == WIDE_OUT ? 32 * HW_STRIDE : 1];
   __shared__ uint32_t tmem_base_s, abort_s;
   volatile uint32_t* abort_flag = &abort_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -221,7 +224,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;
     const int row = quad * 32 + lane;
-    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16) + half * 128;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t release[2] = {map_to_rank(smem_u32(&tempty[0]), 0), map_to_rank(smem_u32(&tempty[1]), 0)};
     uint32_t b = 0, bph = 0;
     bool ok = true;
@@ -230,13 +233,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
       const long long r = (long long)j.rt * 256 + rank * 128 + row;
       const int y = EPI == WIDE_LSE ? p.y[r] : 0;
       const float rp = EPI == WIDE_D ? p.rowp[r] : 0.f;
+      float scale = 1.f;  // OUT: of the row
+      if (EPI == WIDE_OUT && p.row_scale != nullptr) scale = r < p.rows ? __ldg(p.row_scale + r) : 0.f;
+      else if (EPI == WIDE_OUT && p.scale != nullptr) scale = __ldg(p.scale);
+      // D: rows behind the piece's last class (up to the 64 that the products read) are left as they are
+      const bool live = EPI != WIDE_D || r < p.rows;
       float m = -INFINITY, s = 0.f, tl = 0.f, db = 0.f;
       int best = INT_MAX;
       for (int t = j.t0; t < j.t1; ++t) {
         if (!mbar_wait_cl(&tfull[b], bph, abort_flag, p.status, 105)) { ok = false; break; }
         tc_fence_after();
-        const int nc = cols_of(t) - half * 128, c_abs = t * 256 + half * 128;
-        for (int c0 = 0; c0 < 128 && c0 < nc; c0 += 32) {
+        const int nc = live ? cols_of(t) : 0, c_abs = t * 256;
+        for (int c0 = half * 32; c0 < nc; c0 += 64) {  // every second 32 columns are the other group's
           uint32_t v[32];
           tmem_ld_32x32(lane_base + b * 256 + c0, v);
           tmem_ld_wait();
@@ -313,19 +321,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
                 st_global_v8(dst + 2 * i, make_uint4(o[8 * i], o[8 * i + 1], o[8 * i + 2], o[8 * i + 3]),
                              make_uint4(o[8 * i + 4], o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]));
             }
-          } else if (r < p.rows) {
-            float* acc = p.kslices > 1 ? p.slices + (long long)j.sp * p.rows * p.cols : p.acc;
-            const bool whole = p.kslices == 1;
-            const float scale = p.row_scale != nullptr ? __ldg(p.row_scale + r) : p.scale != nullptr ? __ldg(p.scale) : 1.f;
+          } else {
+            // A lane holds a row, and its stores would each be in another line: the warp's rows go through shared memory,
+            // so that four lanes store 64 bytes of a row (bf16) or of half a row's 32 columns (fp32).
+            float* stage = s_stage[warp - 2];
+            const int rr = lane >> 2, piece = lane & 3;  // row rr + 8 i, quarter of it
+            if (p.kslices == 1 && p.out16 != nullptr && !p.add) {
+              uint32_t o[16];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int col = c_abs + c0 + g * 8;
-              if (col < p.cols) {
-                float e[8];
+              for (int i = 0; i < 16; ++i) {
+                // a voxel that takes no part has no gradient, whatever its features hold
+                const float lo = scale == 0.f ? 0.f : scale * __uint_as_float(v[2 * i]);
+                const float hi = scale == 0.f ? 0.f : scale * __uint_as_float(v[2 * i + 1]);
+                o[i] = pack_bf16x2(lo, hi);
+              }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = __uint_as_float(v[g * 8 + i]);
-                hw_sink(acc, whole ? p.add : 0, whole ? p.out16 : nullptr, whole ? p.out32 : nullptr, scale,
-                        r * p.cols + col, e);
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint4*>(stage + lane * HW_STRIDE + 4 * i) =
+                    make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              __syncwarp();
+              const int col = c_abs + c0 + piece * 8;
+              __nv_bfloat16* dst = p.out16 + (r - lane + rr) * p.cols + col;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (r - lane + rr + 8 * i < p.rows && col < p.cols)
+                  *reinterpret_cast<uint4*>(dst + (long long)(8 * i) * p.cols) =
+                      *reinterpret_cast<const uint4*>(stage + (rr + 8 * i) * HW_STRIDE + piece * 4);
+              __syncwarp();
+            } else {
+              float* acc = p.kslices > 1 ? p.slices + (long long)j.sp * p.rows * p.cols : p.acc;
+              const bool whole = p.kslices == 1;
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  *reinterpret_cast<uint4*>(stage + lane * HW_STRIDE + 4 * i) =
+                      make_uint4(v[16 * h + 4 * i], v[16 * h + 4 * i + 1], v[16 * h + 4 * i + 2], v[16 * h + 4 * i + 3]);
+                const int col = c_abs + c0 + h * 16 + piece * 4;
+                const long long at = (r - lane + rr) * p.cols + col, step = 8LL * p.cols;
+                float4 before[4];  // what is added to, requested ahead of everything
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  before[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                  if (whole && p.add && r - lane + rr + 8 * i < p.rows && col < p.cols)
+                    before[i] = *reinterpret_cast<const float4*>(acc + at + i * step);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float k = __shfl_sync(0xffffffffu, scale, rr + 8 * i);
+                  float4 f = *reinterpret_cast<const float4*>(stage + (rr + 8 * i) * HW_STRIDE + piece * 4);
+                  f.x += before[i].x; f.y += before[i].y; f.z += before[i].z; f.w += before[i].w;
+                  if (r - lane + rr + 8 * i < p.rows && col < p.cols)
+                    hw_sink(acc, 0, whole ? p.out16 : nullptr, whole ? p.out32 : nullptr, k, at + i * step, f);
+                }
+                __syncwarp();
               }
             }
           }
@@ -352,7 +402,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
           const float m1 = s_m[row], mm = fmaxf(m, m1);
           const float base = mm == -INFINITY ? 0.f : mm;
           p.part[(long long)j.sp * p.rows_pad + r] = make_float2(mm, s * hd_ex2(m - base) + s_s[row] * hd_ex2(m1 - base));
-          if (y >= j.t0 * 256 && y < j.t1 * 256) p.tl[r] = (y & 255) < 128 ? tl : s_t[row];
+          if (y >= j.t0 * 256 && y < j.t1 * 256) p.tl[r] = (y & 32) == 0 ? tl : s_t[row];
         }
         hd_vote(1, 256, true);  // the merge has read what the next job's will overwrite
       }
@@ -375,32 +425,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
   }
 }
 
-// [rows][C] = (add ? acc : 0) + the slices in order, scaled to an output or back to acc (C a multiple of 8)
+// [rows][C] = (add ? acc : 0) + the slices, scaled to an output or back to acc; four columns a thread. TEAM threads share
+// an output, each adds every TEAM-th slice and the first one their sums in order: few outputs have many slices, and one
+// thread would wait an L2 trip for a few of them at a time.
+template <int TEAM>
 __global__ void __launch_bounds__(256) head_slices_kernel(const float* __restrict__ slices, int n, long long elems, int C,
                                                           float* acc, int add, __nv_bfloat16* out16, float* out32,
                                                           const float* __restrict__ row_scale,
                                                           const float* __restrict__ scale) {
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < elems / 8; i += (long long)gridDim.x * 256) {
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  constexpr int OUT = 256 / TEAM;
+  __shared__ float4 s_part[TEAM > 1 ? TEAM : 1][OUT];
+  const int me = threadIdx.x / OUT, o = threadIdx.x % OUT;
+  for (long long i0 = (long long)blockIdx.x * OUT; i0 < elems / 4; i0 += (long long)gridDim.x * OUT) {
+    const long long i = i0 + o;
+    const bool in = i < elems / 4;
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (in) {
 #pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      const float* src = slices + (long long)k * elems + i * 8;
-      const float4 a = __ldcs(reinterpret_cast<const float4*>(src)), b = __ldcs(reinterpret_cast<const float4*>(src + 4));
-      f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
-      f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+      for (int k = me; k < n; k += TEAM) {
+        const float4 a = __ldcs(reinterpret_cast<const float4*>(slices + (long long)k * elems) + i);
+        f.x += a.x; f.y += a.y; f.z += a.z; f.w += a.w;
+      }
     }
-    hw_sink(acc, add, out16, out32, row_scale != nullptr ? row_scale[i * 8 / C] : scale != nullptr ? scale[0] : 1.f, i * 8, f);
+    if (TEAM > 1) {
+      s_part[me][o] = f;
+      __syncthreads();
+      if (me == 0)
+        for (int k = 1; k < TEAM; ++k) {
+          const float4 a = s_part[k][o];
+          f.x += a.x; f.y += a.y; f.z += a.z; f.w += a.w;
+        }
+    }
+    if (in && me == 0)
+      hw_sink(acc, add, out16, out32, row_scale != nullptr ? row_scale[i * 4 / C] : scale != nullptr ? scale[0] : 1.f, i * 4, f);
+    if (TEAM > 1) __syncthreads();
   }
 }
-// the same for the bias's sums: slices [n][ld], rows of them
+// the same for the bias's sums: slices [n][ld], rows of them; a warp has 32 rows and every eighth slice
 __global__ void __launch_bounds__(256) head_slices_b_kernel(const float* __restrict__ slices, int n, long long ld,
                                                             int rows, float* acc, int add, __nv_bfloat16* out16,
                                                             float* out32, const float* __restrict__ scale) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows) return;
+  __shared__ float s_part[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = blockIdx.x * 32 + lane;
   float f = 0.f;
+  if (i < rows) {
 #pragma unroll 8
-  for (int k = 0; k < n; ++k) f += slices[(long long)k * ld + i];
+    for (int k = warp; k < n; k += 8) f += slices[(long long)k * ld + i];
+  }
+  s_part[warp][lane] = f;
+  __syncthreads();
+  if (warp != 0 || i >= rows) return;
+  for (int k = 1; k < 8; ++k) f += s_part[k][lane];
   if (add) f += acc[i];
   if (out16 != nullptr) out16[i] = __float2bfloat16(f * scale[0]);
   else if (out32 != nullptr) out32[i] = f * scale[0];
@@ -581,7 +656,7 @@ static int wide_product(const HeadCall& a, const void* dl, long long ldd, long l
                         const float* row_scale, const float* scale, void* out16, void* out32, cudaStream_t stream) {
   WideParams p;
   memset(&p, 0, sizeof(p));
-  const long long ext = A_MN ? kext : vext;  // of the reduction
+  const long long ext = A_MN ? up(b_rows, 64) : vext;  // of the reduction: the piece's classes, or its voxels
   p.kc0 = (int)(ext / 64);
   p.kc = lo_rows ? 2 * p.kc0 : p.kc0;
   p.lo_rows = lo_rows;
@@ -606,9 +681,14 @@ static int wide_product(const HeadCall& a, const void* dl, long long ldd, long l
   if (rc) return rc;
   rc = wide_launch<WIDE_OUT, A_MN, 1>(p, stream);
   if (rc || p.kslices == 1) return rc;
-  const long long elems = rows * a.C, blocks = (elems / 8 + 255) / 256;
-  head_slices_kernel<<<(int)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(
-      ws, p.kslices, elems, a.C, acc, add, p.out16, p.out32, row_scale, scale);
+  const long long elems = rows * a.C;
+  const bool team = p.kslices >= 8 && elems < 148LL * 8 * 256 * 4;
+  const long long blocks = (elems / 4 + (team ? 31 : 255)) / (team ? 32 : 256);
+  const int grid = (int)(blocks < 148 * 8 ? blocks : 148 * 8);
+  if (team)
+    head_slices_kernel<8><<<grid, 256, 0, stream>>>(ws, p.kslices, elems, a.C, acc, add, p.out16, p.out32, row_scale, scale);
+  else
+    head_slices_kernel<1><<<grid, 256, 0, stream>>>(ws, p.kslices, elems, a.C, acc, add, p.out16, p.out32, row_scale, scale);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
@@ -643,6 +723,7 @@ int head_wide_backward(const HeadCall& a, cudaStream_t stream) {
       p.splits = (p.col_tiles + q.d_per - 1) / q.d_per;
       p.kc = (a.C + 63) / 64;
       p.cols = (int)vext;
+      p.rows = up(krows, 64);
       p.rows_pad = q.kp;
       p.y = a.y + v0;
       p.colp = a.lse2p + v0;
@@ -661,7 +742,7 @@ int head_wide_backward(const HeadCall& a, cudaStream_t stream) {
       rc = wide_launch<WIDE_D, 0, 0>(p, stream);
       if (rc) return rc;
       if (a.db != nullptr) {
-        head_slices_b_kernel<<<(int)((krows + 255) / 256), 256, 0, stream>>>(
+        head_slices_b_kernel<<<(int)((krows + 31) / 32), 256, 0, stream>>>(
             ws_b, 2 * p.splits, q.kp, (int)krows, a.scratch + q.acc_b + k0, iv > 0,
             v_last && a.db_kind == 0 ? (__nv_bfloat16*)a.db + k0 : nullptr,
             v_last && a.db_kind == 2 ? (float*)a.db + k0 : nullptr, a.scale);

@@ -102,9 +102,11 @@ def test_without_a_bias_and_with_an_fp32_weight(c):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("v,c,k", [(20000, 264, 3000), (40000, 512, 700), (300, 320, 120000)])
+@pytest.mark.parametrize("v,c,k", [(20000, 264, 3000), (40000, 512, 700), (300, 320, 120000),
+                                   (24000, 264, 3500), (600, 320, 120000), (20000, 264, 5000)])
 def test_the_wide_gradient_in_several_pieces(v, c, k):
-    """More classes and voxels than one piece of the gradient's matrix holds: against fp32 products of the formula."""
+    """More classes, more voxels, more of both than one piece of the gradient's matrix holds: against fp32 products of
+    the formula."""
     x, w, b, y, cw = _inputs(v, c, k, weighted=True)
     x, w, b = (t.requires_grad_() for t in (x, w, b))
     loss = head_cross_entropy(x, w, b, y.int(), cw)
