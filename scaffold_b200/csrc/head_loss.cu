@@ -2,15 +2,15 @@
 //   s_ij = x_i . w_j + b_j,  lse_i = log sum_j exp s_ij,  L = sum_i u_i (lse_i - s_i,y(i)) / sum_i u_i,  u_i = class weight
 //   p_ij = exp(s_ij - lse_i),  D_ij = g_i (p_ij - [j = y_i]),  g_i = dL u_i / sum u
 //   dX = D W,  dW = D^T X,  db_j = sum_i D_ij
-// The logits (voxels x classes) are never written: each of the three kernels multiplies the tiles of X and W again, keeps
-// a 128 x 128 tile of s in tensor memory and uses it up there.
+// The logits (voxels x classes) are never written: every kernel multiplies the tiles of X and W again, keeps a 128 x 128
+// tile of s in tensor memory and uses it up on the chip.
 //
 // Bias and log-sum-exp ride along the reduction: X and W have sixteen columns more (x16, w16), in which b_j, -lse_i and
 // log u_i stand as three bf16 each (24 bits) against ones of the other side, so the tensor cores hand over
 // s_ij + b_j - lse_i and an entry costs the epilogue a multiplication by log2(e) and an exponential. Column parameters
 // out of shared memory cost it a data-pipe cycle per warp and column each, more than the exponential unit's share.
 //
-// A CTA keeps tiles of 128 ROWS resident and walks 128-wide tiles of COLUMNS, two kernels:
+// A CTA keeps tiles of 128 ROWS resident and walks 128-wide tiles of COLUMNS, three kernels:
 //   head_rows_kernel  rows = voxels, columns = classes: running maximum and sum of every row (one row per thread, no
 //                     exchange between threads), or (ARG) the largest logit and its class
 //   head_grad_kernel  HEAD_DX  rows = voxels, columns = classes: P = p - [j = y] in bf16 goes back to tensor memory over
@@ -18,6 +18,7 @@
 //                     tile is the same shared memory, read MN-major); the row's g multiplies the finished sum
 //                     HEAD_DW  rows = classes, columns = voxels: the same with X and W exchanged, P = u (p - [j = y]); a
 //                     row of P^T is a class, so db is a sum inside a thread; dL / sum u multiplies the finished sums
+//   head_both_kernel  both gradients from one P, where the weight and its gradient fit into a CTA
 //
 // Roundings. P has 8 significant bits, all sums are fp32. The target's one is taken off in fp32, before the rounding:
 // behind it a confident voxel (p near 1) would keep nothing but the rounding of p. Common factors stay out of P, so that
@@ -48,13 +49,15 @@ constexpr int HD_BOX16 = HD_TILE * 32; // and of the sixteen columns more
 constexpr int HD_MAX_STAGES = 8;
 constexpr int HD_MAX_C = 256;          // TMEM: two or three tiles of s and the accumulator in 512 columns
 
-enum HeadMode { HEAD_ROWS = 0, HEAD_DX = 1, HEAD_DW = 2 };
+enum HeadMode { HEAD_ROWS = 0, HEAD_DX = 1, HEAD_DW = 2, HEAD_BOTH = 3 };
 
 struct HeadParams {
   CUtensorMap mapR, mapQ, mapR16, mapQ16;  // rows and columns, and their sixteen columns more
+  CUtensorMap mapO;                        // both: dX
   const int* coly;      // DW: label (-1: none)
   const float* roww;    // DW: class weight of a row, or null
-  const float* rowg;    // DX: g
+  const float* rowg;    // DX, both: g of a voxel
+  const uint32_t* colhit;  // both: label of a column (16 bits), p - 1 of it (bf16)
   const int* rowy;      // ROWS / DX: label
   float2* part;         // ROWS: [splits, times four with `together` 1][rows padded] running maximum and sum
   float* tl;            // ROWS: [rows padded] s log2(e) at the label
@@ -89,6 +92,19 @@ __device__ __forceinline__ void hd_tmem_st_x16(uint32_t taddr, const uint32_t* v
       : "memory");
 }
 __device__ __forceinline__ void hd_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void hd_tma_store_2d(const CUtensorMap* m, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void hd_sts4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void hd_sts16(uint32_t at, uint32_t v) {
+  asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"((uint16_t)v) : "memory");
+}
 // two fp32 in one instruction
 __device__ __forceinline__ float2 hd_fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -224,7 +240,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
     // one tile into buffer g: rows out of r_slot, columns out of the current stage
     auto tile = [&](uint32_t g, uint32_t r_slot, int t) -> bool {
       const uint32_t u = uses[g >> 1]++;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_done[g], (u & 1u) ^ 1u, abort_flag, p.status, 96))) return false;
+      if (!hd_wait(&s_done[g], (u & 1u) ^ 1u, abort_flag, p.status, 96)) return false;
       tc_fence_after();
       if (leader) {
         hd_first_mma(tmem + g * HD_TILE, r0 + r_slot * tile_bytes, q0 + st * tile_bytes, box16, cols_of(t), p.ksteps);
@@ -238,13 +254,13 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
       const int t0 = sp * p.tiles_per_split;
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
       bool used = false;
-      if (!four && !__all_sync(0xffffffffu, mbar_wait(&r_full[rb], rph, abort_flag, p.status, 94))) break;
+      if (!four && !hd_wait(&r_full[rb], rph, abort_flag, p.status, 94)) break;
       for (int t = t0; t < t1 && ok; ++t, ++fi) {
         if (four || (fi & 1u) == mine) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95))) { ok = false; break; }
+          if (!hd_wait(&q_full[st], ph, abort_flag, p.status, 95)) { ok = false; break; }
           if (four) {
             for (uint32_t g = mine; g < 4u && ok; g += 2u) {
-              if (t == t0) ok = __all_sync(0xffffffffu, mbar_wait(&r_full[g], rph, abort_flag, p.status, 94));
+              if (t == t0) ok = hd_wait(&r_full[g], rph, abort_flag, p.status, 94);
               ok = ok && tile(g, g, t);
               if (ok && leader && t == t1 - 1) tc_commit(&r_empty[g]);
               __syncwarp();
@@ -295,7 +311,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
       int t = four ? t0 : t0 + (int)((group - fi) & 3u);
       fi += t1 - t0;
       for (; t < t1; t += four ? 1 : 4, ++uses) {
-        if (!mbar_wait(&s_full[group], uses & 1u, abort_flag, p.status, 98)) { ok = false; break; }
+        if (!hd_wait(&s_full[group], uses & 1u, abort_flag, p.status, 98)) { ok = false; break; }
         tc_fence_after();
         const int nc = cols_of(t), c_abs = t * HD_TILE;
 #pragma unroll 1
@@ -454,14 +470,14 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
       const int sp = job / p.row_tiles;
       const int t0 = sp * p.tiles_per_split;
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
-      if (!__all_sync(0xffffffffu, mbar_wait(&r_full[rb], rph, abort_flag, p.status, 94))) { ok = false; break; }
+      if (!hd_wait(&r_full[rb], rph, abort_flag, p.status, 94)) { ok = false; break; }
       for (int t = t0; t < t1; ++t, ++tc) {
         // the buffer is free: its P was read by the second MMA that used it
         if (tc >= NB) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[old_st], old_ph, abort_flag, p.status, 96))) { ok = false; break; }
+          if (!hd_wait(&q_empty[old_st], old_ph, abort_flag, p.status, 96)) { ok = false; break; }
           if (++old_st == (uint32_t)p.stages) { old_st = 0; old_ph ^= 1u; }
         }
-        if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95))) { ok = false; break; }
+        if (!hd_wait(&q_full[st], ph, abort_flag, p.status, 95)) { ok = false; break; }
         tc_fence_after();
         if (leader) {
           hd_first_mma(tmem + b * HD_TILE, r0 + rb * tile_bytes, q0 + st * tile_bytes, box16, cols_of(t), p.ksteps);
@@ -487,15 +503,15 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
       const int sp = job / p.row_tiles;
       const int t0 = sp * p.tiles_per_split;
       const int t1 = t0 + p.tiles_per_split < p.col_tiles ? t0 + p.tiles_per_split : p.col_tiles;
-      if (!__all_sync(0xffffffffu, mbar_wait(&acc_empty[ab], aph ^ 1u, abort_flag, p.status, 92))) { ok = false; break; }
+      if (!hd_wait(&acc_empty[ab], aph ^ 1u, abort_flag, p.status, 92)) { ok = false; break; }
       const uint32_t acc = tmem + ACC + ab * 64u;
       for (int t = t0; t < t1; ++t) {
         const int ksteps = cols_of(t) / 16;
         const uint32_t lo = desc_lo(q0 + st * tile_bytes, lbo);
         const uint32_t a = tmem + b * HD_TILE;
         // (the other issuing warp has waited for the tile's loads; this one has to see them too)
-        if (!__all_sync(0xffffffffu, mbar_wait(&q_full[st], ph, abort_flag, p.status, 95) &&
-                                         mbar_wait(&s_done[b], bph, abort_flag, p.status, 93))) { ok = false; break; }
+        if (!(hd_wait(&q_full[st], ph, abort_flag, p.status, 95) &&
+              hd_wait(&s_done[b], bph, abort_flag, p.status, 93))) { ok = false; break; }
         tc_fence_after();
         if (leader) {
 #pragma unroll
@@ -528,7 +544,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
     }
     // the accumulator of a finished job
     auto drain = [&]() -> bool {
-      if (!mbar_wait(&acc_full[ab], aph, abort_flag, p.status, 97)) return false;
+      if (!hd_wait(&acc_full[ab], aph, abort_flag, p.status, 97)) return false;
       tc_fence_after();
       const long long r = (long long)pend_rt * HD_TILE + row;
       for (int c0 = group * 16; c0 < p.cpad; c0 += 64) {
@@ -601,7 +617,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
         label[1] = __ldg(labels + (long long)t * HD_TILE + 32);
       }
       for (; t < t1; t += 2) {
-          if (!mbar_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
+          if (!hd_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
           int rel[2] = {label[0] - (int)(r - lane), label[1] - (int)(r - lane)};
           if (MODE == HEAD_DW && t + 2 < t1) {
             label[0] = __ldg(labels + (long long)(t + 2) * HD_TILE);
@@ -682,6 +698,323 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
       sp = next_sp;
     }
     if (ok && pending) drain();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 0) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Both gradients from one matrix P^T = p - [j = y], rows = classes, columns = voxels (unweighted calls whose weight and
+// whose dW fit into a CTA). A CTA keeps all tiles of W in shared memory and dW's sums in tensor memory and walks tiles of
+// 128 voxels; of each 128 x 128 tile of s^T the epilogue makes a tile of P^T in shared memory, [class][voxel], and two
+// MMAs read it from there: dW += P^T X with the voxels along the reduction (K-major A), dX += P W with the classes along
+// it (the same bytes as an MN-major A). An exponential serves both gradients, X is read once, and in shared memory the
+// target's entry can be put right alone: every thread stores its row of p, then the lanes that hold the columns' labels
+// store p - 1 of the target there (expm1 of the voxel's loss term, which keeps its relative precision). In tensor memory
+// each of a row's entries has to be looked at for it, three instructions more than the three or so of the rest.
+// Roles: warp 0 loads, warps 1 to 3 issue the MMAs of s, dW and dX (a warp loses some 300 clocks at each commit: dW and dX
+// out of one warp 492 instead of 424 us at 128 classes, below), four groups of the epilogue (two take a tile's halves, by
+// tile parity), and the last four warps take dX out of tensor memory, scale it and store it by TMA: row pieces stored by
+// the epilogue itself, 16 bytes a row and instruction, kept the shared memory pipe from P's stores (860 us).
+// Bound: neither the exponential unit (1024 clocks a tile of 128 x 128, some 2100 are taken) nor the MMAs or the stores,
+// but a tile's way through them, two tiles at a time: tensor memory holds no third one of s.
+// 2 x 128^3 voxels, 64 channels, 257 classes: 742 us with all that stands around it, the two kernels above 1160; 128
+// classes 368 / 722; 16 channels and 34 classes 302 / 633; 32 channels and 500 classes 982 / 1456.
+constexpr int HB_FIRST_EPI = 4;
+constexpr int HB_DX_WARPS = 4;  // behind the epilogue's
+constexpr int HB_THREADS = 32 * (HB_FIRST_EPI + HD_EPI_WARPS + HB_DX_WARPS);
+__global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_constant__ HeadParams p) {
+  constexpr uint32_t SB = 2, PB = 2;  // tiles of s in tensor memory and of P in shared memory: one for each pair of groups
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t w_full, x_full[HD_MAX_STAGES], x_empty[HD_MAX_STAGES], s_full[SB], s_empty[SB], p_full[PB],
+      p_empty[PB], acc_full[2], acc_empty[2], dw_full;
+  __shared__ uint32_t tmem_base_s, abort_s;
+  volatile uint32_t* abort_flag = &abort_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kt = p.row_tiles;
+  const uint32_t box16 = (uint32_t)p.kboxes * HD_BOX, tile_bytes = box16 + HD_BOX16;
+  const uint32_t naccs = (uint32_t)p.accs;
+  const uint32_t ACC_X = SB * HD_TILE, ACC_W = ACC_X + naccs * p.cpad;  // columns of the sums
+  uint8_t* smem_p = smem;
+  uint8_t* smem_w = smem_p + PB * 2 * HD_BOX;
+  uint8_t* smem_x = smem_w + kt * tile_bytes;
+  uint8_t* smem_o = smem_x + p.stages * tile_bytes;                     // [dX warps][kboxes][32 rows of 128 bytes]
+  float* smem_db = reinterpret_cast<float*>(smem_o + p.kboxes * HD_BOX);  // [kt][groups][128]
+
+  if (threadIdx.x == 0) {
+    abort_s = 0;
+    mbar_init(&w_full, 1);
+    mbar_init(&dw_full, 1);
+    for (int i = 0; i < p.stages; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1); }
+    for (uint32_t i = 0; i < SB; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], HD_EPI_WARPS / 2); }
+    for (uint32_t i = 0; i < PB; ++i) { mbar_init(&p_full[i], HD_EPI_WARPS / 2); mbar_init(&p_empty[i], 2); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], HB_DX_WARPS); }
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&tmem_base_s, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+  // classes of a tile, up to a multiple of 32
+  const int last_rows = ((int)(p.rows - (long long)(kt - 1) * HD_TILE) + 31) & ~31;
+  auto rows_of = [&](int i) -> int { return i + 1 < kt ? HD_TILE : last_rows; };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&p.mapR);
+      tma_prefetch_desc(&p.mapQ);
+      mbar_expect_tx(&w_full, kt * tile_bytes);
+      for (int i = 0; i < kt; ++i) {
+        for (int k = 0; k < p.kboxes; ++k)
+          hd_tma_2d(smem_w + i * tile_bytes + k * HD_BOX, &p.mapR, &w_full, k * 64, i * HD_TILE);
+        hd_tma_2d(smem_w + i * tile_bytes + box16, &p.mapR16, &w_full, 0, i * HD_TILE);
+      }
+      uint32_t st = 0, ph = 0;
+      for (int v = blockIdx.x; v < p.col_tiles; v += gridDim.x) {
+        if (!mbar_wait(&x_empty[st], ph ^ 1u, abort_flag, p.status, 91)) break;
+        mbar_expect_tx(&x_full[st], tile_bytes);
+        for (int k = 0; k < p.kboxes; ++k)
+          hd_tma_2d(smem_x + st * tile_bytes + k * HD_BOX, &p.mapQ, &x_full[st], k * 64, v * HD_TILE);
+        hd_tma_2d(smem_x + st * tile_bytes + box16, &p.mapQ16, &x_full[st], 0, v * HD_TILE);
+        if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t w0 = smem_u32(smem_w), x0 = smem_u32(smem_x);
+    uint32_t st = 0, ph = 0, b = 0, bph = 0;
+    bool ok = hd_wait(&w_full, 0, abort_flag, p.status, 94);
+    for (int v = blockIdx.x; v < p.col_tiles && ok; v += gridDim.x) {
+      if (!hd_wait(&x_full[st], ph, abort_flag, p.status, 95)) break;
+      for (int i = 0; i < kt; ++i) {
+        if (!hd_wait(&s_empty[b], bph ^ 1u, abort_flag, p.status, 96)) { ok = false; break; }
+        tc_fence_after();
+        if (leader) {
+          hd_first_mma(tmem + b * HD_TILE, w0 + i * tile_bytes, x0 + st * tile_bytes, box16, HD_TILE, p.ksteps);
+          tc_commit(&s_full[b]);
+        }
+        __syncwarp();
+        if (++b == SB) { b = 0; bph ^= 1u; }
+      }
+      if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
+    }
+  } else if (warp == 2) {
+    // dW += P^T X
+    const bool leader = elect_one();
+    const uint32_t hi = desc_hi(8u * 128u, 2u), idesc = make_idesc_bf16(128, p.cpad, 0, 1);
+    const uint32_t p0 = smem_u32(smem_p), x0 = smem_u32(smem_x), lbo = p.kboxes > 1 ? (uint32_t)HD_BOX : 0u;
+    uint32_t st = 0, ph = 0, pb = 0, pph = 0;
+    bool ok = true;
+    for (int v = blockIdx.x; v < p.col_tiles && ok; v += gridDim.x) {
+      // (the first issuing warp has waited for the loads; this one has to see them too)
+      if (!hd_wait(&x_full[st], ph, abort_flag, p.status, 95)) { ok = false; break; }
+      const uint32_t x_lo = desc_lo(x0 + st * tile_bytes, lbo);
+      for (int i = 0; i < kt; ++i) {
+        if (!hd_wait(&p_full[pb], pph, abort_flag, p.status, 93)) { ok = false; break; }
+        tc_fence_after();
+        if (leader) {
+          const uint32_t a_lo = desc_lo(p0 + pb * 2 * HD_BOX, 16u), d = tmem + ACC_W + i * p.cpad;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            tc_mma_bf16_pred(d, a_lo + (uint32_t)(k >> 2) * (HD_BOX >> 4) + (uint32_t)(k & 3) * 2u, hi, x_lo + k * 128u, hi,
+                             idesc, v == (int)blockIdx.x && k == 0 ? 0u : 1u);
+          tc_commit(&p_empty[pb]);
+          if (i + 1 == kt) tc_commit(&x_empty[st]);
+        }
+        __syncwarp();
+        if (++pb == PB) { pb = 0; pph ^= 1u; }
+      }
+      if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
+    }
+    if (ok && leader) tc_commit(&dw_full);
+    __syncwarp();
+  } else if (warp == 3) {
+    // dX = P W
+    const bool leader = elect_one();
+    const uint32_t hi = desc_hi(8u * 128u, 2u), idesc = make_idesc_bf16(128, p.cpad, 1, 1);
+    const uint32_t p0 = smem_u32(smem_p), w0 = smem_u32(smem_w), lbo = p.kboxes > 1 ? (uint32_t)HD_BOX : 0u;
+    uint32_t pb = 0, pph = 0, ab = 0, aph = 0;
+    bool ok = hd_wait(&w_full, 0, abort_flag, p.status, 94);
+    for (int v = blockIdx.x; v < p.col_tiles && ok; v += gridDim.x) {
+      if (!hd_wait(&acc_empty[ab], aph ^ 1u, abort_flag, p.status, 92)) break;
+      for (int i = 0; i < kt; ++i) {
+        if (!hd_wait(&p_full[pb], pph, abort_flag, p.status, 93)) { ok = false; break; }
+        tc_fence_after();
+        if (leader) {
+          const uint32_t a_lo = desc_lo(p0 + pb * 2 * HD_BOX, HD_BOX), w_lo = desc_lo(w0 + i * tile_bytes, lbo);
+          const int ksteps = rows_of(i) / 16;
+          for (int k = 0; k < ksteps; ++k)
+            tc_mma_bf16_pred(tmem + ACC_X + ab * p.cpad, a_lo + k * 128u, hi, w_lo + k * 128u, hi, idesc,
+                             i == 0 && k == 0 ? 0u : 1u);
+          tc_commit(&p_empty[pb]);
+          if (i + 1 == kt) tc_commit(&acc_full[ab]);
+        }
+        __syncwarp();
+        if (++pb == PB) { pb = 0; pph ^= 1u; }
+      }
+      if (++ab == naccs) { ab = 0; aph ^= 1u; }
+    }
+  } else if (warp >= HB_FIRST_EPI + HD_EPI_WARPS) {
+    // dX of a finished voxel tile, a row per thread; each warp stores its 32 rows
+    const int quad = warp & 3;
+    const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + ACC_X;
+    uint8_t* stage = smem_o + quad * p.kboxes * 4096;
+    uint32_t ab = 0, aph = 0;
+    const float* gp = p.rowg + quad * 32 + lane;
+    float g_next = __ldg(gp + (long long)blockIdx.x * HD_TILE);
+    for (int v = blockIdx.x; v < p.col_tiles; v += gridDim.x) {
+      const float g = g_next;
+      if (v + (int)gridDim.x < p.col_tiles) g_next = __ldg(gp + ((long long)v + gridDim.x) * HD_TILE);
+      if (!hd_wait(&acc_full[ab], aph, abort_flag, p.status, 97)) break;
+      tc_fence_after();
+      if (lane == 0) bulk_wait_read_all();  // the last rows have left
+      __syncwarp();
+      for (int c0 = 0; c0 < p.cpad; c0 += 32) {
+        uint32_t u[32];
+        tmem_ld_32x32(acc + ab * p.cpad + c0, u);  // (past cpad: columns of the next sums, which nothing looks at)
+        tmem_ld_wait();
+        if (c0 + 32 >= p.cpad) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[ab]);
+        }
+        // a voxel that takes no part has no gradient, whatever its features hold
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          u[j] = g == 0.f ? 0u : pack_bf16x2(__uint_as_float(u[2 * j]) * g, __uint_as_float(u[2 * j + 1]) * g);
+        uint8_t* dst = stage + (c0 >> 6) * 4096 + lane * 128;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint4*>(dst + (((((c0 & 32) >> 3) + j) ^ (lane & 7)) << 4)) =
+              make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      const long long r = (long long)v * HD_TILE + quad * 32;
+      if (lane == 0 && r < p.cols) {
+        for (int k = 0; k < p.kboxes; ++k) hd_tma_store_2d(&p.mapO, stage + k * 4096, k * 64, (int)r);
+        bulk_commit();
+      }
+      if (++ab == naccs) { ab = 0; aph ^= 1u; }
+    }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
+  } else {
+    const int quad = warp & 3, group = (warp - HB_FIRST_EPI) >> 2, half = group & 1;
+    const uint32_t par = group >> 1;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t swz = row * 128 + ((row & 7) << 4);  // the row's first 16 bytes of voxels in a 128-byte swizzled box
+    const uint32_t s_tile = lane_base + par * HD_TILE + half * 64;
+    uint32_t ph = 0, tc = 0;
+    bool ok = true;
+    float* const db = smem_db + group * HD_TILE + row;  // this thread's alone
+    for (int i = 0; i < kt; ++i) db[i * 4 * HD_TILE] = 0.f;
+    // every second tile over all voxel tiles is this pair of groups'
+    const int step = kt == 1 ? 2 * gridDim.x : gridDim.x;
+    const int v0 = kt == 1 ? blockIdx.x + par * gridDim.x : blockIdx.x;
+    for (int v = v0; v < p.col_tiles && ok; v += step) {
+      // label and p - 1 of the columns `lane` and 32 further of its half; needed behind the first exponentials
+      const uint32_t* at = p.colhit + (long long)v * HD_TILE + half * 64 + lane;
+      const uint32_t hit[2] = {__ldg(at), __ldg(at + 32)};
+      if (v + step < p.col_tiles) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + (long long)step * HD_TILE));
+      int i = kt == 1 ? 0 : (int)((tc ^ par) & 1u);
+      tc += kt;
+      for (; i < kt && ok; i += 2) {
+        if (!hd_wait(&s_full[par], ph, abort_flag, p.status, 98)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t out = smem_u32(smem_p) + par * 2 * HD_BOX + half * HD_BOX;
+        float sum = 0.f;
+        const bool live = quad * 32 < rows_of(i);
+#pragma unroll
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          uint32_t u[32];
+          if (live) {
+            tmem_ld_32x32(s_tile + c0, u);
+            tmem_ld_wait();
+          }
+          if (c0 == 32) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[par]);
+          }
+          if (live) {
+            float2 d[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float2 f = hd_fma2(make_float2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])),
+                                 make_float2(HD_LOG2E, HD_LOG2E), make_float2(0.f, 0.f));
+              f.x = hd_ex2(f.x);
+              f.y = hd_ex2(f.y);
+              d[j & 1] = hd_add2(d[j & 1], f);
+              u[j] = pack_bf16x2(f.x, f.y);
+            }
+            d[0] = hd_add2(d[0], d[1]);
+            sum += d[0].x + d[0].y;
+          }
+          // the buffer is free: both products of its last tile are done
+          if (c0 == 0) ok = hd_wait(&p_empty[par], ph ^ 1u, abort_flag, p.status, 96);
+          if (live) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              hd_sts4((out + swz) ^ (c0 / 8 + j) << 4, u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+            __syncwarp();  // rows before single entries
+            // lane c has the label of column c: a row's targets are the columns whose label has the row's five bits
+            const int rel = (int)(hit[c0 / 32] & 0xFFFFu) - (i * HD_TILE + quad * 32);
+            uint32_t hits = __ballot_sync(0xffffffffu, (unsigned)rel < 32u);
+            if (hits != 0u) {
+#pragma unroll
+              for (int k = 0; k < 5; ++k) hits &= __ballot_sync(0xffffffffu, rel >> k & 1) ^ (lane >> k & 1 ? 0u : ~0u);
+              sum -= (float)__popc(hits);
+              if ((unsigned)rel < 32u) {
+                const int c = c0 + lane, r = quad * 32 + rel;
+                hd_sts16(out + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2, hit[c0 / 32] >> 16);
+              }
+            }
+          }
+        }
+        if (!ok) break;
+        if (live) db[i * 4 * HD_TILE] += sum;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[par]);
+        ph ^= 1u;
+      }
+    }
+    // dW and db of this CTA's voxels
+    if (ok && hd_wait(&dw_full, 0, abort_flag, p.status, 97)) {
+      tc_fence_after();
+      for (int i = 0; i < kt; ++i) {
+        const long long r = (long long)i * HD_TILE + row;
+        p.ws_b[((long long)blockIdx.x * 4 + group) * p.rows_pad + r] = db[i * 4 * HD_TILE];
+        for (int c0 = group * 16; c0 < p.cpad; c0 += 64) {
+          uint32_t v[16];
+          tmem_ld_32x16(lane_base + ACC_W + i * p.cpad + c0, v);
+          tmem_ld_wait();
+          float4* dst = reinterpret_cast<float4*>(p.ws + ((long long)blockIdx.x * p.rows_pad + r) * p.cpad + c0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            dst[j] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
+                                 __uint_as_float(v[4 * j + 3]));
+        }
+      }
+      tc_fence_before();
+    }
   }
 
   tc_fence_before();
@@ -844,25 +1177,31 @@ template <int TEAM>
 __global__ void __launch_bounds__(256) head_merge_kernel(const float2* __restrict__ part, const float* __restrict__ tl,
                                                          const int* __restrict__ y, const float* __restrict__ cw,
                                                          int shares, long long V, long long v_pad,
-                                                         float* __restrict__ lse2, double* __restrict__ sums,
-                                                         double* __restrict__ total, float* __restrict__ loss,
+                                                         float* __restrict__ lse2, uint32_t* __restrict__ hit,
+                                                         double* __restrict__ sums, double* __restrict__ total, float* __restrict__ loss,
                                                          float* __restrict__ den) {
   HeadSum a{0.0, 0.0};
   const int lane = threadIdx.x % TEAM;
   for (long long i = (long long)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM; i < v_pad;
        i += (long long)gridDim.x * (256 / TEAM)) {
     float l = INFINITY;
+    uint32_t h = 0xFFFFu;
     if (i < V) {  // (the same in a team's lanes)
       const float2 e = hd_merge_sums<TEAM>(part, shares, v_pad, i, lane);
       l = e.x < 0.1f * HD_LOWEST ? NAN : e.x + log2f(e.y);  // every class is off: 0 / 0
       const int c = y[i];
       if (c >= 0 && lane == 0) {
         const float u = cw == nullptr ? 1.f : cw[c];
-        a.num += (double)u * ((double)(l - tl[i]) * (double)HD_LN2);
+        const float t = l - tl[i];
+        a.num += (double)u * ((double)t * (double)HD_LN2);
         a.den += (double)u;
+        h = (uint32_t)__bfloat16_as_ushort(__float2bfloat16(expm1f(-t * HD_LN2))) << 16 | (uint32_t)c;
       }
     }
-    if (lane == 0) lse2[i] = l;
+    if (lane == 0) {
+      lse2[i] = l;
+      if (hit != nullptr) hit[i] = h;
+    }
   }
   a = hd_block_sum(a);
   if (threadIdx.x == 0) {
@@ -938,8 +1277,6 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(const HeadReduce a, co
   }
 }
 
-static bool wide(const HeadCall& a) { return a.C > HD_MAX_C; }
-
 static int hd_blocks(long long n, int per_sm) {
   const long long b = (n + 255) / 256;
   return (int)(b < 148LL * per_sm ? (b < 1 ? 1 : b) : 148LL * per_sm);
@@ -956,20 +1293,39 @@ static void head_split(int row_tiles, int col_tiles, int* splits, int* tps) {
   }
 }
 
+static bool wide(const HeadCall& a) { return a.C > HD_MAX_C; }
+constexpr int HD_BOXES = 54;  // of HD_BOX16 in shared memory; a tile of rows or columns is 4 kboxes + 1 of them
+
+// Both gradients in one kernel: all of W next to two tiles of P and two of X in shared memory, dW and a dX next to two
+// tiles of s in tensor memory. Few voxels and class weights want P in two parts.
+static bool head_both(const HeadCall& a) {
+  const int cpad = (a.C + 15) / 16 * 16, kboxes = (a.C + 63) / 64;
+  const long long kt = ((long long)a.K + HD_TILE - 1) / HD_TILE;
+  return a.V > HD_FEW && a.cw == nullptr && kt <= 4 && (kt + 1) * cpad <= 256 &&
+         (kt + 2) * (4 * kboxes + 1) + 16 + 4 * kboxes + (kt + 1) / 2 <= HD_BOXES;
+}
+
 static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
   memset(&p, 0, sizeof(p));
   p.C = a.C;
   p.cpad = (a.C + 15) / 16 * 16;
   p.kboxes = (a.C + 63) / 64;
   p.ksteps = p.cpad / 16;
-  p.rows = mode == HEAD_DW ? a.K : a.V;
-  p.cols = mode == HEAD_DW ? a.V : a.K;
+  p.rows = mode >= HEAD_DW ? a.K : a.V;
+  p.cols = mode >= HEAD_DW ? a.V : a.K;
   p.row_tiles = (int)((p.rows + HD_TILE - 1) / HD_TILE);
   p.col_tiles = (int)((p.cols + HD_TILE - 1) / HD_TILE);
   p.rows_pad = hd_pad(p.rows);
   p.status = a.status;
+  if (mode == HEAD_BOTH) {
+    p.splits = p.col_tiles < 148 ? p.col_tiles : 148;  // CTAs, each with sums of its own
+    p.accs = (p.row_tiles + 2) * p.cpad <= 256 ? 2 : 1;
+    const int tile = 4 * p.kboxes + 1, left = HD_BOXES - p.row_tiles * tile - 4 * p.kboxes - (p.row_tiles + 1) / 2;
+    p.stages = (left - 16) / tile;
+    if (p.stages > 6) p.stages = 6;
+    return;
+  }
   head_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
-  // shared memory holds 54 boxes of 4 KB, a tile of rows or columns is 4 kboxes + 1 of them
   if (mode == HEAD_ROWS) {
     // with four row tiles a job the rounds have four tiles for each of theirs; with one, four of a job's tiles run side by
     // side, so one with fewer is as long
@@ -1000,7 +1356,7 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
 
 template <int MODE, bool FLAG>
 static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
-  constexpr bool rows = MODE == HEAD_ROWS, dw = MODE == HEAD_DW;
+  constexpr bool rows = MODE == HEAD_ROWS, both = MODE == HEAD_BOTH, dw = MODE >= HEAD_DW;
   const long long dv[2] = {a.C, a.V}, dk[2] = {a.C, a.K}, st[2] = {1, a.C};
   const int box[2] = {64, HD_TILE};
   int rc = make_map_bf16(&p.mapR, dw ? a.w : a.x, 2, dw ? dk : dv, st, box, 128);
@@ -1009,27 +1365,35 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
   if (rc) return rc;
   const long long st16[2] = {1, 16}, xv[2] = {16, hd_pad(a.V)}, wk[2] = {16, hd_pad(a.K)};
   const int box16[2] = {16, HD_TILE};
-  const uint4* w16 = a.w16 + (dw ? 2 * hd_pad(a.K) : 0);
+  const uint4* w16 = a.w16 + (MODE == HEAD_DW ? 2 * hd_pad(a.K) : 0);
   if (!rows) {
     rc = make_map_bf16(&p.mapR16, dw ? w16 : a.x16, 2, dw ? wk : xv, st16, box16, 32);
     if (rc) return rc;
   }
   rc = make_map_bf16(&p.mapQ16, dw ? a.x16 : w16, 2, dw ? xv : wk, st16, box16, 32);
   if (rc) return rc;
+  if (both) {
+    const int boxo[2] = {64, 32};
+    rc = make_map_bf16(&p.mapO, a.dx, 2, dv, st, boxo, 128);
+    if (rc) return rc;
+  }
   void (*kernel)(HeadParams) = nullptr;
   if constexpr (rows) kernel = head_rows_kernel<FLAG>;
+  else if constexpr (both) kernel = head_both_kernel;
   else kernel = head_grad_kernel<MODE, FLAG>;
-  const size_t smem = 1024 + (size_t)(p.rbufs + p.stages) * (p.kboxes * HD_BOX + HD_BOX16);
+  const size_t smem = 1024 + (size_t)((both ? p.row_tiles : p.rbufs) + p.stages) * (p.kboxes * HD_BOX + HD_BOX16) +
+                      (both ? 4 * HD_BOX + p.kboxes * HD_BOX + p.row_tiles * 4 * HD_TILE * 4 : 0);
   static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have as much as it can need
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return SB_ERR_DRIVER;
   if (dev > 63 || !(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + 54 * HD_BOX16) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + HD_BOXES * HD_BOX16) != cudaSuccess)
       return SB_ERR_DRIVER;
     if (dev <= 63) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  const long long jobs = (long long)(rows && p.together == 4 ? (p.row_tiles + 3) / 4 : p.row_tiles) * p.splits;
-  kernel<<<(int)(jobs < 148 ? jobs : 148), HD_THREADS, smem, stream>>>(p);
+  const long long jobs =
+      both ? p.splits : (long long)(rows && p.together == 4 ? (p.row_tiles + 3) / 4 : p.row_tiles) * p.splits;
+  kernel<<<(int)(jobs < 148 ? jobs : 148), both ? HB_THREADS : HD_THREADS, smem, stream>>>(p);
   sb_count_launch(1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
 }
@@ -1050,7 +1414,10 @@ static long long head_state(HeadCall& a, void* base) {
   a.lse2 = (float*)take(4 * hd_pad(a.V));
   a.y = (int*)take(4 * hd_pad(a.V));
   a.bias2 = (float*)take(4 * hd_pad(a.K));
-  if (!wide(a)) a.w16 = (uint4*)take(64 * hd_pad(a.K));
+  if (!wide(a)) {
+    a.w16 = (uint4*)take(64 * hd_pad(a.K));
+    if (head_both(a)) a.hit = (uint32_t*)take(4 * hd_pad(a.V));
+  }
   return at - (char*)base;
 }
 struct HeadFwdScratch {
@@ -1086,7 +1453,12 @@ static long long head_bwd_scratch(HeadCall& a, void* base) {
   head_geometry(a, HEAD_DX, p);
   const long long dx = p.splits == 1 ? 0 : p.splits * p.rows_pad * p.cpad;
   head_geometry(a, HEAD_DW, p);
-  const long long dw = p.splits * p.rows_pad * (p.cpad + 4);
+  long long dw = p.splits * p.rows_pad * (p.cpad + 4);
+  if (head_both(a)) {
+    head_geometry(a, HEAD_BOTH, p);
+    const long long both = p.splits * p.rows_pad * (p.cpad + 4);
+    if (both > dw) dw = both;
+  }
   return at - (char*)base + 4 * (dx > dw ? dx : dw);
 }
 
@@ -1107,6 +1479,19 @@ static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
   HeadParams p;
   int rc = 0;
   const bool few = a.V <= HD_FEW;
+  if (a.dx != nullptr && (a.dw != nullptr || a.db != nullptr) && head_both(a)) {
+    head_geometry(a, HEAD_BOTH, p);
+    p.rowg = a.g;
+    p.colhit = a.hit;
+    p.out = a.dx;
+    p.ws = a.scratch;
+    p.ws_b = a.scratch + p.splits * p.rows_pad * p.cpad;
+    rc = head_launch<HEAD_BOTH, false>(a, p, stream);
+    if (rc) return rc;
+    head_reduce(reduce_of(p.ws, p.splits, p, p.C, p.cpad, a.dw_kind, a.dw),
+                reduce_of(p.ws_b, 4 * p.splits, p, 1, 1, a.db_kind, a.db), a.scale, stream);
+    return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+  }
   if (a.dx != nullptr) {
     head_geometry(a, HEAD_DX, p);
     p.rowg = a.g;
@@ -1188,10 +1573,10 @@ extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, i
   // one block, which goes on to the loss, where its rounds cost less than another launch
   const int blocks = v_pad <= (team ? 256 : 4096) ? 1 : hd_blocks(team ? v_pad * 32 : v_pad, HD_SUM_BLOCKS / 148);
   if (team)
-    head_merge_kernel<32><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, f.sums, a.total,
+    head_merge_kernel<32><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, a.hit, f.sums, a.total,
                                                       loss, a.den);
   else
-    head_merge_kernel<1><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, f.sums, a.total,
+    head_merge_kernel<1><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, a.hit, f.sums, a.total,
                                                      loss, a.den);
   if (blocks > 1) head_total_kernel<<<1, 256, 0, stream>>>(f.sums, blocks, a.total, loss, a.den);
   sb_count_launch(blocks > 1 ? 2 : 1);

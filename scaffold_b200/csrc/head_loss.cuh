@@ -31,6 +31,7 @@ struct HeadCall {
   int* y;         // voxels: label, -1 where a voxel takes no part
   float* bias2;   // classes: bias log2(e), -inf behind the last
   uint4* w16;     // narrow heads, classes, twice: sixteen columns more of w
+  uint32_t* hit;  // voxels, for both gradients at once (head_both): label (16 bits) and p - 1 of it (bf16)
   // of the backward pass
   float* scale;   // [1] dL / den
   float* g;       // voxels: scale u, u the class weight of the label, 0 where a voxel takes no part
@@ -56,6 +57,11 @@ __device__ __forceinline__ void hd_tma_2d(void* dst, const CUtensorMap* m, uint6
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
       : "memory");
+}
+// a warp's wait, with the same answer in all lanes (one that gives up must not leave the others in a ballot)
+__device__ __forceinline__ bool hd_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status,
+                                        int site) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, site));
 }
 // named barrier `id` of `threads` threads; the same answer in all of them: whether every one said `ok`
 __device__ __forceinline__ bool hd_vote(int id, int threads, bool ok) {

@@ -241,7 +241,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
       float m = -INFINITY, s = 0.f, tl = 0.f, db = 0.f;
       int best = INT_MAX;
       for (int t = j.t0; t < j.t1; ++t) {
-        if (!mbar_wait_cl(&tfull[b], bph, abort_flag, p.status, 105)) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait_cl(&tfull[b], bph, abort_flag, p.status, 105))) { ok = false; break; }
         tc_fence_after();
         const int nc = live ? cols_of(t) : 0, c_abs = t * 256;
         for (int c0 = half * 32; c0 < nc; c0 += 64) {  // every second 32 columns are the other group's

@@ -87,6 +87,41 @@ def test_loss_and_gradients(v, c, k):
     _check(*_inputs(v, c, k))
 
 
+# both gradients in one kernel: one to four tiles of classes, one and more voxel tiles a CTA, its limits and just behind
+BOTH = [(129, 8, 1), (200, 64, 32), (256, 16, 33), (19000, 64, 128), (38100, 24, 40), (57000, 64, 257), (40000, 32, 500),
+        (40000, 128, 100), (19073, 128, 128), (1000, 128, 129), (300, 64, 384), (300, 64, 385), (500, 48, 512),
+        (500, 32, 513), (38017, 40, 130)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v,c,k", BOTH)
+def test_both_gradients_at_once(v, c, k):
+    x, w, b, y, _ = _inputs(v, c, k, ignored=0.1)
+    _, dx, dw, db = _check(x, w, b, y, None)
+    # and each of them alone, where one is asked for: the same sums from other kernels
+    one = [t.clone().requires_grad_() for t in (x, w, b)]
+    dx1, = torch.autograd.grad(head_cross_entropy(one[0], w, b, y, ignore_label=IGNORED), one[:1])
+    dw1, db1 = torch.autograd.grad(head_cross_entropy(x, *one[1:], y, ignore_label=IGNORED), one[1:])
+    # each side is within 4e-3 of the truth by its roundings to bf16 (_check), and within what fp32 leaves of D: e_term
+    # of p and of the target's one, so twice e_term / V a voxel at most, along rows of W, rows of X and ones
+    logits = x.double() @ w.double().T + b.double()
+    e = 4 * 2 * 2 ** -21 * (1 + 2 * float(logits.abs().amax())) / int((y != IGNORED).sum())
+    for got, want, size in ((dx1, dx, v ** 0.5 * float(w.double().norm(dim=1).max())),
+                            (dw1, dw, float(x.double().norm(dim=1).sum())), (db1, db, v)):
+        assert float((got.double() - want.double()).norm()) <= 8e-3 * float(want.double().norm()) + 2 * e * size
+
+
+@pytest.mark.gpu
+def test_both_gradients_are_the_same_each_time():
+    x, w, b, y, _ = _inputs(30000, 64, 257)
+    runs = []
+    for _ in range(3):
+        ps = [t.clone().requires_grad_() for t in (x, w, b)]
+        runs.append(torch.autograd.grad(head_cross_entropy(*ps, y), ps))
+    for other in runs[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(runs[0], other))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("v,c,k", [(300, 64, 147), (513, 256, 300), (400, 320, 300)])
 @pytest.mark.parametrize("label_type", [torch.int16, torch.int32, torch.int64])
