@@ -134,11 +134,12 @@ __device__ __forceinline__ void hd_sub_if(float& v, float d, uint32_t bits, uint
       : "f"(d), "r"(bits), "r"(bit));
 }
 // s = R Q^T of a tile: the sixteen columns more, then the channels
-__device__ __forceinline__ void hd_first_mma(uint32_t d, uint32_t r, uint32_t q, uint32_t box16, int cols, int ksteps) {
+__device__ __forceinline__ void hd_first_mma(uint32_t d, uint32_t r, uint32_t r16, uint32_t q, uint32_t q16, int cols,
+                                             int ksteps) {
   const uint32_t hi = desc_hi(8u * 128u, 2u), hi16 = desc_hi(8u * 32u, 6u);
   const uint32_t idesc = make_idesc_bf16(128, cols, 0, 0);
   const uint32_t a_lo = desc_lo(r, 16u), b_lo = desc_lo(q, 16u);
-  tc_mma_bf16_pred(d, desc_lo(r + box16, 16u), hi16, desc_lo(q + box16, 16u), hi16, idesc, 0u);
+  tc_mma_bf16_pred(d, desc_lo(r16, 16u), hi16, desc_lo(q16, 16u), hi16, idesc, 0u);
   for (int k = 0; k < ksteps; ++k) {
     const uint32_t off = (uint32_t)(k >> 2) * (HD_BOX >> 4) + (uint32_t)(k & 3) * 2u;
     tc_mma_bf16_pred(d, a_lo + off, hi, b_lo + off, hi, idesc, 1u);
@@ -156,7 +157,7 @@ template <bool ARG>
 __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_constant__ HeadParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t r_full[4], r_empty[4], q_full[HD_MAX_STAGES], q_empty[HD_MAX_STAGES], s_full[4], s_done[4];
+  __shared__ uint64_t r_full[8], r_empty[8], q_full[HD_MAX_STAGES], q_empty[HD_MAX_STAGES], s_full[4], s_done[4];
   __shared__ uint32_t tmem_base_s, abort_s;
   volatile uint32_t* abort_flag = &abort_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -164,13 +165,16 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
   const int row_jobs = four ? (p.row_tiles + 3) / 4 : p.row_tiles, jobs = row_jobs * p.splits;
   const uint32_t box16 = (uint32_t)p.kboxes * HD_BOX, tile_bytes = box16 + HD_BOX16;
   uint8_t* smem_r = smem;
-  uint8_t* smem_q = smem + (size_t)p.rbufs * tile_bytes;
+  uint8_t* smem_q = smem + (size_t)p.rbufs * box16;
+  uint8_t* smem_r16 = smem_q + (size_t)p.stages * tile_bytes;  // the rows' columns more, of all rows the same
 
   if (threadIdx.x == 0) {
     abort_s = 0;
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < p.rbufs; ++i) {
       mbar_init(&r_full[i], 1);
       mbar_init(&r_empty[i], four ? 1 : 2);  // a row tile of several is one issuing warp's, a single one both warps'
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_done[i], HD_EPI_WARPS / 4);
     }
@@ -181,14 +185,12 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
     mbar_fence_init();
   }
   if (threadIdx.x < HD_TILE) {
-    // the rows' columns more: ones against the three parts of the bias (32-byte rows, 16-byte halves exchanged in every
-    // second group of four rows: the 32-byte swizzle)
-    for (int b = 0; b < p.rbufs; ++b) {
-      uint4* at = reinterpret_cast<uint4*>(smem_r + b * tile_bytes + box16 + threadIdx.x * 32);
-      const int half = (threadIdx.x >> 2) & 1;
-      at[half] = make_uint4(0x3F803F80u, 0x00003F80u, 0u, 0u);
-      at[half ^ 1] = make_uint4(0u, 0u, 0u, 0u);
-    }
+    // ones against the three parts of the bias (32-byte rows, 16-byte halves exchanged in every second group of four rows:
+    // the 32-byte swizzle)
+    uint4* at = reinterpret_cast<uint4*>(smem_r16 + threadIdx.x * 32);
+    const int half = (threadIdx.x >> 2) & 1;
+    at[half] = make_uint4(0x3F803F80u, 0x00003F80u, 0u, 0u);
+    at[half ^ 1] = make_uint4(0u, 0u, 0u, 0u);
     fence_proxy_async();
   }
   if (warp == 0) {
@@ -218,7 +220,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
             if (!mbar_wait(&r_empty[rb], rph ^ 1u, abort_flag, p.status, 91)) { ok = false; break; }
             mbar_expect_tx(&r_full[rb], box16);
             for (int k = 0; k < p.kboxes; ++k)
-              hd_tma_2d(smem_r + rb * tile_bytes + k * HD_BOX, &p.mapR, &r_full[rb], k * 64, (rt + g) * HD_TILE);
+              hd_tma_2d(smem_r + rb * box16 + k * HD_BOX, &p.mapR, &r_full[rb], k * 64, (rt + g) * HD_TILE);
             if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
           }
           if (!ok || !mbar_wait(&q_empty[st], ph ^ 1u, abort_flag, p.status, 91)) { ok = false; break; }
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
   } else if (warp <= 2) {
     const bool leader = elect_one();
     const uint32_t mine = (uint32_t)warp - 1u;
-    const uint32_t r0 = smem_u32(smem_r), q0 = smem_u32(smem_q);
+    const uint32_t r0 = smem_u32(smem_r), r16 = smem_u32(smem_r16), q0 = smem_u32(smem_q);
     uint32_t rb = 0, rph = 0, st = 0, ph = 0, fi = 0;  // fi: column tiles so far (together = 1)
     uint32_t uses[2] = {0u, 0u};                       // of this warp's two tiles of s
     bool ok = true;
@@ -243,7 +245,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
       if (!hd_wait(&s_done[g], (u & 1u) ^ 1u, abort_flag, p.status, 96)) return false;
       tc_fence_after();
       if (leader) {
-        hd_first_mma(tmem + g * HD_TILE, r0 + r_slot * tile_bytes, q0 + st * tile_bytes, box16, cols_of(t), p.ksteps);
+        const uint32_t q = q0 + st * tile_bytes;
+        hd_first_mma(tmem + g * HD_TILE, r0 + r_slot * box16, r16, q, q + box16, cols_of(t), p.ksteps);
         tc_commit(&s_full[g]);
       }
       __syncwarp();
@@ -260,9 +263,9 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
           if (!hd_wait(&q_full[st], ph, abort_flag, p.status, 95)) { ok = false; break; }
           if (four) {
             for (uint32_t g = mine; g < 4u && ok; g += 2u) {
-              if (t == t0) ok = hd_wait(&r_full[g], rph, abort_flag, p.status, 94);
-              ok = ok && tile(g, g, t);
-              if (ok && leader && t == t1 - 1) tc_commit(&r_empty[g]);
+              if (t == t0) ok = hd_wait(&r_full[rb + g], rph, abort_flag, p.status, 94);
+              ok = ok && tile(g, rb + g, t);
+              if (ok && leader && t == t1 - 1) tc_commit(&r_empty[rb + g]);
               __syncwarp();
             }
           } else {
@@ -274,16 +277,15 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
         }
         if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
       }
-      if (four) {
-        rph ^= 1u;
-      } else {
+      if (!four) {
         if (ok && leader) {  // this warp is done with the resident tile
           if (used) tc_commit(&r_empty[rb]);
           else mbar_arrive(&r_empty[rb]);
         }
         __syncwarp();
-        if (++rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
       }
+      rb += p.together;
+      if (rb == (uint32_t)p.rbufs) { rb = 0; rph ^= 1u; }
     }
   } else {
     const int quad = warp & 3, group = (warp - HD_FIRST_EPI) >> 2;
@@ -480,7 +482,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
         if (!hd_wait(&q_full[st], ph, abort_flag, p.status, 95)) { ok = false; break; }
         tc_fence_after();
         if (leader) {
-          hd_first_mma(tmem + b * HD_TILE, r0 + rb * tile_bytes, q0 + st * tile_bytes, box16, cols_of(t), p.ksteps);
+          const uint32_t r = r0 + rb * tile_bytes, q = q0 + st * tile_bytes;
+          hd_first_mma(tmem + b * HD_TILE, r, r + box16, q, q + box16, cols_of(t), p.ksteps);
           tc_commit(&s_full[b]);
           if (t == t1 - 1) tc_commit(&r_empty[rb]);
         }
@@ -805,7 +808,8 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
         if (!hd_wait(&s_empty[b], bph ^ 1u, abort_flag, p.status, 96)) { ok = false; break; }
         tc_fence_after();
         if (leader) {
-          hd_first_mma(tmem + b * HD_TILE, w0 + i * tile_bytes, x0 + st * tile_bytes, box16, HD_TILE, p.ksteps);
+          const uint32_t r = w0 + i * tile_bytes, q = x0 + st * tile_bytes;
+          hd_first_mma(tmem + b * HD_TILE, r, r + box16, q, q + box16, HD_TILE, p.ksteps);
           tc_commit(&s_full[b]);
         }
         __syncwarp();
@@ -997,11 +1001,15 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
       }
     }
     // dW and db of this CTA's voxels
-    if (ok && hd_wait(&dw_full, 0, abort_flag, p.status, 97)) {
+    if (hd_vote(1, 32 * HD_EPI_WARPS, ok) && hd_wait(&dw_full, 0, abort_flag, p.status, 97)) {
       tc_fence_after();
+      for (int i = group; i < kt; i += 4) {  // the groups' sums, in order
+        const float* all = smem_db + i * 4 * HD_TILE + row;
+        p.ws_b[(long long)blockIdx.x * p.rows_pad + (long long)i * HD_TILE + row] =
+            all[0] + all[HD_TILE] + all[2 * HD_TILE] + all[3 * HD_TILE];
+      }
       for (int i = 0; i < kt; ++i) {
         const long long r = (long long)i * HD_TILE + row;
-        p.ws_b[((long long)blockIdx.x * 4 + group) * p.rows_pad + r] = db[i * 4 * HD_TILE];
         for (int c0 = group * 16; c0 < p.cpad; c0 += 64) {
           uint32_t v[16];
           tmem_ld_32x16(lane_base + ACC_W + i * p.cpad + c0, v);
@@ -1262,7 +1270,7 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(const HeadReduce a, co
     float sum = 0.f;
     if (i < n) {
       const float* src = p.ws + i / p.C * p.ld + i % p.C;
-#pragma unroll 4
+#pragma unroll 8
       for (int s = warp; s < p.slices; s += 8) sum += src[s * slice];
     }
     s_part[warp][lane] = sum;
@@ -1342,8 +1350,8 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
         p.tiles_per_split = per4;
       }
     }
-    p.rbufs = p.together == 4 ? 4 : p.kboxes <= 2 ? 2 : 1;
-    p.stages = p.kboxes == 1 ? (p.together == 4 ? 6 : 8) : p.kboxes == 2 ? (p.together == 4 ? 2 : 4) : p.kboxes == 3 ? 3 : 2;
+    p.rbufs = p.together == 4 ? (p.kboxes == 1 ? 8 : 4) : p.kboxes <= 2 ? 2 : 1;
+    p.stages = p.kboxes == 1 ? (p.together == 4 ? 4 : 8) : p.kboxes == 2 ? (p.together == 4 ? 2 : 4) : p.kboxes == 3 ? 3 : 2;
     return;
   }
   p.bufs = p.cpad <= 128 ? 3 : 2;
@@ -1381,7 +1389,8 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
   if constexpr (rows) kernel = head_rows_kernel<FLAG>;
   else if constexpr (both) kernel = head_both_kernel;
   else kernel = head_grad_kernel<MODE, FLAG>;
-  const size_t smem = 1024 + (size_t)((both ? p.row_tiles : p.rbufs) + p.stages) * (p.kboxes * HD_BOX + HD_BOX16) +
+  const size_t smem = 1024 + (size_t)((both ? p.row_tiles : p.rbufs) + p.stages) * p.kboxes * HD_BOX +
+                      (size_t)((both ? p.row_tiles : rows ? 1 : p.rbufs) + p.stages) * HD_BOX16 +
                       (both ? 4 * HD_BOX + p.kboxes * HD_BOX + p.row_tiles * 4 * HD_TILE * 4 : 0);
   static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have as much as it can need
   int dev = 0;
@@ -1489,7 +1498,7 @@ static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
     rc = head_launch<HEAD_BOTH, false>(a, p, stream);
     if (rc) return rc;
     head_reduce(reduce_of(p.ws, p.splits, p, p.C, p.cpad, a.dw_kind, a.dw),
-                reduce_of(p.ws_b, 4 * p.splits, p, 1, 1, a.db_kind, a.db), a.scale, stream);
+                reduce_of(p.ws_b, p.splits, p, 1, 1, a.db_kind, a.db), a.scale, stream);
     return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
   }
   if (a.dx != nullptr) {
