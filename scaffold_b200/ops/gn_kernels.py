@@ -240,11 +240,10 @@ def gn8_forward(x, w, b, groups: int, eps: float = 1e-5, relu: bool = True, fin:
     the same memory layout for y, whatever its shape."""
     n, d, h, wd, c = x.shape
     s = d * h * wd
-    dev = x.device
     y = torch.empty_like(x) if out is None else out
-    kept = torch.empty(kept_bytes(n * s * c), dtype=torch.uint8, device=dev)
-    stats = torch.empty((2, n, groups), dtype=torch.float32, device=dev)
-    scratch = torch.empty(_scratch8(0, n, s, c, groups), dtype=torch.float32, device=dev) if fin is None else None
+    kept = x.new_empty(kept_bytes(n * s * c), dtype=torch.uint8)
+    stats = w.new_empty((2, n, groups))
+    scratch = w.new_empty(_scratch8(0, n, s, c, groups)) if fin is None else None
     _lib.check(_lib.lib().sb_gn8_forward(
         x.data_ptr(), w.data_ptr(), b.data_ptr(), n, s, c, groups, eps, relu, _lib.ptr(fin),
         fin is None and _fused_finalize(n * groups), y.data_ptr(), kept.data_ptr(), stats.data_ptr(), _lib.ptr(scratch),
@@ -256,10 +255,9 @@ def gn8_backward(dy, kept, w, b, stats, groups: int, relu: bool = True, into=Non
     """(dx, dw, db) from the 8-bit copy; ``into`` as in :func:`gn_bwd_dx`, ``out`` (for dx) as in :func:`gn8_forward`."""
     n, d, h, wd, c = dy.shape
     s = d * h * wd
-    dev = dy.device
     dx = torch.empty_like(dy) if out is None else out
-    dw, db = into if into is not None else (torch.empty(c, dtype=torch.float32, device=dev) for _ in range(2))
-    scratch = torch.empty(_scratch8(1, n, s, c, groups), dtype=torch.float32, device=dev)
+    dw, db = into if into is not None else (torch.empty_like(w), torch.empty_like(b))
+    scratch = w.new_empty(_scratch8(1, n, s, c, groups))
     _lib.check(_lib.lib().sb_gn8_backward(
         dy.data_ptr(), kept.data_ptr(), w.data_ptr(), b.data_ptr(), stats.data_ptr(), n, s, c, groups, relu, dx.data_ptr(),
         dw.data_ptr(), db.data_ptr(), into is not None, scratch.data_ptr(), _lib.stream_ptr()), "sb_gn8_backward")

@@ -67,15 +67,15 @@ class _Gn8Fn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, relu, partials):
-        shape, x = x.shape, to_vm(x)
+        # (no view of another tensor: autograd keeps a record of such a result's base)
+        y = torch.empty_like(x, memory_format=torch.channels_last_3d)
+        x = to_vm(x)
         w32, b32 = _fp32(weight), _fp32(bias)
         fin = None
         if partials is not None:
             part, splits, pg = partials
             if pg == groups and part.numel() == x.shape[0] * splits * groups * 3:
                 fin = gk.gn_finalize(part, x.shape[0], groups, splits)
-        # (no view of another tensor: autograd keeps a record of such a result's base)
-        y = torch.empty(shape, dtype=x.dtype, device=x.device, memory_format=torch.channels_last_3d)
         _, kept, stats = gk.gn8_forward(x, w32, b32, groups, eps, relu, fin=fin, out=y)
         ctx.save_for_backward(kept, w32, b32, stats)
         ctx.cfg = (groups, relu)
@@ -93,7 +93,7 @@ class _Gn8Fn(torch.autograd.Function):
             if any(t is None for t in into):
                 into = None
         with on_device(gy.device):
-            dx = torch.empty(gy.shape, dtype=torch.bfloat16, device=gy.device, memory_format=torch.channels_last_3d)
+            dx = torch.empty_like(gy, dtype=torch.bfloat16, memory_format=torch.channels_last_3d)
             _, dw, db = gk.gn8_backward(to_vm(gy), kept, w32, b32, stats, groups, relu, into=into, out=dx)
         if into is not None:
             dw = db = None

@@ -61,9 +61,9 @@ class _HeadLossFn(torch.autograd.Function):
         v, c = x.shape
         k = w16.shape[0]
         n_state, n_scratch, _ = _bytes(v, k, c, cw is not None)
-        state = torch.empty(n_state, dtype=torch.uint8, device=dev)
-        scratch = torch.empty(n_scratch, dtype=torch.uint8, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
+        state = x.new_empty(n_state, dtype=torch.uint8)
+        scratch = state.new_empty(n_scratch)
+        loss = x.new_empty((), dtype=torch.float32)
         st = _lib.stream_ptr()
         _lib.check(_lib.lib().sb_head_forward(
             x.data_ptr(), w16.data_ptr(), _lib.ptr(bias), 0 if bias is None else _KIND[bias.dtype], labels.data_ptr(),
@@ -88,9 +88,9 @@ class _HeadLossFn(torch.autograd.Function):
         gout = gout.float()
         with on_device(dev):
             dx = torch.empty_like(x) if want_x else None
-            dw = torch.empty((k, c), dtype=w_type, device=dev) if want_w else None
-            db = torch.empty(k, dtype=b_type, device=dev) if want_b else None
-            scratch = torch.empty(_bytes(v, k, c, cw is not None)[2], dtype=torch.uint8, device=dev)
+            dw = torch.empty_like(w16, dtype=w_type) if want_w else None
+            db = w16.new_empty(k, dtype=b_type) if want_b else None
+            scratch = state.new_empty(_bytes(v, k, c, cw is not None)[2])
             _lib.check(_lib.lib().sb_head_backward(
                 x.data_ptr(), w16.data_ptr(), _lib.ptr(cw), v, k, c, state.data_ptr(), scratch.data_ptr(), gout.data_ptr(),
                 _lib.ptr(dx), _lib.ptr(dw), _KIND[w_type], _lib.ptr(db), _KIND[b_type] if want_b else 0,
@@ -108,8 +108,8 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
     ``class_weights [K]`` (not negative) weigh the voxels by their label; the result is the sum of the weighted terms over
     the sum of the weights, over all shards with ``spatial``. Voxels of ``ignore_label`` take no part; without any other
     voxel the loss and its gradients are zero. A label outside the classes takes no part either and is reported by
-    :func:`scaffold_b200.ops._lib.check_status`. Features of voxels that take no part have to be finite, as for the
-    formula: they reach the weight's gradient as ``0 * x``.
+    :func:`scaffold_b200.ops._lib.check_status`. Features of voxels that take no part have to be finite for the
+    kernels: they reach the weight's gradient as ``0 * x``, as in any matrix product with rows of zeros.
 
     The kernels read bf16: an fp32 ``weight`` is rounded, its gradient comes back in fp32. Gradients: features in bf16,
     weight and bias in their own types.

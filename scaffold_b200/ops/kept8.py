@@ -15,6 +15,7 @@ On CUDA the copy is made by ``csrc/kept8.cu`` on the current stream; on the CPU 
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import NamedTuple, Tuple
 
 import torch
@@ -44,14 +45,7 @@ class Kept8(NamedTuple):
         return self.data.device
 
     def numel(self) -> int:
-        return _numel(self.shape)
-
-
-def _numel(shape) -> int:
-    n = 1
-    for s in shape:
-        n *= s
-    return n
+        return math.prod(self.shape)
 
 
 def kept_bytes(numel: int) -> int:
@@ -74,8 +68,9 @@ def _dense(x: torch.Tensor) -> bool:
 def keep8(x: torch.Tensor) -> Kept8:
     """The 8-bit copy of a bf16, fp16 or fp32 tensor of any shape. Blocks follow the tensor's memory; a tensor that does
     not cover one run of memory (a slice, an expanded view) is copied to one first, in the order of its indices."""
-    if x.dtype not in KINDS:
-        raise TypeError(f"keep8 takes bf16, fp16 or fp32; got {x.dtype}")
+    dtype, shape = x.dtype, x.shape
+    if dtype not in KINDS:
+        raise TypeError(f"keep8 takes bf16, fp16 or fp32; got {dtype}")
     if x.layout != torch.strided or x.is_conj() or x.is_neg():
         raise TypeError("keep8 takes plain strided tensors")
     if not _dense(x):
@@ -85,9 +80,9 @@ def keep8(x: torch.Tensor) -> Kept8:
         return Kept8(_keep_formula(x.detach().as_strided((n,), (1,), x.storage_offset())), tuple(x.shape), x.stride(), x.dtype)
     dev = x.device
     with on_device(dev):
-        data = torch.empty(kept_bytes(n), dtype=torch.uint8, device=dev)
-        _lib.check(_lib.lib().sb_keep8(x.data_ptr(), KINDS[x.dtype], n, data.data_ptr(), _lib.stream_ptr()), "sb_keep8")
-    return Kept8(data, tuple(x.shape), x.stride(), x.dtype)
+        data = x.new_empty(kept_bytes(n), dtype=torch.uint8)
+        _lib.check(_lib.lib().sb_keep8(x.data_ptr(), KINDS[dtype], n, data.data_ptr(), _lib.stream_ptr()), "sb_keep8")
+    return Kept8(data, tuple(shape), x.stride(), dtype)
 
 
 def restore8(kept: Kept8) -> torch.Tensor:
