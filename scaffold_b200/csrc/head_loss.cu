@@ -47,7 +47,9 @@ constexpr int HD_TILE = 128;
 constexpr int HD_BOX = HD_TILE * 128;  // bytes of a 128-row box of 64 channels
 constexpr int HD_BOX16 = HD_TILE * 32; // and of the sixteen columns more
 constexpr int HD_MAX_STAGES = 8;
-constexpr int HD_MAX_C = 256;          // TMEM: two or three tiles of s and the accumulator in 512 columns
+// TMEM: two or three tiles of s and the accumulator in 512 columns. At that width head_wide.cu is slower still: dX of 131072
+// voxels x 256 channels x 2048 classes 238 us here and 570 there.
+constexpr int HD_MAX_C = 256;
 
 enum HeadMode { HEAD_ROWS = 0, HEAD_DX = 1, HEAD_DW = 2, HEAD_BOTH = 3 };
 
@@ -151,8 +153,11 @@ __device__ __forceinline__ void hd_first_mma(uint32_t d, uint32_t r, uint32_t r1
 //                 loaded once for 512 rows and a row's statistics stay in one thread: nothing is merged in the CTA
 //   together = 1: a job is one row tile; group g takes every fourth column tile and leaves statistics of its own
 // The second one is for calls that have no four row tiles for every SM, and for tiles of which shared memory holds few.
-// Bound: the exponential unit, 1024 clocks a tile of 128 x 128. Merging two halves of a tile's columns over two groups by
-// tile parity instead (a barrier and an exchange in every job): 631 us for 2 x 128^3 voxels, 64 channels and 257 classes.
+// Row tiles come in twice the number of a job, so that the next job's are there when this one ends (485 -> 427 us for the
+// whole loss below). Bound: the exponential unit, 1024 clocks a tile of 128 x 128, at long runs of columns (75 % of it at
+// 500 classes), and between jobs the way of a tile through tensor memory. 2 x 128^3 voxels, 64 channels and 257 classes: 381
+// us (237 for the exponentials alone). Merging two halves of a tile's columns over two groups by tile parity instead (a
+// barrier and an exchange in every job): 631.
 template <bool ARG>
 __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_constant__ HeadParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -392,6 +397,10 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
   }
 }
 
+// One gradient (the header has the mathematics). Two or three tiles of s in tensor memory, whose P replaces it: two groups
+// take a tile's halves, by tile parity. Bound: the instructions of the epilogue (about 8 an entry, 2300 clocks a tile of 128
+// x 128, of which the exponential unit takes 1024), three of them for the target in its row. 2 x 128^3 voxels, 64 channels
+// and 257 classes: 540 us each for dX and dW; 2^20 voxels and 512 classes 213 and 224 with all that stands around them.
 template <int MODE, bool LO>
 __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_constant__ HeadParams p) {
   constexpr int MAXB = 3;
@@ -620,79 +629,79 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
         label[1] = __ldg(labels + (long long)t * HD_TILE + 32);
       }
       for (; t < t1; t += 2) {
-          if (!hd_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
-          int rel[2] = {label[0] - (int)(r - lane), label[1] - (int)(r - lane)};
-          if (MODE == HEAD_DW && t + 2 < t1) {
-            label[0] = __ldg(labels + (long long)(t + 2) * HD_TILE);
-            label[1] = __ldg(labels + (long long)(t + 2) * HD_TILE + 32);
+        if (!hd_wait(&s_full[b], bph, abort_flag, p.status, 98)) { ok = false; break; }
+        int rel[2] = {label[0] - (int)(r - lane), label[1] - (int)(r - lane)};
+        if (MODE == HEAD_DW && t + 2 < t1) {
+          label[0] = __ldg(labels + (long long)(t + 2) * HD_TILE);
+          label[1] = __ldg(labels + (long long)(t + 2) * HD_TILE + 32);
+        }
+        tc_fence_after();
+        const int nc = cols_of(t) - half * 64;  // this group's columns: none, 32 or (64 and more) 64
+        const int c_abs = t * HD_TILE + half * 64;
+        const uint32_t tile = lane_base + b * HD_TILE + half * 64;
+#pragma unroll
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          if (c0 >= nc) break;
+          uint32_t v[32];
+          tmem_ld_32x32(tile + c0, v);
+          tmem_ld_wait();
+          float f[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+          // bit j: column j is the row's label
+          uint32_t hits;
+          if (MODE == HEAD_DX) {
+            const int at = y - (c_abs + c0);
+            hits = (unsigned)at < 32u ? 1u << at : 0u;
+          } else {
+            // lane c has the label of column c; a row's columns are those whose label has the row's five bits
+            hits = __ballot_sync(0xffffffffu, (unsigned)rel[c0 / 32] < 32u);
+#pragma unroll
+            for (int k = 0; k < 5; ++k)
+              hits &= __ballot_sync(0xffffffffu, rel[c0 / 32] >> k & 1) ^ rank_bits[k];
           }
-          tc_fence_after();
-          const int nc = cols_of(t) - half * 64;  // this group's columns: none, 32 or (64 and more) 64
-          const int c_abs = t * HD_TILE + half * 64;
-          const uint32_t tile = lane_base + b * HD_TILE + half * 64;
+          const bool any = __any_sync(0xffffffffu, hits != 0u);
 #pragma unroll
-          for (int c0 = 0; c0 < 64; c0 += 32) {
-            if (c0 >= nc) break;
-            uint32_t v[32];
-            tmem_ld_32x32(tile + c0, v);
-            tmem_ld_wait();
-            float f[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-            // bit j: column j is the row's label
-            uint32_t hits;
-            if (MODE == HEAD_DX) {
-              const int at = y - (c_abs + c0);
-              hits = (unsigned)at < 32u ? 1u << at : 0u;
-            } else {
-              // lane c has the label of column c; a row's columns are those whose label has the row's five bits
-              hits = __ballot_sync(0xffffffffu, (unsigned)rel[c0 / 32] < 32u);
-#pragma unroll
-              for (int k = 0; k < 5; ++k)
-                hits &= __ballot_sync(0xffffffffu, rel[c0 / 32] >> k & 1) ^ rank_bits[k];
-            }
-            const bool any = __any_sync(0xffffffffu, hits != 0u);
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const float2 t = hd_fma2(make_float2(f[j], f[j + 1]), make_float2(HD_LOG2E, HD_LOG2E), make_float2(0.f, 0.f));
-                f[j] = hd_ex2(t.x);
-                f[j + 1] = hd_ex2(t.y);
-              }
-              if (any) {
-                const float one = MODE == HEAD_DW ? g : 1.f;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) hd_sub_if(f[j], one, hits, 1u << j);
-              }
-              if (MODE == HEAD_DW) {
-                float2 d[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) d[j / 2 & 1] = hd_add2(d[j / 2 & 1], make_float2(f[j], f[j + 1]));
-                d[0] = hd_add2(d[0], d[1]);
-                db += d[0].x + d[0].y;
-              }
-              uint32_t o[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
-              // over the 32 columns of s that this thread has just read: 16 columns of P, 16 of its remainder
-              hd_tmem_st_x16(tile + c0, o);
-              if (LO) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  o[j] = pack_bf16x2(f[2 * j] - __uint_as_float(o[j] << 16),
-                                     f[2 * j + 1] - __uint_as_float(o[j] & 0xFFFF0000u));
-                hd_tmem_st_x16(tile + c0 + 16, o);
-              }
+          for (int j = 0; j < 32; j += 2) {
+            const float2 t = hd_fma2(make_float2(f[j], f[j + 1]), make_float2(HD_LOG2E, HD_LOG2E), make_float2(0.f, 0.f));
+            f[j] = hd_ex2(t.x);
+            f[j + 1] = hd_ex2(t.y);
           }
-          hd_tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_done[b]);
-          if (pending) {
-            if (!drain()) { ok = false; break; }
-            pending = false;
+          if (any) {
+            const float one = MODE == HEAD_DW ? g : 1.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) hd_sub_if(f[j], one, hits, 1u << j);
           }
-          b += 2;
-          if (b >= NB) { b -= NB; bph ^= 1u; }
+          if (MODE == HEAD_DW) {
+            float2 d[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) d[j / 2 & 1] = hd_add2(d[j / 2 & 1], make_float2(f[j], f[j + 1]));
+            d[0] = hd_add2(d[0], d[1]);
+            db += d[0].x + d[0].y;
+          }
+          uint32_t o[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+          // over the 32 columns of s that this thread has just read: 16 columns of P, 16 of its remainder
+          hd_tmem_st_x16(tile + c0, o);
+          if (LO) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              o[j] = pack_bf16x2(f[2 * j] - __uint_as_float(o[j] << 16),
+                                 f[2 * j + 1] - __uint_as_float(o[j] & 0xFFFF0000u));
+            hd_tmem_st_x16(tile + c0 + 16, o);
+          }
+        }
+        hd_tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_done[b]);
+        if (pending) {
+          if (!drain()) { ok = false; break; }
+          pending = false;
+        }
+        b += 2;
+        if (b >= NB) { b -= NB; bph ^= 1u; }
       }
       if (ok && pending) ok = drain();  // this job had no tile for this group
       pending = true;
@@ -1255,17 +1264,33 @@ struct HeadReduce {
   long long rows, rows_pad;
   void* out;
 };
-// The first a.blocks blocks take a, the others b (dw and db). A block takes 32 neighbouring outputs, each of its eight
-// warps every eighth slice: a thread that walks all slices waits an L2 trip for a few of them at a time.
+// The first a.blocks blocks take a, the others b (dw and db). Up to HD_FEW_SLICES a thread walks the slices of its outputs.
+// More of them: a block takes 32 neighbouring outputs, each of its eight warps every eighth slice, since a thread would
+// wait an L2 trip for a few of them at a time. (Loss and gradients of 1 voxel x 256 channels x 32768 classes,
+// one slice: 105 us, in the second form 347; 300 x 64 x 20000 52 and 89; 2 x 128^3 x 64 x 257, 148 slices: 1152 us, in the
+// first form 1162.)
+constexpr int HD_FEW_SLICES = 4;
 __global__ void __launch_bounds__(256) head_reduce_kernel(const HeadReduce a, const HeadReduce b,
                                                           const float* __restrict__ scale) {
   __shared__ float s_part[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool first = (int)blockIdx.x < a.blocks;
   const HeadReduce& p = first ? a : b;
+  const int block = first ? blockIdx.x : blockIdx.x - a.blocks;
   const long long n = p.rows * p.C, slice = p.rows_pad * p.ld;
   const float k = scale != nullptr ? scale[0] : 1.f;
-  for (long long i0 = (long long)(first ? blockIdx.x : blockIdx.x - a.blocks) * 32; i0 < n; i0 += (long long)p.blocks * 32) {
+  if (p.slices <= HD_FEW_SLICES) {
+    for (long long i = (long long)block * 256 + threadIdx.x; i < n; i += (long long)p.blocks * 256) {
+      const float* src = p.ws + i / p.C * p.ld + i % p.C;
+      float sum = 0.f;
+      for (int s = 0; s < p.slices; ++s) sum += src[s * slice];
+      sum *= k;
+      if (p.kind == 2) reinterpret_cast<float*>(p.out)[i] = sum;
+      else reinterpret_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16(sum);
+    }
+    return;
+  }
+  for (long long i0 = (long long)block * 32; i0 < n; i0 += (long long)p.blocks * 32) {
     const long long i = i0 + lane;
     float sum = 0.f;
     if (i < n) {
@@ -1291,6 +1316,8 @@ static int hd_blocks(long long n, int per_sm) {
 }
 
 // How many ways the columns are cut: fewest rounds of (tiles per job + about one tile of fixed cost), fewest cuts first.
+// Loss of 300 voxels x 64 channels x 20000 classes 19 us, without cuts 113; 1000 x 256 x 1000 17 and 25; loss and gradients
+// of 40000 x 32 x 1001 130 and 318; 5000 x 64 x 300, whose row tiles are cut into few, 39 and 37.
 static void head_split(int row_tiles, int col_tiles, int* splits, int* tps) {
   long long best = -1;
   for (int want = 1; want <= col_tiles && want <= 296; ++want) {
@@ -1335,8 +1362,9 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
   }
   head_split(p.row_tiles, p.col_tiles, &p.splits, &p.tiles_per_split);
   if (mode == HEAD_ROWS) {
-    // with four row tiles a job the rounds have four tiles for each of theirs; with one, four of a job's tiles run side by
-    // side, so one with fewer is as long
+    // With four row tiles a job the rounds have four tiles for each of theirs; with one, four of a job's tiles run side by
+    // side, so one with fewer is as long. Four and one: 407 and 494 us for 2 x 128^3 voxels x 64 channels x 257 classes, 34
+    // and 37 for 64^3 x 64 x 147; 37 and 35 for 100000 x 128 x 500, where it takes one.
     p.together = 1;
     if (p.kboxes <= 2) {
       int s4 = 1, per4 = 1;
@@ -1475,7 +1503,8 @@ static HeadReduce reduce_of(const float* ws, int slices, const HeadParams& p, in
   HeadReduce r;
   r.ws = ws; r.slices = slices; r.C = C; r.ld = ld; r.kind = kind; r.out = out;
   r.rows = p.rows; r.rows_pad = p.rows_pad;
-  const long long blocks = out == nullptr ? 0 : (p.rows * C + 31) / 32;
+  const int each = slices <= HD_FEW_SLICES ? 256 : 32;  // outputs of a block
+  const long long blocks = out == nullptr ? 0 : (p.rows * C + each - 1) / each;
   r.blocks = (int)(blocks < 148 * 8 ? blocks : 148 * 8);
   return r;
 }
@@ -1578,8 +1607,11 @@ extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, i
     rc = head_launch<HEAD_ROWS, false>(a, p, stream);
   }
   if (rc) return rc;
+  // a warp for a voxel: loss of 300 voxels x 64 channels x 20000 classes 19 us, a thread for each 90; of 40000 x 32 x 1001
+  // (four shares) 45 and 33
   const bool team = splits > 4;
-  // one block, which goes on to the loss, where its rounds cost less than another launch
+  // one block, which goes on to the loss, where its rounds cost less than another launch (18 us for 5000 x 64 x 300 both
+  // ways on the device, and the launch's 3 us on the host)
   const int blocks = v_pad <= (team ? 256 : 4096) ? 1 : hd_blocks(team ? v_pad * 32 : v_pad, HD_SUM_BLOCKS / 148);
   if (team)
     head_merge_kernel<32><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, a.hit, f.sums, a.total,
