@@ -58,8 +58,14 @@ struct HeadParams {
   CUtensorMap mapO;                        // both: dX
   const int* coly;      // DW: label (-1: none)
   const float* roww;    // DW: class weight of a row, or null
-  const float* rowg;    // DX, both: g of a voxel
-  const uint32_t* colhit;  // both: label of a column (16 bits), p - 1 of it (bf16)
+  const float* rowg;    // DX: g of a voxel
+  // both: a column's label (16 bits, all ones: it takes no part) and p - 1 of it (bf16); its log2 of the sum of
+  // exponentials; dL, the loss's denominator and where their quotient goes
+  const uint32_t* colhit;
+  const float* lse2;
+  const float* gout;
+  const float* den;
+  float* scale;
   const int* rowy;      // ROWS / DX: label
   float2* part;         // ROWS: [splits, times four with `together` 1][rows padded] running maximum and sum
   float* tl;            // ROWS: [rows padded] s log2(e) at the label
@@ -124,6 +130,17 @@ __device__ __forceinline__ float2 hd_add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+// a number as three bf16 that add up to it (two in the first word, one in the second)
+__device__ __forceinline__ uint2 hd_three(float v) {
+  const __nv_bfloat16 a = __float2bfloat16(v);
+  float rest = v - __bfloat162float(a);
+  if (!isfinite(rest)) rest = 0.f;  // an infinity or a NaN is all in the first
+  const __nv_bfloat16 b = __float2bfloat16(rest), c = __float2bfloat16(rest - __bfloat162float(b));
+  return make_uint2((uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16,
+                    (uint32_t)__bfloat16_as_ushort(c));
+}
+constexpr uint32_t HD_ONE = 0x3F80u;  // 1 in bf16
+
 __device__ __forceinline__ float hd_max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -768,7 +785,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
     abort_s = 0;
     mbar_init(&w_full, 1);
     mbar_init(&dw_full, 1);
-    for (int i = 0; i < p.stages; ++i) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 1); }
+    for (int i = 0; i < p.stages; ++i) { mbar_init(&x_full[i], 1 + HB_DX_WARPS); mbar_init(&x_empty[i], 1); }
     for (uint32_t i = 0; i < SB; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], HD_EPI_WARPS / 2); }
     for (uint32_t i = 0; i < PB; ++i) { mbar_init(&p_full[i], HD_EPI_WARPS / 2); mbar_init(&p_empty[i], 2); }
     for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], HB_DX_WARPS); }
@@ -799,10 +816,9 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
       uint32_t st = 0, ph = 0;
       for (int v = blockIdx.x; v < p.col_tiles; v += gridDim.x) {
         if (!mbar_wait(&x_empty[st], ph ^ 1u, abort_flag, p.status, 91)) break;
-        mbar_expect_tx(&x_full[st], tile_bytes);
+        mbar_expect_tx(&x_full[st], box16);
         for (int k = 0; k < p.kboxes; ++k)
           hd_tma_2d(smem_x + st * tile_bytes + k * HD_BOX, &p.mapQ, &x_full[st], k * 64, v * HD_TILE);
-        hd_tma_2d(smem_x + st * tile_bytes + box16, &p.mapQ16, &x_full[st], 0, v * HD_TILE);
         if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
       }
     }
@@ -883,16 +899,43 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
       if (++ab == naccs) { ab = 0; aph ^= 1u; }
     }
   } else if (warp >= HB_FIRST_EPI + HD_EPI_WARPS) {
-    // dX of a finished voxel tile, a row per thread; each warp stores its 32 rows
-    const int quad = warp & 3;
+    // A thread has a row of voxels: it writes the row's sixteen columns more when a stage is free, and takes dX of a
+    // finished voxel tile; each warp stores its 32 rows.
+    const int quad = warp & 3, row = quad * 32 + lane;
     const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + ACC_X;
     uint8_t* stage = smem_o + quad * p.kboxes * 4096;
-    uint32_t ab = 0, aph = 0;
-    const float* gp = p.rowg + quad * 32 + lane;
-    float g_next = __ldg(gp + (long long)blockIdx.x * HD_TILE);
-    for (int v = blockIdx.x; v < p.col_tiles; v += gridDim.x) {
-      const float g = g_next;
-      if (v + (int)gridDim.x < p.col_tiles) g_next = __ldg(gp + ((long long)v + gridDim.x) * HD_TILE);
+    const float k = __ldg(p.gout) / __ldg(p.den);
+    if (blockIdx.x == 0 && row == 0) p.scale[0] = k;
+    uint32_t ab = 0, aph = 0, st = 0, ph = 0;
+    int ahead = blockIdx.x;  // the next voxel tile whose columns are written; what they are of is read one more ahead
+    float lse_next = __ldg(p.lse2 + (long long)ahead * HD_TILE + row);
+    uint32_t hit_next = __ldg(p.colhit + (long long)ahead * HD_TILE + row);
+    auto columns = [&]() -> bool {
+      const float l = lse_next;
+      const bool live = (hit_next & 0xFFFFu) != 0xFFFFu;
+      ahead += gridDim.x;
+      if (ahead < p.col_tiles) {
+        lse_next = __ldg(p.lse2 + (long long)ahead * HD_TILE + row);
+        hit_next = __ldg(p.colhit + (long long)ahead * HD_TILE + row);
+      }
+      if (!hd_wait(&x_empty[st], ph ^ 1u, abort_flag, p.status, 91)) return false;
+      const uint2 c = hd_three(live ? -l * HD_LN2 : HD_LOWEST);
+      const uint32_t at = smem_u32(smem_x) + st * tile_bytes + box16 + row * 32;
+      const uint32_t second = (row >> 2) & 1;  // (32-byte rows, halves exchanged in every second group of four)
+      hd_sts4(at + 16 * second, HD_ONE | HD_ONE << 16, HD_ONE | c.x << 16, c.x >> 16 | c.y << 16, 0u);
+      hd_sts4(at + 16 * (second ^ 1u), 0u, 0u, 0u, 0u);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&x_full[st]);
+      if (++st == (uint32_t)p.stages) { st = 0; ph ^= 1u; }
+      return true;
+    };
+    bool ok = true;
+    for (int i = 0; i < p.stages && ahead < p.col_tiles && ok; ++i) ok = columns();
+    uint32_t out_next = __ldg(p.colhit + (long long)blockIdx.x * HD_TILE + row);
+    for (int v = blockIdx.x; v < p.col_tiles && ok; v += gridDim.x) {
+      const float g = (out_next & 0xFFFFu) != 0xFFFFu ? k : 0.f;
+      if (v + (int)gridDim.x < p.col_tiles) out_next = __ldg(p.colhit + ((long long)v + gridDim.x) * HD_TILE + row);
       if (!hd_wait(&acc_full[ab], aph, abort_flag, p.status, 97)) break;
       tc_fence_after();
       if (lane == 0) bulk_wait_read_all();  // the last rows have left
@@ -924,6 +967,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
         bulk_commit();
       }
       if (++ab == naccs) { ab = 0; aph ^= 1u; }
+      if (ahead < p.col_tiles) ok = columns();
     }
     if (lane == 0) bulk_wait_all();
     __syncwarp();
@@ -1054,17 +1098,6 @@ __device__ __forceinline__ long long hd_label(const void* labels, int kind, long
   if (kind == 4) return reinterpret_cast<const int*>(labels)[i];
   return reinterpret_cast<const long long*>(labels)[i];
 }
-
-// a number as three bf16 that add up to it (two in the first word, one in the second)
-__device__ __forceinline__ uint2 hd_three(float v) {
-  const __nv_bfloat16 a = __float2bfloat16(v);
-  float rest = v - __bfloat162float(a);
-  if (!isfinite(rest)) rest = 0.f;  // an infinity or a NaN is all in the first
-  const __nv_bfloat16 b = __float2bfloat16(rest), c = __float2bfloat16(rest - __bfloat162float(b));
-  return make_uint2((uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16,
-                    (uint32_t)__bfloat16_as_ushort(c));
-}
-constexpr uint32_t HD_ONE = 0x3F80u;  // 1 in bf16
 
 // y[i]: the label, or -1 for a voxel that takes no part (the ignored label; one outside the classes, which is reported)
 // and behind the last voxel; bias2[j] = bias_j log2(e), -inf behind the last class. w16 (narrow heads): a class's sixteen
@@ -1406,9 +1439,10 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
     rc = make_map_bf16(&p.mapR16, dw ? w16 : a.x16, 2, dw ? wk : xv, st16, box16, 32);
     if (rc) return rc;
   }
-  rc = make_map_bf16(&p.mapQ16, dw ? a.x16 : w16, 2, dw ? xv : wk, st16, box16, 32);
-  if (rc) return rc;
-  if (both) {
+  if (!both) {
+    rc = make_map_bf16(&p.mapQ16, dw ? a.x16 : w16, 2, dw ? xv : wk, st16, box16, 32);
+    if (rc) return rc;
+  } else {
     const int boxo[2] = {64, 32};
     rc = make_map_bf16(&p.mapO, a.dx, 2, dv, st, boxo, 128);
     if (rc) return rc;
@@ -1473,10 +1507,20 @@ static long long head_fwd_scratch(const HeadCall& a, HeadFwdScratch& f, void* ba
   f.tl = (float*)take(4 * p.rows_pad);
   return at - (char*)base;
 }
+// both gradients wanted, and one kernel makes them
+static bool at_once(const HeadCall& a) {
+  return !wide(a) && a.dx != nullptr && (a.dw != nullptr || a.db != nullptr) && head_both(a);
+}
 static long long head_bwd_scratch(HeadCall& a, void* base) {
   char* at = (char*)base;
   auto take = [&](long long bytes) { char* o = at; at += (bytes + 255) / 256 * 256; return o; };
   a.scale = (float*)take(4);
+  if (at_once(a)) {
+    HeadParams p;
+    head_geometry(a, HEAD_BOTH, p);
+    a.scratch = (float*)at;
+    return at - (char*)base + 4 * p.splits * p.rows_pad * (p.cpad + 1);
+  }
   a.g = (float*)take(4 * hd_pad(a.V));
   if (wide(a)) {
     a.u = (float*)take(4 * hd_pad(a.V));
@@ -1490,12 +1534,7 @@ static long long head_bwd_scratch(HeadCall& a, void* base) {
   head_geometry(a, HEAD_DX, p);
   const long long dx = p.splits == 1 ? 0 : p.splits * p.rows_pad * p.cpad;
   head_geometry(a, HEAD_DW, p);
-  long long dw = p.splits * p.rows_pad * (p.cpad + 4);
-  if (head_both(a)) {
-    head_geometry(a, HEAD_BOTH, p);
-    const long long both = p.splits * p.rows_pad * (p.cpad + 4);
-    if (both > dw) dw = both;
-  }
+  const long long dw = p.splits * p.rows_pad * (p.cpad + 4);
   return at - (char*)base + 4 * (dx > dw ? dx : dw);
 }
 
@@ -1517,10 +1556,13 @@ static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
   HeadParams p;
   int rc = 0;
   const bool few = a.V <= HD_FEW;
-  if (a.dx != nullptr && (a.dw != nullptr || a.db != nullptr) && head_both(a)) {
+  if (at_once(a)) {
     head_geometry(a, HEAD_BOTH, p);
-    p.rowg = a.g;
     p.colhit = a.hit;
+    p.lse2 = a.lse2;
+    p.gout = a.gout;
+    p.den = a.den;
+    p.scale = a.scale;
     p.out = a.dx;
     p.ws = a.scratch;
     p.ws_b = a.scratch + p.splits * p.rows_pad * p.cpad;
@@ -1560,15 +1602,17 @@ static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
 
 using namespace sb;
 
-// bytes of the state (0) and of the scratch of the forward (1) and the backward pass (2); -1: outside the range
+// bytes of the state (0) and of the scratch of the forward (1) and the backward pass (2: one gradient, 3: of features and
+// weight or bias); -1: outside the range
 extern "C" long long sb_head_bytes(int what, long long V, int K, int C, int weighted) {
-  if (!shape_ok(V, K, C) || what < 0 || what > 2) return -1;
+  if (!shape_ok(V, K, C) || what < 0 || what > 3) return -1;
   HeadCall a;
   memset(&a, 0, sizeof(a));
   a.V = V;
   a.K = K;
   a.C = C;
   a.cw = weighted ? (const float*)1 : nullptr;  // looked at, not followed
+  if (what == 3) { a.dx = (__nv_bfloat16*)1; a.dw = (void*)1; }
   HeadFwdScratch f;
   return what == 0 ? head_state(a, nullptr) : what == 1 ? head_fwd_scratch(a, f, nullptr) : head_bwd_scratch(a, nullptr);
 }
@@ -1696,9 +1740,12 @@ extern "C" int sb_head_backward(const void* x, const void* w, const float* cw, l
   a.dw = dw; a.dw_kind = dw_kind;
   a.db = db; a.db_kind = db_kind;
   head_state(a, state);
+  a.gout = gout;
   head_bwd_scratch(a, scratch);
-  const long long v_pad = hd_pad(V);
-  head_weights_kernel<<<hd_blocks(v_pad, 8), 256, 0, stream>>>(a, gout, v_pad);
-  sb_count_launch(1);
+  if (!at_once(a)) {
+    const long long v_pad = hd_pad(V);
+    head_weights_kernel<<<hd_blocks(v_pad, 8), 256, 0, stream>>>(a, gout, v_pad);
+    sb_count_launch(1);
+  }
   return wide(a) ? head_wide_backward(a, stream) : head_narrow_backward(a, stream);
 }

@@ -33,6 +33,7 @@ struct HeadCall {
   uint4* w16;     // narrow heads, classes, twice: sixteen columns more of w
   uint32_t* hit;  // voxels, for both gradients at once (head_both): label (16 bits) and p - 1 of it (bf16)
   // of the backward pass
+  const float* gout;  // [1] dL
   float* scale;   // [1] dL / den
   float* g;       // voxels: scale u, u the class weight of the label, 0 where a voxel takes no part
   uint4* x16;     // narrow heads, voxels: sixteen columns more of x

@@ -45,8 +45,8 @@ def head_supported(width: int) -> bool:
 
 @functools.lru_cache(maxsize=256)
 def _bytes(v: int, k: int, c: int, weighted: bool):
-    """Bytes of the state, of the forward pass's scratch and of the backward pass's."""
-    out = tuple(_lib.lib().sb_head_bytes(what, v, k, c, weighted) for what in range(3))
+    """Bytes of the state, of the forward pass's scratch and of the backward pass's: for one gradient, for both."""
+    out = tuple(_lib.lib().sb_head_bytes(what, v, k, c, weighted) for what in range(4))
     if min(out) < 0:
         raise _lib.NativeError(f"sb_head_bytes refused {v} voxels, {k} classes, width {c}")
     return out
@@ -60,7 +60,7 @@ class _HeadLossFn(torch.autograd.Function):
         w16 = weight if weight.dtype == torch.bfloat16 else weight.to(torch.bfloat16)
         v, c = x.shape
         k = w16.shape[0]
-        n_state, n_scratch, _ = _bytes(v, k, c, cw is not None)
+        n_state, n_scratch, *_ = _bytes(v, k, c, cw is not None)
         state = x.new_empty(n_state, dtype=torch.uint8)
         scratch = state.new_empty(n_scratch)
         loss = x.new_empty((), dtype=torch.float32)
@@ -90,7 +90,7 @@ class _HeadLossFn(torch.autograd.Function):
             dx = torch.empty_like(x) if want_x else None
             dw = torch.empty_like(w16, dtype=w_type) if want_w else None
             db = w16.new_empty(k, dtype=b_type) if want_b else None
-            scratch = state.new_empty(_bytes(v, k, c, cw is not None)[2])
+            scratch = state.new_empty(_bytes(v, k, c, cw is not None)[3 if want_x and (want_w or want_b) else 2])
             _lib.check(_lib.lib().sb_head_backward(
                 x.data_ptr(), w16.data_ptr(), _lib.ptr(cw), v, k, c, state.data_ptr(), scratch.data_ptr(), gout.data_ptr(),
                 _lib.ptr(dx), _lib.ptr(dw), _KIND[w_type], _lib.ptr(db), _KIND[b_type] if want_b else 0,
