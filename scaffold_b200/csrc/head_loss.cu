@@ -69,6 +69,12 @@ struct HeadParams {
   const int* rowy;      // ROWS / DX: label
   float2* part;         // ROWS: [splits, times four with `together` 1][rows padded] running maximum and sum
   float* tl;            // ROWS: [rows padded] s log2(e) at the label
+  // ROWS, `whole`: a thread has all of a row, so what head_merge_kernel would make of it is made here (and cw, or null)
+  int whole;
+  float* lse2_out;
+  uint32_t* hit_out;    // or null
+  const float* cw;
+  double* sums;         // [CTAs][2]
   __nv_bfloat16* out;   // DX with one split: [rows][C]
   float* ws;            // DX / DW: [splits][rows padded][cpad]
   float* ws_b;          // DW: [4 splits][rows padded]
@@ -165,11 +171,48 @@ __device__ __forceinline__ void hd_first_mma(uint32_t d, uint32_t r, uint32_t r1
   }
 }
 
+struct HeadSum {
+  double num, den;
+};
+// the sums over a block's warps, in thread 0; all its threads take part
+template <int WARPS>
+__device__ __forceinline__ HeadSum hd_block_sum(HeadSum a) {
+  __shared__ double s_n[WARPS], s_d[WARPS];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.num += __shfl_xor_sync(0xffffffffu, a.num, o);
+    a.den += __shfl_xor_sync(0xffffffffu, a.den, o);
+  }
+  if ((threadIdx.x & 31) == 0) { s_n[threadIdx.x >> 5] = a.num; s_d[threadIdx.x >> 5] = a.den; }
+  __syncthreads();
+  HeadSum t{0.0, 0.0};
+  if (threadIdx.x == 0)
+    for (int w = 0; w < WARPS; ++w) { t.num += s_n[w]; t.den += s_d[w]; }
+  return t;
+}
+
+// A voxel's log2 of the sum of exponentials, from maximum (log2) and sum; u nll and u are added, and the label's p - 1 and
+// the label go to `hit`. i < V; y -1: takes no part.
+__device__ __forceinline__ float hd_voxel(float m2, float sum, float tl, int y, const float* cw, HeadSum& a, uint32_t& hit) {
+  const float l = m2 < 0.1f * HD_LOWEST ? NAN : m2 + log2f(sum);  // every class is off: 0 / 0
+  hit = 0xFFFFu;
+  if (y >= 0) {
+    const float u = cw == nullptr ? 1.f : cw[y], t = l - tl;
+    a.num += (double)u * ((double)t * (double)HD_LN2);
+    a.den += (double)u;
+    hit = (uint32_t)__bfloat16_as_ushort(__float2bfloat16(expm1f(-t * HD_LN2))) << 16 | ((uint32_t)y & 0xFFFFu);
+  }
+  return l;
+}
+
 // Log-sum-exp of the rows (or ARG: their largest logit). Tensor memory holds four tiles of s, one for each epilogue group.
 //   together = 4: a job is four row tiles by a run of column tiles; group g has row tile g all along, so a column tile is
 //                 loaded once for 512 rows and a row's statistics stay in one thread: nothing is merged in the CTA
 //   together = 1: a job is one row tile; group g takes every fourth column tile and leaves statistics of its own
 // The second one is for calls that have no four row tiles for every SM, and for tiles of which shared memory holds few.
+// `whole`: four row tiles and all columns in a job, so a thread ends with all of a row and makes the voxel's term of the loss
+// and what the backward pass needs itself; else head_merge_kernel does, from the shares (2 x 128^3 voxels, 16 channels, 34
+// classes: 136 instead of 215 us; 16^3: 14 instead of 25).
 // Row tiles come in twice the number of a job, so that the next job's are there when this one ends (485 -> 427 us for the
 // whole loss below). Bound: the exponential unit, 1024 clocks a tile of 128 x 128, at long runs of columns (75 % of it at
 // 500 classes), and between jobs the way of a tile through tensor memory. 2 x 128^3 voxels, 64 channels and 257 classes: 381
@@ -226,6 +269,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
   const int last_cols = ((int)(p.cols - (long long)(p.col_tiles - 1) * HD_TILE) + 31) & ~31;
   auto cols_of = [&](int t) -> int { return t + 1 < p.col_tiles ? HD_TILE : last_cols; };  // up to a multiple of 32
 
+  HeadSum total{0.0, 0.0};
   if (warp == 0) {
     if (lane == 0) {
       tma_prefetch_desc(&p.mapR);
@@ -393,13 +437,24 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
           }
         }
       }
-      if (ok && r < p.rows_pad) {
+      if (!ARG && p.whole) {
+        if (ok && r < p.rows_pad) {
+          uint32_t hit = 0xFFFFu;
+          p.lse2_out[r] = r < p.rows ? hd_voxel(m * HD_LOG2E, s, tl * HD_LOG2E, y, p.cw, total, hit) : INFINITY;
+          if (p.hit_out != nullptr) p.hit_out[r] = hit;
+        }
+      } else if (ok && r < p.rows_pad) {
         p.part[(long long)slot * p.rows_pad + r] = ARG ? make_float2(m, __int_as_float(best)) : make_float2(m * HD_LOG2E, s);
         if (!ARG && met) p.tl[r] = tl * HD_LOG2E;
       }
     }
   }
 
+  if (!ARG && p.whole) {
+    __syncwarp();
+    total = hd_block_sum<HD_THREADS / 32>(total);
+    if (threadIdx.x == 0) { p.sums[2 * blockIdx.x] = total.num; p.sums[2 * blockIdx.x + 1] = total.den; }
+  }
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
@@ -1195,24 +1250,6 @@ __global__ void __launch_bounds__(256) head_arg_kernel(const float2* __restrict_
   }
 }
 
-struct HeadSum {
-  double num, den;
-};
-__device__ __forceinline__ HeadSum hd_block_sum(HeadSum a) {
-  __shared__ double s_n[8], s_d[8];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a.num += __shfl_xor_sync(0xffffffffu, a.num, o);
-    a.den += __shfl_xor_sync(0xffffffffu, a.den, o);
-  }
-  if ((threadIdx.x & 31) == 0) { s_n[threadIdx.x >> 5] = a.num; s_d[threadIdx.x >> 5] = a.den; }
-  __syncthreads();
-  HeadSum t{0.0, 0.0};
-  if (threadIdx.x == 0)
-    for (int w = 0; w < 8; ++w) { t.num += s_n[w]; t.den += s_d[w]; }
-  return t;
-}
-
 // loss = num / max(den, eps), den the clamped denominator
 __device__ __forceinline__ void hd_loss(const HeadSum& a, double* total, float* loss, float* den) {
   const double eps = 1.1920928955078125e-7, d = a.den < eps ? eps : a.den;  // NaN stays
@@ -1238,22 +1275,14 @@ __global__ void __launch_bounds__(256) head_merge_kernel(const float2* __restric
     uint32_t h = 0xFFFFu;
     if (i < V) {  // (the same in a team's lanes)
       const float2 e = hd_merge_sums<TEAM>(part, shares, v_pad, i, lane);
-      l = e.x < 0.1f * HD_LOWEST ? NAN : e.x + log2f(e.y);  // every class is off: 0 / 0
-      const int c = y[i];
-      if (c >= 0 && lane == 0) {
-        const float u = cw == nullptr ? 1.f : cw[c];
-        const float t = l - tl[i];
-        a.num += (double)u * ((double)t * (double)HD_LN2);
-        a.den += (double)u;
-        h = (uint32_t)__bfloat16_as_ushort(__float2bfloat16(expm1f(-t * HD_LN2))) << 16 | (uint32_t)c;
-      }
+      if (lane == 0) l = hd_voxel(e.x, e.y, tl[i], y[i], cw, a, h);
     }
     if (lane == 0) {
       lse2[i] = l;
       if (hit != nullptr) hit[i] = h;
     }
   }
-  a = hd_block_sum(a);
+  a = hd_block_sum<8>(a);
   if (threadIdx.x == 0) {
     if (gridDim.x == 1) hd_loss(a, total, loss, den);
     else { sums[2 * blockIdx.x] = a.num; sums[2 * blockIdx.x + 1] = a.den; }
@@ -1266,7 +1295,7 @@ __global__ void __launch_bounds__(256) head_total_kernel(const double* __restric
                                                          float* __restrict__ den) {
   HeadSum a{0.0, 0.0};
   for (int i = threadIdx.x; i < blocks; i += 256) { a.num += sums[2 * i]; a.den += sums[2 * i + 1]; }
-  a = hd_block_sum(a);
+  a = hd_block_sum<8>(a);
   if (threadIdx.x == 0) hd_loss(a, total, loss, den);
 }
 
@@ -1409,6 +1438,7 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
         p.together = 4;
         p.splits = s4;
         p.tiles_per_split = per4;
+        p.whole = s4 == 1;
       }
     }
     p.rbufs = p.together == 4 ? (p.kboxes == 1 ? 8 : 4) : p.kboxes <= 2 ? 2 : 1;
@@ -1647,8 +1677,19 @@ extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, i
     p.part = f.part;
     p.tl = f.tl;
     p.rowy = a.y;
+    p.lse2_out = a.lse2;
+    p.hit_out = a.hit;
+    p.cw = cw;
+    p.sums = f.sums;
     splits = head_shares(p);
     rc = head_launch<HEAD_ROWS, false>(a, p, stream);
+    if (rc) return rc;
+    if (p.whole) {
+      const int jobs = (p.row_tiles + 3) / 4;
+      head_total_kernel<<<1, 256, 0, stream>>>(f.sums, jobs < 148 ? jobs : 148, a.total, loss, a.den);
+      sb_count_launch(1);
+      return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
+    }
   }
   if (rc) return rc;
   // a warp for a voxel: loss of 300 voxels x 64 channels x 20000 classes 19 us, a thread for each 90; of 40000 x 32 x 1001
