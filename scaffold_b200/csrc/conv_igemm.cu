@@ -479,10 +479,17 @@ int make_map_bf16(CUtensorMap* m, const void* base, int rank, const long long* d
   if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return SB_ERR_ALIGN;
   for (int i = 0; i + 1 < rank; ++i)
     if (gstr[i] % 16 != 0) return SB_ERR_ALIGN;
-  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstr,
-                   bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swz_enum(rowb), CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : SB_ERR_TENSORMAP;
+  auto encode = [&] {
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), gdim, gstr, bx, es,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, swz_enum(rowb), CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  if (encode() == CUDA_SUCCESS) return 0;
+  // a thread that has not used the device yet (autograd's, in a process's first backward pass) has no context: make the
+  // current device's current, which the runtime would do at the thread's first launch
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return SB_ERR_DRIVER;
+  return encode() == CUDA_SUCCESS ? 0 : SB_ERR_TENSORMAP;
 }
 
 static int pow2_floor(int v) {

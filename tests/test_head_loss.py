@@ -1,5 +1,8 @@
 """The cross entropy of a head with many classes, taken from its features: against the definition in 64 bits."""
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -110,6 +113,25 @@ def test_both_gradients_at_once(v, c, k):
     for got, want, size in ((dx1, dx, v ** 0.5 * float(w.double().norm(dim=1).max())),
                             (dw1, dw, float(x.double().norm(dim=1).sum())), (db1, db, v)):
         assert float((got.double() - want.double()).norm()) <= 8e-3 * float(want.double().norm()) + 2 * e * size
+
+
+FIRST = """
+import torch
+from scaffold_b200.ops.head_loss import head_cross_entropy
+x, w = (torch.randn(n, %d, device="cuda").bfloat16().requires_grad_() for n in (4096, %d))
+y = torch.zeros(4096, dtype=torch.int32, device="cuda")
+dx, dw = torch.autograd.grad(head_cross_entropy(x, w, None, y), (x, w))
+assert torch.isfinite(dx.float()).all() and dw.abs().sum() > 0
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c,k", [(16, 34), (64, 1000), (320, 40)])
+def test_the_first_backward_pass_of_a_process(c, k):
+    """autograd's thread has used the device for nothing yet: the first call there is the one under test."""
+    root = Path(__file__).resolve().parents[1]
+    run = subprocess.run([sys.executable, "-c", FIRST % (c, k)], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
 
 
 @pytest.mark.gpu
