@@ -812,8 +812,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
 // the epilogue itself, 16 bytes a row and instruction, kept the shared memory pipe from P's stores (860 us).
 // Bound: neither the exponential unit (1024 clocks a tile of 128 x 128, some 2100 are taken) nor the MMAs or the stores,
 // but a tile's way through them, two tiles at a time: tensor memory holds no third one of s.
-// 2 x 128^3 voxels, 64 channels, 257 classes: 742 us with all that stands around it, the two kernels above 1160; 128
-// classes 368 / 722; 16 channels and 34 classes 302 / 633; 32 channels and 500 classes 982 / 1456.
+// 2 x 128^3 voxels, 64 channels, 257 classes: 690 us with the sums behind it, the two kernels above and what they need 1160;
+// 128 classes 349 / 722; 16 channels and 34 classes 293 / 633; 32 channels and 500 classes 849 / 1456.
 constexpr int HB_FIRST_EPI = 4;
 constexpr int HB_DX_WARPS = 4;  // behind the epilogue's
 constexpr int HB_THREADS = 32 * (HB_FIRST_EPI + HD_EPI_WARPS + HB_DX_WARPS);
