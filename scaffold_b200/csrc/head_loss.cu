@@ -1218,12 +1218,20 @@ __device__ __forceinline__ void hd_merge_best(const float2* part, int shares, lo
 }
 template <int TEAM>
 __device__ __forceinline__ float2 hd_merge_sums(const float2* part, int shares, long long v_pad, long long i, int lane) {
+  constexpr int BATCH = TEAM == 1 ? 4 : 8;  // loads and exponentials that do not wait for one another
   float m = -INFINITY, s = 0.f;
-#pragma unroll 4
-  for (int k = lane; k < shares; k += TEAM) {
-    const float2 e = part[(long long)k * v_pad + i];
-    const float mm = fmaxf(m, e.x), base = mm == -INFINITY ? 0.f : mm;
-    s = s * hd_ex2(m - base) + e.y * hd_ex2(e.x - base);
+  for (int k0 = lane; k0 < shares; k0 += BATCH * TEAM) {
+    float2 e[BATCH];
+    float mm = m;
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      e[j] = k0 + j * TEAM < shares ? part[(long long)(k0 + j * TEAM) * v_pad + i] : make_float2(-INFINITY, 0.f);
+      mm = fmaxf(mm, e[j].x);
+    }
+    const float base = mm == -INFINITY ? 0.f : mm;
+    s *= hd_ex2(m - base);
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) s += e[j].y * hd_ex2(e[j].x - base);
     m = mm;
   }
 #pragma unroll
