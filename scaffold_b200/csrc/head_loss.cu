@@ -83,6 +83,9 @@ struct HeadParams {
   int C, cpad, kboxes, ksteps;
   int row_tiles, col_tiles, splits, tiles_per_split;
   int stages, rbufs, bufs, accs;
+  int row0;             // both: first class of this launch
+  float4* part_x;       // both: dX of the launches so far, [voxel tiles][cpad / 4][128]
+  int first, last;      // both: nothing to add, nothing to keep
   int together;         // ROWS: row tiles of a job, 4 or 1
 };
 
@@ -799,7 +802,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
 }
 
 // Both gradients from one matrix P^T = p - [j = y], rows = classes, columns = voxels (unweighted calls whose weight and
-// whose dW fit into a CTA). A CTA keeps all tiles of W in shared memory and dW's sums in tensor memory and walks tiles of
+// whose dW fit into a CTA, or a part of them at a time: head_both). A CTA keeps all tiles of W in shared memory and dW's sums in tensor memory and walks tiles of
 // 128 voxels; of each 128 x 128 tile of s^T the epilogue makes a tile of P^T in shared memory, [class][voxel], and two
 // MMAs read it from there: dW += P^T X with the voxels along the reduction (K-major A), dX += P W with the classes along
 // it (the same bytes as an MN-major A). An exponential serves both gradients, X is read once, and in shared memory the
@@ -865,8 +868,8 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
       mbar_expect_tx(&w_full, kt * tile_bytes);
       for (int i = 0; i < kt; ++i) {
         for (int k = 0; k < p.kboxes; ++k)
-          hd_tma_2d(smem_w + i * tile_bytes + k * HD_BOX, &p.mapR, &w_full, k * 64, i * HD_TILE);
-        hd_tma_2d(smem_w + i * tile_bytes + box16, &p.mapR16, &w_full, 0, i * HD_TILE);
+          hd_tma_2d(smem_w + i * tile_bytes + k * HD_BOX, &p.mapR, &w_full, k * 64, p.row0 + i * HD_TILE);
+        hd_tma_2d(smem_w + i * tile_bytes + box16, &p.mapR16, &w_full, 0, p.row0 + i * HD_TILE);
       }
       uint32_t st = 0, ph = 0;
       for (int v = blockIdx.x; v < p.col_tiles; v += gridDim.x) {
@@ -1004,6 +1007,26 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
           __syncwarp();
           if (lane == 0) mbar_arrive(&acc_empty[ab]);
         }
+        if (!p.first || !p.last) {
+          float4* at = p.part_x + ((long long)v * (p.cpad / 4) + c0 / 4) * HD_TILE + quad * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (c0 + 4 * j >= p.cpad) break;
+            float4 f = make_float4(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1]), __uint_as_float(u[4 * j + 2]),
+                                   __uint_as_float(u[4 * j + 3]));
+            if (!p.first) {
+              const float4 before = at[j * HD_TILE];
+              f.x += before.x; f.y += before.y; f.z += before.z; f.w += before.w;
+            }
+            if (!p.last) {
+              at[j * HD_TILE] = f;
+            } else {
+              u[4 * j] = __float_as_uint(f.x); u[4 * j + 1] = __float_as_uint(f.y);
+              u[4 * j + 2] = __float_as_uint(f.z); u[4 * j + 3] = __float_as_uint(f.w);
+            }
+          }
+          if (!p.last) continue;
+        }
         // a voxel that takes no part has no gradient, whatever its features hold
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -1017,7 +1040,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
       fence_proxy_async();
       __syncwarp();
       const long long r = (long long)v * HD_TILE + quad * 32;
-      if (lane == 0 && r < p.cols) {
+      if (lane == 0 && r < p.cols && p.last) {
         for (int k = 0; k < p.kboxes; ++k) hd_tma_store_2d(&p.mapO, stage + k * 4096, k * 64, (int)r);
         bulk_commit();
       }
@@ -1087,7 +1110,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
               hd_sts4((out + swz) ^ (c0 / 8 + j) << 4, u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
             __syncwarp();  // rows before single entries
             // lane c has the label of column c: a row's targets are the columns whose label has the row's five bits
-            const int rel = (int)(hit[c0 / 32] & 0xFFFFu) - (i * HD_TILE + quad * 32);
+            const int rel = (int)(hit[c0 / 32] & 0xFFFFu) - (p.row0 + i * HD_TILE + quad * 32);
             uint32_t hits = __ballot_sync(0xffffffffu, (unsigned)rel < 32u);
             if (hits != 0u) {
 #pragma unroll
@@ -1401,13 +1424,25 @@ static void head_split(int row_tiles, int col_tiles, int* splits, int* tps) {
 static bool wide(const HeadCall& a) { return a.C > HD_MAX_C; }
 constexpr int HD_BOXES = 54;  // of HD_BOX16 in shared memory; a tile of rows or columns is 4 kboxes + 1 of them
 
-// Both gradients in one kernel: all of W next to two tiles of P and two of X in shared memory, dW and a dX next to two
-// tiles of s in tensor memory. Few voxels and class weights want P in two parts.
-static bool head_both(const HeadCall& a) {
-  const int cpad = (a.C + 15) / 16 * 16, kboxes = (a.C + 63) / 64;
-  const long long kt = ((long long)a.K + HD_TILE - 1) / HD_TILE;
-  return a.V > HD_FEW && a.cw == nullptr && kt <= 4 && (kt + 1) * cpad <= 256 &&
-         (kt + 2) * (4 * kboxes + 1) + 16 + 4 * kboxes + (kt + 1) / 2 <= HD_BOXES;
+// Class tiles of one launch for both gradients, 0: two kernels. Shared memory holds the W of a launch next to two tiles of P
+// and two of X, tensor memory its dW and a dX next to two tiles of s. Up to 32 channels more classes take several launches,
+// which carry dX on in fp32, where a launch has four tiles, the voxels give every CTA four, and the sums stay about as large
+// as L2. Loss and gradients of 401280 voxels x 32 channels x 1001 classes 366 us, in two kernels 431; 2^18 x 16 x 2000 420 and
+// 514; 2^19 x 24 x 3000 1425 and 1549; but 2^20 x 32 x 600 (three tiles) 701 and 663, 40000 x 32 x 1500 119 and 111, and the
+// gradients alone of 2^20 x 64 x 385 749 where 512 classes take 417 in two kernels. Few voxels and class weights want P in two
+// parts.
+static int head_both(const HeadCall& a) {
+  if (a.V <= HD_FEW || a.cw != nullptr || a.K > 65000) return 0;
+  const int cpad = (a.C + 15) / 16 * 16, kboxes = (a.C + 63) / 64, kt = (a.K + HD_TILE - 1) / HD_TILE;
+  auto fits = [&](int n) {
+    return (n + 1) * cpad <= 256 && (n + 2) * (4 * kboxes + 1) + 16 + 4 * kboxes + (n + 1) / 2 <= HD_BOXES;
+  };
+  int most = 0;
+  while (most < 4 && fits(most + 1)) ++most;
+  if (most >= kt) return kt;
+  if (cpad > 32 || a.V < 4 * 148 * HD_TILE || hd_pad(a.V) * cpad * 4 > (128LL << 20)) return 0;
+  const int launches = (kt + most - 1) / most, each = (kt + launches - 1) / launches;
+  return each == 4 ? 4 : 0;
 }
 
 static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
@@ -1418,6 +1453,7 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
   p.ksteps = p.cpad / 16;
   p.rows = mode >= HEAD_DW ? a.K : a.V;
   p.cols = mode >= HEAD_DW ? a.V : a.K;
+  if (mode == HEAD_BOTH && p.rows > (long long)head_both(a) * HD_TILE) p.rows = (long long)head_both(a) * HD_TILE;  // of a launch
   p.row_tiles = (int)((p.rows + HD_TILE - 1) / HD_TILE);
   p.col_tiles = (int)((p.cols + HD_TILE - 1) / HD_TILE);
   p.rows_pad = hd_pad(p.rows);
@@ -1557,7 +1593,7 @@ static long long head_bwd_scratch(HeadCall& a, void* base) {
     HeadParams p;
     head_geometry(a, HEAD_BOTH, p);
     a.scratch = (float*)at;
-    return at - (char*)base + 4 * p.splits * p.rows_pad * (p.cpad + 1);
+    return at - (char*)base + 4 * (p.splits * p.rows_pad * (p.cpad + 1) + (p.rows < a.K ? hd_pad(a.V) * p.cpad : 0));
   }
   a.g = (float*)take(4 * hd_pad(a.V));
   if (wide(a)) {
@@ -1603,11 +1639,23 @@ static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
     p.scale = a.scale;
     p.out = a.dx;
     p.ws = a.scratch;
-    p.ws_b = a.scratch + p.splits * p.rows_pad * p.cpad;
-    rc = head_launch<HEAD_BOTH, false>(a, p, stream);
-    if (rc) return rc;
-    head_reduce(reduce_of(p.ws, p.splits, p, p.C, p.cpad, a.dw_kind, a.dw),
-                reduce_of(p.ws_b, p.splits, p, 1, 1, a.db_kind, a.db), a.scale, stream);
+    p.ws_b = p.ws + p.splits * p.rows_pad * p.cpad;
+    p.part_x = reinterpret_cast<float4*>(p.ws_b + p.splits * p.rows_pad);
+    const long long most = p.rows;
+    for (long long row0 = 0; row0 < a.K; row0 += most) {
+      p.row0 = (int)row0;
+      p.rows = a.K - row0 < most ? a.K - row0 : most;
+      p.row_tiles = (int)((p.rows + HD_TILE - 1) / HD_TILE);
+      p.first = row0 == 0;
+      p.last = row0 + most >= a.K;
+      rc = head_launch<HEAD_BOTH, false>(a, p, stream);
+      if (rc) return rc;
+      auto from = [&](void* out, int kind, long long i) {
+        return out == nullptr ? nullptr : (void*)((char*)out + i * (kind == 2 ? 4 : 2));
+      };
+      head_reduce(reduce_of(p.ws, p.splits, p, p.C, p.cpad, a.dw_kind, from(a.dw, a.dw_kind, row0 * a.C)),
+                  reduce_of(p.ws_b, p.splits, p, 1, 1, a.db_kind, from(a.db, a.db_kind, row0)), a.scale, stream);
+    }
     return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;
   }
   if (a.dx != nullptr) {

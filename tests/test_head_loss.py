@@ -94,7 +94,8 @@ def test_loss_and_gradients(v, c, k):
 # several launches
 BOTH = [(129, 8, 1), (200, 64, 32), (256, 16, 33), (19000, 64, 128), (38100, 24, 40), (57000, 64, 257), (40000, 32, 500),
         (40000, 128, 100), (19073, 128, 128), (1000, 128, 129), (300, 64, 384), (300, 64, 385), (500, 48, 512),
-        (500, 32, 513), (38017, 40, 130), (20000, 32, 1001), (300, 64, 769), (2000, 16, 1537)]
+        (500, 32, 513), (38017, 40, 130), (20000, 32, 1001), (300, 64, 769), (2000, 16, 1537),
+        (76000, 32, 1001), (80001, 16, 1537), (90000, 24, 513), (76543, 32, 800)]
 
 
 @pytest.mark.gpu
