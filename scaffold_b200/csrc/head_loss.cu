@@ -24,7 +24,7 @@
 // behind it a confident voxel (p near 1) would keep nothing but the rounding of p. Common factors stay out of P, so that
 // a target's entry is near -1 (exact when p is small) instead of -1 / V, whose rounding error all voxels would share.
 // Where one rounding can make up a result (LO: up to HD_FEW voxels; class weights in HEAD_DW, whose rounding the voxels
-// of a class share) P is kept as two bf16, value and remainder, and the second MMA runs once for each.
+// of a class share; head_both_kernel weighs X instead) P is kept as two bf16, value and remainder, and the second MMA runs once for each.
 //
 // Roles: warp 0 loads (TMA), warps 1 and 2 issue MMAs, warps 3-18 are the epilogue, four groups of four warps (a row per
 // thread). All waits are bounded.
@@ -118,6 +118,11 @@ __device__ __forceinline__ void hd_tma_store_2d(const CUtensorMap* m, const void
 __device__ __forceinline__ void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void hd_sts4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float2 hd_lds2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
 }
 __device__ __forceinline__ void hd_sts16(uint32_t at, uint32_t v) {
   asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"((uint16_t)v) : "memory");
@@ -801,8 +806,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
   }
 }
 
-// Both gradients from one matrix P^T = p - [j = y], rows = classes, columns = voxels (unweighted calls whose weight and
-// whose dW fit into a CTA, or a part of them at a time: head_both). A CTA keeps all tiles of W in shared memory and dW's sums in tensor memory and walks tiles of
+// Both gradients from one matrix P^T = p - [j = y], rows = classes, columns = voxels (calls whose weight and whose dW fit
+// into a CTA, or a part of them at a time: head_both). A CTA keeps all tiles of W in shared memory and dW's sums in tensor memory and walks tiles of
 // 128 voxels; of each 128 x 128 tile of s^T the epilogue makes a tile of P^T in shared memory, [class][voxel], and two
 // MMAs read it from there: dW += P^T X with the voxels along the reduction (K-major A), dX += P W with the classes along
 // it (the same bytes as an MN-major A). An exponential serves both gradients, X is read once, and in shared memory the
@@ -813,19 +818,25 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_grad_kernel(const __grid_c
 // out of one warp 492 instead of 424 us at 128 classes, below), four groups of the epilogue (two take a tile's halves, by
 // tile parity), and the last four warps take dX out of tensor memory, scale it and store it by TMA: row pieces stored by
 // the epilogue itself, 16 bytes a row and instruction, kept the shared memory pipe from P's stores (860 us).
+// WEIGHTED: P stays without the weights u, for dX, whose rows take g = k u at the end; for dW the last four warps put u X in
+// the place of X as soon as the last product of s has read it. Its rounding goes by the feature, so the voxels of a class do
+// not share it (u P would be off by the same for all of a class's targets), and db takes u in fp32.
 // Bound: neither the exponential unit (1024 clocks a tile of 128 x 128, some 2100 are taken) nor the MMAs or the stores,
 // but a tile's way through them, two tiles at a time: tensor memory holds no third one of s.
 // 2 x 128^3 voxels, 64 channels, 257 classes: 690 us with the sums behind it, the two kernels above and what they need 1160;
-// 128 classes 349 / 722; 16 channels and 34 classes 293 / 633; 32 channels and 500 classes 849 / 1456.
+// 128 classes 349 / 722; 16 channels and 34 classes 293 / 633; 32 channels and 500 classes 849 / 1456. Loss and gradients
+// with class weights, in this kernel and in two: 64^3 x 64 x 147 92 / 113, 2 x 128^3 x 64 x 257 1510 / 1675, x 16 x 34 721 /
+// 741, x 32 x 500 1829 / 2253.
 constexpr int HB_FIRST_EPI = 4;
 constexpr int HB_DX_WARPS = 4;  // behind the epilogue's
 constexpr int HB_THREADS = 32 * (HB_FIRST_EPI + HD_EPI_WARPS + HB_DX_WARPS);
+template <bool WEIGHTED>
 __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_constant__ HeadParams p) {
   constexpr uint32_t SB = 2, PB = 2;  // tiles of s in tensor memory and of P in shared memory: one for each pair of groups
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t w_full, x_full[HD_MAX_STAGES], x_empty[HD_MAX_STAGES], s_full[SB], s_empty[SB], p_full[PB],
-      p_empty[PB], acc_full[2], acc_empty[2], dw_full;
+      p_empty[PB], acc_full[2], acc_empty[2], dw_full, s_last[HD_MAX_STAGES], u_full[HD_MAX_STAGES];
   __shared__ uint32_t tmem_base_s, abort_s;
   volatile uint32_t* abort_flag = &abort_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -838,17 +849,22 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
   uint8_t* smem_x = smem_w + kt * tile_bytes;
   uint8_t* smem_o = smem_x + p.stages * tile_bytes;                     // [dX warps][kboxes][32 rows of 128 bytes]
   float* smem_db = reinterpret_cast<float*>(smem_o + p.kboxes * HD_BOX);  // [kt][groups][128]
+  float* smem_cw = smem_db + kt * 4 * HD_TILE;                            // WEIGHTED: [kt][128], of the classes
+  float* smem_u = smem_cw + kt * HD_TILE;                                 // and [stages][128], of the voxels
 
   if (threadIdx.x == 0) {
     abort_s = 0;
     mbar_init(&w_full, 1);
     mbar_init(&dw_full, 1);
     for (int i = 0; i < p.stages; ++i) { mbar_init(&x_full[i], 1 + HB_DX_WARPS); mbar_init(&x_empty[i], 1); }
+    for (int i = 0; WEIGHTED && i < p.stages; ++i) { mbar_init(&s_last[i], 1); mbar_init(&u_full[i], HB_DX_WARPS); }
     for (uint32_t i = 0; i < SB; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], HD_EPI_WARPS / 2); }
     for (uint32_t i = 0; i < PB; ++i) { mbar_init(&p_full[i], HD_EPI_WARPS / 2); mbar_init(&p_empty[i], 2); }
     for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], HB_DX_WARPS); }
     mbar_fence_init();
   }
+  if (WEIGHTED)
+    for (int i = threadIdx.x; i < kt * HD_TILE; i += HB_THREADS) smem_cw[i] = i < p.rows ? __ldg(p.cw + i) : 0.f;
   if (warp == 0) {
     tmem_alloc(&tmem_base_s, 512);
     tmem_relinquish();
@@ -894,6 +910,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
           const uint32_t r = w0 + i * tile_bytes, q = x0 + st * tile_bytes;
           hd_first_mma(tmem + b * HD_TILE, r, r + box16, q, q + box16, HD_TILE, p.ksteps);
           tc_commit(&s_full[b]);
+          if (WEIGHTED && i + 1 == kt) tc_commit(&s_last[st]);
         }
         __syncwarp();
         if (++b == SB) { b = 0; bph ^= 1u; }
@@ -908,8 +925,8 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
     uint32_t st = 0, ph = 0, pb = 0, pph = 0;
     bool ok = true;
     for (int v = blockIdx.x; v < p.col_tiles && ok; v += gridDim.x) {
-      // (the first issuing warp has waited for the loads; this one has to see them too)
-      if (!hd_wait(&x_full[st], ph, abort_flag, p.status, 95)) { ok = false; break; }
+      // (the first issuing warp has waited for the loads; this one has to see them too, or their weighting)
+      if (!hd_wait(WEIGHTED ? &u_full[st] : &x_full[st], ph, abort_flag, p.status, 95)) { ok = false; break; }
       const uint32_t x_lo = desc_lo(x0 + st * tile_bytes, lbo);
       for (int i = 0; i < kt; ++i) {
         if (!hd_wait(&p_full[pb], pph, abort_flag, p.status, 93)) { ok = false; break; }
@@ -970,14 +987,17 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
     uint32_t hit_next = __ldg(p.colhit + (long long)ahead * HD_TILE + row);
     auto columns = [&]() -> bool {
       const float l = lse_next;
-      const bool live = (hit_next & 0xFFFFu) != 0xFFFFu;
+      const uint32_t label = hit_next & 0xFFFFu;
+      const bool live = label != 0xFFFFu;
+      const float u = WEIGHTED && live ? smem_cw[label] : 0.f;
       ahead += gridDim.x;
       if (ahead < p.col_tiles) {
         lse_next = __ldg(p.lse2 + (long long)ahead * HD_TILE + row);
         hit_next = __ldg(p.colhit + (long long)ahead * HD_TILE + row);
       }
       if (!hd_wait(&x_empty[st], ph ^ 1u, abort_flag, p.status, 91)) return false;
-      const uint2 c = hd_three(live ? -l * HD_LN2 : HD_LOWEST);
+      const uint2 c = hd_three(live && (!WEIGHTED || u != 0.f) ? -l * HD_LN2 : HD_LOWEST);
+      if (WEIGHTED) smem_u[st * HD_TILE + row] = u;  // (the epilogue is done with the stage's last one: its dX is out)
       const uint32_t at = smem_u32(smem_x) + st * tile_bytes + box16 + row * 32;
       const uint32_t second = (row >> 2) & 1;  // (32-byte rows, halves exchanged in every second group of four)
       hd_sts4(at + 16 * second, HD_ONE | HD_ONE << 16, HD_ONE | c.x << 16, c.x >> 16 | c.y << 16, 0u);
@@ -990,10 +1010,35 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
     };
     bool ok = true;
     for (int i = 0; i < p.stages && ahead < p.col_tiles && ok; ++i) ok = columns();
-    uint32_t out_next = __ldg(p.colhit + (long long)blockIdx.x * HD_TILE + row);
+    uint32_t out_next = WEIGHTED ? 0u : __ldg(p.colhit + (long long)blockIdx.x * HD_TILE + row);
+    uint32_t wst = 0, wph = 0;
     for (int v = blockIdx.x; v < p.col_tiles && ok; v += gridDim.x) {
-      const float g = (out_next & 0xFFFFu) != 0xFFFFu ? k : 0.f;
-      if (v + (int)gridDim.x < p.col_tiles) out_next = __ldg(p.colhit + ((long long)v + gridDim.x) * HD_TILE + row);
+      float g;
+      if (WEIGHTED) {
+        // u X in the place of X, as soon as the last product of s has read it
+        const float u = smem_u[wst * HD_TILE + row];
+        g = u == 0.f ? 0.f : k * u;
+        if (!(hd_wait(&x_full[wst], wph, abort_flag, p.status, 95) &&
+              hd_wait(&s_last[wst], wph, abort_flag, p.status, 93))) { ok = false; break; }
+#pragma unroll 4
+        for (int c = 0; c < p.cpad / 8; ++c) {
+          uint4* at = reinterpret_cast<uint4*>(smem_x + wst * tile_bytes + (c >> 3) * HD_BOX + row * 128 +
+                                               (((c & 7) ^ (row & 7)) << 4));
+          uint4 x = *at;
+          uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            w[j] = u == 0.f ? 0u : pack_bf16x2(__uint_as_float(w[j] << 16) * u, __uint_as_float(w[j] & 0xFFFF0000u) * u);
+          *at = x;
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&u_full[wst]);
+        if (++wst == (uint32_t)p.stages) { wst = 0; wph ^= 1u; }
+      } else {
+        g = (out_next & 0xFFFFu) != 0xFFFFu ? k : 0.f;
+        if (v + (int)gridDim.x < p.col_tiles) out_next = __ldg(p.colhit + ((long long)v + gridDim.x) * HD_TILE + row);
+      }
       if (!hd_wait(&acc_full[ab], aph, abort_flag, p.status, 97)) break;
       tc_fence_after();
       if (lane == 0) bulk_wait_read_all();  // the last rows have left
@@ -1057,6 +1102,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
     const uint32_t swz = row * 128 + ((row & 7) << 4);  // the row's first 16 bytes of voxels in a 128-byte swizzled box
     const uint32_t s_tile = lane_base + par * HD_TILE + half * 64;
     uint32_t ph = 0, tc = 0;
+    uint32_t st = kt == 1 ? par : 0u, xph = 0;  // WEIGHTED: stage of the voxel tile (there are two or more)
     bool ok = true;
     float* const db = smem_db + group * HD_TILE + row;  // this thread's alone
     for (int i = 0; i < kt; ++i) db[i * 4 * HD_TILE] = 0.f;
@@ -1070,6 +1116,12 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
       if (v + step < p.col_tiles) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + (long long)step * HD_TILE));
       int i = kt == 1 ? 0 : (int)((tc ^ par) & 1u);
       tc += kt;
+      const uint32_t us = smem_u32(smem_u) + (st * HD_TILE + half * 64) * 4;
+      if (WEIGHTED) {
+        ok = hd_wait(&x_full[st], xph, abort_flag, p.status, 95);  // the weights of its columns are there
+        st += kt == 1 ? 2u : 1u;
+        if (st >= (uint32_t)p.stages) { st -= p.stages; xph ^= 1u; }
+      }
       for (; i < kt && ok; i += 2) {
         if (!hd_wait(&s_full[par], ph, abort_flag, p.status, 98)) { ok = false; break; }
         tc_fence_after();
@@ -1078,36 +1130,46 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
         const bool live = quad * 32 < rows_of(i);
 #pragma unroll
         for (int c0 = 0; c0 < 64; c0 += 32) {
-          uint32_t u[32];
-          if (live) {
-            tmem_ld_32x32(s_tile + c0, u);
-            tmem_ld_wait();
-          }
-          if (c0 == 32) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[par]);
-          }
-          if (live) {
-            float2 d[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          // WEIGHTED: 16 columns at a time, for their weights' registers (80 bytes spilled otherwise: 1789 us instead of 1510
+          // for the loss and gradients of 2 x 128^3 voxels x 64 channels x 257 classes; without weights 1094 instead of 1072)
+          constexpr int CH = WEIGHTED ? 16 : 32;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float2 f = hd_fma2(make_float2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])),
-                                 make_float2(HD_LOG2E, HD_LOG2E), make_float2(0.f, 0.f));
-              f.x = hd_ex2(f.x);
-              f.y = hd_ex2(f.y);
-              d[j & 1] = hd_add2(d[j & 1], f);
-              u[j] = pack_bf16x2(f.x, f.y);
+          for (int c1 = c0; c1 < c0 + 32; c1 += CH) {
+            uint32_t u[CH];
+            if (live) {
+              if constexpr (WEIGHTED) tmem_ld_32x16(s_tile + c1, u);
+              else tmem_ld_32x32(s_tile + c1, u);
+              tmem_ld_wait();
             }
-            d[0] = hd_add2(d[0], d[1]);
-            sum += d[0].x + d[0].y;
-          }
-          // the buffer is free: both products of its last tile are done
-          if (c0 == 0) ok = hd_wait(&p_empty[par], ph ^ 1u, abort_flag, p.status, 96);
-          if (live) {
+            if (c1 + CH == 64) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s_empty[par]);
+            }
+            if (live) {
+              float2 d[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              hd_sts4((out + swz) ^ (c0 / 8 + j) << 4, u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+              for (int j = 0; j < CH / 2; ++j) {
+                float2 f = hd_fma2(make_float2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])),
+                                   make_float2(HD_LOG2E, HD_LOG2E), make_float2(0.f, 0.f));
+                f.x = hd_ex2(f.x);
+                f.y = hd_ex2(f.y);
+                if constexpr (WEIGHTED) d[j & 1] = hd_fma2(f, hd_lds2(us + (c1 + 2 * j) * 4), d[j & 1]);
+                else d[j & 1] = hd_add2(d[j & 1], f);
+                u[j] = pack_bf16x2(f.x, f.y);
+              }
+              d[0] = hd_add2(d[0], d[1]);
+              sum += d[0].x + d[0].y;
+            }
+            // the buffer is free: both products of its last tile are done
+            if (c1 == 0) ok = hd_wait(&p_empty[par], ph ^ 1u, abort_flag, p.status, 96);
+            if (live) {
+#pragma unroll
+              for (int j = 0; j < CH / 8; ++j)
+                hd_sts4((out + swz) ^ (c1 / 8 + j) << 4, u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+            }
+          }
+          if (live) {
             __syncwarp();  // rows before single entries
             // lane c has the label of column c: a row's targets are the columns whose label has the row's five bits
             const int rel = (int)(hit[c0 / 32] & 0xFFFFu) - (p.row0 + i * HD_TILE + quad * 32);
@@ -1115,7 +1177,7 @@ __global__ void __launch_bounds__(HB_THREADS, 1) head_both_kernel(const __grid_c
             if (hits != 0u) {
 #pragma unroll
               for (int k = 0; k < 5; ++k) hits &= __ballot_sync(0xffffffffu, rel >> k & 1) ^ (lane >> k & 1 ? 0u : ~0u);
-              sum -= (float)__popc(hits);
+              sum -= (float)__popc(hits) * (WEIGHTED ? smem_cw[i * HD_TILE + row] : 1.f);
               if ((unsigned)rel < 32u) {
                 const int c = c0 + lane, r = quad * 32 + rel;
                 hd_sts16(out + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2, hit[c0 / 32] >> 16);
@@ -1429,18 +1491,21 @@ constexpr int HD_BOXES = 54;  // of HD_BOX16 in shared memory; a tile of rows or
 // which carry dX on in fp32, where a launch has four tiles, the voxels give every CTA four, and the sums stay about as large
 // as L2. Loss and gradients of 401280 voxels x 32 channels x 1001 classes 366 us, in two kernels 431; 2^18 x 16 x 2000 420 and
 // 514; 2^19 x 24 x 3000 1425 and 1549; but 2^20 x 32 x 600 (three tiles) 701 and 663, 40000 x 32 x 1500 119 and 111, and the
-// gradients alone of 2^20 x 64 x 385 749 where 512 classes take 417 in two kernels. Few voxels and class weights want P in two
-// parts.
+// gradients alone of 2^20 x 64 x 385 749 where 512 classes take 417 in two kernels; class weights 474 and 463 for 401280 x 32 x 1001. Few voxels want P
+// in two parts; with class weights more are few, since the rounding of u X stands next to P's: at 129 voxels, 60 % of them
+// ignored, single elements of dW were off by more than P's alone explains.
+constexpr int HB_FEW_WEIGHTED = 4096;
 static int head_both(const HeadCall& a) {
-  if (a.V <= HD_FEW || a.cw != nullptr || a.K > 65000) return 0;
+  if (a.V <= (a.cw == nullptr ? HD_FEW : HB_FEW_WEIGHTED) || a.K > 65000) return 0;
   const int cpad = (a.C + 15) / 16 * 16, kboxes = (a.C + 63) / 64, kt = (a.K + HD_TILE - 1) / HD_TILE;
   auto fits = [&](int n) {
-    return (n + 1) * cpad <= 256 && (n + 2) * (4 * kboxes + 1) + 16 + 4 * kboxes + (n + 1) / 2 <= HD_BOXES;
+    return (n + 1) * cpad <= 256 &&
+           (n + 2) * (4 * kboxes + 1) + 16 + 4 * kboxes + (n + 1) / 2 + (a.cw != nullptr) <= HD_BOXES;
   };
   int most = 0;
   while (most < 4 && fits(most + 1)) ++most;
   if (most >= kt) return kt;
-  if (cpad > 32 || a.V < 4 * 148 * HD_TILE || hd_pad(a.V) * cpad * 4 > (128LL << 20)) return 0;
+  if (a.cw != nullptr || cpad > 32 || a.V < 4 * 148 * HD_TILE || hd_pad(a.V) * cpad * 4 > (128LL << 20)) return 0;
   const int launches = (kt + most - 1) / most, each = (kt + launches - 1) / launches;
   return each == 4 ? 4 : 0;
 }
@@ -1461,7 +1526,8 @@ static void head_geometry(const HeadCall& a, int mode, HeadParams& p) {
   if (mode == HEAD_BOTH) {
     p.splits = p.col_tiles < 148 ? p.col_tiles : 148;  // CTAs, each with sums of its own
     p.accs = (p.row_tiles + 2) * p.cpad <= 256 ? 2 : 1;
-    const int tile = 4 * p.kboxes + 1, left = HD_BOXES - p.row_tiles * tile - 4 * p.kboxes - (p.row_tiles + 1) / 2;
+    const int tile = 4 * p.kboxes + 1, left = HD_BOXES - p.row_tiles * tile - 4 * p.kboxes - (p.row_tiles + 1) / 2 -
+                                              (a.cw != nullptr);
     p.stages = (left - 16) / tile;
     if (p.stages > 6) p.stages = 6;
     return;
@@ -1523,11 +1589,11 @@ static int head_launch(const HeadCall& a, HeadParams& p, cudaStream_t stream) {
   }
   void (*kernel)(HeadParams) = nullptr;
   if constexpr (rows) kernel = head_rows_kernel<FLAG>;
-  else if constexpr (both) kernel = head_both_kernel;
+  else if constexpr (both) kernel = head_both_kernel<FLAG>;
   else kernel = head_grad_kernel<MODE, FLAG>;
   const size_t smem = 1024 + (size_t)((both ? p.row_tiles : p.rbufs) + p.stages) * p.kboxes * HD_BOX +
                       (size_t)((both ? p.row_tiles : rows ? 1 : p.rbufs) + p.stages) * HD_BOX16 +
-                      (both ? 4 * HD_BOX + p.kboxes * HD_BOX + p.row_tiles * 4 * HD_TILE * 4 : 0);
+                      (both ? 4 * HD_BOX + p.kboxes * HD_BOX + (p.row_tiles * 4 + (FLAG ? p.row_tiles + p.stages : 0)) * HD_TILE * 4 : 0);
   static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have as much as it can need
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return SB_ERR_DRIVER;
@@ -1637,6 +1703,7 @@ static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
     p.gout = a.gout;
     p.den = a.den;
     p.scale = a.scale;
+    p.cw = a.cw;
     p.out = a.dx;
     p.ws = a.scratch;
     p.ws_b = p.ws + p.splits * p.rows_pad * p.cpad;
@@ -1648,7 +1715,7 @@ static int head_narrow_backward(const HeadCall& a, cudaStream_t stream) {
       p.row_tiles = (int)((p.rows + HD_TILE - 1) / HD_TILE);
       p.first = row0 == 0;
       p.last = row0 + most >= a.K;
-      rc = head_launch<HEAD_BOTH, false>(a, p, stream);
+      rc = a.cw != nullptr ? head_launch<HEAD_BOTH, true>(a, p, stream) : head_launch<HEAD_BOTH, false>(a, p, stream);
       if (rc) return rc;
       auto from = [&](void* out, int kind, long long i) {
         return out == nullptr ? nullptr : (void*)((char*)out + i * (kind == 2 ? 4 : 2));

@@ -102,6 +102,9 @@ BOTH = [(129, 8, 1), (200, 64, 32), (256, 16, 33), (19000, 64, 128), (38100, 24,
 @pytest.mark.parametrize("v,c,k", BOTH)
 def test_both_gradients_at_once(v, c, k):
     x, w, b, y, _ = _inputs(v, c, k, ignored=0.1)
+    cw = torch.rand(k, device="cuda") + 0.5
+    cw[::3] = 0.0 if k > 2 else 2.0
+    _check(x, w, b, y, cw)
     _, dx, dw, db = _check(x, w, b, y, None)
     # and each of them alone, where one is asked for: the same sums from other kernels
     one = [t.clone().requires_grad_() for t in (x, w, b)]
