@@ -60,7 +60,11 @@ def _check(x, w, b, y, cw, ignore=IGNORED, scale=1.0, label_type=torch.int32):
     # D's entries are rounded to bf16 (2^-8 of the value at most, 2^-8 of one for the target is covered by its value),
     # after errors of e_term relative to p; then the products' fp32 sums and the result's own rounding
     rel = 2 ** -8 + 4 * e_term
-    g = d.abs().amax(1, keepdim=True)  # the size of a voxel's weight: D's errors of fp32 are relative to it
+    # D = g (p - [j = y]): p is off by e_term p at most, the one by nothing, so fp32 leaves errors of e_term g, however
+    # small p - 1 itself is (one class: exactly 0); g is the voxel's weight over their sum
+    live = (y >= 0) & (y < w16.shape[0]) & (y != ignore)
+    u = live.double() if cw is None else torch.where(live, cw.double()[torch.where(live, y, 0)], 0.0)
+    g = (u / u.sum().clamp_min(torch.finfo(torch.float32).eps) * scale)[:, None].abs()
     slack = 4 * e_term * g
     ex = (d.abs() * rel + slack) @ w16.double().abs()
     ew = (d.abs() * rel + slack).T @ x.detach().double().abs()
