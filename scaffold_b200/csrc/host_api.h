@@ -196,7 +196,8 @@ int sb_gn8_backward(const void* dy, const void* kept, const float* w, const floa
 // 8 int64; `ignore`, if has_ignore, takes no part), cw optional class weights [K], not negative. The forward pass fills
 // `state` for the backward pass; its first 16 bytes are the sums of u nll and of u. state and scratch: sb_head_bytes()
 // bytes, 256-byte aligned. Backward: dx bf16 [V][C], dw [K][C] and db [K] (kind 0 bf16, 2 fp32) are each optional.
-long long sb_head_bytes(int what, long long V, int K, int C, int weighted);  // 0 state, 1 forward, 2 / 3 backward: one / both gradients
+// what: 0 state, 1 scratch of the forward pass, 2 / 3 of the backward pass (one gradient / of x and of w or the bias)
+long long sb_head_bytes(int what, long long V, int K, int C, int weighted);
 int sb_head_forward(const void* x, const void* w, const void* bias, int bias_kind, const void* labels, int label_kind,
                     int has_ignore, long long ignore, const float* cw, long long V, int K, int C, void* state,
                     void* scratch, float* loss, uint32_t* status, cudaStream_t stream);
