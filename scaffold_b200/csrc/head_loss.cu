@@ -404,6 +404,12 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
 #pragma unroll
           for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
           if (ARG) {
+            // columns behind the last class take no part: zeros of w there, and 0 * inf of a feature is a NaN
+            const int left = (int)p.cols - (c_abs + c0);
+            if (left < 32) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j] = j < left ? f[j] : -INFINITY;
+            }
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (f[j] > m || (f[j] != f[j] && m == m)) { m = f[j]; best = c_abs + c0 + j; }

@@ -262,6 +262,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(HW_THREADS, 1)
             }
           }
           if (EPI == WIDE_ARG) {
+            // columns behind the last class take no part: zeros of w there, and 0 * inf of a feature is a NaN
+            const int left = p.cols - (c_abs + c0);
+            if (left < 32) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) f[i] = i < left ? f[i] : -INFINITY;
+            }
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (f[i] > m || (f[i] != f[i] && m == m)) { m = f[i]; best = c_abs + c0 + i; }

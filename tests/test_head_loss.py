@@ -429,6 +429,25 @@ def test_the_predicted_class(v, c, k):
     assert H.head_predict(x[:0], w).shape == (0,)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("v,c,k", [(1, 8, 1), (5, 64, 33), (40, 64, 147), (600, 16, 1001), (129, 256, 1025), (9, 320, 40),
+                                   (300, 320, 513)])
+def test_the_predicted_class_is_a_class_whatever_the_features_hold(v, c, k):
+    """Infinite features make every logit infinite or NaN, and NaN of the zeros behind the last class."""
+    g = torch.Generator(device="cuda").manual_seed(v + k)
+    sign = lambda *s: (torch.randint(0, 2, s, generator=g, device="cuda") * 2 - 1).to(torch.bfloat16)  # noqa: E731
+    x, w = sign(v, c), sign(k, c)
+    w[:, 1] = -1
+    x[::3, 0] = float("inf")   # logits of +inf and -inf: the first class of +inf
+    x[1::3, 1] = float("inf")  # -inf in every class: the first one
+    got = H.head_predict(x, w)
+    want = (x.float() @ w.float().T).argmax(1)
+    assert torch.equal(got, want) and int(want[1::3].max() if v > 1 else 0) == 0
+    # large finite logits of one sign are smaller than the zeros behind the last class
+    big = torch.full((3, c), 1e36, dtype=torch.bfloat16, device="cuda")
+    assert torch.equal(H.head_predict(big, -w.abs()), torch.zeros(3, dtype=torch.int64, device="cuda"))
+
+
 def test_the_predicted_class_on_the_cpu():
     x, w, b, *_ = _inputs(50, 16, 9, dev="cpu")
     assert torch.equal(H.head_predict(x, w, b), (x.float() @ w.float().T + b.float()).argmax(1))
