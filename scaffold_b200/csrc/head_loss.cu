@@ -74,6 +74,8 @@ struct HeadParams {
   float* lse2_out;
   uint32_t* hit_out;    // or null
   const float* cw;
+  const void* bias;
+  int bias_kind;
   double* sums;         // [CTAs][2]
   __nv_bfloat16* out;   // DX with one split: [rows][C]
   float* ws;            // DX / DW: [splits][rows padded][cpad]
@@ -199,14 +201,28 @@ __device__ __forceinline__ HeadSum hd_block_sum(HeadSum a) {
   return t;
 }
 
+// bias: null, bf16 (kind 0) or fp32
+__device__ __forceinline__ float hd_bias(const void* bias, int kind, long long i) {
+  return bias == nullptr ? 0.f
+         : kind == 0     ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(bias)[i])
+                         : reinterpret_cast<const float*>(bias)[i];
+}
 // A voxel's log2 of the sum of exponentials, from maximum (log2) and sum; u nll and u are added, and the label's p - 1 and
-// the label go to `hit`. i < V; y -1: takes no part.
-__device__ __forceinline__ float hd_voxel(float m2, float sum, float tl, int y, const float* cw, HeadSum& a, uint32_t& hit) {
+// the label go to `hit`. i < V; y -1: takes no part. A label whose class its bias turns off (-inf, or the type's lowest
+// number) was given HD_LOWEST or -inf as its logit: the bias itself takes that place, the products beside it are below its
+// rounding.
+__device__ __forceinline__ float hd_voxel(float m2, float sum, float tl, int y, const float* cw, const void* bias,
+                                          int bias_kind, HeadSum& a, uint32_t& hit) {
   const float l = m2 < 0.1f * HD_LOWEST ? NAN : m2 + log2f(sum);  // every class is off: 0 / 0
   hit = 0xFFFFu;
   if (y >= 0) {
     const float u = cw == nullptr ? 1.f : cw[y], t = l - tl;
-    a.num += (double)u * ((double)t * (double)HD_LN2);
+    double nll = (double)t * (double)HD_LN2;
+    if (tl < 0.1f * HD_LOWEST) {
+      const float b = hd_bias(bias, bias_kind, y);
+      if (b < HD_LOWEST) nll = (double)l * (double)HD_LN2 - (double)b;
+    }
+    if (u != 0.f) a.num += (double)u * nll;  // (a class of weight zero takes no part: not 0 * inf)
     a.den += (double)u;
     hit = (uint32_t)__bfloat16_as_ushort(__float2bfloat16(expm1f(-t * HD_LN2))) << 16 | ((uint32_t)y & 0xFFFFu);
   }
@@ -454,7 +470,8 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
       if (!ARG && p.whole) {
         if (ok && r < p.rows_pad) {
           uint32_t hit = 0xFFFFu;
-          p.lse2_out[r] = r < p.rows ? hd_voxel(m * HD_LOG2E, s, tl * HD_LOG2E, y, p.cw, total, hit) : INFINITY;
+          p.lse2_out[r] = r < p.rows ? hd_voxel(m * HD_LOG2E, s, tl * HD_LOG2E, y, p.cw, p.bias, p.bias_kind, total, hit)
+                                       : INFINITY;
           if (p.hit_out != nullptr) p.hit_out[r] = hit;
         }
       } else if (ok && r < p.rows_pad) {
@@ -1270,10 +1287,7 @@ __global__ void __launch_bounds__(256) head_prep_kernel(const void* __restrict__
     }
     if (i < k_pad) {
       float b = -INFINITY;
-      if (i < K)
-        b = bias == nullptr ? 0.f
-            : bias_kind == 0 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(bias)[i])
-                             : reinterpret_cast<const float*>(bias)[i];
+      if (i < K) b = hd_bias(bias, bias_kind, i);
       bias2[i] = b * HD_LOG2E;
       if (w16 != nullptr) {
         const uint2 t = hd_three(b < HD_LOWEST ? HD_LOWEST : b);
@@ -1362,7 +1376,7 @@ __device__ __forceinline__ void hd_loss(const HeadSum& a, double* total, float* 
 template <int TEAM>
 __global__ void __launch_bounds__(256) head_merge_kernel(const float2* __restrict__ part, const float* __restrict__ tl,
                                                          const int* __restrict__ y, const float* __restrict__ cw,
-                                                         int shares, long long V, long long v_pad,
+                                                         const void* __restrict__ bias, int bias_kind, int shares, long long V, long long v_pad,
                                                          float* __restrict__ lse2, uint32_t* __restrict__ hit,
                                                          double* __restrict__ sums, double* __restrict__ total, float* __restrict__ loss,
                                                          float* __restrict__ den) {
@@ -1374,7 +1388,7 @@ __global__ void __launch_bounds__(256) head_merge_kernel(const float2* __restric
     uint32_t h = 0xFFFFu;
     if (i < V) {  // (the same in a team's lanes)
       const float2 e = hd_merge_sums<TEAM>(part, shares, v_pad, i, lane);
-      if (lane == 0) l = hd_voxel(e.x, e.y, tl[i], y[i], cw, a, h);
+      if (lane == 0) l = hd_voxel(e.x, e.y, tl[i], y[i], cw, bias, bias_kind, a, h);
     }
     if (lane == 0) {
       lse2[i] = l;
@@ -1809,6 +1823,8 @@ extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, i
     p.lse2_out = a.lse2;
     p.hit_out = a.hit;
     p.cw = cw;
+    p.bias = bias;
+    p.bias_kind = bias_kind;
     p.sums = f.sums;
     splits = head_shares(p);
     rc = head_launch<HEAD_ROWS, false>(a, p, stream);
@@ -1828,11 +1844,11 @@ extern "C" int sb_head_forward(const void* x, const void* w, const void* bias, i
   // ways on the device, and the launch's 3 us on the host)
   const int blocks = v_pad <= (team ? 256 : 4096) ? 1 : hd_blocks(team ? v_pad * 32 : v_pad, HD_SUM_BLOCKS / 148);
   if (team)
-    head_merge_kernel<32><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, a.hit, f.sums, a.total,
-                                                      loss, a.den);
+    head_merge_kernel<32><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, bias, bias_kind, splits, V, v_pad, a.lse2, a.hit,
+                                                      f.sums, a.total, loss, a.den);
   else
-    head_merge_kernel<1><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, splits, V, v_pad, a.lse2, a.hit, f.sums, a.total,
-                                                     loss, a.den);
+    head_merge_kernel<1><<<blocks, 256, 0, stream>>>(f.part, f.tl, a.y, cw, bias, bias_kind, splits, V, v_pad, a.lse2, a.hit,
+                                                     f.sums, a.total, loss, a.den);
   if (blocks > 1) head_total_kernel<<<1, 256, 0, stream>>>(f.sums, blocks, a.total, loss, a.den);
   sb_count_launch(blocks > 1 ? 2 : 1);
   return cudaGetLastError() == cudaSuccess ? 0 : SB_ERR_LAUNCH;

@@ -106,8 +106,9 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
     ``features [..., C]`` (voxel-major, the classes' axis of the logits is the last), ``weight [K, C]`` (or the
     ``[K, C, 1, 1, 1]`` of a 1x1x1 convolution), ``bias [K]`` or None, ``labels [...]`` int16, int32 or int64.
     ``class_weights [K]`` (not negative) weigh the voxels by their label; the result is the sum of the weighted terms over
-    the sum of the weights, over all shards with ``spatial``. Voxels of ``ignore_label`` take no part; without any other
-    voxel the loss and its gradients are zero. A label outside the classes takes no part either and is reported by
+    the sum of the weights, over all shards with ``spatial``. Voxels of ``ignore_label`` and of a class whose weight is zero
+    take no part; without any other voxel the loss and its gradients are zero. A bias of -inf turns its class off; a voxel
+    that is labelled with it makes the loss +inf. A label outside the classes takes no part either and is reported by
     :func:`scaffold_b200.ops._lib.check_status`. Features of voxels that take no part have to be finite for the
     kernels: they reach the weight's gradient as ``0 * x``, as in any matrix product with rows of zeros.
 
@@ -213,6 +214,8 @@ def _formula(features, weight, bias, labels, class_weights, ignore_label, spatia
     live = (y >= 0) & (y < k)
     if ignore_label is not None:
         live &= y != ignore_label
+    if class_weights is not None:
+        live &= class_weights[y.clamp(0, k - 1)] != 0
     x, y = features.reshape(-1, features.shape[-1])[live], y[live]
     logits = _logits(x, weight, bias)
     kind = logits.dtype

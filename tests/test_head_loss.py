@@ -276,6 +276,37 @@ def test_infinite_logits(c):
     assert loss.isfinite() and xs.grad[:3].isfinite().all() and xs.grad[4:].isfinite().all()
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("v,c,k", [(300, 64, 70), (5000, 16, 34), (400, 128, 300), (7, 256, 3000), (300, 320, 70), (5, 320, 3000)])
+def test_a_label_on_a_class_that_is_off(v, c, k, dev):
+    """Its bias is -inf: the loss is +inf. The type's lowest number: as large, not the stand-in that the kernels multiply
+    with. A class weight of zero takes the voxel out."""
+    x, w, b, y, _ = _inputs(v, c, k, dev=dev)
+    y[y == 5] = 6
+    fine = float(head_cross_entropy(x, w, b, y))
+    assert math.isfinite(fine)
+    y[v // 2] = 5
+    b[5] = float("-inf")
+    xs, ws, bs = (t.clone().requires_grad_() for t in (x, w, b))
+    loss = head_cross_entropy(xs, ws, bs, y)
+    assert float(loss.detach()) == math.inf
+    if dev == "cuda":  # (in 32 bits the formula's gradients are those of inf - inf)
+        loss.backward()
+        for got, want in zip((xs.grad, ws.grad, bs.grad), _definition(x, w, b, y, None)[1:4]):
+            assert got.isfinite().all() and float((got.double() - want).norm()) <= 4e-3 * float(want.norm())
+    cw = torch.ones(k, device=dev)
+    cw[5] = 0
+    keep = torch.where(y == 5, IGNORED, y)
+    assert float(head_cross_entropy(x, w, b, y, cw)) == float(head_cross_entropy(x, w, b, keep, torch.ones_like(cw),
+                                                                                 ignore_label=IGNORED))
+    b = b.float()
+    for low in (torch.finfo(torch.bfloat16).min, torch.finfo(torch.float32).min, -1e31):
+        b[5] = low
+        got = float(head_cross_entropy(x, w, b, y))
+        # one term of the size of -low among v: fp32's roundings of the logit and of the result
+        assert abs(got - -float(b[5]) / v) <= 2 ** -22 * -float(b[5]) / v, (got, low)
+
+
 @pytest.mark.gpu
 def test_shapes_views_and_evaluation():
     x, w, b, y, cw = _inputs(2 * 3 * 4 * 5, 48, 50, weighted=True)
