@@ -131,9 +131,10 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
     if class_weights is not None and (class_weights.dtype != torch.float32 or class_weights.requires_grad
                                       or not class_weights.is_contiguous()):
         class_weights = class_weights.detach().float().contiguous()
-    if x.shape[0] == 0:  # a shard without voxels: its terms are zero, the other shards' sums are not
-        return _formula(x.float(), weight.float(), None if bias is None else bias.float(), labels, class_weights,
-                        ignore_label, spatial)
+    if x.shape[0] == 0:
+        # a shard without voxels: its terms are zero, the other shards' sums are not, and are two fp64 numbers
+        return _formula(x.double(), weight.double(), None if bias is None else bias.double(), labels, class_weights,
+                        ignore_label, spatial).float()
     with on_device(x.device):
         return _HeadLossFn.apply(x, weight, None if bias is None else bias.contiguous(), labels, class_weights,
                                  ignore_label, spatial)
