@@ -203,7 +203,8 @@ def _operands(features, weight, bias):
 
 def _logits(x, weight, bias):
     kind = torch.promote_types(torch.promote_types(x.dtype, weight.dtype), torch.float32)
-    logits = x.to(kind) @ weight.to(kind).T
+    with torch.autocast(x.device.type, enabled=False):  # which would make a product of 16 bits of it
+        logits = x.to(kind) @ weight.to(kind).T
     return logits if bias is None else logits + bias.to(kind)
 
 

@@ -498,6 +498,17 @@ def test_the_formula_on_the_cpu_and_its_gradients():
     assert low.dtype == torch.float32 and abs(float(low) - float(rl)) < 1e-5
 
 
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autocast_leaves_the_formula_in_32_bits(dtype, bias):
+    x, w, b, y, cw = _inputs(700, 24, 40, weighted=True, bias=bias, w_type=torch.float32, dev="cpu")
+    want, pred = head_cross_entropy(x, w, b, y, cw), H.head_predict(x, w, b)
+    with torch.autocast("cpu", dtype=dtype):
+        loss = head_cross_entropy(x, w, b, y, cw)
+        assert loss.dtype == torch.float32 and torch.equal(loss, want)
+        assert torch.equal(H.head_predict(x, w, b), pred)
+
+
 def test_the_gradient_against_differences():
     x, w, b, y, cw = _inputs(7, 8, 12, weighted=True, dev="cpu")
     leaves = [t.double().requires_grad_() for t in (x, w, b)]
