@@ -228,10 +228,16 @@ def _bias_grad(ctx, gy: torch.Tensor, n_out: int, bias) -> Optional[torch.Tensor
     return None
 
 
-def _save(ctx, mod, weight, xs) -> None:
-    """Save a layer's inputs for its weight gradient, as 8-bit copies where the layer was told to (``keep_bits``)."""
+def _keeps8(mod) -> bool:
+    """Whether a layer keeps 8-bit copies of its inputs: told to, with a backward pass to come. Asked outside of the
+    autograd functions, in whose forward passes the gradient mode is always off."""
+    return mod.keep_bits == 8 and torch.is_grad_enabled()
+
+
+def _save(ctx, keep8bit, weight, xs) -> None:
+    """Save a layer's inputs for its weight gradient, as 8-bit copies where the layer keeps such (:func:`_keeps8`)."""
     ctx.kept = None
-    if mod.keep_bits == 8 and ctx.needs_input_grad[0]:
+    if keep8bit and ctx.needs_input_grad[0]:
         kept = [keep8(x) for x in xs]
         xs = [k.data for k in kept]
         ctx.kept = [tuple(k)[1:] for k in kept]
@@ -249,7 +255,7 @@ class _ConvSameFn(torch.autograd.Function):
     """k in {1,3} stride-1 'same' conv over voxel-major bf16 sources."""
 
     @staticmethod
-    def forward(ctx, weight, bias, mod, in_off, fwd_xs, *xs):
+    def forward(ctx, weight, bias, mod, keep8bit, in_off, fwd_xs, *xs):
         """``xs`` are saved for backward; ``fwd_xs`` (or None) are the same sources padded to more channels,
         read by the forward kernel only (a few-channel stem runs the kd-fused kernel on 32 padded channels)."""
         ks = weight.shape[2]
@@ -283,7 +289,7 @@ class _ConvSameFn(torch.autograd.Function):
         ctx.src_c, ctx.real_c = src_c, real_c
         ctx.tap_swap = ts
         ctx.has_bias = bias is not None
-        _save(ctx, mod, weight, xs)
+        _save(ctx, keep8bit, weight, xs)
         return y
 
     @staticmethod
@@ -294,7 +300,7 @@ class _ConvSameFn(torch.autograd.Function):
         gy = gy.contiguous()
         src_c, real_c = ctx.src_c, ctx.real_c
         gxs: List[Optional[torch.Tensor]] = [None] * len(xs)
-        need_gx = [ctx.needs_input_grad[5 + i] for i in range(len(xs))]
+        need_gx = [ctx.needs_input_grad[6 + i] for i in range(len(xs))]
         if any(need_gx):
             if ks == 3:
                 # rows = input channels of the layer, K = gy's channels (Cout padded to a multiple of 16)
@@ -330,7 +336,7 @@ class _ConvSameFn(torch.autograd.Function):
                 gw = torch.cat(parts, 1).contiguous()
         if ctx.has_bias and ctx.needs_input_grad[1]:
             gb = _bias_grad(ctx, gy, weight.shape[0], ctx.bparam)
-        return (gw, gb, None, None, None, *gxs)
+        return (gw, gb, None, None, None, None, *gxs)
 
 
 class _StemFn(torch.autograd.Function):
@@ -338,7 +344,7 @@ class _StemFn(torch.autograd.Function):
     neighbourhoods; nothing but the staged copy is kept for backward."""
 
     @staticmethod
-    def forward(ctx, weight, bias, mod, x):
+    def forward(ctx, weight, bias, mod, keep8bit, x):
         xs = ck.stage_stem(x)
         wf = mod._cache.get(weight, "stem", ck.pack_stem)
         cout_pad = wf.shape[1]
@@ -350,7 +356,7 @@ class _StemFn(torch.autograd.Function):
         (y,) = ck.conv_same([xs], wf, 3, [cout_pad], bias=bpad, gn_groups=gn, gn_sink=sink, stem=True)
         mod._gn_partials = sink[0] if sink else None
         ctx.wparam, ctx.bparam = weight, bias
-        _save(ctx, mod, weight, [xs])
+        _save(ctx, keep8bit, weight, [xs])
         return y
 
     @staticmethod
@@ -369,7 +375,7 @@ class _StemFn(torch.autograd.Function):
                 ck.conv_wgrad(gy, [xs], 3, gw, stem=True)
         if ctx.bparam is not None and ctx.needs_input_grad[1]:
             gb = _bias_grad(ctx, gy, weight.shape[0], ctx.bparam)
-        return gw, gb, None, None
+        return gw, gb, None, None, None
 
 
 class _ConvHaloFn(torch.autograd.Function):
@@ -510,7 +516,7 @@ class Conv3d(nn.Conv3d):
                 and x.is_contiguous() and x.dtype in (torch.float32, torch.bfloat16)
                 and x.shape[1] == self.in_channels
                 and ck.stem_eligible(self.in_channels, ck.pad_channels(self.out_channels), x.shape[2:])):
-            return _StemFn.apply(self.weight, self.bias, self, x)
+            return _StemFn.apply(self.weight, self.bias, self, _keeps8(self), x)
         vms = [to_vm(t, pad16=True) for t in xs]
         fwd_vms = None
         if (len(xs) == 1 and self.kernel_size[0] == 3 and self.in_channels < 16 and not xs[0].requires_grad
@@ -518,7 +524,7 @@ class Conv3d(nn.Conv3d):
             # few input channels (a stem of four and more, or sharded): the forward pass reads a copy padded to 32
             # channels so that it runs the kd-fused kernel; the weight gradient keeps the 16-channel copy
             fwd_vms = (to_vm(xs[0], pad16=True, pad_to=32),)
-        return _ConvSameFn.apply(self.weight, self.bias, self, off, fwd_vms, *vms)
+        return _ConvSameFn.apply(self.weight, self.bias, self, _keeps8(self), off, fwd_vms, *vms)
 
     def forward_padded(self, x) -> torch.Tensor:
         """CUDA path only: voxel-major output with the channel axis padded to a multiple of 16."""
@@ -528,10 +534,10 @@ class Conv3d(nn.Conv3d):
 
 class _ConvTFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, bias, mod, x):
+    def forward(ctx, weight, bias, mod, keep8bit, x):
         cout = weight.shape[1]
         # with a backward pass to come, both operands from one reading of the weight
-        both = mod._cache.get(weight, "both", lambda w: ck.pack_convT(w, True, True)) if ctx.needs_input_grad[3] else None
+        both = mod._cache.get(weight, "both", lambda w: ck.pack_convT(w, True, True)) if ctx.needs_input_grad[4] else None
         wf = both[0] if both else mod._cache.get(weight, "fwd", lambda w: ck.pack_convT(w, True, False)[0])
         b32 = None
         if bias is not None:
@@ -541,7 +547,7 @@ class _ConvTFn(torch.autograd.Function):
         ctx.wparam, ctx.bparam = weight, bias
         ctx.has_bias = bias is not None
         ctx.in_channels = x.shape[4]
-        _save(ctx, mod, weight, [x])
+        _save(ctx, keep8bit, weight, [x])
         return y
 
     @staticmethod
@@ -550,7 +556,7 @@ class _ConvTFn(torch.autograd.Function):
         mod = ctx.mod
         gy = gy.contiguous()
         gx = gw = gb = None
-        if ctx.needs_input_grad[3]:
+        if ctx.needs_input_grad[4]:
             wd = mod._cache.get(weight, "both", lambda w: ck.pack_convT(w, True, True))[1]
             gx = ck.convT_dgrad(gy, wd, ctx.in_channels)
         if ctx.needs_input_grad[0]:
@@ -564,7 +570,7 @@ class _ConvTFn(torch.autograd.Function):
                 ck.conv_wgrad(gy, [x], 2, gw)
         if ctx.has_bias and ctx.needs_input_grad[1]:
             gb = _bias_grad(ctx, gy, gy.shape[4], ctx.bparam)
-        return gw, gb, None, gx
+        return gw, gb, None, None, gx
 
 
 class ConvTranspose3d(nn.ConvTranspose3d):
@@ -594,7 +600,7 @@ class ConvTranspose3d(nn.ConvTranspose3d):
         if use_cuda_kernels(x):
             if not self._kernel_ok() or output_size is not None:
                 raise NotImplementedError(f"sm_100a transposed-conv kernel covers k=2, s=2, no padding; got {self}")
-            return from_vm(_ConvTFn.apply(self._w(), self.bias, self, to_vm(x)))
+            return from_vm(_ConvTFn.apply(self._w(), self.bias, self, _keeps8(self), to_vm(x)))
         if getattr(self._spatial, "lead_swap", None) is not None:
             return F.conv_transpose3d(x, self._w(), self.bias, self.stride, self.padding, self.output_padding,
                                       self.groups, self.dilation)

@@ -87,6 +87,21 @@ def test_a_captured_step_is_the_ordinary_step():
     assert results[0] == results[1]
 
 
+@pytest.mark.gpu
+def test_a_pass_without_gradients_makes_no_copies():
+    model = _model(width=16)
+    x, y = _batch(6, (16, 20, 16))
+    engine = TrainEngine(model, torch.optim.SGD(model.parameters(), lr=0.0), 6, "cuda")
+    counts, losses = [], []
+    for bits in (16, 8):
+        model.keep_activations(bits)
+        engine.eval_step(x, y)  # operand copies are made
+        before = _lib.launch_count()
+        losses.append(engine.eval_step(x, y)[0])
+        counts.append(_lib.launch_count() - before)
+    assert counts[0] == counts[1] > 0 and torch.equal(*losses)
+
+
 def test_the_setting_on_the_cpu():
     model = _model(dev="cpu", width=8, layers=1)
     x, y = _batch(6, (8, 8, 8), 1, "cpu")
