@@ -499,6 +499,7 @@ class Conv3d(nn.Conv3d):
         """Voxel-major output of the kernel path; on a sharded volume the sources first receive their halo."""
         sp = self._spatial
         off = (0, 0, 0)
+        keep8bit = _keeps8(self)
         if sp is not None and sp.size > 1 and self.kernel_size[0] == 3 and sp.halo_channel is not None:
             vms = [to_vm(t, pad16=True) for t in xs]
             d, h, w = vms[0].shape[1:4]
@@ -511,12 +512,13 @@ class Conv3d(nn.Conv3d):
             halo = self.kernel_size[0] // 2
             xs = [sp.halo_pad(t, halo) for t in xs]
             off = tuple(halo if d in sp.dims else 0 for d in (2, 3, 4))
+            keep8bit = False  # a layer that exchanges with other shards keeps 16 bits, here as with the fused halo
         x = xs[0]
         if (len(xs) == 1 and self.kernel_size[0] == 3 and sp is None and x.dim() == 5 and not x.requires_grad
                 and x.is_contiguous() and x.dtype in (torch.float32, torch.bfloat16)
                 and x.shape[1] == self.in_channels
                 and ck.stem_eligible(self.in_channels, ck.pad_channels(self.out_channels), x.shape[2:])):
-            return _StemFn.apply(self.weight, self.bias, self, _keeps8(self), x)
+            return _StemFn.apply(self.weight, self.bias, self, keep8bit, x)
         vms = [to_vm(t, pad16=True) for t in xs]
         fwd_vms = None
         if (len(xs) == 1 and self.kernel_size[0] == 3 and self.in_channels < 16 and not xs[0].requires_grad
@@ -524,7 +526,7 @@ class Conv3d(nn.Conv3d):
             # few input channels (a stem of four and more, or sharded): the forward pass reads a copy padded to 32
             # channels so that it runs the kd-fused kernel; the weight gradient keeps the 16-channel copy
             fwd_vms = (to_vm(xs[0], pad16=True, pad_to=32),)
-        return _ConvSameFn.apply(self.weight, self.bias, self, _keeps8(self), off, fwd_vms, *vms)
+        return _ConvSameFn.apply(self.weight, self.bias, self, keep8bit, off, fwd_vms, *vms)
 
     def forward_padded(self, x) -> torch.Tensor:
         """CUDA path only: voxel-major output with the channel axis padded to a multiple of 16."""

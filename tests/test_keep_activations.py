@@ -4,6 +4,7 @@ import torch
 
 from scaffold_b200.models.unet import UNet
 from scaffold_b200.ops import _lib, loss as L
+from scaffold_b200.ops.conv3d import Conv3d
 from scaffold_b200.ops.head_loss import head_predict
 from scaffold_b200.ops.optim import FusedClipAdam
 from scaffold_b200.train.engine import TrainEngine
@@ -100,6 +101,40 @@ def test_a_pass_without_gradients_makes_no_copies():
         losses.append(engine.eval_step(x, y)[0])
         counts.append(_lib.launch_count() - before)
     assert counts[0] == counts[1] > 0 and torch.equal(*losses)
+
+
+class _Halo:
+    """A spatial context of two shards along the depth whose neighbours are outside of the volume."""
+
+    size, dims, lead_swap, halo_channel = 2, [2], None, None
+
+    @staticmethod
+    def halo_pad(x, halo):
+        return torch.nn.functional.pad(x, (0, 0, 0, 0, halo, halo))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kernel,kept", [(3, False), (1, True)])
+def test_a_convolution_that_exchanges_with_other_shards_keeps_16_bits(kernel, kept):
+    torch.manual_seed(0)
+    conv = Conv3d(32, 32, kernel, padding=kernel // 2, bias=False).cuda()
+    x = torch.randn(1, 32, 8, 12, 16, device="cuda").to(memory_format=torch.channels_last_3d).requires_grad_()
+    grads = []
+    for bits, spatial in ((16, None), (16, _Halo), (8, _Halo)):
+        conv.keep_bits = bits
+        conv.set_spatial(spatial)
+        saved = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: (saved.append(t.dtype), t)[1], lambda t: t):
+            with torch.autocast("cuda", dtype=torch.bfloat16):
+                y = conv(x)
+        grads.append(torch.autograd.grad(y, (x, conv.weight), torch.ones_like(y)))
+        assert (torch.uint8 in saved) == (kept and bits == 8)
+    _lib.check_status()
+    if not kept:
+        assert all(torch.equal(a, b) for a, b in zip(grads[1], grads[2]))
+    # (a padded volume is cut into other parts: the same products in another order)
+    for a, b in zip(grads[0], grads[1]):
+        assert float((a - b).norm()) <= 1e-3 * float(a.norm())
 
 
 def test_the_setting_on_the_cpu():
