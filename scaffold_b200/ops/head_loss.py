@@ -113,7 +113,7 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
     kernels: they reach the weight's gradient as ``0 * x``, as in any matrix product with rows of zeros.
 
     The kernels read bf16: an fp32 ``weight`` is rounded, its gradient comes back in fp32. Gradients: features in bf16,
-    weight and bias in their own types.
+    weight and bias in their own types; the class weights have none.
     """
     shape = features.shape
     if not shape or labels.shape != shape[:-1]:
@@ -217,6 +217,7 @@ def _formula(features, weight, bias, labels, class_weights, ignore_label, spatia
     if ignore_label is not None:
         live &= y != ignore_label
     if class_weights is not None:
+        class_weights = class_weights.detach()
         live &= class_weights[y.clamp(0, k - 1)] != 0
     x, y = features.reshape(-1, features.shape[-1])[live], y[live]
     logits = _logits(x, weight, bias)

@@ -509,6 +509,16 @@ def test_autocast_leaves_the_formula_in_32_bits(dtype, bias):
         assert torch.equal(H.head_predict(x, w, b), pred)
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_class_weights_have_no_gradient(dev):
+    x, w, b, y, cw = _inputs(60, 24, 40, weighted=True, dev=dev)
+    x.requires_grad_()
+    loss = head_cross_entropy(x, w, b, y, cw.requires_grad_())
+    assert torch.equal(loss, head_cross_entropy(x, w, b, y, cw.detach()))
+    dx, none = torch.autograd.grad(loss, (x, cw), allow_unused=True)
+    assert none is None and dx.any()
+
+
 def test_the_gradient_against_differences():
     x, w, b, y, cw = _inputs(7, 8, 12, weighted=True, dev="cpu")
     leaves = [t.double().requires_grad_() for t in (x, w, b)]
