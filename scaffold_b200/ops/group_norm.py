@@ -69,7 +69,7 @@ class _Gn8Fn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, groups, eps, relu, partials):
         # (no view of another tensor: autograd keeps a record of such a result's base)
         y = torch.empty_like(x, memory_format=torch.channels_last_3d)
-        x = to_vm(x)
+        x = _on_16_bytes(to_vm(x))
         w32, b32 = _fp32(weight), _fp32(bias)
         fin = None
         if partials is not None:
@@ -94,12 +94,17 @@ class _Gn8Fn(torch.autograd.Function):
                 into = None
         with on_device(gy.device):
             dx = torch.empty_like(gy, dtype=torch.bfloat16, memory_format=torch.channels_last_3d)
-            _, dw, db = gk.gn8_backward(to_vm(gy), kept, w32, b32, stats, groups, relu, into=into, out=dx)
+            _, dw, db = gk.gn8_backward(_on_16_bytes(to_vm(gy)), kept, w32, b32, stats, groups, relu, into=into, out=dx)
         if into is not None:
             dw = db = None
             for p in ctx.params:
                 notify_grad_written(p)
         return dx, dw, db, None, None, None, None
+
+
+def _on_16_bytes(x: torch.Tensor) -> torch.Tensor:
+    """``x`` where the kernels' vector loads may start: a view into a larger tensor may lie anywhere."""
+    return x.clone() if x.data_ptr() % 16 else x
 
 
 def _fp32(p: torch.Tensor) -> torch.Tensor:

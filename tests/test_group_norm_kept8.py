@@ -192,6 +192,29 @@ def test_a_captured_pass_is_replayed_on_new_values():
         assert torch.equal(grads[1], want[1]) and torch.equal(grads[2], want[2])
 
 
+@pytest.mark.gpu
+def test_inputs_and_gradients_may_start_anywhere():
+    x, gy, w, b = _inputs((2, 3, 4, 5, 32), 11)
+
+    def off(t, by):
+        buf = torch.empty(t.numel() + by, dtype=t.dtype, device="cuda")
+        return buf[by:].view(t.shape).copy_(t).permute(0, 4, 1, 2, 3)
+
+    results = []
+    for by in (0, 1, 4):
+        leaf = off(x, by).requires_grad_()
+        y = group_norm_kept8(leaf, 8, w, b, activation="relu")
+        # (a gradient that is a piece of a larger one: what a concatenation hands back)
+        (dx,) = torch.autograd.grad(y, leaf, off(gy, by))
+        flat = torch.cat([w.new_zeros(by, dtype=torch.bfloat16), group_norm_kept8(leaf, 8, w, b, activation="relu")
+                          .permute(0, 2, 3, 4, 1).reshape(-1)])
+        (dz,) = torch.autograd.grad(flat, leaf, torch.cat([flat.new_zeros(by), gy.reshape(-1)]))
+        results.append((y.detach(), dx, dz))
+    for other in results[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(results[0], other))
+    assert torch.equal(results[0][1], results[0][2])
+
+
 def test_refusals():
     w, b = torch.ones(32), torch.zeros(32)
     x = torch.zeros(1, 32, 2, 2, 2, dtype=torch.bfloat16)
