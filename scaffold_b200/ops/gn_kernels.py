@@ -231,7 +231,10 @@ def supported_kept8(channels: int, groups: int) -> bool:
 
 @functools.lru_cache(maxsize=256)
 def _scratch8(backward: int, n: int, s: int, c: int, groups: int) -> int:
-    return int(_lib.lib().sb_gn8_scratch(backward, n, s, c, groups))
+    floats = int(_lib.lib().sb_gn8_scratch(backward, n, s, c, groups))
+    if floats < 0:
+        raise _lib.NativeError(f"sb_gn8_scratch refused {n} samples of {s} voxels, {c} channels in {groups} groups")
+    return floats
 
 
 def gn8_forward(x, w, b, groups: int, eps: float = 1e-5, relu: bool = True, fin: Optional[torch.Tensor] = None,

@@ -131,6 +131,8 @@ def group_norm_kept8(x: torch.Tensor, num_groups: int, weight: torch.Tensor, bia
                          "2048, and groups of whole octets (or of 2 or 4 channels)")
     if weight.shape != (c,) or bias.shape != (c,) or weight.device != dev or bias.device != dev:
         raise ValueError(f"weight and bias must be [{c}] on {dev}")
+    if x.shape[0] > 65535:
+        raise ValueError(f"group_norm_kept8 takes up to 65535 samples; got {x.shape[0]}")
     if x.numel() == 0:
         raise ValueError(f"group_norm_kept8 has no statistics of an empty tensor {tuple(x.shape)}")
     with on_device(dev):

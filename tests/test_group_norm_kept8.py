@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from scaffold_b200.ops import gn_kernels as gk
+from scaffold_b200.ops._lib import NativeError
 from scaffold_b200.ops.group_norm import GroupNorm, group_norm_kept8
 from scaffold_b200.ops.kept8 import Kept8, block_steps, restore8
 
@@ -233,3 +234,18 @@ def test_refusals_on_the_device():
                  (x[:, :24], 3, w[:24], b[:24]), (x[:0], 8, w, b)):
         with pytest.raises(ValueError):
             group_norm_kept8(*args)
+
+
+def test_the_scratch_of_sizes_outside_the_range():
+    for n, s in ((65536, 1), (0, 8), (1, 0)):
+        with pytest.raises(NativeError, match="samples"):
+            gk._scratch8(0, n, s, 16, 1)
+
+
+@pytest.mark.gpu
+def test_more_samples_than_a_grid_has():
+    w, b = torch.ones(16, device="cuda"), torch.zeros(16, device="cuda")
+    x = torch.zeros(65536, 16, 1, 1, 1, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="65535"):
+        group_norm_kept8(x, 1, w, b)
+    assert group_norm_kept8(x[:65535], 1, w, b).shape == x[:65535].shape
