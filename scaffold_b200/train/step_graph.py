@@ -252,7 +252,8 @@ class StepGraphs:
     @staticmethod
     def _usable(engine, images, masks) -> bool:
         model = engine.model
-        if not (engine.cuda and engine.fused_loss and engine.flat is not None and type(model) is UNet
+        if not (engine.cuda and engine.fused_loss and engine.loss == "ce_dice" and engine.flat is not None
+                and type(model) is UNet
                 and isinstance(engine.optimizer, FusedClipAdam) and engine.reducer.world == 1
                 and engine.spatial is None and model._spatial is None and not _replaced_steps(engine)):
             return False

@@ -207,6 +207,28 @@ def test_copies_and_the_loss_without_logits_together():
     torch.testing.assert_close(dice, ref, rtol=2e-7, atol=0)
 
 
+@pytest.mark.gpu
+def test_another_loss_ends_the_replays():
+    x, y = _batch(6, (16, 16, 16))
+    model = _model(width=16)
+    engine = TrainEngine(model, FusedClipAdam(model.parameters(), lr=0.0), 6, "cuda")
+    for _ in range(4):
+        engine.step(x, y)
+    for _ in range(4):
+        both = engine.eval_step(x, y)
+    assert all(type(p).__name__ == "_Pass" for p in engine._graphs._passes.values()) and len(engine._graphs._passes) == 2
+    ce = engine.last_ce.clone()
+    assert not engine.last_dice.isnan()
+    engine.loss = "ce"
+    loss = engine.step(x, y)
+    # the head's logits are rounded to bf16 in front of the other loss
+    assert engine.last_dice.isnan() and torch.equal(loss, engine.last_ce) and abs(float(loss - ce)) <= 2 ** -8 * float(ce)
+    assert float(engine.eval_step(x, y)[0]) == float(loss) != float(both[0])
+    engine.loss = "ce_dice"
+    engine.step(x, y)
+    assert torch.equal(engine.last_ce, ce)
+
+
 @pytest.mark.parametrize("amp", [True, False])
 def test_the_engine_on_the_cpu(amp):
     x, y = _batch(40, (8, 8, 8), 1, "cpu")
