@@ -439,6 +439,38 @@ def test_nothing_is_written_beside_the_gradients(v, c, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("v,c,k,weighted", [(130, 24, 35, False), (300, 64, 257, False), (5000, 64, 147, True),
+                                            (76001, 24, 1001, False), (4100, 8, 33, True), (300, 320, 70, True)])
+def test_nothing_is_written_beside_both_gradients(v, c, k, weighted):
+    """As above where both gradients come from one kernel, also in several launches: dX leaves it by TMA."""
+    x, w, b, y, cw = _inputs(v, c, k, ignored=0.1, weighted=weighted)
+    dev, margin = x.device, 4096
+    L, st, status = _lib.lib(), _lib.stream_ptr(), _lib.status_tensor(x.device).data_ptr()
+    y = y.int()
+
+    def guarded(n, t=torch.uint8):
+        buf = torch.full((n + 2 * margin,), 77, dtype=t, device=dev)
+        return buf, buf[margin:].data_ptr()
+
+    n_state, n_fwd, _, n_both = H._bytes(v, k, c, weighted)
+    bufs = [guarded(n) for n in (n_state, n_fwd, n_both)]
+    loss, dx, dw, db = guarded(1, torch.float32), *(guarded(n, torch.bfloat16) for n in (v * c, k * c, k))
+    _lib.check(L.sb_head_forward(x.data_ptr(), w.data_ptr(), b.data_ptr(), 0, y.data_ptr(), 4, 1, IGNORED, _lib.ptr(cw), v, k,
+                                 c, bufs[0][1], bufs[1][1], loss[1], status, st), "sb_head_forward")
+    one = torch.ones(1, device=dev)
+    _lib.check(L.sb_head_backward(x.data_ptr(), w.data_ptr(), _lib.ptr(cw), v, k, c, bufs[0][1], bufs[2][1], one.data_ptr(),
+                                  dx[1], dw[1], 0, db[1], 0, status, st), "sb_head_backward")
+    torch.cuda.synchronize()
+    _lib.check_status()
+    for t, _ in (*bufs, loss, dx, dw, db):
+        assert (t[:margin] == 77).all() and (t[-margin:] == 77).all()
+    xs, ws, bs = (t.clone().requires_grad_() for t in (x, w, b))
+    head_cross_entropy(xs, ws, bs, y, cw, ignore_label=IGNORED).backward()
+    assert torch.equal(dx[0][margin:-margin].view(v, c), xs.grad) and torch.equal(dw[0][margin:-margin].view(k, c), ws.grad)
+    assert torch.equal(db[0][margin:-margin], bs.grad)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("v,c,k", [(1, 8, 1), (1, 64, 5000), (300, 64, 147), (1000, 16, 33), (129, 256, 1000), (257, 320, 513),
                                    (30, 1024, 3000), (70000, 32, 34)])
 def test_the_predicted_class(v, c, k):

@@ -2,10 +2,11 @@
 import pytest
 import torch
 
+from helpers.launch import ROOT, results, torchrun_gloo
 from scaffold_b200.models.unet import UNet
 from scaffold_b200.ops import _lib, loss as L
-from scaffold_b200.ops.conv3d import Conv3d
-from scaffold_b200.ops.head_loss import head_predict
+from scaffold_b200.ops.conv3d import Conv3d, ConvTranspose3d
+from scaffold_b200.ops.head_loss import head_cross_entropy, head_predict
 from scaffold_b200.ops.optim import FusedClipAdam
 from scaffold_b200.train.engine import TrainEngine
 
@@ -101,6 +102,34 @@ def test_a_pass_without_gradients_makes_no_copies():
         losses.append(engine.eval_step(x, y)[0])
         counts.append(_lib.launch_count() - before)
     assert counts[0] == counts[1] > 0 and torch.equal(*losses)
+
+
+@pytest.mark.gpu
+def test_passes_that_were_captured_with_other_bits_are_not_replayed():
+    """Results of the forward pass are the same with 8 and 16 bits, gradients are not: those tell what ran."""
+    x, y = _batch(6, (16, 16, 16))
+    grads = {}
+    for name, bits, captured in (("8", 8, True), ("8 ordinary", 8, False), ("16 ordinary", 16, False)):
+        model = _model(width=16)
+        engine = TrainEngine(model, FusedClipAdam(model.parameters(), lr=0.0), 6, "cuda")
+        if not captured:
+            engine._graphs._usable = lambda *a: False
+        model.keep_activations(bits)
+        for _ in range(4):
+            engine.step(x, y)
+        grads[name] = engine.flat.grad.clone()
+        if captured:
+            (old,) = engine._graphs._passes.values()
+            assert type(old).__name__ == "_Pass" and old.fingerprint.holds(engine)
+            model.keep_activations(16)
+            assert not old.fingerprint.holds(engine)
+            for _ in range(4):
+                engine.step(x, y)
+            (new,) = engine._graphs._passes.values()
+            assert new is not old and type(new).__name__ == "_Pass"
+            grads["16"] = engine.flat.grad.clone()
+    assert torch.equal(grads["8"], grads["8 ordinary"]) and torch.equal(grads["16"], grads["16 ordinary"])
+    assert not torch.equal(grads["8"], grads["16"])
 
 
 class _Halo:
@@ -242,6 +271,97 @@ def test_the_engine_on_the_cpu(amp):
     assert dice.shape == (1, 40) and float(val) == float(val) and first > 0
     with pytest.raises(ValueError, match="loss"):
         TrainEngine(model, torch.optim.SGD(model.parameters(), lr=0.1), 40, "cpu", loss="dice")
+
+
+class _Exchanged:
+    """A spatial context of one shard whose volume is processed with H (or W) exchanged with the depth."""
+
+    size, dims, halo_channel = 1, [2], None
+
+    def __init__(self, lead_swap):
+        self.lead_swap = lead_swap
+
+    def to_kernel_space(self, t, first_spatial=2):
+        return t.transpose(first_spatial, first_spatial + self.lead_swap - 2)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("axis", [3, 4])
+def test_the_loss_of_a_volume_whose_axes_are_exchanged(axis, dev):
+    n_classes = 40
+    x, y = _batch(n_classes, (8, 16, 24) if dev == "cpu" else (16, 32, 24), 1, dev)
+    results = []
+    for spatial in (None, _Exchanged(axis)):
+        model = _model(n_classes, 16, 1, dev)
+        model.set_spatial(spatial)
+        for m in model.modules():
+            if isinstance(m, (Conv3d, ConvTranspose3d)):
+                m.set_spatial(spatial)
+        engine = TrainEngine(model, torch.optim.SGD(model.parameters(), lr=0.0), n_classes, dev, spatial=spatial,
+                             class_weights=torch.linspace(0.5, 2.0, n_classes, device=dev), amp=dev == "cuda", loss="ce",
+                             max_norm=1e9)
+        loss = engine.step(x, y)
+        grads = [p.grad.clone() for p in model.parameters()]
+        val, dice = engine.eval_step(x, y)
+        results.append((loss, grads, val, dice))
+    (loss, grads, val, dice), (loss2, grads2, val2, dice2) = results
+    # the exchanged volume's features against labels that were exchanged by hand: the same calls, to the bit
+    labels = y.transpose(1, axis - 1).contiguous()
+    head = model.up_list[-1].conv
+    with torch.autocast(dev, dtype=torch.bfloat16, enabled=dev == "cuda"):
+        features = model.features(x).permute(0, 2, 3, 4, 1)
+        want = head_cross_entropy(features, head.weight, head.bias, labels, engine.class_weights)
+        pred = head_predict(features, head.weight, head.bias)
+    assert torch.equal(loss2, want)
+    for p, g in zip(model.parameters(), torch.autograd.grad(want, list(model.parameters()))):
+        assert torch.equal(p.grad, g)
+    assert torch.equal(dice2, L.hard_dice_of_prediction(pred, labels, n_classes))
+    if dev == "cpu":  # and in 32 bits the volume as it is gives the same
+        assert abs(float(loss - loss2)) <= 1e-5 * float(loss) and abs(float(val - val2)) <= 1e-5 * float(val)
+        for a, b in zip(grads, grads2):
+            assert float((a - b).norm()) <= 1e-3 * float(a.norm()) + 1e-7
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_the_dice_of_a_prediction_over_shards(dev):
+    _, labels = _batch(7, (6, 10, 8), 2, dev)
+    labels[0, 0, 0, :3] = 9  # outside the classes
+    pred = torch.where(torch.rand(labels.shape, device=dev) < 0.5, labels, 2).clamp(max=6)
+    want = L.hard_dice_of_prediction(pred, labels, 7)
+    cut = [slice(0, 4), slice(4, 10)]
+
+    class Shard:
+        size, lead_swap = 2, None
+
+        def __init__(self, others=None):
+            self.others = others
+
+        def all_reduce_sum(self, t):
+            self.sent = t.clone()
+            if self.others is not None:
+                t += self.others
+
+    sent = []
+    for c in cut:
+        shard = Shard()
+        L.hard_dice_of_prediction(pred[:, :, c], labels[:, :, c], 7, shard)
+        sent.append(shard.sent)
+    for c, others in zip(cut, reversed(sent)):
+        assert torch.equal(L.hard_dice_of_prediction(pred[:, :, c], labels[:, :, c], 7, Shard(others)), want)
+
+
+@pytest.mark.slow
+def test_the_trainer_with_both_options_on_one_rank_and_on_two_shards(tmp_path):
+    script = ROOT / "tests" / "helpers" / "rank_scripts" / "benchmark_tiny.py"
+    runs = []
+    for ranks in (1, 2):
+        proc = torchrun_gloo(script, ranks, [str(tmp_path), str(ranks), "2", "{loss: ce, activation_bits: 8}"])
+        assert proc.returncode == 0, proc.stdout[-3000:] + proc.stderr[-3000:]
+        runs.append(results(proc.stdout))
+    for key in ("epoch1", "epoch2"):
+        a, b = ([float(v) for v in r[key][0].split()] for r in runs)
+        # fp32-level agreement of the losses; hard Dice: a few argmax near-ties may flip
+        assert abs(a[0] - b[0]) <= 5e-4 * a[0] and abs(a[1] - b[1]) <= 5e-4 * a[1] and abs(a[2] - b[2]) <= 5e-3, (key, a, b)
 
 
 def test_configuration_keys(tmp_path):
