@@ -1512,8 +1512,11 @@ constexpr int HD_BOXES = 54;  // of HD_BOX16 in shared memory; a tile of rows or
 // as L2. Loss and gradients of 401280 voxels x 32 channels x 1001 classes 366 us, in two kernels 431; 2^18 x 16 x 2000 420 and
 // 514; 2^19 x 24 x 3000 1425 and 1549; but 2^20 x 32 x 600 (three tiles) 701 and 663, 40000 x 32 x 1500 119 and 111, and the
 // gradients alone of 2^20 x 64 x 385 749 where 512 classes take 417 in two kernels; class weights 474 and 463 for 401280 x 32 x 1001. Few voxels want P
-// in two parts; with class weights more are few, since the rounding of u X stands next to P's: at 129 voxels, 60 % of them
-// ignored, single elements of dW were off by more than P's alone explains.
+// in two parts; with class weights more are few, since the rounding of u X stands next to P's. Error of dW out of this
+// kernel, class weights and 60 % of the voxels ignored, in parts of its norm (24 channels x 35 classes, 64 x 147, 16 x 257):
+// 1.7 to 2.8e-3 at 129 voxels, up to 2.4e-3 at 500, up to 2.0e-3 at 2000, 0.7 to 1.3e-3 at 4000, 0.6 to 0.8e-3 at 8000 and
+// falling; with P in two parts 4e-6. A bf16 dW's own rounding is 1.7e-3: the limit stands where the kernel's error is below
+// it. What that costs (loss and gradients of 64 x 147, this kernel / P in two parts): 29 / 36 us at 200 voxels, 46 / 55 at 4000.
 constexpr int HB_FEW_WEIGHTED = 4096;
 static int head_both(const HeadCall& a) {
   if (a.V <= (a.cw == nullptr ? HD_FEW : HB_FEW_WEIGHTED) || a.K > 65000) return 0;

@@ -2,7 +2,9 @@
 // (e >= -126) with max |x| < 126.5 * 2^e; each is kept as q = rint(x / 2^e), so |q| <= 126 and one whole number is left
 // on either side (GroupNorm uses it to keep a value on its side of the ReLU). A power of two makes every operation on
 // the way in and out exact but that one rounding: the copy does not depend on the order or the kind of arithmetic.
-// Error: half a step, which is at most max|x| / 126 of the block (2^-7 * max|x| on average over the mantissa).
+// Error: half a step, which is at most max|x| / 126 of the block (2^-7 * max|x| on average over the mantissa); 2^-127 where
+// e is held at -126 (max|x| below 63.25 * 2^-126, a block below 2^-127 comes back as zeros); less than a step in the
+// blocks of the last line.
 //
 // Memory: int8 q[blocks][16], then one byte e + 127 per block (1..249; 255: the block held an infinity or a NaN and is
 // restored as NaN, its q are zeros, so that 0 * 2^(255-127) = 0 * inf is the NaN). The last block is padded with zeros.

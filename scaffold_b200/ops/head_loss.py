@@ -5,8 +5,9 @@
 logits: a head of some hundred classes over a 128-cubed volume would keep gigabytes of them, several times over. The fused
 segmentation loss keeps a voxel's classes in registers and ends at 32 classes; this one has no limit on the classes.
 
-On CUDA with bf16 features (or under bf16 autocast) the kernels of ``csrc/head_loss.cu`` multiply features and weight
-tile by tile, once for the loss and once for each gradient; other tensors take the PyTorch formula.
+On CUDA with bf16 features (or under bf16 autocast) the kernels of ``csrc/head_loss.cu`` and ``csrc/head_wide.cu``
+multiply features and weight tile by tile: once for the loss, and once more for both gradients together or, where one
+kernel does not hold both, for each; other tensors take the PyTorch formula.
 """
 from __future__ import annotations
 
@@ -112,7 +113,10 @@ def head_cross_entropy(features: torch.Tensor, weight: torch.Tensor, bias: Optio
     :func:`scaffold_b200.ops._lib.check_status`. Features of voxels that take no part have to be finite for the
     kernels: they reach the weight's gradient as ``0 * x``, as in any matrix product with rows of zeros.
 
-    The kernels read bf16: an fp32 ``weight`` is rounded, its gradient comes back in fp32. Gradients: features in bf16,
+    The kernels read bf16: an fp32 ``weight`` is rounded, its gradient comes back in fp32. Logits, log-sum-exp and all sums
+    are fp32; the entries of ``softmax - onehot`` (and with ``class_weights`` the weighted features) are rounded to bf16 for
+    the gradients' products, except in calls of few voxels, where one rounding could make up a result. A feature of a voxel
+    that takes part which is infinite or NaN makes the loss NaN. Gradients: features in bf16,
     weight and bias in their own types; the class weights have none.
     """
     shape = features.shape

@@ -3,9 +3,10 @@
 ``keep8(x)`` writes the 8-bit copy of a tensor, ``restore8(kept)`` reads it back: 1.0625 bytes per element instead of 2
 (or 4). 16 elements that follow one another in memory share a power of two ``2^e``, the smallest one (``e`` at least
 -126) with ``max |x| < 126.5 * 2^e``; each is kept as the whole number nearest to ``x / 2^e`` (a tie goes to the even
-one), so a restored value is off by at most half a step, ``max |x| / 126`` of its block. A block with an infinity or a
-NaN is restored as NaN: an overflow shows. A value that would be restored beyond its type's largest number is kept as 63
-steps, so what was finite stays so.
+one), so a restored value is off by at most half a step: ``max |x| / 126`` of its block, or ``2^-127`` in blocks so small
+that ``e`` is -126 (a block below that comes back as zeros). A block with an infinity or a NaN is restored as
+NaN: an overflow shows. A value that would be restored beyond its type's largest number is kept as 63 steps, so what was
+finite stays so; it is off by less than a step then.
 
 A kept tensor is what a layer stores for its backward pass; no gradient flows through the copy. The layers of
 :mod:`scaffold_b200.ops` use it when they are told to (``UNet.keep_activations(bits=8)``).
