@@ -308,6 +308,31 @@ def test_a_label_on_a_class_that_is_off(v, c, k, dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("low", [float("-inf"), torch.finfo(torch.bfloat16).min, -1e30, -1e20, -1e10, -3e9, -1e9, -1e6, -1e4])
+@pytest.mark.parametrize("v,c,k", [(300, 64, 147), (5000, 16, 129), (63, 48, 385), (1575, 40, 129), (70000, 24, 100),
+                                   (300, 200, 300), (7, 256, 3000), (300, 320, 300)])
+def test_runs_of_classes_that_are_off(v, c, k, low):
+    """A mask of the classes at the front, at the end and in between, as a bias far below the others: whole runs of columns
+    have nothing else, and their probabilities are zero."""
+    x, w, b, y, _ = _inputs(v, c, k, w_type=torch.float32, scale=4.0)
+    w = w.to(torch.bfloat16)
+    b = b.float()
+    y = y % 5 + 70  # the classes that stay are 64 to 95
+    for off in (slice(0, 64), slice(128, None), slice(0, 1), slice(96, None)):
+        b[off] = low
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        loss = head_cross_entropy(*leaves, y)
+        grads = torch.autograd.grad(loss, leaves)
+        rl, *want, _, s = _definition(x, w, b, y, None)
+        error = c * 2 ** -23 * float((x.double().abs() @ w.double().abs().T).amax()) + 2 ** -20 * (1 + float(s[:, 64:96].abs().amax()))
+        assert abs(float(loss.detach()) - float(rl)) <= 2 * error + 2 ** -23 * float(rl)
+        for got, ref in zip(grads, want):
+            assert got.isfinite().all()
+            assert float((got.double() - ref).norm()) <= 4e-3 * float(ref.norm()) + 4 * error * float(ref.abs().amax()) * ref.numel() ** 0.5
+        assert ((H.head_predict(x, w, b) >= 64) & (H.head_predict(x, w, b) < 128)).all() or off.start == 0
+
+
+@pytest.mark.gpu
 def test_shapes_views_and_evaluation():
     x, w, b, y, cw = _inputs(2 * 3 * 4 * 5, 48, 50, weighted=True)
     ref = head_cross_entropy(x, w, b, y, cw)
