@@ -162,9 +162,10 @@ __device__ __forceinline__ float hd_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// -m log2(e), what the running maximum m adds to an exponent, rounded down: for large m (a run of classes that their biases
-// turn off) m log2(e) less its nearest fp32 may be some hundred and more, whose power of two is an infinity.
-__device__ __forceinline__ float hd_base(float m) { return __fmul_rd(-m, HD_LOG2E); }
+// A row's sum of powers of two, held finite (a NaN stays). Beyond |m| of some 1e9 (a run of classes that their biases turn
+// off) m log2(e) less its nearest fp32, the exponent of the maximum itself, may be some hundred and more. Where other classes
+// follow, what such a run left is multiplied by zero, which an infinity would not survive; else it is below m's rounding.
+__device__ __forceinline__ void hd_hold(float& s) { asm("min.NaN.f32 %0, %0, 0f7149F2CA;" : "+f"(s)); }  // 1e30
 // where `bits & bit`: v -= d; predicated, never a branch
 __device__ __forceinline__ void hd_sub_if(float& v, float d, uint32_t bits, uint32_t bit) {
   asm("{\n\t.reg .pred q;\n\t.reg .b32 t;\n\tand.b32 t, %2, %3;\n\tsetp.ne.u32 q, t, 0;\n\t@q sub.f32 %0, %0, %1;\n\t}"
@@ -400,7 +401,7 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
         rt %= row_jobs;
       }
       if (sp < p.splits) y_next = label_of(rt);
-      float m = ARG ? -INFINITY : HD_LOWEST, from_m = hd_base(HD_LOWEST), s = 0.f, tl = 0.f;
+      float m = ARG ? -INFINITY : HD_LOWEST, s = 0.f, tl = 0.f;
       bool met = false;
       int best = INT_MAX;
       int t = four ? t0 : t0 + (int)((group - fi) & 3u);
@@ -455,12 +456,10 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
             }
             const float top = hd_max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
             if (top > m) {
-              const float before = from_m;
-              from_m = hd_base(top);
-              s *= hd_ex2(from_m - before);
+              s *= hd_ex2((m - top) * HD_LOG2E);
               m = top;
             }
-            const float2 scale = make_float2(HD_LOG2E, HD_LOG2E), base = make_float2(from_m, from_m);
+            const float2 scale = make_float2(HD_LOG2E, HD_LOG2E), base = make_float2(-m * HD_LOG2E, -m * HD_LOG2E);
             float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
@@ -469,19 +468,20 @@ __global__ void __launch_bounds__(HD_THREADS, 1) head_rows_kernel(const __grid_c
             }
             a[0] = hd_add2(a[0], a[1]);
             s += a[0].x + a[0].y;
+            hd_hold(s);
           }
         }
       }
       if (!ARG && p.whole) {
         if (ok && r < p.rows_pad) {
           uint32_t hit = 0xFFFFu;
-          p.lse2_out[r] = r < p.rows ? hd_voxel(-from_m, s, -hd_base(tl), y, p.cw, p.bias, p.bias_kind, total, hit)
+          p.lse2_out[r] = r < p.rows ? hd_voxel(m * HD_LOG2E, s, tl * HD_LOG2E, y, p.cw, p.bias, p.bias_kind, total, hit)
                                        : INFINITY;
           if (p.hit_out != nullptr) p.hit_out[r] = hit;
         }
       } else if (ok && r < p.rows_pad) {
-        p.part[(long long)slot * p.rows_pad + r] = ARG ? make_float2(m, __int_as_float(best)) : make_float2(-from_m, s);
-        if (!ARG && met) p.tl[r] = -hd_base(tl);  // (rounded as the maximum is)
+        p.part[(long long)slot * p.rows_pad + r] = ARG ? make_float2(m, __int_as_float(best)) : make_float2(m * HD_LOG2E, s);
+        if (!ARG && met) p.tl[r] = tl * HD_LOG2E;
       }
     }
   }
