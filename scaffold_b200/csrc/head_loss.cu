@@ -1392,8 +1392,10 @@ __global__ void __launch_bounds__(256) head_merge_kernel(const float2* __restric
     float l = INFINITY;
     uint32_t h = 0xFFFFu;
     if (i < V) {  // (the same in a team's lanes)
+      const float at_label = __ldg(tl + i);  // requested ahead of the shares
+      const int label = __ldg(y + i);
       const float2 e = hd_merge_sums<TEAM>(part, shares, v_pad, i, lane);
-      if (lane == 0) l = hd_voxel(e.x, e.y, tl[i], y[i], cw, bias, bias_kind, a, h);
+      if (lane == 0) l = hd_voxel(e.x, e.y, at_label, label, cw, bias, bias_kind, a, h);
     }
     if (lane == 0) {
       lse2[i] = l;
